@@ -1,4 +1,5 @@
-"""ctypes binding of include/bbh.h (libbbh.so, built in-tree by the Makefile).
+"""ctypes binding of include/bbh.h and include/bbh_int8.h (libbbh.so, built
+in-tree by the Makefile).
 
 There is deliberately no fallback: if libbbh.so is missing or fails to load,
 importing the product path raises.  Nothing here computes anything on the CPU.
@@ -112,6 +113,15 @@ SIGNATURES = {
                              c_void_p, c_void_p]),
 }
 
+# Every symbol declared in include/bbh_int8.h.
+SIGNATURES_INT8 = {
+    "bbh_quantize_rows": (c_int, [c_void_p] * 3 + [c_int, c_int, c_void_p]),
+    "bbh_dequantize_rows": (c_int, [c_void_p] * 3 + [c_int, c_int, c_void_p]),
+    "bbh_rmsnorm_quantize": (c_int, [c_void_p] * 7 + [c_int, c_int, c_float, c_void_p]),
+    "bbh_layernorm_quantize": (c_int, [c_void_p] * 8 + [c_int, c_int, c_float, c_void_p]),
+    "bbh_linear_i8": (c_int, [c_void_p] * 5 + [c_int] * 3 + [c_void_p, c_int, c_void_p]),
+}
+
 # Exported for profile tables only: what the launchers choose.
 QUERIES = {
     "bbh_linear_tile": (c_int, [c_int, c_int, c_int, c_int]),
@@ -149,7 +159,7 @@ def lib():
         import torch  # noqa: F401
 
         L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in {**SIGNATURES, **QUERIES}.items():
+        for name, (res, args) in {**SIGNATURES, **SIGNATURES_INT8, **QUERIES}.items():
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

@@ -460,6 +460,85 @@ def launch_pool_normalize(hidden, mask, out, seq, batch=1, stream=None):
     return out
 
 
+# ---- 8-bit operators (include/bbh_int8.h) -----------------------------------
+
+I8_MAX_K = 131071  # BBH_I8_MAX_K
+I8_MAX_NORM = 16384  # BBH_I8_MAX_NORM
+
+
+def _check_i8(dtypes, numels, **tensors):
+    """Each tensor (None: not passed) is contiguous, of its dtype, on the
+    current device and of at least its number of elements."""
+    if min(numels) < 1:
+        raise ValueError("sizes must be positive")
+    dev = _torch().cuda.current_device() if any(
+        t is not None and t.is_cuda for t in tensors.values()) else None
+    for (name, t), dtype, n in zip(tensors.items(), dtypes, numels):
+        if t is None:
+            continue
+        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
+            raise TypeError(f"{name} must be a contiguous {dtype} CUDA tensor")
+        if t.get_device() != dev:
+            raise ValueError(f"{name} is on cuda:{t.get_device()}, the current device is cuda:{dev}")
+        if t.numel() < n:
+            raise ValueError(f"{name}: expected {n} elements, got {t.numel()}")
+
+
+def launch_quantize_rows(x, q, scale, M, D, stream=None):
+    """x (M, D) fp16 -> q (M, D) int8, scale (M) fp32: one scale a row, the
+    largest magnitude / 127 (bbh_quantize_rows)."""
+    torch = _torch()
+    _check_i8((torch.float16, torch.int8, torch.float32), (M * D, M * D, M), x=x, q=q, scale=scale)
+    call("bbh_quantize_rows", _ptr(x), _ptr(q), _ptr(scale), M, D, _stream(stream))
+    return q, scale
+
+
+def launch_dequantize_rows(q, scale, x, M, D, stream=None):
+    """x (M, D) fp16 = q * scale, row by row (bbh_dequantize_rows)."""
+    torch = _torch()
+    _check_i8((torch.int8, torch.float32, torch.float16), (M * D, M, M * D), q=q, scale=scale, x=x)
+    call("bbh_dequantize_rows", _ptr(q), _ptr(scale), _ptr(x), M, D, _stream(stream))
+    return x
+
+
+def launch_rmsnorm_quantize(x, gamma, q, scale, M, D, eps=1e-6, residual=None, sum=None, y=None,
+                            stream=None):
+    """RMS norm of x [+ residual] times gamma, quantised a row at a time into
+    q, scale; sum (x + residual) and y (the norm) get fp16 where given
+    (bbh_rmsnorm_quantize)."""
+    f16 = _torch().float16
+    _check_i8((f16, f16, f16, f16, f16, _torch().int8, _torch().float32),
+              (M * D, M * D, D, M * D, M * D, M * D, M), x=x, residual=residual, gamma=gamma,
+              sum=sum, y=y, q=q, scale=scale)
+    call("bbh_rmsnorm_quantize", _ptr(x), _ptr(residual), _ptr(gamma), _ptr(sum), _ptr(y), _ptr(q),
+         _ptr(scale), M, D, eps, _stream(stream))
+    return q, scale
+
+
+def launch_layernorm_quantize(x, gamma, beta, q, scale, M, D, eps=LAYER_NORM_EPS, residual=None,
+                              sum=None, y=None, stream=None):
+    """launch_rmsnorm_quantize for LayerNorm (bbh_layernorm_quantize)."""
+    f16 = _torch().float16
+    _check_i8((f16, f16, f16, f16, f16, f16, _torch().int8, _torch().float32),
+              (M * D, M * D, D, D, M * D, M * D, M * D, M), x=x, residual=residual, gamma=gamma,
+              beta=beta, sum=sum, y=y, q=q, scale=scale)
+    call("bbh_layernorm_quantize", _ptr(x), _ptr(residual), _ptr(gamma), _ptr(beta), _ptr(sum),
+         _ptr(y), _ptr(q), _ptr(scale), M, D, eps, _stream(stream))
+    return q, scale
+
+
+def launch_matmul_i8(A, a_scale, B, b_scale, C, M, N, K, bias=None, gelu=False, stream=None):
+    """launch_matmul on 8-bit rows: C (M, N) fp16 = a_scale[m] * b_scale[n] *
+    (A (M, K) . B (N, K)^T) [+ bias] [GELU], the sums exact (bbh_linear_i8)."""
+    torch = _torch()
+    i8, f32, f16 = torch.int8, torch.float32, torch.float16
+    _check_i8((i8, f32, i8, f32, f16, f16), (M * K, M, N * K, N, M * N, N), A=A, a_scale=a_scale,
+              B=B, b_scale=b_scale, C=C, bias=bias)
+    call("bbh_linear_i8", _ptr(A), _ptr(a_scale), _ptr(B), _ptr(b_scale), _ptr(C), M, N, K,
+         _ptr(bias), int(bool(gelu)), _stream(stream))
+    return C
+
+
 class Tokenizer:
     """The uncased BERT WordPiece tokenizer (bbh_tokenizer_load / bbh_tokenize):
     texts -> host int32 (n, seq) ids, types, mask, as

@@ -1,0 +1,335 @@
+// 8-bit rows: quantising, reading back, and the residual norms that quantise
+// what they compute.
+//
+// A row's codes need its largest magnitude first, so the row stays in
+// registers between the reductions and its values are read once and written
+// once: bound by HBM (by the launch below a few hundred rows).  T threads own
+// a row, thread t the 8-wide chunks t, t + T, ..., V of them: 16-byte loads,
+// 8-byte stores of codes, any row length and alignment (the last chunk of a
+// row goes element by element).
+//
+// The largest magnitude is reduced on the bit patterns as unsigned integers:
+// they order like the magnitudes, an infinity above every number and a NaN
+// above that, so one reduction also tells whether the row is finite.
+
+#include <algorithm>
+
+#include "int8.h"
+
+namespace bbh {
+namespace {
+
+typedef f16x8 f16x8_any __attribute__((aligned(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(1)));
+
+enum Kind { kPlain, kRms, kLayer };
+
+struct UMaxOp {
+  __device__ __forceinline__ float operator()(float a, float b) const {
+    return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+  }
+};
+
+// Reduction over the T threads of a row.  T > 64: over the workgroup, through
+// `part` (one array a call: the next call's writes need no barrier before them).
+template <int T, class F>
+__device__ __forceinline__ float row_reduce(float v, F f, float* part) {
+  v = xor_op<8>(v, f);
+  v = xor_op<4>(v, f);
+  v = xor_op<2>(v, f);
+  v = xor_op<1>(v, f);
+  if constexpr (T >= 64) {
+    v = xor_op<32>(v, f);
+    v = xor_op<16>(v, f);
+  }
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int w = 1; w < T / 64; ++w) v = f(v, part[w]);
+  }
+  return v;
+}
+
+// Chunk `c` of a row of D halves as fp32; zeros past the row's end.
+__device__ __forceinline__ void load8(const f16* row, int c, int D, float (&v)[8]) {
+  const int o = c * 8;
+  if (o + 8 <= D) {
+    const f16x8 a = *reinterpret_cast<const f16x8_any*>(row + o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)a[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = o + e < D ? (float)row[o + e] : 0.f;
+  }
+}
+
+__device__ __forceinline__ void store8(f16* row, int c, int D, const float (&v)[8]) {
+  const int o = c * 8;
+  if (o + 8 <= D) {
+    f16x8 a;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = (f16)v[e];
+    *reinterpret_cast<f16x8_any*>(row + o) = a;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (o + e < D) row[o + e] = (f16)v[e];
+  }
+}
+
+// How a row's values become codes: v / scale = 127 v / amax.
+struct Coder {
+  float amax, inv;
+  bool finite;
+  // (Below 2^-120, which no fp16 row reaches, the reciprocal would overflow.)
+  __device__ __forceinline__ explicit Coder(float a) : amax(a) {
+    finite = __float_as_uint(amax) < 0x7f800000u;
+    inv = finite && amax >= 0x1p-120f ? 1.0f / amax : 0.f;
+  }
+  __device__ __forceinline__ float scale() const {
+    return finite ? amax / 127.0f : __uint_as_float(0x7fc00000u);
+  }
+  // The rounded code in the low byte.  The product with the reciprocal is off
+  // by up to 2^-16 of a step near 127, enough to push an exact tie to the wrong
+  // side; one correction by its remainder gives the quotient rounded once.
+  // (127 v is exact for v from fp16.)  Adding 1.5 * 2^23 rounds to an integer,
+  // ties to even, and leaves it in two's complement in the sum's low bits.
+  __device__ __forceinline__ uint32_t code(float v) const {
+    const float t = 127.0f * v, q = t * inv;
+    const float c = fmaf(fmaf(-q, amax, t), inv, q);
+    return __float_as_uint(c + 12582912.0f);
+  }
+  __device__ __forceinline__ uint32_t code4(const float* v) const {
+    // perm selects bytes of {a, b}: 0-3 from b, 4-7 from a
+    const uint32_t lo = __builtin_amdgcn_perm(code(v[1]), code(v[0]), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(code(v[3]), code(v[2]), 0x04000c0cu);
+    return finite ? lo | hi : 0u;
+  }
+};
+
+__device__ __forceinline__ void store_codes(int8_t* row, int c, int D, const Coder& k,
+                                            const float (&v)[8]) {
+  const int o = c * 8;
+  const u32x2 w = {k.code4(v), k.code4(v + 4)};
+  if (o + 8 <= D) {
+    *reinterpret_cast<u32x2_any*>(row + o) = w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (o + e < D) row[o + e] = (int8_t)(w[e / 4] >> (8 * (e % 4)));
+  }
+}
+
+// This workgroup's first row (or item) of a launch of grid2().
+__device__ __forceinline__ int64_t block_id() {
+  return (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+}
+
+struct NormArgs {
+  const f16 *residual, *gamma, *beta;
+  f16 *sum, *y;
+  float eps;
+};
+
+// x and the outputs may be the same rows, so none is __restrict__; every
+// thread writes only the elements it has read.
+template <int T, int V, Kind KIND>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_kernel(const f16* x, int8_t* q,
+                                                                     float* scale, int M, int D,
+                                                                     NormArgs a) {
+  constexpr int R = T < 256 ? 256 / T : 1;  // rows a workgroup
+  __shared__ float part[4][T > 64 ? T / 64 : 1];
+  const int64_t row = block_id() * R + threadIdx.x / T;
+  const int t = threadIdx.x % T;
+  if (row >= M) return;  // T > 64: the whole workgroup
+  const size_t off = (size_t)row * D;
+  const int chunks = (D + 7) / 8;
+  float v[V][8];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = t + T * i;
+    if (c < chunks) {
+      load8(x + off, c, D, v[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    }
+  }
+  float rstd = 1.f;
+  if constexpr (KIND != kPlain) {
+    if (a.residual) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = t + T * i;
+        if (c >= chunks) break;
+        float r[8];
+        load8(a.residual + off, c, D, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] += r[e];
+      }
+    }
+    if (a.sum) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = t + T * i;
+        if (c < chunks) store8(a.sum + off, c, D, v[i]);
+      }
+    }
+    if constexpr (KIND == kLayer) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += v[i][e];
+      const float mean = row_reduce<T>(s, AddOp{}, part[0]) / (float)D;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          v[i][e] = (t + T * i) * 8 + e < D ? v[i][e] - mean : 0.f;
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += v[i][e] * v[i][e];
+    rstd = rsqrtf(row_reduce<T>(s, AddOp{}, part[1]) / (float)D + a.eps);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = t + T * i;
+      if (c >= chunks) break;
+      float g[8], b[8];
+      load8(a.gamma, c, D, g);
+      if constexpr (KIND == kLayer) load8(a.beta, c, D, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[i][e] = v[i][e] * rstd * g[e];
+        if constexpr (KIND == kLayer) v[i][e] += b[e];
+      }
+      if (a.y) store8(a.y + off, c, D, v[i]);
+    }
+  }
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = UMaxOp{}(m, fabsf(v[i][e]));
+  const Coder k(row_reduce<T>(m, UMaxOp{}, part[2]));
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = t + T * i;
+    if (c < chunks) store_codes(q + off, c, D, k, v[i]);
+  }
+  if (t == 0) scale[row] = k.scale();
+}
+
+// Rows longer than 16384: one workgroup a row, read twice (the second time
+// from L2).
+constexpr int kWide = 1024;
+__global__ __launch_bounds__(kWide) void quantize_wide_kernel(const f16* __restrict__ x,
+                                                              int8_t* __restrict__ q,
+                                                              float* __restrict__ scale, int M,
+                                                              int D) {
+  __shared__ float part[kWide / 64];
+  const int64_t row = block_id();
+  if (row >= M) return;
+  const size_t off = (size_t)row * D;
+  const int chunks = (D + 7) / 8;
+  float m = 0.f, v[8];
+  for (int c = threadIdx.x; c < chunks; c += kWide) {
+    load8(x + off, c, D, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = UMaxOp{}(m, fabsf(v[e]));
+  }
+  const Coder k(row_reduce<kWide>(m, UMaxOp{}, part));
+  for (int c = threadIdx.x; c < chunks; c += kWide) {
+    load8(x + off, c, D, v);
+    store_codes(q + off, c, D, k, v);
+  }
+  if (threadIdx.x == 0) scale[row] = k.scale();
+}
+
+// T threads a row, eight codes at a time.
+template <int T>
+__global__ __launch_bounds__(256) void dequantize_kernel(const int8_t* __restrict__ q,
+                                                         const float* __restrict__ scale,
+                                                         f16* __restrict__ x, int M, int D) {
+  const int64_t row = block_id() * (256 / T) + threadIdx.x / T;
+  if (row >= M) return;
+  const size_t off = (size_t)row * D;
+  const float s = scale[row];
+  for (int c = threadIdx.x % T; c < (D + 7) / 8; c += T) {
+    const int o = c * 8;
+    float v[8];
+    if (o + 8 <= D) {
+      const u32x2 w = *reinterpret_cast<const u32x2_any*>(q + off + o);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * s;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = o + e < D ? (float)q[off + o + e] * s : 0.f;
+    }
+    store8(x + off, c, D, v);
+  }
+}
+
+// n workgroups: no launch dimension counts 2^32 threads.
+dim3 grid2(int64_t n) {
+  constexpr int64_t X = 1 << 21;
+  return n <= X ? dim3((uint32_t)n) : dim3((uint32_t)X, (uint32_t)((n + X - 1) / X));
+}
+
+template <int T, int V, Kind KIND>
+hipError_t launch(const f16* x, int8_t* q, float* scale, int M, int D, const NormArgs& a,
+                  hipStream_t s) {
+  constexpr int R = T < 256 ? 256 / T : 1;
+  hipLaunchKernelGGL((quantize_kernel<T, V, KIND>), grid2(((int64_t)M + R - 1) / R),
+                     dim3(T < 256 ? 256 : T), 0, s, x, q, scale, M, D, a);
+  return hipGetLastError();
+}
+
+template <Kind KIND>
+hipError_t quantize(const f16* x, int8_t* q, float* scale, int M, int D, const NormArgs& a,
+                    hipStream_t s) {
+  const int chunks = (D + 7) / 8;
+  if (chunks <= 64) return launch<64, 1, KIND>(x, q, scale, M, D, a, s);
+  if (chunks <= 128) return launch<64, 2, KIND>(x, q, scale, M, D, a, s);
+  if (chunks <= 256) return launch<256, 1, KIND>(x, q, scale, M, D, a, s);
+  if (chunks <= 512) return launch<256, 2, KIND>(x, q, scale, M, D, a, s);
+  if (chunks <= 1024) return launch<256, 4, KIND>(x, q, scale, M, D, a, s);
+  return launch<1024, 2, KIND>(x, q, scale, M, D, a, s);
+}
+
+}  // namespace
+
+hipError_t quantize_rows(const f16* x, int8_t* q, float* scale, int M, int D, hipStream_t s) {
+  if (D <= kMaxNormRow) return quantize<kPlain>(x, q, scale, M, D, NormArgs{}, s);
+  hipLaunchKernelGGL(quantize_wide_kernel, grid2(M), dim3(kWide), 0, s, x, q, scale, M, D);
+  return hipGetLastError();
+}
+
+hipError_t dequantize_rows(const int8_t* q, const float* scale, f16* x, int M, int D,
+                           hipStream_t s) {
+  if (D <= 1024)
+    hipLaunchKernelGGL(dequantize_kernel<64>, grid2(((int64_t)M + 3) / 4), dim3(256), 0, s, q,
+                       scale, x, M, D);
+  else
+    hipLaunchKernelGGL(dequantize_kernel<256>, grid2(M), dim3(256), 0, s, q, scale, x, M, D);
+  return hipGetLastError();
+}
+
+hipError_t rmsnorm_quantize(const f16* x, const f16* residual, const f16* gamma, f16* sum, f16* y,
+                            int8_t* q, float* scale, int M, int D, float eps, hipStream_t s) {
+  return quantize<kRms>(x, q, scale, M, D, NormArgs{residual, gamma, nullptr, sum, y, eps}, s);
+}
+
+hipError_t layernorm_quantize(const f16* x, const f16* residual, const f16* gamma,
+                              const f16* beta, f16* sum, f16* y, int8_t* q, float* scale, int M,
+                              int D, float eps, hipStream_t s) {
+  return quantize<kLayer>(x, q, scale, M, D, NormArgs{residual, gamma, beta, sum, y, eps}, s);
+}
+
+}  // namespace bbh

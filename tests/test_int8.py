@@ -1,0 +1,621 @@
+"""The 8-bit operators (include/bbh_int8.h): refusals on the CPU, numerics on
+the GPU against the formulas in 64 bits.
+
+u is half a step of fp32 relative to the value, 2^-24; H the same of fp16,
+2^-11.  A sum of D products over a workgroup is at most 32 additions a thread
+and 12 levels of a tree: relative error <= 45 u where no term is negative."""
+
+import ctypes
+import os
+import re
+
+import numpy as np
+import pytest
+
+from conftest import ROOT
+
+U, H = 2.0 ** -24, 2.0 ** -11
+TINY = 2.0 ** -25  # half a step of fp16 below its normal range
+gpu = pytest.mark.gpu
+
+
+# ---- CPU: declarations and refusals -------------------------------------------
+
+def _lib():
+    from bbh import capi
+
+    return capi.lib()
+
+
+def test_header_declarations_all_exported():
+    from bbh import capi
+
+    text = open(os.path.join(ROOT, "include", "bbh_int8.h")).read()
+    names = sorted(set(re.findall(r"^bbh_status (bbh_[a-z0-9_]+)\s*\(", text, re.M)))
+    assert len(names) == 5 and sorted(capi.SIGNATURES_INT8) == names
+    for n in names:
+        assert hasattr(_lib(), n), n
+
+
+P = 1 << 20  # fake operands, 1 MB apart; refusals come before any device work
+
+
+def _p(i, off=0):
+    return None if i is None else ctypes.c_void_p(P * i + off)
+
+
+@pytest.mark.parametrize("args, status, message", [
+    ((None, 2, 3, 4, 8), 1, b"null"),
+    ((1, 2, 3, 0, 8), 1, b"positive"),
+    ((1, 2, 3, 4, 0), 1, b"positive"),
+    ((1, 2, 3, -1, 8), 1, b"positive"),
+    ((1, 2, 3, 1, 131072), 7, b"131071"),
+    ((1, 1, 3, 4, 8), 1, b"overlap"),
+    ((1, 2, 1, 4, 8), 1, b"overlap"),
+])
+def test_quantize_refusals(args, status, message):
+    L = _lib()
+    a, b, c, m, d = args
+    assert L.bbh_quantize_rows(_p(a), _p(b), _p(c), m, d, None) == status
+    assert message in L.bbh_last_error()
+    assert L.bbh_dequantize_rows(_p(b), _p(c), _p(a), m, d, None) == (
+        status if args[1:3] != (2, 1) else 1)
+
+
+def test_quantize_misaligned():
+    L = _lib()
+    assert L.bbh_quantize_rows(_p(1, 1), _p(2), _p(3), 4, 8, None) == 1
+    assert L.bbh_quantize_rows(_p(1), _p(2), _p(3, 2), 4, 8, None) == 1
+    assert b"aligned" in L.bbh_last_error()
+    assert L.bbh_dequantize_rows(_p(2), _p(3), _p(1, 1), 4, 8, None) == 1
+
+
+@pytest.mark.parametrize("change, status, message", [
+    (dict(x=None), 1, b"null"), (dict(gamma=None), 1, b"null"), (dict(q=None), 1, b"null"),
+    (dict(scale=None), 1, b"null"), (dict(M=0), 1, b"positive"), (dict(D=-3), 1, b"positive"),
+    (dict(D=16385), 7, b"16384"), (dict(eps=-1e-6), 1, b"eps"), (dict(eps=float("nan")), 1, b"eps"),
+    (dict(eps=float("inf")), 1, b"eps"), (dict(y=7, sum=7), 1, b"overlap"),
+    (dict(q=1), 1, b"overlap"), (dict(q=2), 1, b"overlap"), (dict(scale=7, y=7), 1, b"overlap"),
+    (dict(sum=(1, 16)), 1, b"in part"), (dict(y=(2, 2)), 1, b"in part"),
+    (dict(y=3), 1, b"gamma or beta"), (dict(q=3), 1, b"overlap"),
+    (dict(x=(1, 1)), 1, b"aligned"), (dict(scale=(8, 2)), 1, b"aligned"),
+])
+def test_norm_refusals(change, status, message):
+    L = _lib()
+    a = dict(x=1, residual=2, gamma=3, beta=4, sum=None, y=None, q=5, scale=6, M=4, D=64, eps=1e-6)
+    a.update(change)
+    v = {k: (_p(*t) if isinstance(t, tuple) else _p(t)) for k, t in a.items()
+         if k not in ("M", "D", "eps")}
+    tail = (v["sum"], v["y"], v["q"], v["scale"], a["M"], a["D"], ctypes.c_float(a["eps"]), None)
+    assert L.bbh_rmsnorm_quantize(v["x"], v["residual"], v["gamma"], *tail) == status
+    assert message in L.bbh_last_error()
+    assert L.bbh_layernorm_quantize(v["x"], v["residual"], v["gamma"], v["beta"], *tail) == status
+    assert message in L.bbh_last_error()
+    assert L.bbh_layernorm_quantize(v["x"], v["residual"], v["gamma"], None, *tail) == 1
+
+
+@pytest.mark.parametrize("change, status, message", [
+    (dict(A=None), 1, b"null"), (dict(sa=None), 1, b"null"), (dict(B=None), 1, b"null"),
+    (dict(sb=None), 1, b"null"), (dict(C=None), 1, b"null"), (dict(M=0), 1, b"positive"),
+    (dict(N=0), 1, b"positive"), (dict(K=0), 1, b"positive"), (dict(K=-5), 1, b"positive"),
+    (dict(K=131072), 7, b"131071"), (dict(C=(5, 1)), 1, b"aligned"), (dict(sa=(2, 1)), 1, b"aligned"),
+    (dict(bias=(6, 1)), 1, b"aligned"), (dict(C=1), 1, b"overlap"), (dict(C=3), 1, b"overlap"),
+    (dict(C=2), 1, b"overlap"), (dict(C=4), 1, b"overlap"), (dict(C=6), 1, b"overlap"),
+])
+def test_linear_refusals(change, status, message):
+    L = _lib()
+    a = dict(A=1, sa=2, B=3, sb=4, C=5, bias=6, M=4, N=64, K=64)
+    a.update(change)
+    v = {k: (_p(*t) if isinstance(t, tuple) else _p(t)) for k, t in a.items()
+         if k not in ("M", "N", "K")}
+    assert L.bbh_linear_i8(v["A"], v["sa"], v["B"], v["sb"], v["C"], a["M"], a["N"], a["K"],
+                           v["bias"], 0, None) == status
+    assert message in L.bbh_last_error()
+
+
+def test_python_refuses_host_tensors_and_wrong_types():
+    import torch
+    from bbh import engine
+
+    x, q, s = torch.zeros(4, 8).half(), torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4)
+    with pytest.raises(TypeError):
+        engine.launch_quantize_rows(x, q, s, 4, 8)
+    with pytest.raises(TypeError):
+        engine.launch_dequantize_rows(q, s, x, 4, 8)
+    with pytest.raises(TypeError):
+        engine.launch_rmsnorm_quantize(x, x[0], q, s, 4, 8)
+    with pytest.raises(TypeError):
+        engine.launch_matmul_i8(q, s, q, s, x, 4, 4, 8)
+    with pytest.raises(ValueError):
+        engine.launch_quantize_rows(x, q, s, -4, -8)
+
+
+# ---- GPU -----------------------------------------------------------------------
+
+def _gen(torch, seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _half(torch, g, *shape, scale=1.0):
+    return (scale * torch.randn(shape, device="cuda", generator=g)).half()
+
+
+def _codes64(torch, v):
+    """fp64 rows -> codes (fp64, not yet rounded), scale."""
+    a = v.abs().amax(1)
+    return torch.where(a[:, None] > 0, 127 * v / a[:, None], 0.0), a / 127
+
+
+ROWS = [1, 7, 8, 9, 16, 33, 100, 384, 385, 512, 513, 777, 1024, 1536, 2047, 2048, 2049, 4096, 5000,
+        8192, 8193, 12001, 16384]
+
+
+def _guarded(torch, n, dtype, fill, off=0):
+    """n elements with 64 more after them (and `off` before), all `fill`."""
+    buf = torch.full((off + n + 64,), fill, dtype=dtype, device="cuda")
+    return buf, buf[off:off + n]
+
+
+@gpu
+@pytest.mark.parametrize("D", ROWS + [16385, 40000, 131071])
+def test_quantize_rows_exact(torch_cuda, D):
+    """Codes and scales equal the formula's, bit for bit: 127 x and a are exact in
+    fp32, and the quotient's distance to a tie is either 0 or >= 2^-13."""
+    from bbh import engine
+
+    torch = torch_cuda
+    for M in (1, 5, 130):
+        x = _half(torch, _gen(torch, D + M), M, D, scale=3.0)
+        if D >= 8:
+            x[0, :8] = torch.tensor([127, 63.5, -0.5, 1.5, -2.5, 0.25, 126.5, -127]).half()
+            x[0, 8:] = x[0, 8:].clamp(-100, 100)  # scale 1: codes are x, ties among them
+        buf, q = _guarded(torch, M * D, torch.int8, 99)
+        sbuf, s = _guarded(torch, M, torch.float32, 7.0)
+        engine.launch_quantize_rows(x, q, s, M, D)
+        c64, s64 = _codes64(torch, x.double())
+        assert torch.equal(q.view(M, D).double(), c64.round())
+        assert torch.equal(s, s64.float())
+        assert bool((buf[M * D:] == 99).all()) and bool((sbuf[M:] == 7).all())
+        xbuf, back = _guarded(torch, M * D, torch.float16, 5.0)
+        engine.launch_dequantize_rows(q, s, back, M, D)
+        # code * scale in fp32 (u), then fp16
+        want = q.view(M, D).double() * s.double()[:, None]
+        err = (back.view(M, D).double() - want).abs()
+        assert bool((err <= want.abs() * (H + 2 * U) + TINY).all())
+        assert bool((xbuf[M * D:] == 5).all())
+
+
+@gpu
+def test_quantize_rows_zero_nan_inf_and_extremes(torch_cuda):
+    from bbh import engine
+
+    torch = torch_cuda
+    for D in (5, 64, 1000, 9000, 20000):
+        x = _half(torch, _gen(torch, D), 8, D)
+        x[0] = 0
+        x[1, D // 2] = float("nan")
+        x[2, D - 1] = float("inf")
+        x[3, 0] = float("-inf")
+        x[4] = 0
+        x[4, D - 1] = 2.0 ** -24   # the smallest fp16
+        x[5, 0] = 65504.0          # the largest
+        x[6] = -0.0
+        q = torch.full((8, D), 55, dtype=torch.int8, device="cuda")
+        s = torch.empty(8, device="cuda")
+        back = torch.empty(8, D, dtype=torch.float16, device="cuda")
+        engine.launch_quantize_rows(x, q, s, 8, D)
+        engine.launch_dequantize_rows(q, s, back, 8, D)
+        assert bool((q[[0, 1, 2, 3, 6]] == 0).all())
+        assert float(s[0]) == 0 and float(s[6]) == 0 and bool(torch.isnan(s[1:4]).all())
+        assert bool(torch.isnan(back[1:4]).all()) and bool((back[[0, 6]] == 0).all())
+        c64, s64 = _codes64(torch, x[[4, 5, 7]].double())
+        assert torch.equal(q[[4, 5, 7]].double(), c64.round())
+        assert torch.equal(s[[4, 5, 7]], s64.float())
+        assert int(q[4, D - 1]) == 127 and int(q[5, 0]) == 127
+
+
+def _check_norm(torch, kind, x, r, gamma, beta, eps, q, s, ssum, y):
+    h = x.double() + (0 if r is None else r.double())
+    mean = h.mean(1, keepdim=True) if kind == "layernorm" else 0 * h[:, :1]
+    d = h - mean
+    rstd = 1 / torch.sqrt((d * d).mean(1, keepdim=True) + eps)
+    g = gamma.double()
+    b = beta.double() if kind == "layernorm" else 0 * g
+    v = d * rstd * g + b
+    # h: u |h|.  mean: 45 u of the mean magnitude, which moves d by as much and
+    # the variance by its square.  rstd: half the variance's 45 u + 2 m^2 / var
+    # (m that move of d), and 3 u of its own.  Products and the sum: 3 u.
+    m = (46 * U * h.abs().mean(1, keepdim=True) if kind == "layernorm" else 0.0)
+    move = m + 2 * U * h.abs()
+    e = g.abs() * rstd * move + (d * rstd * g).abs() * (30 * U + 3 * (move.amax(1, keepdim=True) * rstd) ** 2
+                                                      + move.mean(1, keepdim=True) * rstd) + 3 * U * v.abs()
+    a, ea = v.abs().amax(1), e.amax(1)
+    assert bool(((s.double() - a / 127).abs() <= (ea + 2 * U * a) / 127).all())
+    c64, _ = _codes64(torch, v)
+    err = (q.double() - c64).abs()
+    over = a.clamp(min=1e-300)  # a row of zeros: e is 0 too, and so is the code
+    lim = 0.5 + 127 * (e / over[:, None] + (ea / over)[:, None] + 4 * U)
+    ok = bool((err <= lim).all())
+    assert ok, float((err - lim).max())
+    if ssum is not None:
+        assert bool(((ssum.double() - h).abs() <= h.abs() * (H + U) + TINY).all())
+    if y is not None:
+        assert bool(((y.double() - v).abs() <= v.abs() * H + e * (1 + H) + TINY).all())
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["rmsnorm", "layernorm"])
+@pytest.mark.parametrize("D", ROWS)
+def test_norms_against_64_bits(torch_cuda, kind, D):
+    from bbh import engine
+
+    torch = torch_cuda
+    for M, res, keep in ((1, True, "sum"), (3, False, "y"), (67, True, "both"), (130, True, "")):
+        g = _gen(torch, D * 7 + M)
+        x = _half(torch, g, M, D) + (0.5 if M == 67 else 0)
+        r = _half(torch, g, M, D, scale=2.0) if res else None
+        gamma = _half(torch, g, D, scale=0.3) + 1
+        beta = _half(torch, g, D, scale=0.1)
+        eps = 1e-6 if kind == "rmsnorm" else 1e-12
+        if kind == "layernorm" and D == 1:
+            eps = 0.25  # a row of one: the deviation is 0, v = beta
+        buf, q = _guarded(torch, M * D, torch.int8, 99)
+        sbuf, s = _guarded(torch, M, torch.float32, 7.0)
+        hb, hs = _guarded(torch, M * D, torch.float16, 3.0)
+        yb, y = _guarded(torch, M * D, torch.float16, 3.0)
+        kw = dict(eps=eps, residual=r, sum=hs if keep in ("sum", "both") else None,
+                  y=y if keep in ("y", "both") else None)
+        if kind == "rmsnorm":
+            engine.launch_rmsnorm_quantize(x, gamma, q, s, M, D, **kw)
+        else:
+            engine.launch_layernorm_quantize(x, gamma, beta, q, s, M, D, **kw)
+        _check_norm(torch, kind, x, r, gamma, beta, eps, q.view(M, D), s,
+                    hs.view(M, D) if kw["sum"] is not None else None,
+                    y.view(M, D) if kw["y"] is not None else None)
+        for b, n in ((buf, 99), (hb, 3), (yb, 3)):
+            assert bool((b[M * D:] == n).all())
+        assert bool((sbuf[M:] == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["rmsnorm", "layernorm"])
+@pytest.mark.parametrize("D", [40, 384, 1001, 4096, 16384])
+def test_norm_outputs_over_inputs_and_odd_addresses(torch_cuda, kind, D):
+    """sum over x and y over residual (and the other way round) give what
+    separate outputs give, at rows that start 2 bytes off a 16-byte boundary and
+    codes that start at an odd byte."""
+    from bbh import engine
+
+    torch = torch_cuda
+    M = 37
+    g = _gen(torch, D)
+    x0, r0 = _half(torch, g, M, D), _half(torch, g, M, D)
+    gamma, beta = _half(torch, g, D) + 1, _half(torch, g, D)
+
+    def run(x, r, q, s, hs, y):
+        args = (x, gamma) if kind == "rmsnorm" else (x, gamma, beta)
+        getattr(engine, f"launch_{kind}_quantize")(*args, q, s, M, D, eps=1e-5, residual=r, sum=hs,
+                                                   y=y)
+
+    want = [torch.empty(M * D, dtype=t, device="cuda") for t in (torch.float16, torch.float16,
+                                                                  torch.int8)]
+    s0 = torch.empty(M, device="cuda")
+    run(x0, r0, want[2], s0, want[0], want[1])
+    for over in ((0, 1), (1, 0)):
+        xb, x = _guarded(torch, M * D, torch.float16, 3.0, off=1)
+        rb, r = _guarded(torch, M * D, torch.float16, 3.0, off=3)
+        qb, q = _guarded(torch, M * D, torch.int8, 9, off=5)
+        x.copy_(x0.view(-1)), r.copy_(r0.view(-1))
+        s = torch.empty(M, device="cuda")
+        outs = (x, r)
+        run(x, r, q, s, outs[over[0]], outs[over[1]])
+        assert torch.equal(outs[over[0]], want[0]) and torch.equal(outs[over[1]], want[1])
+        assert torch.equal(q, want[2]) and torch.equal(s, s0)
+        for b, o, f in ((xb, 1, 3), (rb, 3, 3), (qb, 5, 9)):
+            assert bool((b[:o] == f).all()) and bool((b[o + M * D:] == f).all())
+
+
+@gpu
+def test_norms_of_zero_and_non_finite_rows(torch_cuda):
+    from bbh import engine
+
+    torch = torch_cuda
+    for D in (24, 500, 3000, 16000):
+        x = _half(torch, _gen(torch, D), 6, D)
+        x[0] = 0
+        x[1, 3] = float("nan")
+        x[2, D - 1] = float("inf")
+        x[3] = 2.0
+        x[4] = 60000.0  # x + x leaves fp16, not fp32
+        gamma = torch.ones(D, device="cuda").half()
+        beta = torch.zeros(D, device="cuda").half()
+        for kind in ("rmsnorm", "layernorm"):
+            q = torch.full((6, D), 55, dtype=torch.int8, device="cuda")
+            s = torch.empty(6, device="cuda")
+            y = torch.empty(6, D, dtype=torch.float16, device="cuda")
+            hs = torch.empty(6, D, dtype=torch.float16, device="cuda")
+            args = (x, gamma) if kind == "rmsnorm" else (x, gamma, beta)
+            getattr(engine, f"launch_{kind}_quantize")(*args, q, s, 6, D, eps=1e-6, residual=x,
+                                                       sum=hs, y=y)
+            assert bool((q[:3] == 0).all()) and float(s[0]) == 0 and bool(torch.isnan(s[1:3]).all())
+            assert bool((y[0] == 0).all()) and bool(torch.isnan(y[1]).all())
+            assert bool(torch.isinf(hs[4]).all())
+            if kind == "rmsnorm":  # constant rows: all ones
+                assert bool((q[3:5] == 127).all()) and bool((y[3:5] == 1).all())
+            else:  # no deviation; 4 D and 120000 D are exact in fp32, so is their mean
+                assert bool((q[3] == 0).all()) and float(s[3]) == 0 and bool((y[3] == 0).all())
+
+
+def _gelu64(torch, v):
+    return v * torch.special.ndtr(v)
+
+
+def _linear_check(torch, A, sa, B, sb, bias, gelu, C):
+    """Exact sums; then (float) acc, two products and an addition (u each), GELU
+    to the error its polynomial states, fp16."""
+    acc = A.double() @ B.double().t().contiguous()  # exact: below 2^53
+    p = acc * sa.double()[:, None] * sb.double()
+    v = p if bias is None else p + bias.double()
+    e = 3 * U * p.abs() + U * v.abs()
+    if gelu:
+        x = v.abs()
+        e = 1.13 * e + torch.where(x < 3, 1.1e-5, torch.where(x < 6, 7.6e-5, 1.8e-4 + 3.5e-6 * x))
+        e = e + 4 * U * x
+        v = _gelu64(torch, v)
+    err = (C.double() - v).abs()
+    lim = v.abs() * H + e * (1 + H) + TINY
+    fine = v.abs() < 65000
+    bad = (err > lim) & fine
+    assert not bool(bad.any()), (float((err / lim)[fine].max()), bad.nonzero()[:4].tolist())
+
+
+def _operands(torch, seed, M, N, K, off=0):
+    g = _gen(torch, seed)
+    mk = lambda n: torch.randint(-128, 128, (n + off,), device="cuda", generator=g,  # noqa: E731
+                                 dtype=torch.int8)[off:]
+    sa = torch.rand(M, device="cuda", generator=g) * 0.02 / K ** 0.5 + 1e-5
+    sb = torch.rand(N, device="cuda", generator=g) * 0.02 + 1e-4
+    return mk(M * K).view(M, K), sa, mk(N * K).view(N, K), sb, _half(torch, g, N)
+
+
+LINEAR = [(1, 1, 1), (1, 1, 16), (1, 3, 5), (1, 64, 128), (1, 1000, 4096), (1, 4097, 777), (2, 33, 48),
+          (3, 5, 17), (4, 384, 1536), (4, 1023, 1000), (5, 130, 384), (8, 257, 2048), (9, 16, 8192), (15, 65, 129), (16, 1536, 384),
+          (17, 384, 1536), (31, 33, 144), (32, 32, 32), (33, 31, 112), (33, 700, 4112), (48, 1152, 384),
+          (64, 1537, 384), (64, 64, 127), (65, 129, 128), (100, 100, 100), (127, 384, 2000),
+          (128, 128, 128), (129, 257, 255), (200, 4096, 512), (256, 256, 256), (257, 1111, 777),
+          (300, 1152, 384), (513, 130, 1040), (600, 2048, 96), (1000, 999, 1001), (2003, 1152, 384),
+          (1, 7, 131071), (40, 70, 131071), (130, 200, 100000), (3000, 20, 384), (20, 9000, 64),
+          (4096, 1536, 384), (2048, 2048, 1024), (2500, 2700, 528), (4100, 4100, 260)]
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", LINEAR)
+def test_linear_i8(torch_cuda, M, N, K):
+    from bbh import engine
+
+    torch = torch_cuda
+    A, sa, B, sb, bias = _operands(torch, M + N + K, M, N, K)
+    for b, gelu in ((None, False), (bias, True)):
+        buf, C = _guarded(torch, M * N, torch.float16, 3.0)
+        engine.launch_matmul_i8(A, sa, B, sb, C, M, N, K, bias=b, gelu=gelu)
+        _linear_check(torch, A, sa, B, sb, b, gelu, C.view(M, N))
+        assert bool((buf[M * N:] == 3).all())
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(1, 100, 256), (3, 64, 1024), (20, 96, 256), (70, 200, 400),
+                                   (300, 520, 384), (2100, 1100, 512), (3000, 3000, 256)])
+def test_linear_i8_same_bits_at_odd_addresses_and_any_rows(torch_cuda, M, N, K):
+    """Operands one byte off, an output two bytes off, and every row alone: the
+    same bits, whichever kernel computes them."""
+    from bbh import engine
+
+    torch = torch_cuda
+    A, sa, B, sb, bias = _operands(torch, 5, M, N, K)
+    C = torch.empty(M, N, dtype=torch.float16, device="cuda")
+    engine.launch_matmul_i8(A, sa, B, sb, C, M, N, K, bias=bias, gelu=True)
+    A1, _, B1, _, _ = _operands(torch, 6, M, N, K, off=1)
+    A1.copy_(A), B1.copy_(B)
+    buf, C1 = _guarded(torch, M * N, torch.float16, 3.0, off=1)
+    engine.launch_matmul_i8(A1, sa, B1, sb, C1, M, N, K, bias=bias, gelu=True)
+    assert torch.equal(C1.view(M, N), C) and float(buf[0]) == 3 and bool((buf[1 + M * N:] == 3).all())
+    for a, b in ((0, 1), (M // 2, M // 2 + 2), (max(0, M - 40), M)):
+        b = min(b, M)
+        Cr = torch.empty(b - a, N, dtype=torch.float16, device="cuda")
+        engine.launch_matmul_i8(A[a:b], sa[a:b], B, sb, Cr, b - a, N, K, bias=bias, gelu=True)
+        assert torch.equal(Cr, C[a:b])
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 40])
+def test_linear_i8_largest_sums(torch_cuda, M):
+    """-128 x -128 over the longest K: 131071 * 2^14 = 2147467264 < 2^31."""
+    from bbh import engine
+
+    torch = torch_cuda
+    N, K = 66, 131071
+    A = torch.full((M, K), -128, dtype=torch.int8, device="cuda")
+    B = torch.full((N, K), -128, dtype=torch.int8, device="cuda")
+    B[N // 2:] = 127
+    sa = torch.full((M,), 2.0 ** -12, device="cuda")
+    sb = torch.full((N,), 2.0 ** -12, device="cuda")
+    C = torch.empty(M, N, dtype=torch.float16, device="cuda")
+    engine.launch_matmul_i8(A, sa, B, sb, C, M, N, K)
+    _linear_check(torch, A, sa, B, sb, None, False, C)
+    assert float(C[0, 0]) == 128 and float(C[0, N - 1]) == -127
+
+
+@gpu
+def test_linear_i8_non_finite_and_zero_scales(torch_cuda):
+    from bbh import engine
+
+    torch = torch_cuda
+    for M in (1, 3, 50, 200):
+        N, K = 300, 160
+        A, sa, B, sb, bias = _operands(torch, 1, M, N, K)
+        sa[M - 1] = float("nan")
+        sb[7] = float("nan")
+        sb[8] = 0
+        C = torch.empty(M, N, dtype=torch.float16, device="cuda")
+        engine.launch_matmul_i8(A, sa, B, sb, C, M, N, K, bias=bias)
+        nan = torch.isnan(C)
+        assert bool(nan[M - 1].all()) and bool(nan[:, 7].all())
+        if M > 1:
+            assert torch.equal(C[:M - 1, 8], bias[8].expand(M - 1))
+            keep = [n for n in range(N) if n != 7]
+            _linear_check(torch, A[:M - 1], sa[:M - 1], B[keep], sb[keep], bias[keep], False,
+                          C[:M - 1][:, keep])
+
+
+@gpu
+def test_offsets_past_32_bits(torch_cuda):
+    """Rows whose elements lie past 2^31 of every operand: the last rows of
+    597001 x 4096 (2.4e9) and of an output of 70001 x 31000 (2.2e9)."""
+    from bbh import engine
+
+    torch = torch_cuda
+    M, D = 597001, 4096
+    x = torch.zeros(M, D, dtype=torch.float16, device="cuda")
+    tail = _half(torch, _gen(torch, 3), 5, D)
+    x[M - 5:] = tail
+    q = torch.empty(M, D, dtype=torch.int8, device="cuda")
+    s = torch.empty(M, device="cuda")
+    engine.launch_quantize_rows(x, q, s, M, D)
+    c64, s64 = _codes64(torch, tail.double())
+    assert torch.equal(q[M - 5:].double(), c64.round()) and torch.equal(s[M - 5:], s64.float())
+    assert not bool(q[:M - 5:1000].any()) and not bool(s[:M - 5].any())
+    y = torch.empty(M, D, dtype=torch.float16, device="cuda")
+    engine.launch_rmsnorm_quantize(x, torch.ones(D, device="cuda").half(), q, s, M, D, y=y, sum=x)
+    _check_norm(torch, "rmsnorm", tail, None, torch.ones(D, device="cuda"), None, 1e-6, q[M - 5:],
+                s[M - 5:], x[M - 5:], y[M - 5:])
+    engine.launch_dequantize_rows(q, s, y, M, D)
+    assert torch.equal(y[M - 5:], (q[M - 5:].float() * s[M - 5:, None]).half())
+    # the same codes as A, one column block of them as B
+    N = 40
+    C = torch.empty(M, N, dtype=torch.float16, device="cuda")
+    B, sb = q[M - N:], s[M - N:].clone()
+    engine.launch_matmul_i8(q, s, B, sb, C, M, N, D)
+    _linear_check(torch, q[M - 5:], s[M - 5:], B, sb, None, False, C[M - 5:])
+    Ct = torch.empty(5, M, dtype=torch.float16, device="cuda")
+    engine.launch_matmul_i8(q[M - 5:], s[M - 5:], q, s, Ct, 5, M, D)
+    assert torch.equal(Ct[:, M - N:], C[M - 5:]) and not bool(Ct[:, :M - N].any())
+    del x, y, q, C, Ct
+    M, N, K = 70001, 31000, 16
+    A, sa, B, sb, bias = _operands(torch, 9, M, N, K)
+    C = torch.empty(M, N, dtype=torch.float16, device="cuda")
+    engine.launch_matmul_i8(A, sa, B, sb, C, M, N, K, bias=bias)
+    for a in (0, 35000, M - 40):
+        _linear_check(torch, A[a:a + 40], sa[a:a + 40], B, sb, bias, False, C[a:a + 40])
+
+
+def _ffn(torch, engine, st, stream=None):
+    m, d, f = st["m"], st["d"], st["f"]
+    engine.launch_layernorm_quantize(st["x"], st["gamma"], st["beta"], st["q"], st["s"], m, d,
+                                     residual=st["r"], y=st["y"], stream=stream)
+    engine.launch_matmul_i8(st["q"], st["s"], st["w1"], st["s1"], st["mid"], m, f, d, bias=st["b1"],
+                            gelu=True, stream=stream)
+    engine.launch_quantize_rows(st["mid"], st["q2"], st["s2"], m, f, stream=stream)
+    engine.launch_matmul_i8(st["q2"], st["s2"], st["w2"], st["s3"], st["out"], m, d, f,
+                            bias=st["b2"], stream=stream)
+
+
+def _ffn_state(torch, engine, m, d, f, seed):
+    g = _gen(torch, seed)
+    h = lambda *s: torch.empty(s, dtype=torch.float16, device="cuda")  # noqa: E731
+    c = lambda *s: torch.empty(s, dtype=torch.int8, device="cuda")  # noqa: E731
+    v = lambda n: torch.empty(n, device="cuda")  # noqa: E731
+    st = dict(m=m, d=d, f=f, x=_half(torch, g, m, d), r=_half(torch, g, m, d), q=c(m, d), s=v(m),
+              q2=c(m, f), s2=v(m), y=h(m, d), mid=h(m, f), out=h(m, d), w1=c(f, d), s1=v(f),
+              w2=c(d, f), s3=v(d), gamma=_half(torch, g, d, scale=0.2) + 1,
+              beta=_half(torch, g, d, scale=0.1), b1=_half(torch, g, f, scale=0.05),
+              b2=_half(torch, g, d, scale=0.05))
+    st["W1"], st["W2"] = _half(torch, g, f, d, scale=0.05), _half(torch, g, d, f, scale=0.05)
+    engine.launch_quantize_rows(st["W1"], st["w1"], st["s1"], f, d)  # a scale an output channel
+    engine.launch_quantize_rows(st["W2"], st["w2"], st["s3"], d, f)
+    return st
+
+
+@gpu
+@pytest.mark.parametrize("m,d,f", [(1, 384, 1536), (77, 384, 1536), (512, 200, 801)])
+def test_ffn_block_in_8_bits(torch_cuda, m, d, f):
+    """The operators together: each step against the formula on what the step
+    before it wrote, and the whole against the fp16 weights unquantised."""
+    from bbh import engine
+
+    torch = torch_cuda
+    st = _ffn_state(torch, engine, m, d, f, m)
+    _ffn(torch, engine, st)
+    _check_norm(torch, "layernorm", st["x"], st["r"], st["gamma"], st["beta"], 1e-12, st["q"],
+                st["s"], None, st["y"])
+    _linear_check(torch, st["q"], st["s"], st["w1"], st["s1"], st["b1"], True, st["mid"])
+    c64, s64 = _codes64(torch, st["mid"].double())
+    assert torch.equal(st["q2"].double(), c64.round()) and torch.equal(st["s2"], s64.float())
+    _linear_check(torch, st["q2"], st["s2"], st["w2"], st["s3"], st["b2"], False, st["out"])
+    mid = _gelu64(torch, st["y"].double() @ st["W1"].double().t() + st["b1"].double())
+    want = mid @ st["W2"].double().t() + st["b2"].double()
+    # codes are off by at most half a scale, a / 254, independent of each other:
+    # rms of a product's error over its rms ~ 0.29 (4 / 127) a tensor at a = 4 rms,
+    # four tensors, and twice that for peaks above 4 rms: 4 %
+    rel = float((st["out"].double() - want).norm() / want.norm())
+    assert rel < 0.04
+
+
+@gpu
+def test_captured_and_replayed_beside_eager_work_on_two_streams(torch_cuda):
+    from bbh import engine
+
+    torch = torch_cuda
+    a = _ffn_state(torch, engine, 130, 384, 1536, 1)
+    b = _ffn_state(torch, engine, 9, 384, 1536, 2)
+    want = []
+    for st in (a, b):
+        _ffn(torch, engine, st)
+        want.append((st["out"].clone(), st["y"].clone(), st["q2"].clone()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        _ffn(torch, engine, a)
+    other = torch.cuda.Stream()
+    for i in range(4):
+        for st in (a, b):
+            for k in ("out", "y", "q2", "q", "mid"):
+                st[k].zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        _ffn(torch, engine, b, stream=other.cuda_stream)
+        torch.cuda.synchronize()
+        for st, w in zip((a, b), want):
+            assert torch.equal(st["out"], w[0]) and torch.equal(st["y"], w[1])
+            assert torch.equal(st["q2"], w[2])
+        x = a["x"].clone()  # eager work of the program between replays
+        a["x"].mul_(2)
+        _ffn(torch, engine, a)
+        a["x"].copy_(x)
+
+
+@gpu
+def test_python_checks_sizes_and_layout(torch_cuda):
+    from bbh import capi, engine
+
+    torch = torch_cuda
+    x = torch.zeros(4, 8, dtype=torch.float16, device="cuda")
+    q = torch.zeros(4, 8, dtype=torch.int8, device="cuda")
+    s = torch.zeros(4, device="cuda")
+    with pytest.raises(ValueError):
+        engine.launch_quantize_rows(x, q, s, 5, 8)
+    with pytest.raises(ValueError):
+        engine.launch_quantize_rows(x, q, s[:3], 4, 8)
+    with pytest.raises(TypeError):
+        engine.launch_quantize_rows(x.t(), q, s, 4, 8)
+    with pytest.raises(TypeError):
+        engine.launch_matmul_i8(q, s, q, s.double(), x, 4, 4, 8)
+    with pytest.raises(ValueError):
+        engine.launch_matmul_i8(q, s, q, s, x, 4, 4, 9)
+    with pytest.raises(ValueError):
+        engine.launch_rmsnorm_quantize(x, x[0, :7], q, s, 4, 8)
+    with pytest.raises(capi.BBHError) as e:
+        engine.launch_rmsnorm_quantize(x, x[0], q, s, 4, 8, sum=x, y=x)
+    assert e.value.name == "BBH_ERR_INVALID_ARG"
+    with pytest.raises(TypeError):
+        engine.launch_dequantize_rows(q.cpu(), s, x, 4, 8)
