@@ -466,38 +466,52 @@ I8_MAX_K = 131071  # BBH_I8_MAX_K
 I8_MAX_NORM = 16384  # BBH_I8_MAX_NORM
 
 
-def _check_i8(dtypes, numels, **tensors):
-    """Each tensor (None: not passed) is contiguous, of its dtype, on the
-    current device and of at least its number of elements."""
-    if min(numels) < 1:
+def _operand(name, t, dtype, n, device):
+    """The address of an operand of n elements or more, contiguous, on the
+    current device (None: of one that is not passed)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or not t.is_contiguous() or t.get_device() < 0:
+        raise TypeError(f"{name} must be a contiguous {dtype} CUDA tensor")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on cuda:{t.get_device()}, the current device is cuda:{device}")
+    if t.numel() < n:
+        raise ValueError(f"{name}: expected {n} elements, got {t.numel()}")
+    return t.data_ptr()
+
+
+def _place(t, stream, *sizes):
+    """(current device, stream) of a launch that has t as an operand.  A launch
+    of a few microseconds on the GPU is bound by the host's part of the call:
+    reading the stream from torch's C layer takes 0.2 us, a torch.cuda.Stream
+    object 3 us."""
+    if min(sizes) < 1:
         raise ValueError("sizes must be positive")
-    dev = _torch().cuda.current_device() if any(
-        t is not None and t.is_cuda for t in tensors.values()) else None
-    for (name, t), dtype, n in zip(tensors.items(), dtypes, numels):
-        if t is None:
-            continue
-        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
-            raise TypeError(f"{name} must be a contiguous {dtype} CUDA tensor")
-        if t.get_device() != dev:
-            raise ValueError(f"{name} is on cuda:{t.get_device()}, the current device is cuda:{dev}")
-        if t.numel() < n:
-            raise ValueError(f"{name}: expected {n} elements, got {t.numel()}")
+    if not t.is_cuda:
+        raise TypeError("operands must be CUDA tensors")
+    c = _torch()._C
+    device = c._cuda_getDevice()
+    return device, c._cuda_getCurrentRawStream(device) if stream is None else stream
 
 
 def launch_quantize_rows(x, q, scale, M, D, stream=None):
     """x (M, D) fp16 -> q (M, D) int8, scale (M) fp32: one scale a row, the
     largest magnitude / 127 (bbh_quantize_rows)."""
     torch = _torch()
-    _check_i8((torch.float16, torch.int8, torch.float32), (M * D, M * D, M), x=x, q=q, scale=scale)
-    call("bbh_quantize_rows", _ptr(x), _ptr(q), _ptr(scale), M, D, _stream(stream))
+    dev, s = _place(x, stream, M, D)
+    call("bbh_quantize_rows", _operand("x", x, torch.float16, M * D, dev),
+         _operand("q", q, torch.int8, M * D, dev), _operand("scale", scale, torch.float32, M, dev),
+         M, D, s)
     return q, scale
 
 
 def launch_dequantize_rows(q, scale, x, M, D, stream=None):
     """x (M, D) fp16 = q * scale, row by row (bbh_dequantize_rows)."""
     torch = _torch()
-    _check_i8((torch.int8, torch.float32, torch.float16), (M * D, M, M * D), q=q, scale=scale, x=x)
-    call("bbh_dequantize_rows", _ptr(q), _ptr(scale), _ptr(x), M, D, _stream(stream))
+    dev, s = _place(q, stream, M, D)
+    call("bbh_dequantize_rows", _operand("q", q, torch.int8, M * D, dev),
+         _operand("scale", scale, torch.float32, M, dev),
+         _operand("x", x, torch.float16, M * D, dev), M, D, s)
     return x
 
 
@@ -506,24 +520,28 @@ def launch_rmsnorm_quantize(x, gamma, q, scale, M, D, eps=1e-6, residual=None, s
     """RMS norm of x [+ residual] times gamma, quantised a row at a time into
     q, scale; sum (x + residual) and y (the norm) get fp16 where given
     (bbh_rmsnorm_quantize)."""
-    f16 = _torch().float16
-    _check_i8((f16, f16, f16, f16, f16, _torch().int8, _torch().float32),
-              (M * D, M * D, D, M * D, M * D, M * D, M), x=x, residual=residual, gamma=gamma,
-              sum=sum, y=y, q=q, scale=scale)
-    call("bbh_rmsnorm_quantize", _ptr(x), _ptr(residual), _ptr(gamma), _ptr(sum), _ptr(y), _ptr(q),
-         _ptr(scale), M, D, eps, _stream(stream))
+    torch = _torch()
+    f16, n = torch.float16, M * D
+    dev, s = _place(x, stream, M, D)
+    call("bbh_rmsnorm_quantize", _operand("x", x, f16, n, dev),
+         _operand("residual", residual, f16, n, dev), _operand("gamma", gamma, f16, D, dev),
+         _operand("sum", sum, f16, n, dev), _operand("y", y, f16, n, dev),
+         _operand("q", q, torch.int8, n, dev), _operand("scale", scale, torch.float32, M, dev), M,
+         D, eps, s)
     return q, scale
 
 
 def launch_layernorm_quantize(x, gamma, beta, q, scale, M, D, eps=LAYER_NORM_EPS, residual=None,
                               sum=None, y=None, stream=None):
     """launch_rmsnorm_quantize for LayerNorm (bbh_layernorm_quantize)."""
-    f16 = _torch().float16
-    _check_i8((f16, f16, f16, f16, f16, f16, _torch().int8, _torch().float32),
-              (M * D, M * D, D, D, M * D, M * D, M * D, M), x=x, residual=residual, gamma=gamma,
-              beta=beta, sum=sum, y=y, q=q, scale=scale)
-    call("bbh_layernorm_quantize", _ptr(x), _ptr(residual), _ptr(gamma), _ptr(beta), _ptr(sum),
-         _ptr(y), _ptr(q), _ptr(scale), M, D, eps, _stream(stream))
+    torch = _torch()
+    f16, n = torch.float16, M * D
+    dev, s = _place(x, stream, M, D)
+    call("bbh_layernorm_quantize", _operand("x", x, f16, n, dev),
+         _operand("residual", residual, f16, n, dev), _operand("gamma", gamma, f16, D, dev),
+         _operand("beta", beta, f16, D, dev), _operand("sum", sum, f16, n, dev),
+         _operand("y", y, f16, n, dev), _operand("q", q, torch.int8, n, dev),
+         _operand("scale", scale, torch.float32, M, dev), M, D, eps, s)
     return q, scale
 
 
@@ -532,10 +550,11 @@ def launch_matmul_i8(A, a_scale, B, b_scale, C, M, N, K, bias=None, gelu=False, 
     (A (M, K) . B (N, K)^T) [+ bias] [GELU], the sums exact (bbh_linear_i8)."""
     torch = _torch()
     i8, f32, f16 = torch.int8, torch.float32, torch.float16
-    _check_i8((i8, f32, i8, f32, f16, f16), (M * K, M, N * K, N, M * N, N), A=A, a_scale=a_scale,
-              B=B, b_scale=b_scale, C=C, bias=bias)
-    call("bbh_linear_i8", _ptr(A), _ptr(a_scale), _ptr(B), _ptr(b_scale), _ptr(C), M, N, K,
-         _ptr(bias), int(bool(gelu)), _stream(stream))
+    dev, s = _place(A, stream, M, N, K)
+    call("bbh_linear_i8", _operand("A", A, i8, M * K, dev), _operand("a_scale", a_scale, f32, M, dev),
+         _operand("B", B, i8, N * K, dev), _operand("b_scale", b_scale, f32, N, dev),
+         _operand("C", C, f16, M * N, dev), M, N, K, _operand("bias", bias, f16, N, dev),
+         int(bool(gelu)), s)
     return C
 
 

@@ -92,8 +92,10 @@ struct Cfg {
   static_assert(LDS <= (int)kLdsMax && THREADS <= 1024, "workgroup");
 };
 
-// Copies of this wavefront's share of slice s: global -> LDS, 1 KB = 8 rows a
-// copy.  Rows and bytes past the operand are out of the resource's bounds.
+// Copies of this wavefront's share of a slice: global -> LDS, 1 KB = 8 rows a
+// copy.  Rows and bytes past the operand are out of the resource's bounds, as
+// is everything at an offset of kNowhere: such copies read no memory.
+constexpr uint32_t kNowhere = 1u << 30;
 struct Copier {
   __amdgpu_buffer_rsrc_t src;
   uint32_t lane[2], step;  // byte offset in an even / odd block of 8 rows; 8 rows
@@ -105,11 +107,11 @@ struct Copier {
       lane[p] = r * K + (((l & 7) ^ (p << 2 | r >> 1)) << 4);
   }
   template <int N>
-  __device__ __forceinline__ void copy(int s, char* dst, int wave) const {
+  __device__ __forceinline__ void copy(uint32_t at, char* dst, int wave) const {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int b = wave * N + j;  // block of 8 rows
-      const uint32_t off = (N % 2 == 0 ? lane[j & 1] : lane[b & 1]) + b * step + s * kSlice;
+      const uint32_t off = (N % 2 == 0 ? lane[j & 1] : lane[b & 1]) + (b * step + at);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           src, (__attribute__((address_space(3))) void*)(dst + b * 1024), 16, (int)off, 0, 0, 0);
     }
@@ -130,10 +132,6 @@ struct Frags {
     for (int f = 0; f < C::FN; ++f)
       b[f] = *reinterpret_cast<const i32x4*>(p + (C::BM + wn * C::TN + f * 32) * kSlice);
   }
-  __device__ __forceinline__ void clear_a() {
-#pragma unroll
-    for (int f = 0; f < C::FM; ++f) a[f] = i32x4{0, 0, 0, 0};
-  }
   __device__ __forceinline__ void mul(i32x16 (&acc)[C::FM][C::FN]) const {
 #pragma unroll
     for (int fm = 0; fm < C::FM; ++fm)
@@ -142,6 +140,17 @@ struct Frags {
         acc[fm][fn] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[fn], a[fm], acc[fm][fn], 0, 0, 0);
   }
 };
+
+// Scheduling groups: (one LDS read, then ~Q / R matrix products) x R.
+template <int R, int Q, int I = 0>
+__device__ __forceinline__ void interleave() {
+  if constexpr (I < R) {
+    constexpr int n = (I < Q % R) ? Q / R + 1 : Q / R;
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    if constexpr (n > 0) __builtin_amdgcn_sched_group_barrier(0x008, n, 0);
+    interleave<R, Q, I + 1>();
+  }
+}
 
 // 16 bytes at k of a row of K, zeros past its end.
 __device__ __forceinline__ i32x4 load_chunk(const int8_t* row, int k, int K) {
@@ -190,90 +199,120 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[fm][fn][i] = 0;
 
+  // Iteration i of a group is slice i * KS + grp.  Every group has `even` whole
+  // slices; then one iteration more, in which a group has a whole slice, the
+  // last part of K or none, unless no group has any.
   const int full = K / kSlice, rem = K % kSlice, total = full + (rem ? 1 : 0);
-  const int iters = (total + C::KS - 1) / C::KS;
-  char* ring = smem + grp * C::R * C::STAGE;
+  const int even = full / C::KS, iters = (total + C::KS - 1) / C::KS;
+  char* const ring = smem + grp * C::R * C::STAGE;
+  char* const ring_end = ring + C::R * C::STAGE;
   const Copier ca(A, rows, K), cb(B, cols, K);
-  i32x4 held[ALIGNED ? 1 : C::CH];
-  auto issue = [&](int i) {  // ALIGNED: the group's slice of iteration i into its slot
+  auto issue = [&](int i, char* dst) {  // ALIGNED: the slice of iteration i into a slot
     const int s = i * C::KS + grp;
-    if (i >= iters || s >= total) return;
-    char* dst = ring + i % C::R * C::STAGE;
-    ca.template copy<C::LA>(s, dst, w);
-    cb.template copy<C::LB>(s, dst + C::BM * kSlice, w);
+    const uint32_t at = s < total ? (uint32_t)s * kSlice : kNowhere;
+    ca.template copy<C::LA>(at, dst, w);
+    cb.template copy<C::LB>(at, dst + C::BM * kSlice, w);
   };
+  i32x4 held[ALIGNED ? 1 : C::CH];
   auto load = [&](int i) {  // the same into registers
     const int s = i * C::KS + grp;
-    if (i >= iters || s >= total) return;
 #pragma unroll
     for (int j = 0; j < C::CH; ++j) {
       const int q = w * 64 + lane + j * 64 * C::GW, r = q >> 3, k = s * kSlice + (q & 7) * kChunk;
-      const bool isA = r < C::BM;
-      const int rr = isA ? r : r - C::BM;
-      held[j] = rr < (isA ? rows : cols) ? load_chunk((isA ? A : B) + (size_t)rr * K, k, K)
-                                         : i32x4{0, 0, 0, 0};
+      // rows past the tile's last: that one again (nothing of theirs is written)
+      const int8_t* row = r < C::BM ? A + (size_t)min(r, rows - 1) * K
+                                    : B + (size_t)min(r - C::BM, cols - 1) * K;
+      if (s < full)
+        held[j] = *reinterpret_cast<const i32x4_any*>(row + k);
+      else
+        held[j] = load_chunk(row, k, K);
     }
   };
-  auto put = [&](int i) {
-    const int s = i * C::KS + grp;
-    if (i >= iters || s >= total) return;
-    char* dst = ring + i % C::R * C::STAGE;
+  auto put = [&](char* dst) {
 #pragma unroll
     for (int j = 0; j < C::CH; ++j) {
       const int q = w * 64 + lane + j * 64 * C::GW, r = q >> 3;
       *reinterpret_cast<i32x4*>(dst + r * kSlice + (((q & 7) ^ (r >> 1 & 7)) << 4)) = held[j];
     }
   };
+  auto next = [&](char* p) { return p + C::STAGE == ring_end ? ring : p + C::STAGE; };
+  char* slot = ring;      // of the slice that is read
+  char* refill = ring;    // the slot that the next copies go to
   if constexpr (ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < C::R - 1; ++i) issue(i);
+    for (int i = 0; i < C::R - 1; ++i) issue(i, ring + i * C::STAGE);
+    refill = ring_end - C::STAGE;
   } else {
     load(0);
-    put(0);
   }
 
   const int r32 = lane & 31, at = r32 * kSlice + ((lane >> 5 ^ (r32 >> 1 & 7)) << 4);
-  Frags<C> f0, f1;
-  for (int i = 0; i < iters; ++i) {
-    if constexpr (ALIGNED) {
-      // slice i landed: the R - 2 later ones may be in flight, unless fewer were issued
-      if (C::R > 2 && i + C::R - 2 < iters - 1)
-        wait_vm<(C::R - 2) * C::L>();
-      else
-        wait_vm<0>();
-    }
-    lds_barrier();  // and every wavefront has read slice i - 1
+  // Makes slice i readable: its copies have landed (those of the R - 2 later
+  // ones may be in flight), and every wavefront has read slice i - 1, whose
+  // slot the next copies fill.
+  auto arrive = [&](int) {
     if constexpr (ALIGNED)
-      issue(i + C::R - 1);
+      wait_vm<(C::R - 2) * C::L>();
     else
+      put(slot);
+    lds_barrier();
+  };
+  auto advance = [&](int i) {  // the copies that follow arrive(i)
+    if constexpr (ALIGNED) {
+      issue(i + C::R - 1, refill);
+      refill = next(refill);
+    } else if (i + 1 < iters) {
       load(i + 1);
-    const int s = i * C::KS + grp;
-    const char* st = ring + i % C::R * C::STAGE;
-    if (s < full) {
-      f0.read(st, 0, at, wm, wn);
-      if (i > 0) f1.mul(acc);
-      f1.read(st, 1, at, wm, wn);
-      f0.mul(acc);
-      f0.read(st, 2, at, wm, wn);
-      f1.mul(acc);
-      f1.read(st, 3, at, wm, wn);
-      f0.mul(acc);
-    } else {
-      if (i > 0) f1.mul(acc);
-      f1.clear_a();
-      if (s < total) {
-        for (int j = 0; j * 32 < rem; ++j) {
-          f0.read(st, j, at, wm, wn);
-          // past K: the next row's bytes in both operands, cleared in one
-          if (ALIGNED && (2 * j + (lane >> 5)) * kChunk >= rem) f0.clear_a();
-          f0.mul(acc);
-        }
-      }
     }
-    if constexpr (!ALIGNED) put(i + 1);
+  };
+  Frags<C> f0, f1;
+  constexpr int RD = C::FM + C::FN, MF = C::FM * C::FN;
+  // K steps 0-2 of the slice, each beside the reads of the next step.
+  auto three = [&] {
+    __builtin_amdgcn_sched_barrier(0);
+    f1.read(slot, 1, at, wm, wn);
+    f0.mul(acc);
+    interleave<RD, MF>();
+    __builtin_amdgcn_sched_barrier(0);
+    f0.read(slot, 2, at, wm, wn);
+    f1.mul(acc);
+    interleave<RD, MF>();
+    __builtin_amdgcn_sched_barrier(0);
+    f1.read(slot, 3, at, wm, wn);
+    f0.mul(acc);
+    interleave<RD, MF>();
+    __builtin_amdgcn_sched_barrier(0);
+    slot = next(slot);
+  };
+  if (even > 0) {
+    arrive(0);
+    f0.read(slot, 0, at, wm, wn);
+    advance(0);
+    for (int i = 1; i < even; ++i) {
+      three();
+      arrive(i);
+      f0.read(slot, 0, at, wm, wn);
+      advance(i);
+      f1.mul(acc);
+      interleave<RD, MF>();
+    }
+    three();
+    f1.mul(acc);
   }
-  f1.mul(acc);
-  lds_barrier();  // the ring is free
+  if (iters > even) {
+    arrive(even);
+    const int s = even * C::KS + grp, left = min(kSlice, K - s * kSlice);
+    for (int j = 0; j * 32 < left; ++j) {
+      f0.read(slot, j, at, wm, wn);
+      // past K: the next row's bytes in both operands, cleared in one
+      if (ALIGNED && (2 * j + (lane >> 5)) * kChunk >= left)
+#pragma unroll
+        for (int f = 0; f < C::FM; ++f) f0.a[f] = i32x4{0, 0, 0, 0};
+      f0.mul(acc);
+    }
+  }
+  if constexpr (ALIGNED) wait_vm<0>();  // copies from nowhere are still copies
+  lds_barrier();                        // the ring is free
 
   if constexpr (C::KS == 1) {
     f16* out = reinterpret_cast<f16*>(smem);
