@@ -471,12 +471,11 @@ def _operand(name, t, dtype, n, device):
     current device (None: of one that is not passed)."""
     if t is None:
         return None
-    if t.dtype != dtype or not t.is_contiguous() or t.get_device() < 0:
+    if t.dtype != dtype or t.get_device() < 0 or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous {dtype} CUDA tensor")
-    if t.get_device() != device:
-        raise ValueError(f"{name} is on cuda:{t.get_device()}, the current device is cuda:{device}")
-    if t.numel() < n:
-        raise ValueError(f"{name}: expected {n} elements, got {t.numel()}")
+    if t.get_device() != device or t.numel() < n:
+        raise ValueError(f"{name}: expected {n} elements on cuda:{device}, the current device, got "
+                         f"{t.numel()} on cuda:{t.get_device()}")
     return t.data_ptr()
 
 

@@ -76,7 +76,10 @@ template <int BM_, int BN_, int WM_, int WN_, int KS_, int R_>
 struct Cfg {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KS = KS_, R = R_;
   static constexpr int GW = WM * WN, THREADS = 64 * GW * KS;  // wavefronts a group
-  static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+  static constexpr int MB = BM < 32 ? 16 : 32;                // matrix block MB x MB
+  static constexpr int KB = MB == 16 ? 64 : 32, STEPS = kSlice / KB;  // bytes of K a product
+  static constexpr int NV = MB * MB / 64;                     // sums a lane a block
+  static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / MB, FN = TN / MB;
   static constexpr int LA = BM / 8 / GW, LB = BN / 8 / GW, L = LA + LB;  // 1 KB copies a wavefront
   static constexpr int STAGE = (BM + BN) * kSlice;
   static constexpr int RING = STAGE * R * KS;
@@ -86,9 +89,10 @@ struct Cfg {
   static constexpr int VEC = RING > OUT ? RING : OUT;       // sa, sb, bias follow
   static constexpr int LDS = VEC + (BM + 2 * BN) * 4;
   static constexpr int CH = (BM + BN) * 8 / (64 * GW);      // chunks a thread (unaligned)
-  static_assert(TM % 32 == 0 && TN % 32 == 0, "whole 32x32 blocks");
+  static_assert(TM % MB == 0 && TN % MB == 0, "whole blocks");
   static_assert(BM % (8 * GW) == 0 && BN % (8 * GW) == 0, "copies");
   static_assert(R >= 2 && (R - 2) * L < 64, "vmcnt range");
+  static_assert(STEPS == 2 || STEPS == 4, "K steps");
   static_assert(LDS <= (int)kLdsMax && THREADS <= 1024, "workgroup");
 };
 
@@ -118,26 +122,48 @@ struct Copier {
   }
 };
 
+template <int MB>
+struct Product;
+template <>
+struct Product<32> {
+  typedef i32x16 Acc;
+  __device__ static __forceinline__ Acc mul(i32x4 b, i32x4 a, Acc c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(b, a, c, 0, 0, 0);
+  }
+};
+template <>
+struct Product<16> {
+  typedef i32x4 Acc;
+  __device__ static __forceinline__ Acc mul(i32x4 b, i32x4 a, Acc c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, c, 0, 0, 0);
+  }
+};
+
+// Operands of one K step: lane l holds 16 bytes of row l % MB, chunk l / MB of
+// the step's, of each block.  A product gives it the columns 8 q + 4 (l / MB)
+// .. + 3, q = 0 .. NV / 4 - 1, of row l % MB.
 template <class C>
 struct Frags {
   i32x4 a[C::FM], b[C::FN];
-  // K step j (32 bytes) of the slice at `st`; lane l reads row l % 32, chunk
-  // 2 j + l / 32.
+  __device__ static __forceinline__ int lane_at(int lane) {
+    const int r = lane % C::MB;
+    return r * kSlice + ((lane / C::MB ^ (r >> 1 & 7)) << 4);
+  }
   __device__ __forceinline__ void read(const char* st, int j, int at, int wm, int wn) {
-    const char* p = st + (at ^ (j << 5));
+    const char* p = st + (at ^ (j * C::KB));
 #pragma unroll
     for (int f = 0; f < C::FM; ++f)
-      a[f] = *reinterpret_cast<const i32x4*>(p + (wm * C::TM + f * 32) * kSlice);
+      a[f] = *reinterpret_cast<const i32x4*>(p + (wm * C::TM + f * C::MB) * kSlice);
 #pragma unroll
     for (int f = 0; f < C::FN; ++f)
-      b[f] = *reinterpret_cast<const i32x4*>(p + (C::BM + wn * C::TN + f * 32) * kSlice);
+      b[f] = *reinterpret_cast<const i32x4*>(p + (C::BM + wn * C::TN + f * C::MB) * kSlice);
   }
-  __device__ __forceinline__ void mul(i32x16 (&acc)[C::FM][C::FN]) const {
+  __device__ __forceinline__ void mul(typename Product<C::MB>::Acc (&acc)[C::FM][C::FN]) const {
 #pragma unroll
     for (int fm = 0; fm < C::FM; ++fm)
 #pragma unroll
       for (int fn = 0; fn < C::FN; ++fn)
-        acc[fm][fn] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[fn], a[fm], acc[fm][fn], 0, 0, 0);
+        acc[fm][fn] = Product<C::MB>::mul(b[fn], a[fm], acc[fm][fn]);
   }
 };
 
@@ -152,19 +178,30 @@ __device__ __forceinline__ void interleave() {
   }
 }
 
-// 16 bytes at k of a row of K, zeros past its end.
+// 16 bytes at k of a row of K, zeros past its end.  A chunk that crosses the end
+// is the row's last 16 bytes shifted down; of a row shorter than that, byte by
+// byte.  (Small: it is unrolled for every chunk a thread copies.)
 __device__ __forceinline__ i32x4 load_chunk(const int8_t* row, int k, int K) {
-  i32x4 v = {0, 0, 0, 0};
-  if (k + kChunk <= K) {
-    v = *reinterpret_cast<const i32x4_any*>(row + k);
-  } else if (k < K) {
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < 15; ++e)
-      if (k + e < K) w[e / 4] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e % 4));
-    v = i32x4{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+  const int n = K - k;
+  if (n >= kChunk) return *reinterpret_cast<const i32x4_any*>(row + k);
+  uint64_t lo = 0, hi = 0;
+  if (n > 0) {
+    if (K >= kChunk) {
+      const i32x4 v = *reinterpret_cast<const i32x4_any*>(row + K - kChunk);
+      lo = (uint32_t)v[0] | (uint64_t)(uint32_t)v[1] << 32;
+      hi = (uint32_t)v[2] | (uint64_t)(uint32_t)v[3] << 32;
+      const int s = 8 * (kChunk - n);
+      lo = s < 64 ? lo >> s | hi << (64 - s) : hi >> (s - 64);
+      hi = s < 64 ? hi >> s : 0;
+    } else {
+#pragma unroll 1
+      for (int e = n - 1; e >= 0; --e) {
+        hi = hi << 8 | lo >> 56;
+        lo = lo << 8 | (uint8_t)row[k + e];
+      }
+    }
   }
-  return v;
+  return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 }
 
 // ALIGNED: K % 16 == 0 and 16-byte aligned operands; the slices are copied
@@ -191,13 +228,13 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     vbias[i] = i < cols && g.bias ? (float)g.bias[n0 + i] : 0.f;
   }
 
-  i32x16 acc[C::FM][C::FN];
+  typename Product<C::MB>::Acc acc[C::FM][C::FN];
 #pragma unroll
   for (int fm = 0; fm < C::FM; ++fm)
 #pragma unroll
     for (int fn = 0; fn < C::FN; ++fn)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[fm][fn][i] = 0;
+      for (int i = 0; i < C::NV; ++i) acc[fm][fn][i] = 0;
 
   // Iteration i of a group is slice i * KS + grp.  Every group has `even` whole
   // slices; then one iteration more, in which a group has a whole slice, the
@@ -214,18 +251,27 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     cb.template copy<C::LB>(at, dst + C::BM * kSlice, w);
   };
   i32x4 held[ALIGNED ? 1 : C::CH];
-  auto load = [&](int i) {  // the same into registers
+  // The same into registers.  Rows past the tile's last: that one again (nothing
+  // of theirs is written).  The branch is outside the loop, so that a whole
+  // slice's loads are issued together.
+  auto row_of = [&](int q) {
+    const int r = q >> 3;
+    return r < C::BM ? A + (size_t)min(r, rows - 1) * K : B + (size_t)min(r - C::BM, cols - 1) * K;
+  };
+  auto load = [&](int i) {
     const int s = i * C::KS + grp;
+    if (s < full) {
 #pragma unroll
-    for (int j = 0; j < C::CH; ++j) {
-      const int q = w * 64 + lane + j * 64 * C::GW, r = q >> 3, k = s * kSlice + (q & 7) * kChunk;
-      // rows past the tile's last: that one again (nothing of theirs is written)
-      const int8_t* row = r < C::BM ? A + (size_t)min(r, rows - 1) * K
-                                    : B + (size_t)min(r - C::BM, cols - 1) * K;
-      if (s < full)
-        held[j] = *reinterpret_cast<const i32x4_any*>(row + k);
-      else
-        held[j] = load_chunk(row, k, K);
+      for (int j = 0; j < C::CH; ++j) {
+        const int q = w * 64 + lane + j * 64 * C::GW;
+        held[j] = *reinterpret_cast<const i32x4_any*>(row_of(q) + s * kSlice + (q & 7) * kChunk);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::CH; ++j) {
+        const int q = w * 64 + lane + j * 64 * C::GW;
+        held[j] = load_chunk(row_of(q), s * kSlice + (q & 7) * kChunk, K);
+      }
     }
   };
   auto put = [&](char* dst) {
@@ -246,7 +292,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     load(0);
   }
 
-  const int r32 = lane & 31, at = r32 * kSlice + ((lane >> 5 ^ (r32 >> 1 & 7)) << 4);
+  const int at = Frags<C>::lane_at(lane), lrow = lane % C::MB, lchunk = lane / C::MB;
   // Makes slice i readable: its copies have landed (those of the R - 2 later
   // ones may be in flight), and every wavefront has read slice i - 1, whose
   // slot the next copies fill.
@@ -267,21 +313,23 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
   };
   Frags<C> f0, f1;
   constexpr int RD = C::FM + C::FN, MF = C::FM * C::FN;
-  // K steps 0-2 of the slice, each beside the reads of the next step.
-  auto three = [&] {
+  // All K steps of the slice but the last, each beside the reads of the next.
+  auto most = [&] {
     __builtin_amdgcn_sched_barrier(0);
     f1.read(slot, 1, at, wm, wn);
     f0.mul(acc);
     interleave<RD, MF>();
     __builtin_amdgcn_sched_barrier(0);
-    f0.read(slot, 2, at, wm, wn);
-    f1.mul(acc);
-    interleave<RD, MF>();
-    __builtin_amdgcn_sched_barrier(0);
-    f1.read(slot, 3, at, wm, wn);
-    f0.mul(acc);
-    interleave<RD, MF>();
-    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (C::STEPS == 4) {
+      f0.read(slot, 2, at, wm, wn);
+      f1.mul(acc);
+      interleave<RD, MF>();
+      __builtin_amdgcn_sched_barrier(0);
+      f1.read(slot, 3, at, wm, wn);
+      f0.mul(acc);
+      interleave<RD, MF>();
+      __builtin_amdgcn_sched_barrier(0);
+    }
     slot = next(slot);
   };
   if (even > 0) {
@@ -289,23 +337,23 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     f0.read(slot, 0, at, wm, wn);
     advance(0);
     for (int i = 1; i < even; ++i) {
-      three();
+      most();
       arrive(i);
       f0.read(slot, 0, at, wm, wn);
       advance(i);
       f1.mul(acc);
       interleave<RD, MF>();
     }
-    three();
+    most();
     f1.mul(acc);
   }
   if (iters > even) {
     arrive(even);
     const int s = even * C::KS + grp, left = min(kSlice, K - s * kSlice);
-    for (int j = 0; j * 32 < left; ++j) {
+    for (int j = 0; j * C::KB < left; ++j) {
       f0.read(slot, j, at, wm, wn);
       // past K: the next row's bytes in both operands, cleared in one
-      if (ALIGNED && (2 * j + (lane >> 5)) * kChunk >= left)
+      if (ALIGNED && j * C::KB + lchunk * kChunk >= left)
 #pragma unroll
         for (int f = 0; f < C::FM; ++f) f0.a[f] = i32x4{0, 0, 0, 0};
       f0.mul(acc);
@@ -318,13 +366,13 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     f16* out = reinterpret_cast<f16*>(smem);
 #pragma unroll
     for (int fm = 0; fm < C::FM; ++fm) {
-      const int m = wm * C::TM + fm * 32 + r32;
+      const int m = wm * C::TM + fm * C::MB + lrow;
       const float sa = vsa[m];
 #pragma unroll
       for (int fn = 0; fn < C::FN; ++fn)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = wn * C::TN + fn * 32 + 8 * q + 4 * (lane >> 5);
+        for (int q = 0; q < C::NV / 4; ++q) {
+          const int n = wn * C::TN + fn * C::MB + 8 * q + 4 * lchunk;
           const f32x4 sb = *reinterpret_cast<const f32x4*>(vsb + n);
           const f32x4 bi = *reinterpret_cast<const f32x4*>(vbias + n);
           f16x4 o;
@@ -340,9 +388,9 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
 #pragma unroll
       for (int fn = 0; fn < C::FN; ++fn)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int m = wm * C::TM + fm * 32 + r32;
-          const int n = wn * C::TN + fn * 32 + 8 * q + 4 * (lane >> 5);
+        for (int q = 0; q < C::NV / 4; ++q) {
+          const int m = wm * C::TM + fm * C::MB + lrow;
+          const int n = wn * C::TN + fn * C::MB + 8 * q + 4 * lchunk;
           *reinterpret_cast<i32x4*>(sums + m * C::SUM_LD + n) =
               i32x4{acc[fm][fn][4 * q], acc[fm][fn][4 * q + 1], acc[fm][fn][4 * q + 2],
                     acc[fm][fn][4 * q + 3]};
@@ -417,10 +465,50 @@ hipError_t launch(const Args& g, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <class C>
-hipError_t launch(const Args& g, bool aligned, bool gelu, hipStream_t s) {
-  if (aligned) return gelu ? launch<C, true, true>(g, s) : launch<C, true, false>(g, s);
-  return gelu ? launch<C, false, true>(g, s) : launch<C, false, false>(g, s);
+template <class C, bool ALIGNED>
+hipError_t run(const Args& g, bool gelu, hipStream_t s) {
+  return gelu ? launch<C, ALIGNED, true>(g, s) : launch<C, ALIGNED, false>(g, s);
+}
+
+// The tiles, and what one costs a CU in cycles: a byte of K costs the larger of
+// its operand bytes at 32 a cycle, which is what the copies sustain from L2, and
+// `mfma`, the measured pace of the tile's products; `fixed` is the rest of a
+// tile's time (first copies, epilogue) that other workgroups on the CU do not
+// hide.  The tile whose ceil(tiles / CUs) rounds cost least is launched.
+struct Tile {
+  int bm, bn;
+  float mfma, fixed;
+};
+constexpr Tile kTiles[] = {{256, 256, 25.f, 6000.f}, {256, 128, 14.5f, 4000.f},
+                           {128, 128, 8.6f, 1200.f}, {64, 128, 4.4f, 1200.f},
+                           {128, 64, 4.4f, 1250.f},  {64, 64, 2.3f, 300.f},
+                           {32, 64, 1.2f, 600.f},    {32, 32, 0.7f, 400.f},
+                           {16, 32, 0.5f, 1500.f},   {16, 16, 0.3f, 600.f}};
+constexpr int kCus = kXcds * kXcdCus;
+// Tiles that unaligned operands take: the copies of the others would need more
+// registers than their wavefronts have.
+constexpr uint32_t kUnaligned = 1u << 2 | 1u << 3 | 1u << 5 | 1u << 6 | 1u << 9;
+
+int64_t rounds_of(const Tile& t, int M, int N) {
+  const int64_t n = (int64_t)((M - 1) / t.bm + 1) * ((N - 1) / t.bn + 1);
+  return (n + kCus - 1) / kCus;
+}
+
+int pick_tile(int M, int N, int K, uint32_t allowed) {
+  int best = -1;
+  float least = 0.f;
+  for (int i = 0; i < (int)(sizeof kTiles / sizeof kTiles[0]); ++i) {
+    if (!(allowed >> i & 1)) continue;
+    const Tile& t = kTiles[i];
+    const float copies = (float)((M < t.bm ? M : t.bm) + (N < t.bn ? N : t.bn)) / 32.f;
+    const float a_byte = copies > t.mfma ? copies : t.mfma;
+    const float cost = (float)rounds_of(t, M, N) * ((float)K * a_byte + t.fixed);
+    if (best < 0 || cost < least) {
+      least = cost;
+      best = i;
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -429,9 +517,43 @@ hipError_t gemm_i8(const int8_t* A, const float* sa, const int8_t* B, const floa
                    const f16* bias, f16* C, int M, int N, int K, bool gelu, hipStream_t s) {
   const Args g{A, B, sa, sb, bias, C, M, N, K};
   const bool aligned = K % kChunk == 0 && (((uintptr_t)A | (uintptr_t)B) & 15) == 0;
-  const int64_t t128 = (int64_t)((M - 1) / 128 + 1) * ((N - 1) / 128 + 1);
-  if (t128 >= 128) return launch<Cfg<128, 128, 2, 2, 1, 3>>(g, aligned, gelu, s);
-  return launch<Cfg<32, 64, 1, 2, 4, 2>>(g, aligned, gelu, s);
+  const int t = pick_tile(M, N, K, aligned ? ~0u : kUnaligned);
+  // One round, a workgroup a CU, and a long K: nothing but its own copies hides
+  // a workgroup's waits, so it has more of them in flight (or more groups).
+  const bool alone = rounds_of(kTiles[t], M, N) == 1 && K >= 1024;
+  if (!aligned) {
+    switch (t) {
+      case 2: return run<Cfg<128, 128, 2, 4, 1, 2>, false>(g, gelu, s);
+      case 3: return run<Cfg<64, 128, 2, 4, 1, 2>, false>(g, gelu, s);
+      case 5: return run<Cfg<64, 64, 2, 2, 1, 2>, false>(g, gelu, s);
+      case 6: return run<Cfg<32, 64, 1, 2, 4, 2>, false>(g, gelu, s);
+      default:
+        return alone ? run<Cfg<16, 16, 1, 1, 8, 2>, false>(g, gelu, s)
+                     : run<Cfg<16, 16, 1, 1, 4, 2>, false>(g, gelu, s);
+    }
+  }
+  switch (t) {
+    case 0: return run<Cfg<256, 256, 2, 4, 1, 2>, true>(g, gelu, s);
+    case 1: return run<Cfg<256, 128, 4, 2, 1, 3>, true>(g, gelu, s);
+    case 2:
+      return alone ? run<Cfg<128, 128, 2, 4, 1, 3>, true>(g, gelu, s)
+                   : run<Cfg<128, 128, 2, 4, 1, 2>, true>(g, gelu, s);
+    case 3:
+      return alone ? run<Cfg<64, 128, 2, 2, 1, 3>, true>(g, gelu, s)
+                   : run<Cfg<64, 128, 1, 4, 1, 2>, true>(g, gelu, s);
+    case 4:
+      return alone ? run<Cfg<128, 64, 2, 2, 1, 3>, true>(g, gelu, s)
+                   : run<Cfg<128, 64, 2, 2, 1, 2>, true>(g, gelu, s);
+    case 5:
+      return alone ? run<Cfg<64, 64, 2, 2, 2, 3>, true>(g, gelu, s)
+                   : run<Cfg<64, 64, 2, 2, 1, 2>, true>(g, gelu, s);
+    case 6: return run<Cfg<32, 64, 1, 2, 2, 3>, true>(g, gelu, s);
+    case 7:
+      return alone ? run<Cfg<32, 32, 1, 1, 4, 4>, true>(g, gelu, s)
+                   : run<Cfg<32, 32, 1, 1, 4, 2>, true>(g, gelu, s);
+    case 8: return run<Cfg<16, 32, 1, 1, 4, 4>, true>(g, gelu, s);
+    default: return run<Cfg<16, 16, 1, 1, 4, 4>, true>(g, gelu, s);
+  }
 }
 
 }  // namespace bbh
