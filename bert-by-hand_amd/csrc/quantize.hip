@@ -53,17 +53,14 @@ __device__ __forceinline__ float row_reduce(float v, F f, float* part) {
   return v;
 }
 
-// Chunk `c` of a row of D halves as fp32; zeros past the row's end.
-__device__ __forceinline__ void load8(const f16* row, int c, int D, float (&v)[8]) {
+// Chunk `c` of a row of D halves; zeros past the row's end.
+__device__ __forceinline__ f16x8 load8(const f16* row, int c, int D) {
   const int o = c * 8;
-  if (o + 8 <= D) {
-    const f16x8 a = *reinterpret_cast<const f16x8_any*>(row + o);
+  if (o + 8 <= D) return *reinterpret_cast<const f16x8_any*>(row + o);
+  f16x8 a;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)a[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = o + e < D ? (float)row[o + e] : 0.f;
-  }
+  for (int e = 0; e < 8; ++e) a[e] = o + e < D ? row[o + e] : (f16)0.f;
+  return a;
 }
 
 __device__ __forceinline__ void store8(f16* row, int c, int D, const float (&v)[8]) {
@@ -147,36 +144,42 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_kernel(const f16* 
   if (row >= M) return;  // T > 64: the whole workgroup
   const size_t off = (size_t)row * D;
   const int chunks = (D + 7) / 8;
-  float v[V][8];
+  // Every load before the first use: x, the residual and the norm's weights
+  // come in one latency.
+  f16x8 hx[V], hr[V], hg[V], hb[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = t + T * i;
-    if (c < chunks) {
-      load8(x + off, c, D, v[i]);
-    } else {
+    hx[i] = f16x8{};
+    if (t + T * i < chunks) hx[i] = load8(x + off, t + T * i, D);
+  }
+  if constexpr (KIND != kPlain) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    for (int i = 0; i < V; ++i) {
+      hr[i] = f16x8{};
+      if (a.residual && t + T * i < chunks) hr[i] = load8(a.residual + off, t + T * i, D);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      hg[i] = hb[i] = f16x8{};
+      if (t + T * i < chunks) {
+        hg[i] = load8(a.gamma, t + T * i, D);
+        if constexpr (KIND == kLayer) hb[i] = load8(a.beta, t + T * i, D);
+      }
     }
   }
-  float rstd = 1.f;
-  if constexpr (KIND != kPlain) {
-    if (a.residual) {
+  float v[V][8];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = t + T * i;
-        if (c >= chunks) break;
-        float r[8];
-        load8(a.residual + off, c, D, r);
+  for (int i = 0; i < V; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] += r[e];
-      }
+    for (int e = 0; e < 8; ++e) {
+      v[i][e] = (float)hx[i][e];
+      if constexpr (KIND != kPlain) v[i][e] += (float)hr[i][e];
     }
+  if constexpr (KIND != kPlain) {
     if (a.sum) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = t + T * i;
-        if (c < chunks) store8(a.sum + off, c, D, v[i]);
-      }
+      for (int i = 0; i < V; ++i)
+        if (t + T * i < chunks) store8(a.sum + off, t + T * i, D, v[i]);
     }
     if constexpr (KIND == kLayer) {
       float s = 0.f;
@@ -196,20 +199,15 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_kernel(const f16* 
     for (int i = 0; i < V; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += v[i][e] * v[i][e];
-    rstd = rsqrtf(row_reduce<T>(s, AddOp{}, part[1]) / (float)D + a.eps);
+    const float rstd = rsqrtf(row_reduce<T>(s, AddOp{}, part[1]) / (float)D + a.eps);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int c = t + T * i;
-      if (c >= chunks) break;
-      float g[8], b[8];
-      load8(a.gamma, c, D, g);
-      if constexpr (KIND == kLayer) load8(a.beta, c, D, b);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        v[i][e] = v[i][e] * rstd * g[e];
-        if constexpr (KIND == kLayer) v[i][e] += b[e];
+        v[i][e] = v[i][e] * rstd * (float)hg[i][e];
+        if constexpr (KIND == kLayer) v[i][e] += (float)hb[i][e];
       }
-      if (a.y) store8(a.y + off, c, D, v[i]);
+      if (a.y && t + T * i < chunks) store8(a.y + off, t + T * i, D, v[i]);
     }
   }
   float m = 0.f;
@@ -238,15 +236,18 @@ __global__ __launch_bounds__(kWide) void quantize_wide_kernel(const f16* __restr
   if (row >= M) return;
   const size_t off = (size_t)row * D;
   const int chunks = (D + 7) / 8;
-  float m = 0.f, v[8];
+  float m = 0.f;
   for (int c = threadIdx.x; c < chunks; c += kWide) {
-    load8(x + off, c, D, v);
+    const f16x8 h = load8(x + off, c, D);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = UMaxOp{}(m, fabsf(v[e]));
+    for (int e = 0; e < 8; ++e) m = UMaxOp{}(m, fabsf((float)h[e]));
   }
   const Coder k(row_reduce<kWide>(m, UMaxOp{}, part));
   for (int c = threadIdx.x; c < chunks; c += kWide) {
-    load8(x + off, c, D, v);
+    const f16x8 h = load8(x + off, c, D);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)h[e];
     store_codes(q + off, c, D, k, v);
   }
   if (threadIdx.x == 0) scale[row] = k.scale();
@@ -282,6 +283,14 @@ dim3 grid2(int64_t n) {
   return n <= X ? dim3((uint32_t)n) : dim3((uint32_t)X, (uint32_t)((n + X - 1) / X));
 }
 
+template <int T>
+hipError_t dequantize(const int8_t* q, const float* scale, f16* x, int M, int D, hipStream_t s) {
+  constexpr int R = 256 / T;
+  hipLaunchKernelGGL(dequantize_kernel<T>, grid2(((int64_t)M + R - 1) / R), dim3(256), 0, s, q,
+                     scale, x, M, D);
+  return hipGetLastError();
+}
+
 template <int T, int V, Kind KIND>
 hipError_t launch(const f16* x, int8_t* q, float* scale, int M, int D, const NormArgs& a,
                   hipStream_t s) {
@@ -294,11 +303,29 @@ hipError_t launch(const f16* x, int8_t* q, float* scale, int M, int D, const Nor
 template <Kind KIND>
 hipError_t quantize(const f16* x, int8_t* q, float* scale, int M, int D, const NormArgs& a,
                     hipStream_t s) {
+  // Threads a row: as few as leave a thread at most four chunks, so that the
+  // lanes are full and the reductions short; more where rows are too few to fill
+  // the GPU and a thread's chunks would queue behind each other.  Measured, us
+  // (quantise / LayerNorm with residual and y):
+  //   131072 x 32     16 threads  8.2 / 15.4   64 threads  27.0 / 52.3
+  //   131072 x 384    16 x 3     28.3 / 63.5   64 x 1      36.6 / 64.8
+  //   2003 x 384      16 x 3      3.1 /  4.5   64 x 1       2.8 /  3.6
+  //   65536 x 1536    64 x 3     54.7 / 119    256 x 1     67.9 / 126
+  //   30000 x 2048    64 x 4     33.5 / 76.0   256 x 1     35.2 / 74.5
+  //   8192 x 8192    256 x 4     37.0 / 84.4   1024 x 1    43.5 / 96.7
+  //   1 x 8192       256 x 4      3.1 /  4.8   1024 x 1     2.7 /  4.0
   const int chunks = (D + 7) / 8;
+  const bool many = M >= 4096;
+  if (chunks <= 16) return launch<16, 1, KIND>(x, q, scale, M, D, a, s);
+  if (chunks <= 32 && many) return launch<16, 2, KIND>(x, q, scale, M, D, a, s);
+  if (chunks <= 48 && many) return launch<16, 3, KIND>(x, q, scale, M, D, a, s);
   if (chunks <= 64) return launch<64, 1, KIND>(x, q, scale, M, D, a, s);
   if (chunks <= 128) return launch<64, 2, KIND>(x, q, scale, M, D, a, s);
+  if (chunks <= 192) return launch<64, 3, KIND>(x, q, scale, M, D, a, s);
   if (chunks <= 256) return launch<256, 1, KIND>(x, q, scale, M, D, a, s);
   if (chunks <= 512) return launch<256, 2, KIND>(x, q, scale, M, D, a, s);
+  if (chunks <= 1024 && M <= 128) return launch<1024, 1, KIND>(x, q, scale, M, D, a, s);
+  if (chunks <= 768) return launch<256, 3, KIND>(x, q, scale, M, D, a, s);
   if (chunks <= 1024) return launch<256, 4, KIND>(x, q, scale, M, D, a, s);
   return launch<1024, 2, KIND>(x, q, scale, M, D, a, s);
 }
@@ -313,12 +340,11 @@ hipError_t quantize_rows(const f16* x, int8_t* q, float* scale, int M, int D, hi
 
 hipError_t dequantize_rows(const int8_t* q, const float* scale, f16* x, int M, int D,
                            hipStream_t s) {
-  if (D <= 1024)
-    hipLaunchKernelGGL(dequantize_kernel<64>, grid2(((int64_t)M + 3) / 4), dim3(256), 0, s, q,
-                       scale, x, M, D);
-  else
-    hipLaunchKernelGGL(dequantize_kernel<256>, grid2(M), dim3(256), 0, s, q, scale, x, M, D);
-  return hipGetLastError();
+  // 131072 x 256 19.2 us with 16 threads a row, 25.9 with 64; 65536 x 1024 39.1
+  // and 35.8; 16384 x 4096 41.2 with 64, 35.9 with 256
+  if (D <= 256) return dequantize<16>(q, scale, x, M, D, s);
+  if (D <= 1024) return dequantize<64>(q, scale, x, M, D, s);
+  return dequantize<256>(q, scale, x, M, D, s);
 }
 
 hipError_t rmsnorm_quantize(const f16* x, const f16* residual, const f16* gamma, f16* sum, f16* y,
