@@ -471,12 +471,12 @@ def _operand(name, t, dtype, n, device):
     current device (None: of one that is not passed)."""
     if t is None:
         return None
-    if t.dtype != dtype or t.get_device() < 0 or not t.is_contiguous():
+    if (t.dtype is dtype and t.get_device() == device and t.numel() >= n and t.is_contiguous()):
+        return t.data_ptr()
+    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous {dtype} CUDA tensor")
-    if t.get_device() != device or t.numel() < n:
-        raise ValueError(f"{name}: expected {n} elements on cuda:{device}, the current device, got "
-                         f"{t.numel()} on cuda:{t.get_device()}")
-    return t.data_ptr()
+    raise ValueError(f"{name}: expected {n} elements on cuda:{device}, the current device, got "
+                     f"{t.numel()} on cuda:{t.get_device()}")
 
 
 def _place(t, stream, *sizes):

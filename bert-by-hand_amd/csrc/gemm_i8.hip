@@ -15,6 +15,7 @@
 // (the layout of pipe.h's 64-wide fp16 slice, byte for byte).
 
 #include <atomic>
+#include <type_traits>
 
 #include "int8.h"
 #include "pipe.h"
@@ -91,8 +92,9 @@ struct Cfg {
   static constexpr int CH = (BM + BN) * 8 / (64 * GW);      // chunks a thread (unaligned)
   static_assert(TM % MB == 0 && TN % MB == 0, "whole blocks");
   static_assert(BM % (8 * GW) == 0 && BN % (8 * GW) == 0, "copies");
-  static_assert(R >= 2 && (R - 2) * L < 64, "vmcnt range");
+  static_assert(R >= 2 && (R - 1) * L < 64, "vmcnt range");
   static_assert(STEPS == 2 || STEPS == 4, "K steps");
+  static_assert(BM <= THREADS && BN <= THREADS, "a thread loads one of each vector");
   static_assert(LDS <= (int)kLdsMax && THREADS <= 1024, "workgroup");
 };
 
@@ -219,13 +221,15 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int grp = wave / C::GW, w = wave % C::GW, wm = w / C::WN, wn = w % C::WN;
 
-  float* vsa = reinterpret_cast<float*>(smem + C::VEC);
-  float* vsb = vsa + C::BM;
-  float* vbias = vsb + C::BN;
-  for (int i = threadIdx.x; i < C::BM; i += C::THREADS) vsa[i] = i < rows ? g.sa[m0 + i] : 0.f;
-  for (int i = threadIdx.x; i < C::BN; i += C::THREADS) {
-    vsb[i] = i < cols ? g.sb[n0 + i] : 0.f;
-    vbias[i] = i < cols && g.bias ? (float)g.bias[n0 + i] : 0.f;
+  // The epilogue's vectors: loaded here, ahead of the copies, and put into LDS
+  // after the K loop, so that nothing waits for them.
+  const int tid = threadIdx.x;
+  float hsa = 0.f, hsb = 0.f;
+  f16 hbias = 0.f;
+  if (tid < rows) hsa = g.sa[m0 + tid];
+  if (tid < cols) {
+    hsb = g.sb[n0 + tid];
+    if (g.bias) hbias = g.bias[n0 + tid];
   }
 
   typename Product<C::MB>::Acc acc[C::FM][C::FN];
@@ -286,24 +290,26 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
   char* refill = ring;    // the slot that the next copies go to
   if constexpr (ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < C::R - 1; ++i) issue(i, ring + i * C::STAGE);
-    refill = ring_end - C::STAGE;
+    for (int i = 0; i < C::R; ++i) issue(i, ring + i * C::STAGE);
   } else {
     load(0);
   }
 
   const int at = Frags<C>::lane_at(lane), lrow = lane % C::MB, lchunk = lane / C::MB;
-  // Makes slice i readable: its copies have landed (those of the R - 2 later
-  // ones may be in flight), and every wavefront has read slice i - 1, whose
-  // slot the next copies fill.
-  auto arrive = [&](int) {
+  // Makes slice i readable: its copies have landed (those of later ones may be
+  // in flight: R - 1 slices behind the first, then R - 2, as the next copies come
+  // after this), and every wavefront has read slice i - 1, whose slot the next
+  // copies fill.
+  auto arrive = [&](auto first) {
     if constexpr (ALIGNED)
-      wait_vm<(C::R - 2) * C::L>();
+      wait_vm<(C::R - (decltype(first)::value ? 1 : 2)) * C::L>();
     else
       put(slot);
     lds_barrier();
   };
-  auto advance = [&](int i) {  // the copies that follow arrive(i)
+  constexpr std::true_type kFirst{};
+  constexpr std::false_type kLater{};
+  auto advance = [&](int i) {  // the copies that follow arrive() of slice i
     if constexpr (ALIGNED) {
       issue(i + C::R - 1, refill);
       refill = next(refill);
@@ -333,12 +339,12 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     slot = next(slot);
   };
   if (even > 0) {
-    arrive(0);
+    arrive(kFirst);
     f0.read(slot, 0, at, wm, wn);
-    advance(0);
+    if constexpr (!ALIGNED) advance(0);
     for (int i = 1; i < even; ++i) {
       most();
-      arrive(i);
+      arrive(kLater);
       f0.read(slot, 0, at, wm, wn);
       advance(i);
       f1.mul(acc);
@@ -348,7 +354,10 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     f1.mul(acc);
   }
   if (iters > even) {
-    arrive(even);
+    if (even > 0)
+      arrive(kLater);
+    else
+      arrive(kFirst);
     const int s = even * C::KS + grp, left = min(kSlice, K - s * kSlice);
     for (int j = 0; j * C::KB < left; ++j) {
       f0.read(slot, j, at, wm, wn);
@@ -358,6 +367,14 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
         for (int f = 0; f < C::FM; ++f) f0.a[f] = i32x4{0, 0, 0, 0};
       f0.mul(acc);
     }
+  }
+  float* vsa = reinterpret_cast<float*>(smem + C::VEC);
+  float* vsb = vsa + C::BM;
+  float* vbias = vsb + C::BN;
+  if (tid < C::BM) vsa[tid] = hsa;
+  if (tid < C::BN) {
+    vsb[tid] = hsb;
+    vbias[tid] = (float)hbias;
   }
   if constexpr (ALIGNED) wait_vm<0>();  // copies from nowhere are still copies
   lds_barrier();                        // the ring is free
