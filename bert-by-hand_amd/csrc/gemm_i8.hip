@@ -92,7 +92,7 @@ struct Cfg {
   static constexpr int CH = (BM + BN) * 8 / (64 * GW);      // chunks a thread (unaligned)
   static_assert(TM % MB == 0 && TN % MB == 0, "whole blocks");
   static_assert(BM % (8 * GW) == 0 && BN % (8 * GW) == 0, "copies");
-  static_assert(R >= 2 && (R - 1) * L < 64, "vmcnt range");
+  static_assert(R >= 1 && (R - 1) * L < 64, "vmcnt range");
   static_assert(STEPS == 2 || STEPS == 4, "K steps");
   static_assert(BM <= THREADS && BN <= THREADS, "a thread loads one of each vector");
   static_assert(LDS <= (int)kLdsMax && THREADS <= 1024, "workgroup");
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
   // copies fill.
   auto arrive = [&](auto first) {
     if constexpr (ALIGNED)
-      wait_vm<(C::R - (decltype(first)::value ? 1 : 2)) * C::L>();
+      wait_vm<(C::R - (decltype(first)::value || C::R == 1 ? 1 : 2)) * C::L>();
     else
       put(slot);
     lds_barrier();
@@ -310,11 +310,17 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
   constexpr std::true_type kFirst{};
   constexpr std::false_type kLater{};
   auto advance = [&](int i) {  // the copies that follow arrive() of slice i
-    if constexpr (ALIGNED) {
+    if constexpr (ALIGNED && C::R > 1) {
       issue(i + C::R - 1, refill);
       refill = next(refill);
-    } else if (i + 1 < iters) {
+    } else if (!ALIGNED && i + 1 < iters) {
       load(i + 1);
+    }
+  };
+  auto reload = [&](int i) {  // R == 1: the next slice over this one
+    if constexpr (ALIGNED && C::R == 1) {
+      lds_barrier();
+      issue(i, ring);
     }
   };
   Frags<C> f0, f1;
@@ -344,6 +350,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     if constexpr (!ALIGNED) advance(0);
     for (int i = 1; i < even; ++i) {
       most();
+      reload(i);
       arrive(kLater);
       f0.read(slot, 0, at, wm, wn);
       advance(i);
@@ -351,6 +358,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
       interleave<RD, MF>();
     }
     most();
+    if (C::R == 1 && iters > even) reload(even);
     f1.mul(acc);
   }
   if (iters > even) {
@@ -488,19 +496,20 @@ hipError_t run(const Args& g, bool gelu, hipStream_t s) {
 }
 
 // The tiles, and what one costs a CU in cycles: a byte of K costs the larger of
-// its operand bytes at 32 a cycle, which is what the copies sustain from L2, and
-// `mfma`, the measured pace of the tile's products; `fixed` is the rest of a
-// tile's time (first copies, epilogue) that other workgroups on the CU do not
-// hide.  The tile whose ceil(tiles / CUs) rounds cost least is launched.
+// its operand bytes at 32 a cycle, which is what the copies sustain from L2 (44
+// where many single-wavefront workgroups share a CU), and `mfma`, the measured
+// pace of the tile's products; `fixed` is the rest of a tile's time (first
+// copies, epilogue) that other workgroups on the CU do not hide.  The tile
+// whose ceil(tiles / CUs) rounds cost least is launched.
 struct Tile {
   int bm, bn;
   float mfma, fixed;
 };
-constexpr Tile kTiles[] = {{256, 256, 25.f, 6000.f}, {256, 128, 14.5f, 4000.f},
-                           {128, 128, 8.6f, 1200.f}, {64, 128, 4.4f, 1200.f},
-                           {128, 64, 4.4f, 1250.f},  {64, 64, 2.3f, 300.f},
-                           {32, 64, 1.2f, 600.f},    {32, 32, 0.7f, 400.f},
-                           {16, 32, 0.5f, 1500.f},   {16, 16, 0.3f, 600.f}};
+constexpr Tile kTiles[] = {{256, 256, 20.5f, 8000.f}, {256, 128, 14.5f, 4000.f},
+                           {128, 128, 8.6f, 1000.f},  {64, 128, 4.4f, 1200.f},
+                           {128, 64, 4.4f, 1250.f},   {64, 64, 2.3f, 300.f},
+                           {32, 64, 1.2f, 600.f},     {32, 32, 0.7f, 900.f},
+                           {16, 32, 0.5f, 1500.f},    {16, 16, 0.3f, 120.f}};
 constexpr int kCus = kXcds * kXcdCus;
 // Tiles that unaligned operands take: the copies of the others would need more
 // registers than their wavefronts have.
@@ -517,9 +526,10 @@ int pick_tile(int M, int N, int K, uint32_t allowed) {
   for (int i = 0; i < (int)(sizeof kTiles / sizeof kTiles[0]); ++i) {
     if (!(allowed >> i & 1)) continue;
     const Tile& t = kTiles[i];
-    const float copies = (float)((M < t.bm ? M : t.bm) + (N < t.bn ? N : t.bn)) / 32.f;
-    const float a_byte = copies > t.mfma ? copies : t.mfma;
-    const float cost = (float)rounds_of(t, M, N) * ((float)K * a_byte + t.fixed);
+    const int64_t rounds = rounds_of(t, M, N);
+    const float copies = (float)((M < t.bm ? M : t.bm) + (N < t.bn ? N : t.bn)) /
+                         (t.bn == 16 && rounds > 2 ? 44.f : 32.f);
+    const float cost = (float)rounds * ((float)K * (copies > t.mfma ? copies : t.mfma) + t.fixed);
     if (best < 0 || cost < least) {
       least = cost;
       best = i;
@@ -537,7 +547,11 @@ hipError_t gemm_i8(const int8_t* A, const float* sa, const int8_t* B, const floa
   const int t = pick_tile(M, N, K, aligned ? ~0u : kUnaligned);
   // One round, a workgroup a CU, and a long K: nothing but its own copies hides
   // a workgroup's waits, so it has more of them in flight (or more groups).
-  const bool alone = rounds_of(kTiles[t], M, N) == 1 && K >= 1024;
+  const int64_t rounds = rounds_of(kTiles[t], M, N);
+  const bool alone = rounds == 1 && K >= 1024;
+  // Several rounds of a short K: a ring of one slice, so that twice the
+  // workgroups share a CU and hide each other's copies and epilogues.
+  const bool shortk = rounds > 1 && K <= 512;
   if (!aligned) {
     switch (t) {
       case 2: return run<Cfg<128, 128, 2, 4, 1, 2>, false>(g, gelu, s);
@@ -554,22 +568,37 @@ hipError_t gemm_i8(const int8_t* A, const float* sa, const int8_t* B, const floa
     case 1: return run<Cfg<256, 128, 4, 2, 1, 3>, true>(g, gelu, s);
     case 2:
       return alone ? run<Cfg<128, 128, 2, 4, 1, 3>, true>(g, gelu, s)
-                   : run<Cfg<128, 128, 2, 4, 1, 2>, true>(g, gelu, s);
+             : shortk ? run<Cfg<128, 128, 2, 4, 1, 1>, true>(g, gelu, s)
+                      : run<Cfg<128, 128, 2, 4, 1, 2>, true>(g, gelu, s);
     case 3:
       return alone ? run<Cfg<64, 128, 2, 2, 1, 3>, true>(g, gelu, s)
-                   : run<Cfg<64, 128, 1, 4, 1, 2>, true>(g, gelu, s);
+             : shortk ? run<Cfg<64, 128, 1, 4, 1, 1>, true>(g, gelu, s)
+                      : run<Cfg<64, 128, 1, 4, 1, 2>, true>(g, gelu, s);
     case 4:
       return alone ? run<Cfg<128, 64, 2, 2, 1, 3>, true>(g, gelu, s)
-                   : run<Cfg<128, 64, 2, 2, 1, 2>, true>(g, gelu, s);
+             : shortk ? run<Cfg<128, 64, 2, 2, 1, 1>, true>(g, gelu, s)
+                      : run<Cfg<128, 64, 2, 2, 1, 2>, true>(g, gelu, s);
     case 5:
       return alone ? run<Cfg<64, 64, 2, 2, 2, 3>, true>(g, gelu, s)
-                   : run<Cfg<64, 64, 2, 2, 1, 2>, true>(g, gelu, s);
-    case 6: return run<Cfg<32, 64, 1, 2, 2, 3>, true>(g, gelu, s);
+             : shortk ? run<Cfg<64, 64, 2, 2, 1, 1>, true>(g, gelu, s)
+             : rounds == 2 && K >= 1024 ? run<Cfg<64, 64, 2, 2, 1, 3>, true>(g, gelu, s)
+                                        : run<Cfg<64, 64, 2, 2, 1, 2>, true>(g, gelu, s);
+    case 6:
+      return shortk       ? run<Cfg<32, 64, 1, 2, 1, 1>, true>(g, gelu, s)
+             : rounds > 2 ? run<Cfg<32, 64, 1, 2, 1, 2>, true>(g, gelu, s)
+                          : run<Cfg<32, 64, 1, 2, 2, 3>, true>(g, gelu, s);
     case 7:
-      return alone ? run<Cfg<32, 32, 1, 1, 4, 4>, true>(g, gelu, s)
-                   : run<Cfg<32, 32, 1, 1, 4, 2>, true>(g, gelu, s);
+      return alone                   ? run<Cfg<32, 32, 1, 1, 4, 4>, true>(g, gelu, s)
+             : K <= 512 || rounds > 2 ? run<Cfg<32, 32, 1, 1, 1, 2>, true>(g, gelu, s)
+                                      : run<Cfg<32, 32, 1, 1, 4, 2>, true>(g, gelu, s);
     case 8: return run<Cfg<16, 32, 1, 1, 4, 4>, true>(g, gelu, s);
-    default: return run<Cfg<16, 16, 1, 1, 4, 4>, true>(g, gelu, s);
+    default:
+      // one wavefront a workgroup where K is short (16 x 1536 x 384 2.7 us
+      // against 3.1) or there are many (8 x 33206 x 2704 17.0 against 19.7), not
+      // too long each (1 x 32000 x 4096 31.5 against 27.6)
+      return K <= 512 || (rounds >= 8 && K < 4096) ? run<Cfg<16, 16, 1, 1, 1, 2>, true>(g, gelu, s)
+             : K <= 1536 ? run<Cfg<16, 16, 1, 1, 2, 2>, true>(g, gelu, s)
+                         : run<Cfg<16, 16, 1, 1, 4, 4>, true>(g, gelu, s);
   }
 }
 
