@@ -388,7 +388,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
   lds_barrier();                        // the ring is free
 
   if constexpr (C::KS == 1) {
-    f16* out = reinterpret_cast<f16*>(smem);
+    f16* tile = reinterpret_cast<f16*>(smem);
 #pragma unroll
     for (int fm = 0; fm < C::FM; ++fm) {
       const int m = wm * C::TM + fm * C::MB + lrow;
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
           f16x4 o;
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] = finish<GELU>(acc[fm][fn][4 * q + e], sa, sb[e], bi[e]);
-          *reinterpret_cast<f16x4*>(out + m * C::OUT_LD + n) = o;
+          *reinterpret_cast<f16x4*>(tile + m * C::OUT_LD + n) = o;
         }
     }
   } else {
@@ -422,9 +422,8 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
         }
   }
   lds_barrier();
-  for (int i = threadIdx.x; i < C::BM * C::BN / 8; i += C::THREADS) {
-    const int m = i / (C::BN / 8), n = i % (C::BN / 8) * 8;
-    if (m >= rows || n >= cols) continue;
+  // Eight columns a thread at a time, 16-byte stores.
+  auto chunk = [&](int m, int n) {
     f16x8 o;
     if constexpr (C::KS == 1) {
       o = *reinterpret_cast<const f16x8*>(reinterpret_cast<const f16*>(smem) + m * C::OUT_LD + n);
@@ -443,7 +442,33 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = finish<GELU>(v[e], vsa[m], vsb[n + e], vbias[n + e]);
     }
-    f16* dst = g.C + (size_t)(m0 + m) * g.N + n0 + n;
+    return o;
+  };
+  constexpr int CPR = C::BN / 8, N8 = C::BM * CPR;  // chunks a row, a tile
+  f16* const out = g.C + (size_t)m0 * g.N + n0;
+  if (N8 % C::THREADS == 0 && rows == C::BM && cols == C::BN) {
+    // a whole tile: up to four reads in flight before their stores
+    constexpr int IT = N8 >= C::THREADS ? N8 / C::THREADS : 1, U = IT % 4 == 0 ? 4 : 1;
+    const int m = tid / CPR, n = tid % CPR * 8;
+    f16* dst = out + (size_t)m * g.N + n;
+#pragma unroll
+    for (int i = 0; i < IT; i += U) {
+      f16x8 o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) o[u] = chunk(m + (i + u) * (C::THREADS / CPR), n);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        *reinterpret_cast<f16x8_any*>(dst) = o[u];
+        dst += (size_t)(C::THREADS / CPR) * g.N;
+      }
+    }
+    return;
+  }
+  for (int i = tid; i < N8; i += C::THREADS) {
+    const int m = i / CPR, n = i % CPR * 8;
+    if (m >= rows || n >= cols) continue;
+    const f16x8 o = chunk(m, n);
+    f16* dst = out + (size_t)m * g.N + n;
     if (n + 8 <= cols) {
       *reinterpret_cast<f16x8_any*>(dst) = o;
     } else {
@@ -505,7 +530,7 @@ struct Tile {
   int bm, bn;
   float mfma, fixed;
 };
-constexpr Tile kTiles[] = {{256, 256, 20.5f, 8000.f}, {256, 128, 14.5f, 4000.f},
+constexpr Tile kTiles[] = {{256, 256, 20.5f, 9500.f}, {256, 128, 14.5f, 4000.f},
                            {128, 128, 8.6f, 1000.f},  {64, 128, 4.4f, 1200.f},
                            {128, 64, 4.4f, 1250.f},   {64, 64, 2.3f, 300.f},
                            {32, 64, 1.2f, 600.f},     {32, 32, 0.7f, 900.f},
