@@ -91,7 +91,7 @@ struct Cfg {
   static constexpr int LDS = VEC + (BM + 2 * BN) * 4;
   static constexpr int CH = (BM + BN) * 8 / (64 * GW);      // chunks a thread (unaligned)
   static_assert(TM % MB == 0 && TN % MB == 0, "whole blocks");
-  static_assert(BM % (8 * GW) == 0 && BN % (8 * GW) == 0, "copies");
+  static_assert(BM % (8 * GW) == 0 && BN % (8 * GW) == 0, "a copy is of one operand");
   static_assert(R >= 1 && (R - 1) * L < 64, "vmcnt range");
   static_assert(STEPS == 2 || STEPS == 4, "K steps");
   static_assert(BM <= THREADS && BN <= THREADS, "a thread loads one of each vector");
@@ -100,7 +100,8 @@ struct Cfg {
 
 // Copies of this wavefront's share of a slice: global -> LDS, 1 KB = 8 rows a
 // copy.  Rows and bytes past the operand are out of the resource's bounds, as
-// is everything at an offset of kNowhere: such copies read no memory.
+// is everything at an offset of kNowhere: such copies read no memory and write
+// zeros.
 constexpr uint32_t kNowhere = 1u << 30;
 struct Copier {
   __amdgpu_buffer_rsrc_t src;
@@ -206,12 +207,23 @@ __device__ __forceinline__ i32x4 load_chunk(const int8_t* row, int k, int K) {
   return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 }
 
-// ALIGNED: K % 16 == 0 and 16-byte aligned operands; the slices are copied
-// global -> LDS with buffer loads to LDS.  Otherwise they go through registers,
-// one slice ahead, the bytes past K cleared.
-template <class C, bool ALIGNED, bool GELU>
+// How slices reach the ring.
+//  kCopies   K % 16 == 0, 16-byte aligned operands: buffer loads to LDS.
+//  kCopies4  K % 4 == 0, 4-byte aligned operands: the same for whole slices (a
+//            copy of 16 bytes needs 4-byte alignment only); the last part of K,
+//            whose chunks would cross a row's end, goes through registers.
+//  kStaged   any K and address: through registers, one slice ahead; kStaged2:
+//            two ahead, for workgroups that have a CU to themselves (2008 x 1904
+//            x 5201 44 us against 52; with two on a CU the registers cost more
+//            than that hides: 4000 x 4000 x 2001 75 against 65).
+// Through registers, the bytes past K are cleared.
+enum Feed { kCopies, kCopies4, kStaged, kStaged2 };
+
+template <class C, int FEED, bool GELU>
 __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int tn) {
   extern __shared__ __align__(16) char smem[];
+  constexpr bool COPIES = FEED <= kCopies4;
+  constexpr int AHEAD = FEED == kStaged2 ? 2 : 1;
   int bm, bn;
   if (!tile_of(tm, tn, bm, bn)) return;
   const int K = g.K, m0 = bm * C::BM, n0 = bn * C::BN;
@@ -248,51 +260,56 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
   char* const ring = smem + grp * C::R * C::STAGE;
   char* const ring_end = ring + C::R * C::STAGE;
   const Copier ca(A, rows, K), cb(B, cols, K);
-  auto issue = [&](int i, char* dst) {  // ALIGNED: the slice of iteration i into a slot
+  auto issue = [&](int i, char* dst) {  // COPIES: the slice of iteration i into a slot
     const int s = i * C::KS + grp;
-    const uint32_t at = s < total ? (uint32_t)s * kSlice : kNowhere;
+    const uint32_t at = s < (FEED == kCopies ? total : full) ? (uint32_t)s * kSlice : kNowhere;
     ca.template copy<C::LA>(at, dst, w);
     cb.template copy<C::LB>(at, dst + C::BM * kSlice, w);
   };
-  i32x4 held[ALIGNED ? 1 : C::CH];
-  // The same into registers.  Rows past the tile's last: that one again (nothing
-  // of theirs is written).  The branch is outside the loop, so that a whole
-  // slice's loads are issued together.
-  auto row_of = [&](int q) {
-    const int r = q >> 3;
-    return r < C::BM ? A + (size_t)min(r, rows - 1) * K : B + (size_t)min(r - C::BM, cols - 1) * K;
+  // Through registers (set: i % AHEAD).  Chunk j of a thread is a row of A or of B
+  // by j alone; rows past the tile's last are that one again (nothing of theirs
+  // is written).
+  constexpr int CH = FEED == kCopies ? 1 : C::CH;
+  i32x4 held[AHEAD][CH];
+  auto from = [&](int j) {
+    const int q = w * 64 + lane + j * 64 * C::GW, r = q >> 3;
+    return (uint32_t)(j * 8 * C::GW < C::BM ? min(r, rows - 1) : min(r - C::BM, cols - 1)) * K +
+           (q & 7) * kChunk;
   };
-  auto load = [&](int i) {
+  auto load = [&](int i, auto set) {
     const int s = i * C::KS + grp;
+    // the branch is outside the loops, so that a slice's loads are issued together
     if (s < full) {
+      const int8_t *a = A + s * kSlice, *b = B + s * kSlice;
 #pragma unroll
-      for (int j = 0; j < C::CH; ++j) {
-        const int q = w * 64 + lane + j * 64 * C::GW;
-        held[j] = *reinterpret_cast<const i32x4_any*>(row_of(q) + s * kSlice + (q & 7) * kChunk);
-      }
-    } else {
+      for (int j = 0; j < CH; ++j)
+        held[set][j] = *reinterpret_cast<const i32x4_any*>((j * 8 * C::GW < C::BM ? a : b) + from(j));
+    } else if (s < total) {
 #pragma unroll
-      for (int j = 0; j < C::CH; ++j) {
-        const int q = w * 64 + lane + j * 64 * C::GW;
-        held[j] = load_chunk(row_of(q), s * kSlice + (q & 7) * kChunk, K);
+      for (int j = 0; j < CH; ++j) {
+        const int k = (lane & 7) * kChunk;  // from(j) less its row's start
+        held[set][j] = load_chunk((j * 8 * C::GW < C::BM ? A : B) + (from(j) - k), s * kSlice + k, K);
       }
     }
   };
-  auto put = [&](char* dst) {
+  auto put = [&](char* dst, auto set) {
 #pragma unroll
-    for (int j = 0; j < C::CH; ++j) {
+    for (int j = 0; j < CH; ++j) {
       const int q = w * 64 + lane + j * 64 * C::GW, r = q >> 3;
-      *reinterpret_cast<i32x4*>(dst + r * kSlice + (((q & 7) ^ (r >> 1 & 7)) << 4)) = held[j];
+      *reinterpret_cast<i32x4*>(dst + r * kSlice + (((q & 7) ^ (r >> 1 & 7)) << 4)) = held[set][j];
     }
   };
   auto next = [&](char* p) { return p + C::STAGE == ring_end ? ring : p + C::STAGE; };
   char* slot = ring;      // of the slice that is read
   char* refill = ring;    // the slot that the next copies go to
-  if constexpr (ALIGNED) {
+  constexpr std::integral_constant<int, 0> kEven{};
+  constexpr std::integral_constant<int, AHEAD - 1> kOdd{};
+  if constexpr (COPIES) {
 #pragma unroll
     for (int i = 0; i < C::R; ++i) issue(i, ring + i * C::STAGE);
   } else {
-    load(0);
+    load(0, kEven);
+    if constexpr (AHEAD == 2) load(1, kOdd);
   }
 
   const int at = Frags<C>::lane_at(lane), lrow = lane % C::MB, lchunk = lane / C::MB;
@@ -300,25 +317,25 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
   // in flight: R - 1 slices behind the first, then R - 2, as the next copies come
   // after this), and every wavefront has read slice i - 1, whose slot the next
   // copies fill.
-  auto arrive = [&](auto first) {
-    if constexpr (ALIGNED)
+  auto arrive = [&](auto first, auto set) {
+    if constexpr (COPIES)
       wait_vm<(C::R - (decltype(first)::value || C::R == 1 ? 1 : 2)) * C::L>();
     else
-      put(slot);
+      put(slot, set);
     lds_barrier();
   };
   constexpr std::true_type kFirst{};
   constexpr std::false_type kLater{};
-  auto advance = [&](int i) {  // the copies that follow arrive() of slice i
-    if constexpr (ALIGNED && C::R > 1) {
+  auto advance = [&](int i, auto set) {  // the copies that follow arrive() of slice i
+    if constexpr (!COPIES) {
+      load(i + AHEAD, set);
+    } else if constexpr (C::R > 1) {
       issue(i + C::R - 1, refill);
       refill = next(refill);
-    } else if (!ALIGNED && i + 1 < iters) {
-      load(i + 1);
     }
   };
   auto reload = [&](int i) {  // R == 1: the next slice over this one
-    if constexpr (ALIGNED && C::R == 1) {
+    if constexpr (COPIES && C::R == 1) {
       lds_barrier();
       issue(i, ring);
     }
@@ -344,33 +361,55 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     }
     slot = next(slot);
   };
-  if (even > 0) {
-    arrive(kFirst);
+  auto step = [&](int i, auto set) {
+    most();
+    reload(i);
+    arrive(kLater, set);
     f0.read(slot, 0, at, wm, wn);
-    if constexpr (!ALIGNED) advance(0);
-    for (int i = 1; i < even; ++i) {
-      most();
-      reload(i);
-      arrive(kLater);
-      f0.read(slot, 0, at, wm, wn);
-      advance(i);
-      f1.mul(acc);
-      interleave<RD, MF>();
+    advance(i, set);
+    f1.mul(acc);
+    interleave<RD, MF>();
+  };
+  if (even > 0) {
+    arrive(kFirst, kEven);
+    f0.read(slot, 0, at, wm, wn);
+    if constexpr (!COPIES) advance(0, kEven);
+    if constexpr (AHEAD == 1) {
+      for (int i = 1; i < even; ++i) step(i, kEven);
+    } else {
+      int i = 1;
+      for (; i + 1 < even; i += 2) {
+        step(i, kOdd);
+        step(i + 1, kEven);
+      }
+      if (i < even) step(i, kOdd);
     }
+    if constexpr (FEED == kCopies4) load(even, kEven);
     most();
     if (C::R == 1 && iters > even) reload(even);
     f1.mul(acc);
+  } else if constexpr (FEED == kCopies4) {
+    load(0, kEven);
   }
   if (iters > even) {
-    if (even > 0)
-      arrive(kLater);
+    if constexpr (FEED == kCopies4) {
+      // A copy from nowhere still writes its slot (zeros): every wavefront's have
+      // landed before any puts what belongs there.
+      wait_vm<0>();
+      lds_barrier();
+      if (even * C::KS + grp == full) put(slot, kEven);
+    }
+    if (even == 0)
+      arrive(kFirst, kEven);
+    else if (AHEAD == 1 || even % 2 == 0)
+      arrive(kLater, kEven);
     else
-      arrive(kFirst);
+      arrive(kLater, kOdd);
     const int s = even * C::KS + grp, left = min(kSlice, K - s * kSlice);
     for (int j = 0; j * C::KB < left; ++j) {
       f0.read(slot, j, at, wm, wn);
       // past K: the next row's bytes in both operands, cleared in one
-      if (ALIGNED && j * C::KB + lchunk * kChunk >= left)
+      if (FEED == kCopies && j * C::KB + lchunk * kChunk >= left)
 #pragma unroll
         for (int f = 0; f < C::FM; ++f) f0.a[f] = i32x4{0, 0, 0, 0};
       f0.mul(acc);
@@ -384,7 +423,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     vsb[tid] = hsb;
     vbias[tid] = (float)hbias;
   }
-  if constexpr (ALIGNED) wait_vm<0>();  // copies from nowhere are still copies
+  if constexpr (COPIES) wait_vm<0>();  // copies from nowhere are still copies
   lds_barrier();                        // the ring is free
 
   if constexpr (C::KS == 1) {
@@ -487,7 +526,7 @@ dim3 grid2(int64_t n) {
 }
 
 // Dynamic LDS above 64 KB has to be allowed once a device.
-template <class C, bool ALIGNED, bool GELU>
+template <class C, int FEED, bool GELU>
 hipError_t allow_lds() {
   static std::atomic<uint64_t> done{0};
   if (C::LDS <= 64 * 1024) return hipSuccess;
@@ -496,28 +535,28 @@ hipError_t allow_lds() {
   if (e != hipSuccess) return e;
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
-  e = hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_kernel<C, ALIGNED, GELU>),
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_i8_kernel<C, FEED, GELU>),
                           hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
   if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
 
-template <class C, bool ALIGNED, bool GELU>
+template <class C, int FEED, bool GELU>
 hipError_t launch(const Args& g, hipStream_t s) {
-  const hipError_t e = allow_lds<C, ALIGNED, GELU>();
+  const hipError_t e = allow_lds<C, FEED, GELU>();
   if (e != hipSuccess) return e;
   const int tm = (g.M - 1) / C::BM + 1, tn = (g.N - 1) / C::BN + 1;
   const int64_t items = (int64_t)tm * tn;
   if (items > INT32_MAX / 2) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((gemm_i8_kernel<C, ALIGNED, GELU>),
+  hipLaunchKernelGGL((gemm_i8_kernel<C, FEED, GELU>),
                      grid2((items + kXcds - 1) / kXcds * kXcds), dim3(C::THREADS), C::LDS, s, g, tm,
                      tn);
   return hipGetLastError();
 }
 
-template <class C, bool ALIGNED>
+template <class C, int FEED>
 hipError_t run(const Args& g, bool gelu, hipStream_t s) {
-  return gelu ? launch<C, ALIGNED, true>(g, s) : launch<C, ALIGNED, false>(g, s);
+  return gelu ? launch<C, FEED, true>(g, s) : launch<C, FEED, false>(g, s);
 }
 
 // The tiles, and what one costs a CU in cycles: a byte of K costs the larger of
@@ -536,24 +575,28 @@ constexpr Tile kTiles[] = {{256, 256, 20.5f, 9500.f}, {256, 128, 14.5f, 4000.f},
                            {32, 64, 1.2f, 600.f},     {32, 32, 0.7f, 900.f},
                            {16, 32, 0.5f, 1500.f},    {16, 16, 0.3f, 120.f}};
 constexpr int kCus = kXcds * kXcdCus;
-// Tiles that unaligned operands take: the copies of the others would need more
-// registers than their wavefronts have.
-constexpr uint32_t kUnaligned = 1u << 2 | 1u << 3 | 1u << 5 | 1u << 6 | 1u << 9;
+// Tiles of operands that are staged, and of those that are copied but for the
+// last part of K.  (The staged chunks of the others would need more registers
+// than their wavefronts have.)
+constexpr uint32_t kStagedTiles = 1u << 2 | 1u << 3 | 1u << 5 | 1u << 6 | 1u << 9;
+constexpr uint32_t kCopies4Tiles = 1u << 0 | kStagedTiles;
 
 int64_t rounds_of(const Tile& t, int M, int N) {
   const int64_t n = (int64_t)((M - 1) / t.bm + 1) * ((N - 1) / t.bn + 1);
   return (n + kCus - 1) / kCus;
 }
 
-int pick_tile(int M, int N, int K, uint32_t allowed) {
+// all_rows: rows past M and N cost what the others do (staged chunks; copies of
+// them read nothing).
+int pick_tile(int M, int N, int K, uint32_t allowed, bool all_rows) {
   int best = -1;
   float least = 0.f;
   for (int i = 0; i < (int)(sizeof kTiles / sizeof kTiles[0]); ++i) {
     if (!(allowed >> i & 1)) continue;
     const Tile& t = kTiles[i];
     const int64_t rounds = rounds_of(t, M, N);
-    const float copies = (float)((M < t.bm ? M : t.bm) + (N < t.bn ? N : t.bn)) /
-                         (t.bn == 16 && rounds > 2 ? 44.f : 32.f);
+    const int rows = all_rows || M > t.bm ? t.bm : M, cols = all_rows || N > t.bn ? t.bn : N;
+    const float copies = (float)(rows + cols) / (t.bn == 16 && rounds > 2 ? 44.f : 32.f);
     const float cost = (float)rounds * ((float)K * (copies > t.mfma ? copies : t.mfma) + t.fixed);
     if (best < 0 || cost < least) {
       least = cost;
@@ -568,62 +611,86 @@ int pick_tile(int M, int N, int K, uint32_t allowed) {
 hipError_t gemm_i8(const int8_t* A, const float* sa, const int8_t* B, const float* sb,
                    const f16* bias, f16* C, int M, int N, int K, bool gelu, hipStream_t s) {
   const Args g{A, B, sa, sb, bias, C, M, N, K};
-  const bool aligned = K % kChunk == 0 && (((uintptr_t)A | (uintptr_t)B) & 15) == 0;
-  const int t = pick_tile(M, N, K, aligned ? ~0u : kUnaligned);
+  const uintptr_t at = (uintptr_t)A | (uintptr_t)B | (uintptr_t)K;
+  const Feed feed = at % 16 == 0 ? kCopies : at % 4 == 0 ? kCopies4 : kStaged;
+  const uint32_t allowed = feed == kCopies    ? ~0u
+                           : feed == kCopies4 ? kCopies4Tiles
+                                              : kStagedTiles;
+  const int t = pick_tile(M, N, K, allowed, feed == kStaged);
   // One round, a workgroup a CU, and a long K: nothing but its own copies hides
   // a workgroup's waits, so it has more of them in flight (or more groups).
   const int64_t rounds = rounds_of(kTiles[t], M, N);
   const bool alone = rounds == 1 && K >= 1024;
+  // Tiles of 16 x 16 by one wavefront a workgroup: where K is short (16 x 1536 x
+  // 384 2.7 us against 3.1) or there are many, not too long each (8 x 33206 x 2704
+  // 17.0 against 19.7, but 1 x 32000 x 4096 31.5 against 27.6).
+  const bool one_wave = K <= 512 || (rounds >= 8 && K < 4096);
+  if (feed == kCopies4) {
+    switch (t) {
+      case 0: return run<Cfg<256, 256, 2, 4, 1, 2>, kCopies4>(g, gelu, s);
+      case 2:
+        return alone ? run<Cfg<128, 128, 2, 4, 1, 3>, kCopies4>(g, gelu, s)
+                     : run<Cfg<128, 128, 2, 4, 1, 2>, kCopies4>(g, gelu, s);
+      case 3: return run<Cfg<64, 128, 2, 2, 1, 3>, kCopies4>(g, gelu, s);
+      case 5: return run<Cfg<64, 64, 2, 2, 1, 2>, kCopies4>(g, gelu, s);
+      case 6: return run<Cfg<32, 64, 1, 2, 2, 3>, kCopies4>(g, gelu, s);
+      default:
+        return one_wave ? run<Cfg<16, 16, 1, 1, 1, 2>, kCopies4>(g, gelu, s)
+                        : run<Cfg<16, 16, 1, 1, 4, 4>, kCopies4>(g, gelu, s);
+    }
+  }
+  if (feed == kStaged) {
+    switch (t) {
+      case 2:
+        return alone ? run<Cfg<128, 128, 2, 4, 1, 2>, kStaged2>(g, gelu, s)
+                     : run<Cfg<128, 128, 2, 4, 1, 2>, kStaged>(g, gelu, s);
+      case 3: return run<Cfg<64, 128, 2, 4, 1, 2>, kStaged>(g, gelu, s);
+      case 5: return run<Cfg<64, 64, 2, 2, 1, 2>, kStaged>(g, gelu, s);
+      case 6:
+        return alone ? run<Cfg<32, 64, 1, 2, 4, 2>, kStaged2>(g, gelu, s)
+                     : run<Cfg<32, 64, 1, 2, 4, 2>, kStaged>(g, gelu, s);
+      default:
+        return alone      ? run<Cfg<16, 16, 1, 1, 8, 2>, kStaged2>(g, gelu, s)
+               : one_wave ? run<Cfg<16, 16, 1, 1, 1, 2>, kStaged>(g, gelu, s)
+                          : run<Cfg<16, 16, 1, 1, 4, 2>, kStaged>(g, gelu, s);
+    }
+  }
   // Several rounds of a short K: a ring of one slice, so that twice the
   // workgroups share a CU and hide each other's copies and epilogues.
   const bool shortk = rounds > 1 && K <= 512;
-  if (!aligned) {
-    switch (t) {
-      case 2: return run<Cfg<128, 128, 2, 4, 1, 2>, false>(g, gelu, s);
-      case 3: return run<Cfg<64, 128, 2, 4, 1, 2>, false>(g, gelu, s);
-      case 5: return run<Cfg<64, 64, 2, 2, 1, 2>, false>(g, gelu, s);
-      case 6: return run<Cfg<32, 64, 1, 2, 4, 2>, false>(g, gelu, s);
-      default:
-        return alone ? run<Cfg<16, 16, 1, 1, 8, 2>, false>(g, gelu, s)
-                     : run<Cfg<16, 16, 1, 1, 4, 2>, false>(g, gelu, s);
-    }
-  }
   switch (t) {
-    case 0: return run<Cfg<256, 256, 2, 4, 1, 2>, true>(g, gelu, s);
-    case 1: return run<Cfg<256, 128, 4, 2, 1, 3>, true>(g, gelu, s);
+    case 0: return run<Cfg<256, 256, 2, 4, 1, 2>, kCopies>(g, gelu, s);
+    case 1: return run<Cfg<256, 128, 4, 2, 1, 3>, kCopies>(g, gelu, s);
     case 2:
-      return alone ? run<Cfg<128, 128, 2, 4, 1, 3>, true>(g, gelu, s)
-             : shortk ? run<Cfg<128, 128, 2, 4, 1, 1>, true>(g, gelu, s)
-                      : run<Cfg<128, 128, 2, 4, 1, 2>, true>(g, gelu, s);
+      return alone ? run<Cfg<128, 128, 2, 4, 1, 3>, kCopies>(g, gelu, s)
+             : shortk ? run<Cfg<128, 128, 2, 4, 1, 1>, kCopies>(g, gelu, s)
+                      : run<Cfg<128, 128, 2, 4, 1, 2>, kCopies>(g, gelu, s);
     case 3:
-      return alone ? run<Cfg<64, 128, 2, 2, 1, 3>, true>(g, gelu, s)
-             : shortk ? run<Cfg<64, 128, 1, 4, 1, 1>, true>(g, gelu, s)
-                      : run<Cfg<64, 128, 1, 4, 1, 2>, true>(g, gelu, s);
+      return alone ? run<Cfg<64, 128, 2, 2, 1, 3>, kCopies>(g, gelu, s)
+             : shortk ? run<Cfg<64, 128, 1, 4, 1, 1>, kCopies>(g, gelu, s)
+                      : run<Cfg<64, 128, 1, 4, 1, 2>, kCopies>(g, gelu, s);
     case 4:
-      return alone ? run<Cfg<128, 64, 2, 2, 1, 3>, true>(g, gelu, s)
-             : shortk ? run<Cfg<128, 64, 2, 2, 1, 1>, true>(g, gelu, s)
-                      : run<Cfg<128, 64, 2, 2, 1, 2>, true>(g, gelu, s);
+      return alone ? run<Cfg<128, 64, 2, 2, 1, 3>, kCopies>(g, gelu, s)
+             : shortk ? run<Cfg<128, 64, 2, 2, 1, 1>, kCopies>(g, gelu, s)
+                      : run<Cfg<128, 64, 2, 2, 1, 2>, kCopies>(g, gelu, s);
     case 5:
-      return alone ? run<Cfg<64, 64, 2, 2, 2, 3>, true>(g, gelu, s)
-             : shortk ? run<Cfg<64, 64, 2, 2, 1, 1>, true>(g, gelu, s)
-             : rounds == 2 && K >= 1024 ? run<Cfg<64, 64, 2, 2, 1, 3>, true>(g, gelu, s)
-                                        : run<Cfg<64, 64, 2, 2, 1, 2>, true>(g, gelu, s);
+      return alone ? run<Cfg<64, 64, 2, 2, 2, 3>, kCopies>(g, gelu, s)
+             : shortk ? run<Cfg<64, 64, 2, 2, 1, 1>, kCopies>(g, gelu, s)
+             : rounds == 2 && K >= 1024 ? run<Cfg<64, 64, 2, 2, 1, 3>, kCopies>(g, gelu, s)
+                                        : run<Cfg<64, 64, 2, 2, 1, 2>, kCopies>(g, gelu, s);
     case 6:
-      return shortk       ? run<Cfg<32, 64, 1, 2, 1, 1>, true>(g, gelu, s)
-             : rounds > 2 ? run<Cfg<32, 64, 1, 2, 1, 2>, true>(g, gelu, s)
-                          : run<Cfg<32, 64, 1, 2, 2, 3>, true>(g, gelu, s);
+      return shortk       ? run<Cfg<32, 64, 1, 2, 1, 1>, kCopies>(g, gelu, s)
+             : rounds > 2 ? run<Cfg<32, 64, 1, 2, 1, 2>, kCopies>(g, gelu, s)
+                          : run<Cfg<32, 64, 1, 2, 2, 3>, kCopies>(g, gelu, s);
     case 7:
-      return alone                   ? run<Cfg<32, 32, 1, 1, 4, 4>, true>(g, gelu, s)
-             : K <= 512 || rounds > 2 ? run<Cfg<32, 32, 1, 1, 1, 2>, true>(g, gelu, s)
-                                      : run<Cfg<32, 32, 1, 1, 4, 2>, true>(g, gelu, s);
-    case 8: return run<Cfg<16, 32, 1, 1, 4, 4>, true>(g, gelu, s);
+      return alone                   ? run<Cfg<32, 32, 1, 1, 4, 4>, kCopies>(g, gelu, s)
+             : K <= 512 || rounds > 2 ? run<Cfg<32, 32, 1, 1, 1, 2>, kCopies>(g, gelu, s)
+                                      : run<Cfg<32, 32, 1, 1, 4, 2>, kCopies>(g, gelu, s);
+    case 8: return run<Cfg<16, 32, 1, 1, 4, 4>, kCopies>(g, gelu, s);
     default:
-      // one wavefront a workgroup where K is short (16 x 1536 x 384 2.7 us
-      // against 3.1) or there are many (8 x 33206 x 2704 17.0 against 19.7), not
-      // too long each (1 x 32000 x 4096 31.5 against 27.6)
-      return K <= 512 || (rounds >= 8 && K < 4096) ? run<Cfg<16, 16, 1, 1, 1, 2>, true>(g, gelu, s)
-             : K <= 1536 ? run<Cfg<16, 16, 1, 1, 2, 2>, true>(g, gelu, s)
-                         : run<Cfg<16, 16, 1, 1, 4, 4>, true>(g, gelu, s);
+      return one_wave    ? run<Cfg<16, 16, 1, 1, 1, 2>, kCopies>(g, gelu, s)
+             : K <= 1536 ? run<Cfg<16, 16, 1, 1, 2, 2>, kCopies>(g, gelu, s)
+                         : run<Cfg<16, 16, 1, 1, 4, 4>, kCopies>(g, gelu, s);
   }
 }
 

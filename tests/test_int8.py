@@ -385,7 +385,11 @@ LINEAR = [(1, 1, 1), (1, 1, 16), (1, 3, 5), (1, 64, 128), (1, 1000, 4096), (1, 4
           (128, 128, 128), (129, 257, 255), (200, 4096, 512), (256, 256, 256), (257, 1111, 777),
           (300, 1152, 384), (513, 130, 1040), (600, 2048, 96), (1000, 999, 1001), (2003, 1152, 384),
           (1, 7, 131071), (40, 70, 131071), (130, 200, 100000), (3000, 20, 384), (20, 9000, 64),
-          (4096, 1536, 384), (2048, 2048, 1024), (2500, 2700, 528), (4100, 4100, 260)]
+          (4096, 1536, 384), (2048, 2048, 1024), (2500, 2700, 528), (4100, 4100, 260),
+          # K a multiple of 4 only: whole slices copied, the last part staged
+          (1, 64, 4), (7, 130, 132), (16, 900, 300), (40, 1000, 1100), (64, 2000, 1004), (100, 3000, 500),
+          (200, 1025, 2052), (300, 4000, 1300), (1000, 999, 300), (1030, 2050, 1412), (3000, 5000, 772),
+          (5000, 700, 100)]
 
 
 @gpu
@@ -404,21 +408,23 @@ def test_linear_i8(torch_cuda, M, N, K):
 
 @gpu
 @pytest.mark.parametrize("M,N,K", [(1, 100, 256), (3, 64, 1024), (20, 96, 256), (70, 200, 400),
-                                   (300, 520, 384), (2100, 1100, 512), (3000, 3000, 256)])
+                                   (300, 520, 384), (2100, 1100, 512), (3000, 3000, 256), (90, 700, 2052)])
 def test_linear_i8_same_bits_at_odd_addresses_and_any_rows(torch_cuda, M, N, K):
-    """Operands one byte off, an output two bytes off, and every row alone: the
-    same bits, whichever kernel computes them."""
+    """Operands one, two and four bytes off, an output two bytes off, and some rows
+    alone: the same bits, whichever kernel computes them."""
     from bbh import engine
 
     torch = torch_cuda
     A, sa, B, sb, bias = _operands(torch, 5, M, N, K)
     C = torch.empty(M, N, dtype=torch.float16, device="cuda")
     engine.launch_matmul_i8(A, sa, B, sb, C, M, N, K, bias=bias, gelu=True)
-    A1, _, B1, _, _ = _operands(torch, 6, M, N, K, off=1)
-    A1.copy_(A), B1.copy_(B)
-    buf, C1 = _guarded(torch, M * N, torch.float16, 3.0, off=1)
-    engine.launch_matmul_i8(A1, sa, B1, sb, C1, M, N, K, bias=bias, gelu=True)
-    assert torch.equal(C1.view(M, N), C) and float(buf[0]) == 3 and bool((buf[1 + M * N:] == 3).all())
+    for off in (1, 2, 4):
+        A1, _, B1, _, _ = _operands(torch, 6, M, N, K, off=off)
+        A1.copy_(A), B1.copy_(B)
+        buf, C1 = _guarded(torch, M * N, torch.float16, 3.0, off=1)
+        engine.launch_matmul_i8(A1, sa, B1, sb, C1, M, N, K, bias=bias, gelu=True)
+        assert torch.equal(C1.view(M, N), C)
+        assert float(buf[0]) == 3 and bool((buf[1 + M * N:] == 3).all())
     for a, b in ((0, 1), (M // 2, M // 2 + 2), (max(0, M - 40), M)):
         b = min(b, M)
         Cr = torch.empty(b - a, N, dtype=torch.float16, device="cuda")
