@@ -8,6 +8,8 @@ and 12 levels of a tree: relative error <= 45 u where no term is negative."""
 import ctypes
 import os
 import re
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -598,6 +600,61 @@ def test_captured_and_replayed_beside_eager_work_on_two_streams(torch_cuda):
         a["x"].mul_(2)
         _ffn(torch, engine, a)
         a["x"].copy_(x)
+
+
+@gpu
+def test_through_the_cpp_layer(torch_cuda, tmp_path):
+    """cpp/int8_check: the operators through bert_by_hand_int8.hpp."""
+    prog = os.path.join(ROOT, "bert-by-hand_amd", "cpp", "int8_check")
+    if not os.path.exists(prog):
+        pytest.fail(f"{prog} is not built (run __graft_entry__.build())")
+    r = subprocess.run([prog], cwd=str(tmp_path), capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout.count(" PASS") == 5, r.stdout + r.stderr
+
+
+@gpu
+def test_captured_before_any_eager_call(torch_cuda):
+    """A launch may be the first of its kernel: nothing of its set-up is refused
+    while a stream is captured (a fresh process, so that no earlier test made
+    one)."""
+    code = """
+import sys; sys.path.insert(0, %r)
+import torch
+from bbh import engine
+M, N, K = 1024, 2048, 512
+A = torch.randint(-128, 128, (M, K), dtype=torch.int8, device="cuda")
+B = torch.randint(-128, 128, (N, K), dtype=torch.int8, device="cuda")
+s = torch.rand(N, device="cuda")
+C = torch.zeros(M, N, dtype=torch.float16, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    engine.launch_matmul_i8(A, s, B, s, C, M, N, K)
+g.replay()
+torch.cuda.synchronize()
+D = torch.empty_like(C)
+engine.launch_matmul_i8(A, s, B, s, D, M, N, K)
+assert bool(C.any()) and torch.equal(C, D)
+print("SAME")
+""" % os.path.join(ROOT, "bert-by-hand_amd")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "SAME" in r.stdout, r.stdout + r.stderr
+
+
+@gpu
+def test_norm_of_zeros_without_eps(torch_cuda):
+    """eps 0 is the formula's: 0 / 0 in a row of zeros, and no other row's matter."""
+    from bbh import engine
+
+    torch = torch_cuda
+    x = _half(torch, _gen(torch, 4), 3, 200)
+    x[1] = 0
+    g = torch.ones(200, device="cuda").half()
+    q = torch.empty(3, 200, dtype=torch.int8, device="cuda")
+    s = torch.empty(3, device="cuda")
+    engine.launch_rmsnorm_quantize(x, g, q, s, 3, 200, eps=0.0)
+    assert bool(torch.isnan(s[1])) and bool((q[1] == 0).all())
+    keep = torch.tensor([0, 2], device="cuda")
+    _check_norm(torch, "rmsnorm", x[keep], None, g, None, 0.0, q[keep], s[keep], None, None)
 
 
 @gpu
