@@ -53,23 +53,33 @@ __device__ __forceinline__ float row_reduce(float v, F f, float* part) {
   return v;
 }
 
-// Chunk `c` of a row of D halves; zeros past the row's end.
+// Chunk `c` of a row of D halves; zeros past the row's end.  STREAM: past the
+// caches' reach (streams(), below).
+template <bool STREAM = false>
 __device__ __forceinline__ f16x8 load8(const f16* row, int c, int D) {
   const int o = c * 8;
-  if (o + 8 <= D) return *reinterpret_cast<const f16x8_any*>(row + o);
+  if (o + 8 <= D) {
+    const f16x8_any* p = reinterpret_cast<const f16x8_any*>(row + o);
+    return STREAM ? __builtin_nontemporal_load(p) : *p;
+  }
   f16x8 a;
 #pragma unroll
   for (int e = 0; e < 8; ++e) a[e] = o + e < D ? row[o + e] : (f16)0.f;
   return a;
 }
 
+template <bool STREAM>
 __device__ __forceinline__ void store8(f16* row, int c, int D, const float (&v)[8]) {
   const int o = c * 8;
   if (o + 8 <= D) {
     f16x8 a;
 #pragma unroll
     for (int e = 0; e < 8; ++e) a[e] = (f16)v[e];
-    *reinterpret_cast<f16x8_any*>(row + o) = a;
+    f16x8_any* p = reinterpret_cast<f16x8_any*>(row + o);
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(a, p);
+    else
+      *p = a;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -133,7 +143,7 @@ struct NormArgs {
 
 // x and the outputs may be the same rows, so none is __restrict__; every
 // thread writes only the elements it has read.
-template <int T, int V, Kind KIND>
+template <int T, int V, Kind KIND, bool STREAM>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_kernel(const f16* x, int8_t* q,
                                                                      float* scale, int M, int D,
                                                                      NormArgs a) {
@@ -150,13 +160,13 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_kernel(const f16* 
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     hx[i] = f16x8{};
-    if (t + T * i < chunks) hx[i] = load8(x + off, t + T * i, D);
+    if (t + T * i < chunks) hx[i] = load8<STREAM>(x + off, t + T * i, D);
   }
   if constexpr (KIND != kPlain) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       hr[i] = f16x8{};
-      if (a.residual && t + T * i < chunks) hr[i] = load8(a.residual + off, t + T * i, D);
+      if (a.residual && t + T * i < chunks) hr[i] = load8<STREAM>(a.residual + off, t + T * i, D);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -179,7 +189,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_kernel(const f16* 
     if (a.sum) {
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (t + T * i < chunks) store8(a.sum + off, t + T * i, D, v[i]);
+        if (t + T * i < chunks) store8<STREAM>(a.sum + off, t + T * i, D, v[i]);
     }
     if constexpr (KIND == kLayer) {
       float s = 0.f;
@@ -207,7 +217,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_kernel(const f16* 
         v[i][e] = v[i][e] * rstd * (float)hg[i][e];
         if constexpr (KIND == kLayer) v[i][e] += (float)hb[i][e];
       }
-      if (a.y && t + T * i < chunks) store8(a.y + off, t + T * i, D, v[i]);
+      if (a.y && t + T * i < chunks) store8<STREAM>(a.y + off, t + T * i, D, v[i]);
     }
   }
   float m = 0.f;
@@ -254,7 +264,7 @@ __global__ __launch_bounds__(kWide) void quantize_wide_kernel(const f16* __restr
 }
 
 // T threads a row, eight codes at a time.
-template <int T>
+template <int T, bool STREAM>
 __global__ __launch_bounds__(256) void dequantize_kernel(const int8_t* __restrict__ q,
                                                          const float* __restrict__ scale,
                                                          f16* __restrict__ x, int M, int D) {
@@ -273,7 +283,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const int8_t* __restric
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = o + e < D ? (float)q[off + o + e] * s : 0.f;
     }
-    store8(x + off, c, D, v);
+    store8<STREAM>(x + off, c, D, v);
   }
 }
 
@@ -283,25 +293,25 @@ dim3 grid2(int64_t n) {
   return n <= X ? dim3((uint32_t)n) : dim3((uint32_t)X, (uint32_t)((n + X - 1) / X));
 }
 
-template <int T>
+template <int T, bool STREAM>
 hipError_t dequantize(const int8_t* q, const float* scale, f16* x, int M, int D, hipStream_t s) {
   constexpr int R = 256 / T;
-  hipLaunchKernelGGL(dequantize_kernel<T>, grid2(((int64_t)M + R - 1) / R), dim3(256), 0, s, q,
+  hipLaunchKernelGGL((dequantize_kernel<T, STREAM>), grid2(((int64_t)M + R - 1) / R), dim3(256), 0, s, q,
                      scale, x, M, D);
   return hipGetLastError();
 }
 
-template <int T, int V, Kind KIND>
+template <int T, int V, Kind KIND, bool STREAM>
 hipError_t launch(const f16* x, int8_t* q, float* scale, int M, int D, const NormArgs& a,
                   hipStream_t s) {
   constexpr int R = T < 256 ? 256 / T : 1;
-  hipLaunchKernelGGL((quantize_kernel<T, V, KIND>), grid2(((int64_t)M + R - 1) / R),
+  hipLaunchKernelGGL((quantize_kernel<T, V, KIND, STREAM>), grid2(((int64_t)M + R - 1) / R),
                      dim3(T < 256 ? 256 : T), 0, s, x, q, scale, M, D, a);
   return hipGetLastError();
 }
 
-template <Kind KIND>
-hipError_t quantize(const f16* x, int8_t* q, float* scale, int M, int D, const NormArgs& a,
+template <Kind KIND, bool STREAM>
+hipError_t quantize_as(const f16* x, int8_t* q, float* scale, int M, int D, const NormArgs& a,
                     hipStream_t s) {
   // Threads a row: as few as leave a thread at most four chunks, so that the
   // lanes are full and the reductions short; more where rows are too few to fill
@@ -316,18 +326,46 @@ hipError_t quantize(const f16* x, int8_t* q, float* scale, int M, int D, const N
   //   1 x 8192       256 x 4      3.1 /  4.8   1024 x 1     2.7 /  4.0
   const int chunks = (D + 7) / 8;
   const bool many = M >= 4096;
-  if (chunks <= 16) return launch<16, 1, KIND>(x, q, scale, M, D, a, s);
-  if (chunks <= 32 && many) return launch<16, 2, KIND>(x, q, scale, M, D, a, s);
-  if (chunks <= 48 && many) return launch<16, 3, KIND>(x, q, scale, M, D, a, s);
-  if (chunks <= 64) return launch<64, 1, KIND>(x, q, scale, M, D, a, s);
-  if (chunks <= 128) return launch<64, 2, KIND>(x, q, scale, M, D, a, s);
-  if (chunks <= 192) return launch<64, 3, KIND>(x, q, scale, M, D, a, s);
-  if (chunks <= 256) return launch<256, 1, KIND>(x, q, scale, M, D, a, s);
-  if (chunks <= 512) return launch<256, 2, KIND>(x, q, scale, M, D, a, s);
-  if (chunks <= 1024 && M <= 128) return launch<1024, 1, KIND>(x, q, scale, M, D, a, s);
-  if (chunks <= 768) return launch<256, 3, KIND>(x, q, scale, M, D, a, s);
-  if (chunks <= 1024) return launch<256, 4, KIND>(x, q, scale, M, D, a, s);
-  return launch<1024, 2, KIND>(x, q, scale, M, D, a, s);
+  if (chunks <= 16) return launch<16, 1, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if (chunks <= 32 && many) return launch<16, 2, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if (chunks <= 48 && many) return launch<16, 3, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if (chunks <= 64) return launch<64, 1, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if (chunks <= 128) return launch<64, 2, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if (chunks <= 192) return launch<64, 3, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if (chunks <= 256) return launch<256, 1, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if (chunks <= 512) return launch<256, 2, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if (chunks <= 1024 && M <= 128) return launch<1024, 1, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if (chunks <= 768) return launch<256, 3, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if (chunks <= 1024) return launch<256, 4, KIND, STREAM>(x, q, scale, M, D, a, s);
+  return launch<1024, 2, KIND, STREAM>(x, q, scale, M, D, a, s);
+}
+
+// fp16 rows of this many bytes and more are read and written past the caches
+// (non-temporal): they would push out of the memory-side cache what the next
+// operators find there, the codes among it, and be gone themselves before anyone
+// came back to them.  Quantising and reading back 131072 x 384 (96 MB) 55.2 us
+// without, 50.0 with; LayerNorm with residual and y, read back, and the values
+// quantised again, where the reader right behind finds less: 115 and 104; the
+// first of 43690 x 384 (32 MB) 19.8 and 20.8.  Values read back stay in the
+// caches up to twice the size.
+constexpr int64_t kStreamBytes = 48 << 20;
+bool streams(int M, int D, int64_t bytes) { return (int64_t)M * D * 2 >= bytes; }
+
+template <Kind KIND>
+hipError_t quantize(const f16* x, int8_t* q, float* scale, int M, int D, const NormArgs& a,
+                    hipStream_t s) {
+  return streams(M, D, kStreamBytes) ? quantize_as<KIND, true>(x, q, scale, M, D, a, s)
+                                     : quantize_as<KIND, false>(x, q, scale, M, D, a, s);
+}
+
+template <bool STREAM>
+hipError_t dequantize_as(const int8_t* q, const float* scale, f16* x, int M, int D,
+                         hipStream_t s) {
+  // 131072 x 256 19.2 us with 16 threads a row, 25.9 with 64; 65536 x 1024 39.1
+  // and 35.8; 16384 x 4096 41.2 with 64, 35.9 with 256
+  if (D <= 256) return dequantize<16, STREAM>(q, scale, x, M, D, s);
+  if (D <= 1024) return dequantize<64, STREAM>(q, scale, x, M, D, s);
+  return dequantize<256, STREAM>(q, scale, x, M, D, s);
 }
 
 }  // namespace
@@ -340,11 +378,8 @@ hipError_t quantize_rows(const f16* x, int8_t* q, float* scale, int M, int D, hi
 
 hipError_t dequantize_rows(const int8_t* q, const float* scale, f16* x, int M, int D,
                            hipStream_t s) {
-  // 131072 x 256 19.2 us with 16 threads a row, 25.9 with 64; 65536 x 1024 39.1
-  // and 35.8; 16384 x 4096 41.2 with 64, 35.9 with 256
-  if (D <= 256) return dequantize<16>(q, scale, x, M, D, s);
-  if (D <= 1024) return dequantize<64>(q, scale, x, M, D, s);
-  return dequantize<256>(q, scale, x, M, D, s);
+  return streams(M, D, 2 * kStreamBytes) ? dequantize_as<true>(q, scale, x, M, D, s)
+                                         : dequantize_as<false>(q, scale, x, M, D, s);
 }
 
 hipError_t rmsnorm_quantize(const f16* x, const f16* residual, const f16* gamma, f16* sum, f16* y,

@@ -280,6 +280,36 @@ def test_norms_against_64_bits(torch_cuda, kind, D):
 
 
 @gpu
+@pytest.mark.parametrize("M,D", [(131072, 384), (70001, 385), (200003, 129), (27001, 1000),
+                                 (3333, 16384), (9001, 8191)])
+def test_rows_read_and_written_past_the_caches(torch_cuda, M, D):
+    """From 48 MB of fp16 rows on the accesses are non-temporal (from 96 MB what is
+    read back, too): the same results, outputs over inputs among them."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, D)
+    x, r = _half(torch, g, M, D), _half(torch, g, M, D)
+    gamma, beta = _half(torch, g, D, scale=0.3) + 1, _half(torch, g, D, scale=0.1)
+    q = torch.empty(M, D, dtype=torch.int8, device="cuda")
+    s = torch.empty(M, device="cuda")
+    engine.launch_quantize_rows(x, q, s, M, D)
+    back = torch.empty_like(x)
+    engine.launch_dequantize_rows(q, s, back, M, D)
+    part = slice(0, M, 37)
+    c64, s64 = _codes64(torch, x[part].double())
+    assert torch.equal(q[part].double(), c64.round()) and torch.equal(s[part], s64.float())
+    assert torch.equal(back, (q.float() * s[:, None]).half())
+    for kind in ("rmsnorm", "layernorm"):
+        hx, hr = x.clone(), r.clone()
+        args = (hx, gamma) if kind == "rmsnorm" else (hx, gamma, beta)
+        getattr(engine, f"launch_{kind}_quantize")(*args, q, s, M, D, eps=1e-6, residual=hr, sum=hx,
+                                                   y=hr)
+        _check_norm(torch, kind, x[part], r[part], gamma, beta, 1e-6, q[part], s[part], hx[part],
+                    hr[part])
+
+
+@gpu
 @pytest.mark.parametrize("kind", ["rmsnorm", "layernorm"])
 @pytest.mark.parametrize("D", [40, 384, 1001, 4096, 16384])
 def test_norm_outputs_over_inputs_and_odd_addresses(torch_cuda, kind, D):
@@ -380,7 +410,7 @@ def _operands(torch, seed, M, N, K, off=0):
     return mk(M * K).view(M, K), sa, mk(N * K).view(N, K), sb, _half(torch, g, N)
 
 
-LINEAR = [(1, 1, 1), (1, 1, 16), (1, 3, 5), (1, 64, 128), (1, 1000, 4096), (1, 4097, 777), (2, 33, 48),
+LINEAR = [(1, 1, 1), (1, 1, 16), (5000, 1, 384), (1, 1, 131071), (3, 1, 131056), (1, 3, 5), (1, 64, 128), (1, 1000, 4096), (1, 4097, 777), (2, 33, 48),
           (3, 5, 17), (4, 384, 1536), (4, 1023, 1000), (5, 130, 384), (8, 257, 2048), (9, 16, 8192), (15, 65, 129), (16, 1536, 384),
           (17, 384, 1536), (31, 33, 144), (32, 32, 32), (33, 31, 112), (33, 700, 4112), (48, 1152, 384),
           (64, 1537, 384), (64, 64, 127), (65, 129, 128), (100, 100, 100), (127, 384, 2000),
