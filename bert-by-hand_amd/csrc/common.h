@@ -152,8 +152,7 @@ __device__ inline float gelu_erf(float v) {
 // 13 VALU operations (one med3, one mul, ten fma, one mul) where the rcp +
 // exp form costs the VALU time of ~25: the epilogue of the K = 384 GEMMs runs
 // on the same SIMD issue as their MFMAs.
-__device__ inline float gelu_poly(float x) {
-  const float u = __builtin_amdgcn_fmed3f(x, -4.5f, 4.5f);
+__device__ inline float gelu_phi(float u) {  // |u| <= 4.5
   const float t = u * u;
   float p = -1.726400164e-12f;
   p = fmaf(p, t, 2.022508966e-10f);
@@ -165,7 +164,19 @@ __device__ inline float gelu_poly(float x) {
   p = fmaf(p, t, 9.891781956e-03f);
   p = fmaf(p, t, -6.642068923e-02f);
   p = fmaf(p, t, 3.989246786e-01f);
-  return x * fmaf(u, p, 0.5f);
+  return fmaf(u, p, 0.5f);
+}
+__device__ inline float gelu_poly(float x) {
+  const float u = __builtin_amdgcn_fmed3f(x, -4.5f, 4.5f);
+  return x * gelu_phi(u);
+}
+// gelu_poly with tails of any length, for sums whose size nothing bounds: the
+// same bits to |x| = 4.5 and past it max(x - u, 0) more than at the clamp, so the
+// error stays below 7.6e-5 there (gelu_poly's grows as 6.8e-6 |x|: 0.44 at
+// -65504).  NaN stays NaN.  Two more operations.
+__device__ inline float gelu_wide(float x) {
+  const float u = __builtin_amdgcn_fmed3f(x, -4.5f, 4.5f);
+  return fmaf(u, gelu_phi(u), __builtin_elementwise_maximum(x - u, 0.f));
 }
 
 // LayerNorm of one 384-wide row held by a wavefront: lane l holds columns

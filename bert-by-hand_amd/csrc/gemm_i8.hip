@@ -45,7 +45,7 @@ struct Args {
 template <bool GELU>
 __device__ __forceinline__ f16 finish(int acc, float sa, float sb, float bias) {
   const float v = fmaf((float)acc * sa, sb, bias);
-  return to_half(GELU ? gelu_poly(v) : v);
+  return to_half(GELU ? gelu_wide(v) : v);
 }
 
 __device__ __forceinline__ int64_t block_id() {

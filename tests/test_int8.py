@@ -484,6 +484,45 @@ def test_linear_i8_largest_sums(torch_cuda, M):
 
 
 @gpu
+@pytest.mark.parametrize("M,N", [(17, 33), (300, 520)])
+def test_linear_i8_gelu_of_large_values(torch_cuda, M, N):
+    """GELU of values of any size: its absolute error past 4.5 does not grow with
+    them (7.6e-5, the stated bound of the polynomial to 6), on either side."""
+    from bbh import engine
+
+    torch = torch_cuda
+    A = (torch.arange(M * 2, device="cuda") % 255 - 127).to(torch.int8).view(M, 2)
+    B = torch.ones(N, 2, dtype=torch.int8, device="cuda")
+    sa = torch.ones(M, device="cuda")
+    sb = torch.logspace(-3, 2.4, N, device="cuda")  # to 64000
+    C = torch.empty(M, N, dtype=torch.float16, device="cuda")
+    engine.launch_matmul_i8(A, sa, B, sb, C, M, N, 2, gelu=True)
+    v = A.double().sum(1)[:, None] * sb.double()
+    want = _gelu64(torch, v)
+    # one rounding of the product (the sum of two codes is exact), a subtraction
+    # and an fma of |v| at most, fp16's
+    lim = want.abs() * H + (7.6e-5 + 3.13 * U * v.abs()) * (1 + H) + TINY
+    err = (C.double() - want).abs()
+    assert v.abs().max() > 60000 and bool((err <= lim).all()), float((err / lim).max())
+
+
+@gpu
+def test_linear_i8_gelu_of_non_finite_values(torch_cuda):
+    from bbh import engine
+
+    torch = torch_cuda
+    inf, nan = float("inf"), float("nan")
+    for N in (1, 40):
+        A = torch.tensor([[1], [-1], [5], [0]], dtype=torch.int8, device="cuda")
+        sa = torch.tensor([inf, inf, nan, inf], device="cuda")  # inf, -inf, NaN, 0 x inf
+        B = torch.ones(N, 1, dtype=torch.int8, device="cuda")
+        C = torch.empty(4, N, dtype=torch.float16, device="cuda")
+        engine.launch_matmul_i8(A, sa, B, torch.ones(N, device="cuda"), C, 4, N, 1, gelu=True)
+        assert bool((C[0] == inf).all()) and bool((C[1].abs() <= 7.6e-5 * (1 + H)).all())
+        assert bool(torch.isnan(C[2:]).all())
+
+
+@gpu
 def test_linear_i8_non_finite_and_zero_scales(torch_cuda):
     from bbh import engine
 
