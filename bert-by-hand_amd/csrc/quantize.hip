@@ -3,10 +3,13 @@
 //
 // A row's codes need its largest magnitude first, so the row stays in
 // registers between the reductions and its values are read once and written
-// once: bound by HBM (by the launch below a few hundred rows).  T threads own
-// a row, thread t the 8-wide chunks t, t + T, ..., V of them: 16-byte loads,
-// 8-byte stores of codes, any row length and alignment (the last chunk of a
-// row goes element by element).
+// once: bound by HBM, at 5.8-6.5 TB/s of those bytes from 100 MB of rows on
+// (65536 x 1536 quantised in 52 us and read back in 50; LayerNorm of 131072 x
+// 384 with residual and y 55, RMS norm of 16384 x 4096 73), and by a launch and
+// its first latency below a few hundred rows (2003 x 384: 2.8-3.6 us).  T
+// threads own a row, thread t the 8-wide chunks t, t + T, ..., V of them:
+// 16-byte loads, 8-byte stores of codes, any row length and alignment (the last
+// chunk of a row goes element by element).
 //
 // The largest magnitude is reduced on the bit patterns as unsigned integers:
 // they order like the magnitudes, an infinity above every number and a NaN
@@ -312,17 +315,19 @@ hipError_t launch(const f16* x, int8_t* q, float* scale, int M, int D, const Nor
 
 template <Kind KIND, bool STREAM>
 hipError_t quantize_as(const f16* x, int8_t* q, float* scale, int M, int D, const NormArgs& a,
-                    hipStream_t s) {
+                       hipStream_t s) {
   // Threads a row: as few as leave a thread at most four chunks, so that the
   // lanes are full and the reductions short; more where rows are too few to fill
   // the GPU and a thread's chunks would queue behind each other.  Measured, us
   // (quantise / LayerNorm with residual and y):
-  //   131072 x 32     16 threads  8.2 / 15.4   64 threads  27.0 / 52.3
-  //   131072 x 384    16 x 3     28.3 / 63.5   64 x 1      36.6 / 64.8
+  //   131072 x 32     16 threads  8.4 / 15.4   64 threads  27.5 / 52.1
+  //   131072 x 384    16 x 3     26.1 / 55.3   64 x 1      37.2 / 62.7
   //   2003 x 384      16 x 3      3.1 /  4.5   64 x 1       2.8 /  3.6
-  //   65536 x 1536    64 x 3     54.7 / 119    256 x 1     67.9 / 126
-  //   30000 x 2048    64 x 4     33.5 / 76.0   256 x 1     35.2 / 74.5
-  //   8192 x 8192    256 x 4     37.0 / 84.4   1024 x 1    43.5 / 96.7
+  //   65536 x 1536    64 x 3     52.2 / 112    256 x 1     66.2 / 128
+  //   65536 x 1792    64 x 4     60.3 / 134    256 x 1     73.4 / 141
+  //   5000 x 1700     64 x 4      8.8 / 17.5   256 x 1      8.2 / 16.9
+  //   700 x 2048      64 x 4      3.6 /  5.4   256 x 1      3.1 /  4.5
+  //   8192 x 8192    256 x 4     34.3 / 76.1   1024 x 1    43.2 / 93.2
   //   1 x 8192       256 x 4      3.1 /  4.8   1024 x 1     2.7 /  4.0
   const int chunks = (D + 7) / 8;
   const bool many = M >= 4096;
@@ -332,9 +337,14 @@ hipError_t quantize_as(const f16* x, int8_t* q, float* scale, int M, int D, cons
   if (chunks <= 64) return launch<64, 1, KIND, STREAM>(x, q, scale, M, D, a, s);
   if (chunks <= 128) return launch<64, 2, KIND, STREAM>(x, q, scale, M, D, a, s);
   if (chunks <= 192) return launch<64, 3, KIND, STREAM>(x, q, scale, M, D, a, s);
-  if (chunks <= 256) return launch<256, 1, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if constexpr (STREAM) {
+    if (chunks <= 256) return launch<64, 4, KIND, true>(x, q, scale, M, D, a, s);
+  } else {
+    if (chunks <= 256) return launch<256, 1, KIND, false>(x, q, scale, M, D, a, s);
+    if (chunks > 512 && chunks <= 1024 && M <= 128)
+      return launch<1024, 1, KIND, false>(x, q, scale, M, D, a, s);
+  }
   if (chunks <= 512) return launch<256, 2, KIND, STREAM>(x, q, scale, M, D, a, s);
-  if (chunks <= 1024 && M <= 128) return launch<1024, 1, KIND, STREAM>(x, q, scale, M, D, a, s);
   if (chunks <= 768) return launch<256, 3, KIND, STREAM>(x, q, scale, M, D, a, s);
   if (chunks <= 1024) return launch<256, 4, KIND, STREAM>(x, q, scale, M, D, a, s);
   return launch<1024, 2, KIND, STREAM>(x, q, scale, M, D, a, s);
@@ -361,8 +371,8 @@ hipError_t quantize(const f16* x, int8_t* q, float* scale, int M, int D, const N
 template <bool STREAM>
 hipError_t dequantize_as(const int8_t* q, const float* scale, f16* x, int M, int D,
                          hipStream_t s) {
-  // 131072 x 256 19.2 us with 16 threads a row, 25.9 with 64; 65536 x 1024 39.1
-  // and 35.8; 16384 x 4096 41.2 with 64, 35.9 with 256
+  // 131072 x 256 18.9 us with 16 threads a row, 25.5 with 64; 65536 x 1024 31.2
+  // and 29.8; 700 x 2048 3.3 with 64, 2.7 with 256, 16384 x 4096 31.5 and 29.4
   if (D <= 256) return dequantize<16, STREAM>(q, scale, x, M, D, s);
   if (D <= 1024) return dequantize<64, STREAM>(q, scale, x, M, D, s);
   return dequantize<256, STREAM>(q, scale, x, M, D, s);

@@ -281,7 +281,9 @@ def test_norms_against_64_bits(torch_cuda, kind, D):
 
 @gpu
 @pytest.mark.parametrize("M,D", [(131072, 384), (70001, 385), (200003, 129), (27001, 1000),
-                                 (3333, 16384), (9001, 8191)])
+                                 (3333, 16384), (9001, 8191), (400003, 63), (60001, 500),
+                                 (17001, 1536), (13001, 2047), (30001, 1700), (6401, 4000),
+                                 (4501, 5999)])
 def test_rows_read_and_written_past_the_caches(torch_cuda, M, D):
     """From 48 MB of fp16 rows on the accesses are non-temporal (from 96 MB what is
     read back, too): the same results, outputs over inputs among them."""
