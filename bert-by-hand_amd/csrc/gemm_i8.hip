@@ -10,10 +10,18 @@
 // transposed tile D(n, m) = B . A^T, so that a lane holds runs of four
 // consecutive output columns of one row.
 //
+// Bounds, measured on MI355X: large products the matrix cores at the clock that
+// power leaves them (8192^3 440 us, 2.5 POP/s, at 1.65 GHz; independent products
+// on random codes reach 3.5); few rows against many the reading of B (64 x 200003
+// x 384 18.8 us, 5.5 TB/s with its output); a short K its copies from L2, epilogue
+// and stores in turn (8192 x 1536 x 384 with GELU 14.4 us); the smallest a launch
+// and one latency (16 x 1536 x 384 2.7 us, 1 x 4096 x 4096 5.4).
+//
 // K goes in slices of 128 bytes: a row of a slice is one cache line, eight
 // 16-byte chunks, and logical chunk c of row r sits in slot c ^ ((r >> 1) & 7)
 // (the layout of pipe.h's 64-wide fp16 slice, byte for byte).
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -25,7 +33,6 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
-typedef i32x4 i32x4_any __attribute__((aligned(1)));
 typedef f16x8 f16x8_any __attribute__((aligned(2)));
 
 constexpr int kSlice = 128;  // bytes of K a slice
@@ -90,7 +97,7 @@ struct Cfg {
   static constexpr int OUT = KS == 1 ? BM * OUT_LD * 2 : KS * BM * SUM_LD * 4;
   static constexpr int VEC = RING > OUT ? RING : OUT;       // sa, sb, bias follow
   static constexpr int LDS = VEC + (BM + 2 * BN) * 4;
-  static constexpr int CH = (BM + BN) * 8 / (64 * GW);      // chunks a thread (unaligned)
+  static constexpr int CH = (BM + BN) * 8 / (64 * GW);      // chunks a thread (last slice)
   static_assert(TM % MB == 0 && TN % MB == 0, "whole blocks");
   static_assert(BM % (8 * GW) == 0 && BN % (8 * GW) == 0, "a copy is of one operand");
   static_assert(R >= 1 && (R - 1) * L < 64, "vmcnt range");
@@ -104,15 +111,17 @@ struct Cfg {
 // is everything at an offset of kNowhere: such copies read no memory and write
 // zeros.
 constexpr uint32_t kNowhere = 1u << 30;
+__device__ __forceinline__ uint32_t head(const int8_t* p) { return (uint32_t)(uintptr_t)p & 3; }
 struct Copier {
   __amdgpu_buffer_rsrc_t src;
   uint32_t lane[2], step;  // byte offset in an even / odd block of 8 rows; 8 rows
   __device__ __forceinline__ Copier(const int8_t* base, int rows, int K)
-      : src(buffer_of(base, (uint32_t)rows * K)), step(8u * K) {
+      : src(buffer_of(base - head(base), (head(base) + (uint32_t)rows * K + 3) & ~3u)),
+        step(8u * K) {
     const int l = threadIdx.x & 63, r = l >> 3;
 #pragma unroll
     for (int p = 0; p < 2; ++p)
-      lane[p] = r * K + (((l & 7) ^ (p << 2 | r >> 1)) << 4);
+      lane[p] = ((head(base) + r * K) & ~3u) + (((l & 7) ^ (p << 2 | r >> 1)) << 4);
   }
   template <int N>
   __device__ __forceinline__ void copy(uint32_t at, char* dst, int wave) const {
@@ -146,14 +155,24 @@ struct Product<16> {
 // Operands of one K step: lane l holds 16 bytes of row l % MB, chunk l / MB of
 // the step's, of each block.  A product gives it the columns 8 q + 4 (l / MB)
 // .. + 3, q = 0 .. NV / 4 - 1, of row l % MB.
-template <class C>
+template <class C, bool SHIFTED>
 struct Frags {
   i32x4 a[C::FM], b[C::FN];
+  static constexpr bool BEFORE = SHIFTED && C::MB == 16;
+  int pa[BEFORE ? C::FM : 1] = {}, pb[BEFORE ? C::FN : 1] = {};  // the dwords before (Carry)
   __device__ static __forceinline__ int lane_at(int lane) {
     const int r = lane % C::MB;
     return r * kSlice + ((lane / C::MB ^ (r >> 1 & 7)) << 4);
   }
-  __device__ __forceinline__ void read(const char* st, int j, int at, int wm, int wn) {
+  // kShifted: where a lane finds the dword before its chunk: in the chunk before
+  // of the same step, or, for the step's first chunk, in the last chunk of the
+  // step before.  So the lanes of the first read the last one's, for the step
+  // that follows (Carry).
+  __device__ static __forceinline__ int lane_before(int lane) {
+    const int r = lane % C::MB, c = lane / C::MB, last = 64 / C::MB - 1;
+    return r * kSlice + (((c ? c - 1 : last) ^ (r >> 1 & 7)) << 4) + 12;
+  }
+  __device__ __forceinline__ void read(const char* st, int j, int at, int before, int wm, int wn) {
     const char* p = st + (at ^ (j * C::KB));
 #pragma unroll
     for (int f = 0; f < C::FM; ++f)
@@ -161,6 +180,15 @@ struct Frags {
 #pragma unroll
     for (int f = 0; f < C::FN; ++f)
       b[f] = *reinterpret_cast<const i32x4*>(p + (C::BM + wn * C::TN + f * C::MB) * kSlice);
+    if constexpr (BEFORE) {
+      const char* e = st + (before ^ (j * C::KB));
+#pragma unroll
+      for (int f = 0; f < C::FM; ++f)
+        pa[f] = *reinterpret_cast<const int*>(e + (wm * C::TM + f * C::MB) * kSlice);
+#pragma unroll
+      for (int f = 0; f < C::FN; ++f)
+        pb[f] = *reinterpret_cast<const int*>(e + (C::BM + wn * C::TN + f * C::MB) * kSlice);
+    }
   }
   __device__ __forceinline__ void mul(typename Product<C::MB>::Acc (&acc)[C::FM][C::FN]) const {
 #pragma unroll
@@ -168,6 +196,41 @@ struct Frags {
 #pragma unroll
       for (int fn = 0; fn < C::FN; ++fn)
         acc[fm][fn] = Product<C::MB>::mul(b[fn], a[fm], acc[fm][fn]);
+  }
+};
+
+// kShifted: of the 20 raw bytes that end with a lane's chunk, the 16 from byte
+// `sa` (or `sb`) on are its bytes of K.  The first four are the last of the chunk
+// before: that of the lane MB below, or, for the step's first chunk, of the
+// step before, kept here.  With MB = 32 both come from one exchange of the
+// wavefront's halves; with 16 the dword is read from LDS (with 32, too, that took
+// the LDS half as long again as the chunks do).
+template <class C>
+struct Carry {
+  int a[C::FM], b[C::FN];
+  uint32_t sa, sb;
+  bool first;  // of the step's chunks
+  __device__ __forceinline__ void one(i32x4& v, int& keep, int before, uint32_t by) const {
+    int p;
+    if constexpr (C::MB == 32) {
+      const auto h = __builtin_amdgcn_permlane32_swap((uint32_t)keep, (uint32_t)v[3], false, false);
+      p = (int)(first ? h[1] : h[0]);
+      keep = v[3];
+    } else {
+      p = first ? keep : before;
+      keep = before;
+    }
+    v[3] = __builtin_amdgcn_alignbyte(v[3], v[2], by);
+    v[2] = __builtin_amdgcn_alignbyte(v[2], v[1], by);
+    v[1] = __builtin_amdgcn_alignbyte(v[1], v[0], by);
+    v[0] = __builtin_amdgcn_alignbyte(v[0], p, by);
+  }
+  __device__ __forceinline__ void shift(Frags<C, true>& f) {
+    constexpr bool B = Frags<C, true>::BEFORE;
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i) one(f.a[i], a[i], f.pa[B ? i : 0], sa);
+#pragma unroll
+    for (int i = 0; i < C::FN; ++i) one(f.b[i], b[i], f.pb[B ? i : 0], sb);
   }
 };
 
@@ -182,49 +245,26 @@ __device__ __forceinline__ void interleave() {
   }
 }
 
-// 16 bytes at k of a row of K, zeros past its end.  A chunk that crosses the end
-// is the row's last 16 bytes shifted down; of a row shorter than that, byte by
-// byte.  (Small: it is unrolled for every chunk a thread copies.)
-__device__ __forceinline__ i32x4 load_chunk(const int8_t* row, int k, int K) {
-  const int n = K - k;
-  if (n >= kChunk) return *reinterpret_cast<const i32x4_any*>(row + k);
-  uint64_t lo = 0, hi = 0;
-  if (n > 0) {
-    if (K >= kChunk) {
-      const i32x4 v = *reinterpret_cast<const i32x4_any*>(row + K - kChunk);
-      lo = (uint32_t)v[0] | (uint64_t)(uint32_t)v[1] << 32;
-      hi = (uint32_t)v[2] | (uint64_t)(uint32_t)v[3] << 32;
-      const int s = 8 * (kChunk - n);
-      lo = s < 64 ? lo >> s | hi << (64 - s) : hi >> (s - 64);
-      hi = s < 64 ? hi >> s : 0;
-    } else {
-#pragma unroll 1
-      for (int e = n - 1; e >= 0; --e) {
-        hi = hi << 8 | lo >> 56;
-        lo = lo << 8 | (uint8_t)row[k + e];
-      }
-    }
-  }
-  return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
-}
-
-// How slices reach the ring.
-//  kCopies   K % 16 == 0, 16-byte aligned operands: buffer loads to LDS.
-//  kCopies4  K % 4 == 0, 4-byte aligned operands: the same for whole slices (a
-//            copy of 16 bytes needs 4-byte alignment only); the last part of K,
+// How slices reach the ring: by buffer loads to LDS, 16 bytes a lane, which need
+// 4-byte alignment only.
+//  kCopies   K % 16 == 0, 16-byte aligned operands.
+//  kCopies4  K % 4 == 0, 4-byte aligned operands: whole slices; the last part of K,
 //            whose chunks would cross a row's end, goes through registers.
-//  kStaged   any K and address: through registers, one slice ahead; kStaged2:
-//            two ahead, for workgroups that have a CU to themselves (2008 x 1904
-//            x 5201 44 us against 52; with two on a CU the registers cost more
-//            than that hides: 4000 x 4000 x 2001 75 against 65).
-// Through registers, the bytes past K are cleared.
-enum Feed { kCopies, kCopies4, kStaged, kStaged2 };
+//  kShifted  any K and address: a row's raw bytes from the 4-byte boundary at or
+//            before its first, and again the last part through registers.  Bytes
+//            of K come from the raw ones by a shift that is the lane's own, as
+//            its rows are equal modulo 4 (Carry): slice s holds k = 128 s - 4 ..
+//            128 s + 123.  Only dwords that hold a byte of the operand are read,
+//            and what else they hold is cleared in A before the product.
+// 4000 x 4000 x 2001 49 us, 2004 43, 2000 40 (through registers altogether 65);
+// 2003 x 1111 x 777 10.9, 780 9.6, 768 8.4 (12.4).
+enum Feed { kCopies, kCopies4, kShifted };
 
 template <class C, int FEED, bool GELU>
 __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int tn) {
   extern __shared__ __align__(16) char smem[];
-  constexpr bool COPIES = FEED <= kCopies4;
-  constexpr int AHEAD = FEED == kStaged2 ? 2 : 1;
+  constexpr bool SHIFTED = FEED == kShifted;
+  constexpr bool TAIL = FEED != kCopies;  // the last slice goes through registers
   int bm, bn;
   if (!tile_of(tm, tn, bm, bn)) return;
   const int K = g.K, m0 = bm * C::BM, n0 = bn * C::BN;
@@ -256,163 +296,190 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
   // Iteration i of a group is slice i * KS + grp.  Every group has `even` whole
   // slices; then one iteration more, in which a group has a whole slice, the
   // last part of K or none, unless no group has any.
-  const int full = K / kSlice, rem = K % kSlice, total = full + (rem ? 1 : 0);
+  const int full = (SHIFTED ? K + 3 : K) / kSlice;
+  const int total = SHIFTED ? full + 1 : full + (K % kSlice ? 1 : 0);
   const int even = full / C::KS, iters = (total + C::KS - 1) / C::KS;
   char* const ring = smem + grp * C::R * C::STAGE;
   char* const ring_end = ring + C::R * C::STAGE;
   const Copier ca(A, rows, K), cb(B, cols, K);
-  auto issue = [&](int i, char* dst) {  // COPIES: the slice of iteration i into a slot
-    const int s = i * C::KS + grp;
-    const uint32_t at = s < (FEED == kCopies ? total : full) ? (uint32_t)s * kSlice : kNowhere;
+  auto slice = [&](int i) {
+    if constexpr (SHIFTED && C::KS > 1)  // a group's are next to each other
+      return i < even ? grp * even + i : i > even ? total : C::KS * even + grp;
+    else
+      return i * C::KS + grp;
+  };
+  auto issue = [&](int i, char* dst) {  // the slice of iteration i into a slot
+    const int s = slice(i);
+    const uint32_t at = s < (TAIL ? full : total) ? (uint32_t)s * kSlice : kNowhere;
     ca.template copy<C::LA>(at, dst, w);
     cb.template copy<C::LB>(at, dst + C::BM * kSlice, w);
   };
-  // Through registers (set: i % AHEAD).  Chunk j of a thread is a row of A or of B
-  // by j alone; rows past the tile's last are that one again (nothing of theirs
-  // is written).
-  constexpr int CH = FEED == kCopies ? 1 : C::CH;
-  i32x4 held[AHEAD][CH];
-  auto from = [&](int j) {
-    const int q = w * 64 + lane + j * 64 * C::GW, r = q >> 3;
-    return (uint32_t)(j * 8 * C::GW < C::BM ? min(r, rows - 1) : min(r - C::BM, cols - 1)) * K +
-           (q & 7) * kChunk;
-  };
-  auto load = [&](int i, auto set) {
-    const int s = i * C::KS + grp;
-    // the branch is outside the loops, so that a slice's loads are issued together
-    if (s < full) {
-      const int8_t *a = A + s * kSlice, *b = B + s * kSlice;
-#pragma unroll
-      for (int j = 0; j < CH; ++j)
-        held[set][j] = *reinterpret_cast<const i32x4_any*>((j * 8 * C::GW < C::BM ? a : b) + from(j));
-    } else if (s < total) {
-#pragma unroll
-      for (int j = 0; j < CH; ++j) {
-        const int k = (lane & 7) * kChunk;  // from(j) less its row's start
-        held[set][j] = load_chunk((j * 8 * C::GW < C::BM ? A : B) + (from(j) - k), s * kSlice + k, K);
-      }
-    }
-  };
-  auto put = [&](char* dst, auto set) {
+  // The last slice through registers.  Chunk j of a thread is a row of A or of B by
+  // j alone; rows past the tile's last are that one again (nothing of theirs is
+  // written).
+  constexpr int CH = TAIL ? C::CH : 1;
+  i32x4 held[CH];
+  auto load = [&] {
+    if (slice(even) != full) return;
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
-      const int q = w * 64 + lane + j * 64 * C::GW, r = q >> 3;
-      *reinterpret_cast<i32x4*>(dst + r * kSlice + (((q & 7) ^ (r >> 1 & 7)) << 4)) = held[set][j];
+      const int r = w * 8 + (lane >> 3) + j * 8 * C::GW, k = full * kSlice + (lane & 7) * kChunk;
+      const int8_t* row = j * 8 * C::GW < C::BM ? A + (uint32_t)min(r, rows - 1) * K
+                                                : B + (uint32_t)min(r - C::BM, cols - 1) * K;
+      const int8_t* p = row - (SHIFTED ? head(row) : 0) + k;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        held[j][e] = p + 4 * e < row + K ? reinterpret_cast<const int*>(p)[e] : 0;
+    }
+  };
+  auto put = [&](char* dst) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int r = w * 8 + (lane >> 3) + j * 8 * C::GW;
+      *reinterpret_cast<i32x4*>(dst + r * kSlice + (((lane & 7) ^ (r >> 1 & 7)) << 4)) = held[j];
     }
   };
   auto next = [&](char* p) { return p + C::STAGE == ring_end ? ring : p + C::STAGE; };
   char* slot = ring;      // of the slice that is read
   char* refill = ring;    // the slot that the next copies go to
-  constexpr std::integral_constant<int, 0> kEven{};
-  constexpr std::integral_constant<int, AHEAD - 1> kOdd{};
-  if constexpr (COPIES) {
+
+  typedef Frags<C, SHIFTED> F;
+  const int at = F::lane_at(lane), lrow = lane % C::MB, lchunk = lane / C::MB;
+  const int before = SHIFTED ? F::lane_before(lane) : 0;
+  Carry<C> carry{}, later{};
+  auto carry_into = [&](int s, Carry<C>& c) {  // 0 < s <= full
+#pragma unroll
+    for (int f = 0; f < C::FM; ++f) {
+      const int8_t* row = A + (size_t)min(wm * C::TM + f * C::MB + lrow, rows - 1) * K;
+      c.a[f] = *reinterpret_cast<const int*>(row - head(row) + s * kSlice - 4);
+    }
+#pragma unroll
+    for (int f = 0; f < C::FN; ++f) {
+      const int8_t* row = B + (size_t)min(wn * C::TN + f * C::MB + lrow, cols - 1) * K;
+      c.b[f] = *reinterpret_cast<const int*>(row - head(row) + s * kSlice - 4);
+    }
+  };
+  if constexpr (SHIFTED) {
+    carry.sa = later.sa = head(A + lrow * (K & 3));
+    carry.sb = later.sb = head(B + lrow * (K & 3));
+    carry.first = later.first = lchunk == 0;
+    if constexpr (C::KS > 1) {
+      if (even > 0 && grp > 0) carry_into(grp * even, carry);
+      if (slice(even) > 0 && slice(even) <= full) carry_into(slice(even), later);
+    }
+  }
+  if (!TAIL || full > 0) {
 #pragma unroll
     for (int i = 0; i < C::R; ++i) issue(i, ring + i * C::STAGE);
-  } else {
-    load(0, kEven);
-    if constexpr (AHEAD == 2) load(1, kOdd);
   }
-
-  const int at = Frags<C>::lane_at(lane), lrow = lane % C::MB, lchunk = lane / C::MB;
   // Makes slice i readable: its copies have landed (those of later ones may be
   // in flight: R - 1 slices behind the first, then R - 2, as the next copies come
   // after this), and every wavefront has read slice i - 1, whose slot the next
   // copies fill.
-  auto arrive = [&](auto first, auto set) {
-    if constexpr (COPIES)
-      wait_vm<(C::R - (decltype(first)::value || C::R == 1 ? 1 : 2)) * C::L>();
-    else
-      put(slot, set);
+  auto arrive = [&](auto first) {
+    wait_vm<(C::R - (decltype(first)::value || C::R == 1 ? 1 : 2)) * C::L>();
     lds_barrier();
   };
   constexpr std::true_type kFirst{};
   constexpr std::false_type kLater{};
-  auto advance = [&](int i, auto set) {  // the copies that follow arrive() of slice i
-    if constexpr (!COPIES) {
-      load(i + AHEAD, set);
-    } else if constexpr (C::R > 1) {
+  auto advance = [&](int i) {  // the copies that follow arrive() of slice i
+    if constexpr (C::R > 1) {
       issue(i + C::R - 1, refill);
       refill = next(refill);
     }
   };
   auto reload = [&](int i) {  // R == 1: the next slice over this one
-    if constexpr (COPIES && C::R == 1) {
+    if constexpr (C::R == 1) {
       lds_barrier();
       issue(i, ring);
     }
   };
-  Frags<C> f0, f1;
+  F f0, f1;
+  auto mul = [&](F& f) {
+    if constexpr (SHIFTED) carry.shift(f);
+    f.mul(acc);
+  };
+  // kShifted: the bytes before the first of K
+  auto clear_head = [&](int s) {
+    if (SHIFTED && s == 0 && lchunk == 0)
+#pragma unroll
+      for (int f = 0; f < C::FM; ++f) f0.a[f][0] &= (int)(~0u << (8 * carry.sa));
+  };
   constexpr int RD = C::FM + C::FN, MF = C::FM * C::FN;
   // All K steps of the slice but the last, each beside the reads of the next.
   auto most = [&] {
     __builtin_amdgcn_sched_barrier(0);
-    f1.read(slot, 1, at, wm, wn);
-    f0.mul(acc);
+    f1.read(slot, 1, at, before, wm, wn);
+    mul(f0);
     interleave<RD, MF>();
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (C::STEPS == 4) {
-      f0.read(slot, 2, at, wm, wn);
-      f1.mul(acc);
+      f0.read(slot, 2, at, before, wm, wn);
+      mul(f1);
       interleave<RD, MF>();
       __builtin_amdgcn_sched_barrier(0);
-      f1.read(slot, 3, at, wm, wn);
-      f0.mul(acc);
+      f1.read(slot, 3, at, before, wm, wn);
+      mul(f0);
       interleave<RD, MF>();
       __builtin_amdgcn_sched_barrier(0);
     }
     slot = next(slot);
   };
-  auto step = [&](int i, auto set) {
+  auto step = [&](int i) {
     most();
     reload(i);
-    arrive(kLater, set);
-    f0.read(slot, 0, at, wm, wn);
-    advance(i, set);
-    f1.mul(acc);
+    arrive(kLater);
+    f0.read(slot, 0, at, before, wm, wn);
+    advance(i);
+    mul(f1);
     interleave<RD, MF>();
   };
   if (even > 0) {
-    arrive(kFirst, kEven);
-    f0.read(slot, 0, at, wm, wn);
-    if constexpr (!COPIES) advance(0, kEven);
-    if constexpr (AHEAD == 1) {
-      for (int i = 1; i < even; ++i) step(i, kEven);
-    } else {
-      int i = 1;
-      for (; i + 1 < even; i += 2) {
-        step(i, kOdd);
-        step(i + 1, kEven);
-      }
-      if (i < even) step(i, kOdd);
-    }
-    if constexpr (FEED == kCopies4) load(even, kEven);
+    arrive(kFirst);
+    f0.read(slot, 0, at, before, wm, wn);
+    clear_head(slice(0));
+    for (int i = 1; i < even; ++i) step(i);
+    if constexpr (TAIL) load();
     most();
     if (C::R == 1 && iters > even) reload(even);
-    f1.mul(acc);
-  } else if constexpr (FEED == kCopies4) {
-    load(0, kEven);
+    mul(f1);
+  } else if constexpr (TAIL) {
+    load();
   }
   if (iters > even) {
-    if constexpr (FEED == kCopies4) {
+    if constexpr (TAIL) {
       // A copy from nowhere still writes its slot (zeros): every wavefront's have
       // landed before any puts what belongs there.
-      wait_vm<0>();
-      lds_barrier();
-      if (even * C::KS + grp == full) put(slot, kEven);
+      if (full > 0) {
+        wait_vm<0>();
+        lds_barrier();
+      }
+      if (slice(even) == full) put(slot);
     }
     if (even == 0)
-      arrive(kFirst, kEven);
-    else if (AHEAD == 1 || even % 2 == 0)
-      arrive(kLater, kEven);
+      arrive(kFirst);
     else
-      arrive(kLater, kOdd);
-    const int s = even * C::KS + grp, left = min(kSlice, K - s * kSlice);
+      arrive(kLater);
+    // kShifted: a slice's k begin 4 before its raw bytes
+    const int s = slice(even), left = min(kSlice, K - s * kSlice + (SHIFTED ? 4 : 0));
+    if constexpr (SHIFTED && C::KS > 1) carry = later;
     for (int j = 0; j * C::KB < left; ++j) {
-      f0.read(slot, j, at, wm, wn);
+      f0.read(slot, j, at, before, wm, wn);
       // past K: the next row's bytes in both operands, cleared in one
       if (FEED == kCopies && j * C::KB + lchunk * kChunk >= left)
 #pragma unroll
         for (int f = 0; f < C::FM; ++f) f0.a[f] = i32x4{0, 0, 0, 0};
+      if constexpr (SHIFTED) {
+        if (j == 0) clear_head(s);
+        carry.shift(f0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = left - j * C::KB - lchunk * kChunk - 4 * e;  // bytes of this dword in K
+          const int keep = n >= 4 ? -1 : n <= 0 ? 0 : (int)((1u << (8 * n)) - 1);
+#pragma unroll
+          for (int f = 0; f < C::FM; ++f) f0.a[f][e] &= keep;
+        }
+      }
       f0.mul(acc);
     }
   }
@@ -424,8 +491,8 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     vsb[tid] = hsb;
     vbias[tid] = (float)hbias;
   }
-  if constexpr (COPIES) wait_vm<0>();  // copies from nowhere are still copies
-  lds_barrier();                        // the ring is free
+  wait_vm<0>();  // copies from nowhere are still copies
+  lds_barrier();  // the ring is free
 
   if constexpr (C::KS == 1) {
     f16* tile = reinterpret_cast<f16*>(smem);
@@ -509,13 +576,16 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
       }
     };
     // An output beyond an XCD's L2 is written past it, where it would displace the
-    // operands that other tiles read again: 8192 x 1536 x 384 12.1 -> 10.5 us, with
+    // operands that other tiles read again: 8192 x 1536 x 384 12.4 -> 10.7 us, with
     // the quantising that reads it 23.9 -> 22.3; but 512 x 1536 x 384 with that 8.0
     // -> 8.2, and tiles of 256 x 256, whose operands are read less often, 51.8 ->
-    // 55.8 (8192 x 4096 x 1024).
+    // 55.8 (8192 x 4096 x 1024).  Only where its rows are whole lines: parts of lines
+    // need L2 to be put together (8192 x 1537 x 384 15.9 -> 17.7, 11678 x 3845 x 48
+    // 22.6 -> 40.0).
     // (The comments in the assembly keep the compiler from merging the two, which
     // would make every store an ordinary one.)
-    if (C::BM * C::BN < 256 * 256 && (int64_t)g.M * g.N * 2 >= kXcdL2) {
+    if (C::BM * C::BN < 256 * 256 && (int64_t)g.M * g.N * 2 >= kXcdL2 &&
+        ((uintptr_t)g.C | (uint32_t)g.N * 2) % 128 == 0) {
       asm volatile("; past L2" ::: "memory");
       write(std::true_type{});
       asm volatile("; end past L2" ::: "memory");
@@ -596,28 +666,20 @@ constexpr Tile kTiles[] = {{256, 256, 20.5f, 9500.f}, {256, 128, 14.5f, 4000.f},
                            {32, 64, 1.2f, 600.f},     {32, 32, 0.7f, 900.f},
                            {16, 32, 0.5f, 1500.f},    {16, 16, 0.3f, 120.f}};
 constexpr int kCus = kXcds * kXcdCus;
-// Tiles of operands that are staged, and of those that are copied but for the
-// last part of K.  (The staged chunks of the others would need more registers
-// than their wavefronts have.)
-constexpr uint32_t kStagedTiles = 1u << 2 | 1u << 3 | 1u << 5 | 1u << 6 | 1u << 9;
-constexpr uint32_t kCopies4Tiles = 1u << 0 | kStagedTiles;
-
 int64_t rounds_of(const Tile& t, int M, int N) {
   const int64_t n = (int64_t)((M - 1) / t.bm + 1) * ((N - 1) / t.bn + 1);
   return (n + kCus - 1) / kCus;
 }
 
-// all_rows: rows past M and N cost what the others do (staged chunks; copies of
-// them read nothing).
-int pick_tile(int M, int N, int K, uint32_t allowed, bool all_rows) {
+int pick_tile(int M, int N, int K) {
   int best = -1;
   float least = 0.f;
   for (int i = 0; i < (int)(sizeof kTiles / sizeof kTiles[0]); ++i) {
-    if (!(allowed >> i & 1)) continue;
     const Tile& t = kTiles[i];
     const int64_t rounds = rounds_of(t, M, N);
-    const int rows = all_rows || M > t.bm ? t.bm : M, cols = all_rows || N > t.bn ? t.bn : N;
-    const float copies = (float)(rows + cols) / (t.bn == 16 && rounds > 2 ? 44.f : 32.f);
+    // rows past M and N are not read
+    const float copies = (float)(std::min(M, t.bm) + std::min(N, t.bn)) /
+                         (t.bn == 16 && rounds > 2 ? 44.f : 32.f);
     const float cost = (float)rounds * ((float)K * (copies > t.mfma ? copies : t.mfma) + t.fixed);
     if (best < 0 || cost < least) {
       least = cost;
@@ -627,92 +689,65 @@ int pick_tile(int M, int N, int K, uint32_t allowed, bool all_rows) {
   return best;
 }
 
+template <int FEED>
+hipError_t dispatch(const Args& g, bool gelu, hipStream_t s) {
+  const int K = g.K, t = pick_tile(g.M, g.N, K);
+  // One round, a workgroup a CU, and a long K: nothing but its own copies hides
+  // a workgroup's waits, so it has more of them in flight (or more groups).
+  const int64_t rounds = rounds_of(kTiles[t], g.M, g.N);
+  const bool alone = rounds == 1 && K >= 1024;
+  // Tiles of 16 x 16 by one wavefront a workgroup: where K is short (16 x 1536 x
+  // 384 2.7 us against 3.1) or there are many, not too long each (8 x 33206 x 2704
+  // 17.0 against 19.7, but 1 x 32000 x 4096 31.5 against 27.6).
+  const bool one_wave = K <= 512 || (rounds >= 8 && K < 4096);
+  // Several rounds of a short K: a ring of one slice, so that twice the
+  // workgroups share a CU and hide each other's copies and epilogues.
+  const bool shortk = rounds > 1 && K <= 512;
+  switch (t) {
+    case 0: return run<Cfg<256, 256, 2, 4, 1, 2>, FEED>(g, gelu, s);
+    case 1: return run<Cfg<256, 128, 4, 2, 1, 3>, FEED>(g, gelu, s);
+    case 2:
+      return alone    ? run<Cfg<128, 128, 2, 4, 1, 3>, FEED>(g, gelu, s)
+             : shortk ? run<Cfg<128, 128, 2, 4, 1, 1>, FEED>(g, gelu, s)
+                      : run<Cfg<128, 128, 2, 4, 1, 2>, FEED>(g, gelu, s);
+    case 3:
+      return alone    ? run<Cfg<64, 128, 2, 2, 1, 3>, FEED>(g, gelu, s)
+             : shortk ? run<Cfg<64, 128, 1, 4, 1, 1>, FEED>(g, gelu, s)
+                      : run<Cfg<64, 128, 1, 4, 1, 2>, FEED>(g, gelu, s);
+    case 4:
+      return alone    ? run<Cfg<128, 64, 2, 2, 1, 3>, FEED>(g, gelu, s)
+             : shortk ? run<Cfg<128, 64, 2, 2, 1, 1>, FEED>(g, gelu, s)
+                      : run<Cfg<128, 64, 2, 2, 1, 2>, FEED>(g, gelu, s);
+    case 5:
+      return alone                    ? run<Cfg<64, 64, 2, 2, 2, 3>, FEED>(g, gelu, s)
+             : shortk                 ? run<Cfg<64, 64, 2, 2, 1, 1>, FEED>(g, gelu, s)
+             : rounds == 2 && K >= 1024 ? run<Cfg<64, 64, 2, 2, 1, 3>, FEED>(g, gelu, s)
+                                        : run<Cfg<64, 64, 2, 2, 1, 2>, FEED>(g, gelu, s);
+    case 6:
+      return shortk       ? run<Cfg<32, 64, 1, 2, 1, 1>, FEED>(g, gelu, s)
+             : rounds > 2 ? run<Cfg<32, 64, 1, 2, 1, 2>, FEED>(g, gelu, s)
+                          : run<Cfg<32, 64, 1, 2, 2, 3>, FEED>(g, gelu, s);
+    case 7:
+      return alone                    ? run<Cfg<32, 32, 1, 1, 4, 4>, FEED>(g, gelu, s)
+             : K <= 512 || rounds > 2 ? run<Cfg<32, 32, 1, 1, 1, 2>, FEED>(g, gelu, s)
+                                      : run<Cfg<32, 32, 1, 1, 4, 2>, FEED>(g, gelu, s);
+    case 8: return run<Cfg<16, 32, 1, 1, 4, 4>, FEED>(g, gelu, s);
+    default:
+      return one_wave    ? run<Cfg<16, 16, 1, 1, 1, 2>, FEED>(g, gelu, s)
+             : K <= 1536 ? run<Cfg<16, 16, 1, 1, 2, 2>, FEED>(g, gelu, s)
+                         : run<Cfg<16, 16, 1, 1, 4, 4>, FEED>(g, gelu, s);
+  }
+}
+
 }  // namespace
 
 hipError_t gemm_i8(const int8_t* A, const float* sa, const int8_t* B, const float* sb,
                    const f16* bias, f16* C, int M, int N, int K, bool gelu, hipStream_t s) {
   const Args g{A, B, sa, sb, bias, C, M, N, K};
   const uintptr_t at = (uintptr_t)A | (uintptr_t)B | (uintptr_t)K;
-  const Feed feed = at % 16 == 0 ? kCopies : at % 4 == 0 ? kCopies4 : kStaged;
-  const uint32_t allowed = feed == kCopies    ? ~0u
-                           : feed == kCopies4 ? kCopies4Tiles
-                                              : kStagedTiles;
-  const int t = pick_tile(M, N, K, allowed, feed == kStaged);
-  // One round, a workgroup a CU, and a long K: nothing but its own copies hides
-  // a workgroup's waits, so it has more of them in flight (or more groups).
-  const int64_t rounds = rounds_of(kTiles[t], M, N);
-  const bool alone = rounds == 1 && K >= 1024;
-  // Tiles of 16 x 16 by one wavefront a workgroup: where K is short (16 x 1536 x
-  // 384 2.7 us against 3.1) or there are many, not too long each (8 x 33206 x 2704
-  // 17.0 against 19.7, but 1 x 32000 x 4096 31.5 against 27.6).
-  const bool one_wave = K <= 512 || (rounds >= 8 && K < 4096);
-  if (feed == kCopies4) {
-    switch (t) {
-      case 0: return run<Cfg<256, 256, 2, 4, 1, 2>, kCopies4>(g, gelu, s);
-      case 2:
-        return alone ? run<Cfg<128, 128, 2, 4, 1, 3>, kCopies4>(g, gelu, s)
-                     : run<Cfg<128, 128, 2, 4, 1, 2>, kCopies4>(g, gelu, s);
-      case 3: return run<Cfg<64, 128, 2, 2, 1, 3>, kCopies4>(g, gelu, s);
-      case 5: return run<Cfg<64, 64, 2, 2, 1, 2>, kCopies4>(g, gelu, s);
-      case 6: return run<Cfg<32, 64, 1, 2, 2, 3>, kCopies4>(g, gelu, s);
-      default:
-        return one_wave ? run<Cfg<16, 16, 1, 1, 1, 2>, kCopies4>(g, gelu, s)
-                        : run<Cfg<16, 16, 1, 1, 4, 4>, kCopies4>(g, gelu, s);
-    }
-  }
-  if (feed == kStaged) {
-    switch (t) {
-      case 2:
-        return alone ? run<Cfg<128, 128, 2, 4, 1, 2>, kStaged2>(g, gelu, s)
-                     : run<Cfg<128, 128, 2, 4, 1, 2>, kStaged>(g, gelu, s);
-      case 3: return run<Cfg<64, 128, 2, 4, 1, 2>, kStaged>(g, gelu, s);
-      case 5: return run<Cfg<64, 64, 2, 2, 1, 2>, kStaged>(g, gelu, s);
-      case 6:
-        return alone ? run<Cfg<32, 64, 1, 2, 4, 2>, kStaged2>(g, gelu, s)
-                     : run<Cfg<32, 64, 1, 2, 4, 2>, kStaged>(g, gelu, s);
-      default:
-        return alone      ? run<Cfg<16, 16, 1, 1, 8, 2>, kStaged2>(g, gelu, s)
-               : one_wave ? run<Cfg<16, 16, 1, 1, 1, 2>, kStaged>(g, gelu, s)
-                          : run<Cfg<16, 16, 1, 1, 4, 2>, kStaged>(g, gelu, s);
-    }
-  }
-  // Several rounds of a short K: a ring of one slice, so that twice the
-  // workgroups share a CU and hide each other's copies and epilogues.
-  const bool shortk = rounds > 1 && K <= 512;
-  switch (t) {
-    case 0: return run<Cfg<256, 256, 2, 4, 1, 2>, kCopies>(g, gelu, s);
-    case 1: return run<Cfg<256, 128, 4, 2, 1, 3>, kCopies>(g, gelu, s);
-    case 2:
-      return alone ? run<Cfg<128, 128, 2, 4, 1, 3>, kCopies>(g, gelu, s)
-             : shortk ? run<Cfg<128, 128, 2, 4, 1, 1>, kCopies>(g, gelu, s)
-                      : run<Cfg<128, 128, 2, 4, 1, 2>, kCopies>(g, gelu, s);
-    case 3:
-      return alone ? run<Cfg<64, 128, 2, 2, 1, 3>, kCopies>(g, gelu, s)
-             : shortk ? run<Cfg<64, 128, 1, 4, 1, 1>, kCopies>(g, gelu, s)
-                      : run<Cfg<64, 128, 1, 4, 1, 2>, kCopies>(g, gelu, s);
-    case 4:
-      return alone ? run<Cfg<128, 64, 2, 2, 1, 3>, kCopies>(g, gelu, s)
-             : shortk ? run<Cfg<128, 64, 2, 2, 1, 1>, kCopies>(g, gelu, s)
-                      : run<Cfg<128, 64, 2, 2, 1, 2>, kCopies>(g, gelu, s);
-    case 5:
-      return alone ? run<Cfg<64, 64, 2, 2, 2, 3>, kCopies>(g, gelu, s)
-             : shortk ? run<Cfg<64, 64, 2, 2, 1, 1>, kCopies>(g, gelu, s)
-             : rounds == 2 && K >= 1024 ? run<Cfg<64, 64, 2, 2, 1, 3>, kCopies>(g, gelu, s)
-                                        : run<Cfg<64, 64, 2, 2, 1, 2>, kCopies>(g, gelu, s);
-    case 6:
-      return shortk       ? run<Cfg<32, 64, 1, 2, 1, 1>, kCopies>(g, gelu, s)
-             : rounds > 2 ? run<Cfg<32, 64, 1, 2, 1, 2>, kCopies>(g, gelu, s)
-                          : run<Cfg<32, 64, 1, 2, 2, 3>, kCopies>(g, gelu, s);
-    case 7:
-      return alone                   ? run<Cfg<32, 32, 1, 1, 4, 4>, kCopies>(g, gelu, s)
-             : K <= 512 || rounds > 2 ? run<Cfg<32, 32, 1, 1, 1, 2>, kCopies>(g, gelu, s)
-                                      : run<Cfg<32, 32, 1, 1, 4, 2>, kCopies>(g, gelu, s);
-    case 8: return run<Cfg<16, 32, 1, 1, 4, 4>, kCopies>(g, gelu, s);
-    default:
-      return one_wave    ? run<Cfg<16, 16, 1, 1, 1, 2>, kCopies>(g, gelu, s)
-             : K <= 1536 ? run<Cfg<16, 16, 1, 1, 2, 2>, kCopies>(g, gelu, s)
-                         : run<Cfg<16, 16, 1, 1, 4, 4>, kCopies>(g, gelu, s);
-  }
+  return at % 16 == 0  ? dispatch<kCopies>(g, gelu, s)
+         : at % 4 == 0 ? dispatch<kCopies4>(g, gelu, s)
+                       : dispatch<kShifted>(g, gelu, s);
 }
 
 }  // namespace bbh

@@ -486,6 +486,56 @@ def test_linear_i8_largest_sums(torch_cuda, M):
 
 
 @gpu
+@pytest.mark.parametrize("K", [1, 2, 3, 5, 61, 123, 124, 125, 126, 127, 128, 129, 131, 132, 251, 252, 253,
+                               255, 257, 381, 384, 511, 512, 513, 514, 637, 641, 765, 1021, 1025, 1535,
+                               1537, 1661, 1664, 2047, 2050, 4099, 4221])
+def test_linear_i8_every_offset(torch_cuda, K):
+    """Rows that start at any byte, ends of K on either side of a slice's: the
+    integers are those of aligned copies, in bits, and nothing beside the operands
+    counts (the bytes there are not what the sums of a wrong window would need)."""
+    from bbh import engine
+
+    torch = torch_cuda
+    for M, N in ((1, 5), (40, 70), (130, 90)):
+        g = _gen(torch, K + M)
+        mk = lambda n: torch.randint(-128, 128, (n + 96,), device="cuda", generator=g,  # noqa: E731
+                                     dtype=torch.int8)
+        a, b = mk(M * K), mk(N * K)
+        sa = torch.full((M,), 2.0 ** -7, device="cuda")
+        sb = torch.full((N,), 2.0 ** -5, device="cuda")
+        for oa, ob in ((0, 0), (1, 0), (0, 3), (2, 1), (3, 3), (4, 2), (16, 4)):
+            A, B = a[oa:oa + M * K].view(M, K), b[ob:ob + N * K].view(N, K)
+            C = torch.empty(M, N, dtype=torch.float16, device="cuda")
+            engine.launch_matmul_i8(A, sa, B, sb, C, M, N, K)
+            # sums below 2^27 / 2^12, a power of two apart from the integers
+            want = (A.double() @ B.double().t().contiguous()).float() * 2.0 ** -12
+            assert torch.equal(C, want.half()), (M, N, oa, ob)
+
+
+# One shape for each tile and way to run it, with odd K.
+TILES = [(1, 17, 523), (1, 17, 1785), (1, 16, 37), (2429, 19, 1829), (17, 2202, 1873), (3106, 57, 469),
+         (18, 6612, 617), (4136, 17, 395), (8, 12772, 1049), (1, 8817, 33), (8, 29729, 1107),
+         (1, 21477, 33), (20, 19787, 1027), (8297, 71, 185), (154, 17305, 305), (17352, 22, 1105),
+         (73, 8539, 193), (16913, 131, 337), (76, 16445, 1047), (18750, 67, 33), (66, 44845, 37),
+         (137, 23991, 763), (51309, 139, 403), (4001, 3999, 517)]
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_linear_i8_every_tile(torch_cuda, M, N, K):
+    """Each tile with rows of K bytes: odd, a multiple of 4 and one of 16."""
+    from bbh import engine
+
+    torch = torch_cuda
+    for k in (K, (K + 3) // 4 * 4, (K + 15) // 16 * 16):
+        A, sa, B, sb, bias = _operands(torch, M + N + k, M, N, k)
+        buf, C = _guarded(torch, M * N, torch.float16, 3.0)
+        engine.launch_matmul_i8(A, sa, B, sb, C, M, N, k, bias=bias)
+        _linear_check(torch, A, sa, B, sb, bias, False, C.view(M, N))
+        assert bool((buf[M * N:] == 3).all())
+
+
+@gpu
 @pytest.mark.parametrize("M,N", [(17, 33), (300, 520)])
 def test_linear_i8_gelu_of_large_values(torch_cuda, M, N):
     """GELU of values of any size: its absolute error past 4.5 does not grow with
