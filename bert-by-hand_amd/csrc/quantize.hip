@@ -323,6 +323,8 @@ hipError_t quantize_as(const f16* x, int8_t* q, float* scale, int M, int D, cons
   //   131072 x 32     16 threads  8.4 / 15.4   64 threads  27.5 / 52.1
   //   131072 x 384    16 x 3     26.1 / 55.3   64 x 1      37.2 / 62.7
   //   2003 x 384      16 x 3      3.1 /  4.5   64 x 1       2.8 /  3.6
+  //   131072 x 512    16 x 4     33.4 / 72.1   64 x 1      37.9 / 73.9
+  //   30000 x 512     16 x 4     10.1 / 22.1   64 x 1       9.7 / 20.4
   //   65536 x 1536    64 x 3     52.2 / 112    256 x 1     66.2 / 128
   //   65536 x 1792    64 x 4     60.3 / 134    256 x 1     73.4 / 141
   //   5000 x 1700     64 x 4      8.8 / 17.5   256 x 1      8.2 / 16.9
@@ -334,7 +336,11 @@ hipError_t quantize_as(const f16* x, int8_t* q, float* scale, int M, int D, cons
   if (chunks <= 16) return launch<16, 1, KIND, STREAM>(x, q, scale, M, D, a, s);
   if (chunks <= 32 && many) return launch<16, 2, KIND, STREAM>(x, q, scale, M, D, a, s);
   if (chunks <= 48 && many) return launch<16, 3, KIND, STREAM>(x, q, scale, M, D, a, s);
-  if (chunks <= 64) return launch<64, 1, KIND, STREAM>(x, q, scale, M, D, a, s);
+  if constexpr (STREAM) {
+    if (chunks <= 64) return launch<16, 4, KIND, true>(x, q, scale, M, D, a, s);
+  } else {
+    if (chunks <= 64) return launch<64, 1, KIND, false>(x, q, scale, M, D, a, s);
+  }
   if (chunks <= 128) return launch<64, 2, KIND, STREAM>(x, q, scale, M, D, a, s);
   if (chunks <= 192) return launch<64, 3, KIND, STREAM>(x, q, scale, M, D, a, s);
   if constexpr (STREAM) {

@@ -47,7 +47,8 @@ bbh_status bbh_dequantize_rows(const int8_t *q, const float *scale, void *x, int
  * sum (optional, fp16) gets h, the residual stream of a pre-norm block; y
  * (optional, fp16) gets v, which a post-norm block adds later.  x, residual,
  * gamma, beta: fp16.  sum and y may each be x or residual, but not each other;
- * q and scale overlap nothing. */
+ * q and scale overlap nothing.  With eps 0 a row of zeros (rmsnorm) or of equal
+ * values (layernorm) is the formula's 0 / 0: a row with a NaN. */
 bbh_status bbh_rmsnorm_quantize(const void *x, const void *residual, const void *gamma,
                                 void *sum, void *y, int8_t *q, float *scale, int M, int D,
                                 float eps, bbh_stream_t stream);
