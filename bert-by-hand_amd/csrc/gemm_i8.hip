@@ -13,7 +13,7 @@
 // Bounds, measured on MI355X: large products the matrix cores at the clock that
 // power leaves them (8192^3 440 us, 2.5 POP/s, at 1.65 GHz; independent products
 // on random codes reach 3.5); few rows against many the reading of B (64 x 200003
-// x 384 18.8 us, 5.5 TB/s with its output); a short K its copies from L2, epilogue
+// x 384 21.0 us, 4.9 TB/s with its output); a short K its copies from L2, epilogue
 // and stores in turn (8192 x 1536 x 384 with GELU 14.4 us); the smallest a launch
 // and one latency (16 x 1536 x 384 2.7 us, 1 x 4096 x 4096 5.4).
 //
@@ -579,13 +579,15 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
     // operands that other tiles read again: 8192 x 1536 x 384 12.4 -> 10.7 us, with
     // the quantising that reads it 23.9 -> 22.3; but 512 x 1536 x 384 with that 8.0
     // -> 8.2, and tiles of 256 x 256, whose operands are read less often, 51.8 ->
-    // 55.8 (8192 x 4096 x 1024).  Only where its rows are whole lines: parts of lines
-    // need L2 to be put together (8192 x 1537 x 384 15.9 -> 17.7, 11678 x 3845 x 48
-    // 22.6 -> 40.0).
+    // 55.8 (8192 x 4096 x 1024).  Rows that are not whole lines, whose parts L2 would
+    // put together, only beside larger operands that no L2 holds (64 x 200003 x 384
+    // 24.3 -> 21.3, but 8192 x 1537 x 384 15.9 -> 17.7, 11678 x 3845 x 48 27 -> 40).
     // (The comments in the assembly keep the compiler from merging the two, which
     // would make every store an ordinary one.)
-    if (C::BM * C::BN < 256 * 256 && (int64_t)g.M * g.N * 2 >= kXcdL2 &&
-        ((uintptr_t)g.C | (uint32_t)g.N * 2) % 128 == 0) {
+    const int64_t written = (int64_t)g.M * g.N * 2, read = ((int64_t)g.M + g.N) * K;
+    const bool lines = ((uintptr_t)g.C | (uint32_t)g.N * 2) % 128 == 0;
+    if (C::BM * C::BN < 256 * 256 && written >= kXcdL2 &&
+        (lines || read > max(written, kXcds * kXcdL2))) {
       asm volatile("; past L2" ::: "memory");
       write(std::true_type{});
       asm volatile("; end past L2" ::: "memory");
@@ -660,9 +662,9 @@ struct Tile {
   int bm, bn;
   float mfma, fixed;
 };
-constexpr Tile kTiles[] = {{256, 256, 20.5f, 9500.f}, {256, 128, 14.5f, 4000.f},
+constexpr Tile kTiles[] = {{256, 256, 22.f, 11400.f}, {256, 128, 15.8f, 4000.f},
                            {128, 128, 8.6f, 1000.f},  {64, 128, 4.4f, 1200.f},
-                           {128, 64, 4.4f, 1250.f},   {64, 64, 2.3f, 300.f},
+                           {128, 64, 5.4f, 2200.f},   {64, 64, 2.3f, 300.f},
                            {32, 64, 1.2f, 600.f},     {32, 32, 0.7f, 900.f},
                            {16, 32, 0.5f, 1500.f},    {16, 16, 0.3f, 120.f}};
 constexpr int kCus = kXcds * kXcdCus;
@@ -700,16 +702,23 @@ hipError_t dispatch(const Args& g, bool gelu, hipStream_t s) {
   // 384 2.7 us against 3.1) or there are many, not too long each (8 x 33206 x 2704
   // 17.0 against 19.7, but 1 x 32000 x 4096 31.5 against 27.6).
   const bool one_wave = K <= 512 || (rounds >= 8 && K < 4096);
-  // Several rounds of a short K: a ring of one slice, so that twice the
-  // workgroups share a CU and hide each other's copies and epilogues.
-  const bool shortk = rounds > 1 && K <= 512;
+  // Several rounds: a ring of one slice, so that twice the workgroups share a CU
+  // and hide each other's copies and epilogues (128 x 128 tiles, 16388 x 3190 x 368
+  // 41.2 us against 43.9 with two, 44705 x 1024 x 800 58.3 and 62.1), until a long
+  // K leaves little to hide (4004 x 3648 x 4240 98.2 and 86.9); smaller tiles only
+  // where K is short (64 x 128, 18842 x 512 x 256 7.5 and 9.0, but 4749 x 1984 x
+  // 3488 60.8 and 58.6).  Where the last slice goes through registers a second
+  // slice hides that better (4000 x 4000 x 2004 52.0 and 50.0, 5336 x 3392 x 1969
+  // 77.0 and 67.5).
+  const bool one_slice = FEED == kCopies && rounds > 1 && K < 4096;
+  const bool shortk = one_slice && K <= 512;
   switch (t) {
     case 0: return run<Cfg<256, 256, 2, 4, 1, 2>, FEED>(g, gelu, s);
     case 1: return run<Cfg<256, 128, 4, 2, 1, 3>, FEED>(g, gelu, s);
     case 2:
-      return alone    ? run<Cfg<128, 128, 2, 4, 1, 3>, FEED>(g, gelu, s)
-             : shortk ? run<Cfg<128, 128, 2, 4, 1, 1>, FEED>(g, gelu, s)
-                      : run<Cfg<128, 128, 2, 4, 1, 2>, FEED>(g, gelu, s);
+      return alone       ? run<Cfg<128, 128, 2, 4, 1, 3>, FEED>(g, gelu, s)
+             : one_slice ? run<Cfg<128, 128, 4, 2, 1, 1>, FEED>(g, gelu, s)
+                         : run<Cfg<128, 128, 4, 2, 1, 2>, FEED>(g, gelu, s);
     case 3:
       return alone    ? run<Cfg<64, 128, 2, 2, 1, 3>, FEED>(g, gelu, s)
              : shortk ? run<Cfg<64, 128, 1, 4, 1, 1>, FEED>(g, gelu, s)
