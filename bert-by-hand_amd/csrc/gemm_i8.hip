@@ -663,8 +663,8 @@ struct Tile {
   float mfma, fixed;
 };
 constexpr Tile kTiles[] = {{256, 256, 22.f, 11400.f}, {256, 128, 15.8f, 4000.f},
-                           {128, 128, 8.6f, 1000.f},  {64, 128, 4.4f, 1200.f},
-                           {128, 64, 5.4f, 2200.f},   {64, 64, 2.3f, 300.f},
+                           {128, 128, 8.6f, 1000.f},  {64, 128, 4.4f, 2000.f},
+                           {128, 64, 5.4f, 2200.f},   {64, 64, 2.3f, 500.f},
                            {32, 64, 1.2f, 600.f},     {32, 32, 0.7f, 900.f},
                            {16, 32, 0.5f, 1500.f},    {16, 16, 0.3f, 120.f}};
 constexpr int kCus = kXcds * kXcdCus;
@@ -724,9 +724,8 @@ hipError_t dispatch(const Args& g, bool gelu, hipStream_t s) {
              : shortk ? run<Cfg<64, 128, 1, 4, 1, 1>, FEED>(g, gelu, s)
                       : run<Cfg<64, 128, 1, 4, 1, 2>, FEED>(g, gelu, s);
     case 4:
-      return alone    ? run<Cfg<128, 64, 2, 2, 1, 3>, FEED>(g, gelu, s)
-             : shortk ? run<Cfg<128, 64, 2, 2, 1, 1>, FEED>(g, gelu, s)
-                      : run<Cfg<128, 64, 2, 2, 1, 2>, FEED>(g, gelu, s);
+      return alone ? run<Cfg<128, 64, 2, 2, 1, 3>, FEED>(g, gelu, s)
+                   : run<Cfg<128, 64, 2, 2, 1, 2>, FEED>(g, gelu, s);
     case 5:
       return alone                    ? run<Cfg<64, 64, 2, 2, 2, 3>, FEED>(g, gelu, s)
              : shortk                 ? run<Cfg<64, 64, 2, 2, 1, 1>, FEED>(g, gelu, s)
@@ -742,6 +741,10 @@ hipError_t dispatch(const Args& g, bool gelu, hipStream_t s) {
                                       : run<Cfg<32, 32, 1, 1, 4, 2>, FEED>(g, gelu, s);
     case 8: return run<Cfg<16, 32, 1, 1, 4, 4>, FEED>(g, gelu, s);
     default:
+      // (Shifting takes a wavefront's time, so fewer slices each: 5 x 384 x 9677 7.3 us
+      // with eight groups, 8.9 with four; 2 x 148 x 2227 4.8 and 5.1.)
+      if constexpr (FEED == kShifted)
+        if (rounds == 1 && K > 1536) return run<Cfg<16, 16, 1, 1, 8, 2>, FEED>(g, gelu, s);
       return one_wave    ? run<Cfg<16, 16, 1, 1, 1, 2>, FEED>(g, gelu, s)
              : K <= 1536 ? run<Cfg<16, 16, 1, 1, 2, 2>, FEED>(g, gelu, s)
                          : run<Cfg<16, 16, 1, 1, 4, 4>, FEED>(g, gelu, s);

@@ -517,7 +517,10 @@ TILES = [(1, 17, 523), (1, 17, 1785), (1, 16, 37), (2429, 19, 1829), (17, 2202, 
          (18, 6612, 617), (4136, 17, 395), (8, 12772, 1049), (1, 8817, 33), (8, 29729, 1107),
          (1, 21477, 33), (20, 19787, 1027), (8297, 71, 185), (154, 17305, 305), (17352, 22, 1105),
          (73, 8539, 193), (16913, 131, 337), (76, 16445, 1047), (18750, 67, 33), (66, 44845, 37),
-         (137, 23991, 763), (51309, 139, 403), (4001, 3999, 517)]
+         (137, 23991, 763), (51309, 139, 403), (4001, 3999, 517), (17, 7229, 409), (17, 6344, 557),
+         (18231, 17, 1913), (66, 9224, 105), (10, 12423, 1125), (17, 8775, 37), (18543, 18, 1029),
+         (17, 17406, 2005), (8634, 75, 281), (551, 6690, 505), (16582, 42, 1141), (68, 11134, 465),
+         (139, 21858, 1477), (130, 52084, 641)]
 
 
 @gpu
