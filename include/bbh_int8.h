@@ -60,8 +60,11 @@ bbh_status bbh_layernorm_quantize(const void *x, const void *residual, const voi
  * sum_k A[m,k] B[n,k] [+ bias[n]] [then GELU]; A (M, K) and B (N, K) int8,
  * a_scale (M) and b_scale (N) fp32, bias (N) fp16 or NULL.  The sum is exact in
  * int32, the rest fp32, rounded to fp16 once, so a result does not depend on M
- * or on how the work is split.  Any M, N >= 1 and 1 <= K <= BBH_I8_MAX_K, any
- * alignment of A and B; K % 16 == 0 with A and B 16-byte aligned is fastest. */
+ * or on how the work is split.  GELU is within 7.6e-5 of the exact-erf form for
+ * values of any size.  Any M, N >= 1 and 1 <= K <= BBH_I8_MAX_K, any alignment
+ * of A and B (of which, where it is no multiple of 4, the 4-byte words around
+ * the first and last bytes are read); fastest where K and the addresses of A and
+ * B are multiples of 16, then of 4. */
 bbh_status bbh_linear_i8(const int8_t *A, const float *a_scale, const int8_t *B,
                          const float *b_scale, void *C, int M, int N, int K, const void *bias,
                          int gelu, bbh_stream_t stream);
