@@ -640,6 +640,56 @@ def test_offsets_past_32_bits(torch_cuda):
         _linear_check(torch, A[a:a + 40], sa[a:a + 40], B, sb, bias, False, C[a:a + 40])
 
 
+@gpu
+def test_offsets_past_32_bits_at_odd_addresses(torch_cuda):
+    """600001 rows of 4093 codes (2.5e9) from an odd address, as A and as B."""
+    from bbh import engine
+
+    torch = torch_cuda
+    M, K = 600001, 4093
+    a = torch.zeros(M * K + 1, dtype=torch.int8, device="cuda")
+    A = a[1:].view(M, K)
+    g = _gen(torch, 8)
+    A[M - 7:] = torch.randint(-128, 128, (7, K), device="cuda", generator=g).to(torch.int8)
+    sa = torch.rand(M, device="cuda", generator=g) * 1e-3
+    B, sb = A[M - 7:], sa[M - 7:].clone()
+    C = torch.empty(M, 7, dtype=torch.float16, device="cuda")
+    engine.launch_matmul_i8(A, sa, B, sb, C, M, 7, K)
+    _linear_check(torch, A[M - 7:], sa[M - 7:], B, sb, None, False, C[M - 7:])
+    assert not bool(C[:M - 7].any())
+    Ct = torch.empty(7, M, dtype=torch.float16, device="cuda")
+    engine.launch_matmul_i8(B, sb, A, sa, Ct, 7, M, K)
+    _linear_check(torch, B, sb, A[M - 7:], sa[M - 7:], None, False, Ct[:, M - 7:])
+    assert not bool(Ct[:, :M - 7].any())
+
+
+@gpu
+def test_more_workgroups_than_one_grid_dimension(torch_cuda):
+    """Launches of more than 2^21 workgroups: 34 million rows of 3, 40 million
+    output columns."""
+    from bbh import engine
+
+    torch = torch_cuda
+    M, D = (1 << 21) * 16 + 37, 3
+    x = _half(torch, _gen(torch, 1), M, D)
+    q = torch.empty(M, D, dtype=torch.int8, device="cuda")
+    s = torch.empty(M, device="cuda")
+    engine.launch_quantize_rows(x, q, s, M, D)
+    a = x.float().abs().amax(1)
+    assert torch.equal(s, (a.double() / 127).float())  # (torch divides fp32 by 1 / 127)
+    assert torch.equal(q[::997].double(), _codes64(torch, x[::997].double())[0].round())
+    assert bool((q[M - 40:].abs().amax(1) == 127).all())
+    engine.launch_dequantize_rows(q, s, x, M, D)
+    assert torch.equal(x, (q.float() * s[:, None]).half())
+    N = 40000003
+    B = torch.randint(-128, 128, (N, 1), device="cuda", dtype=torch.int8)
+    A = torch.tensor([[3]], dtype=torch.int8, device="cuda")
+    sb = torch.full((N,), 0.5, device="cuda")
+    C = torch.empty(1, N, dtype=torch.float16, device="cuda")
+    engine.launch_matmul_i8(A, sb[:1], B, sb, C, 1, N, 1)
+    assert torch.equal(C[0], B[:, 0].half() * 0.75)
+
+
 def _ffn(torch, engine, st, stream=None):
     m, d, f = st["m"], st["d"], st["f"]
     engine.launch_layernorm_quantize(st["x"], st["gamma"], st["beta"], st["q"], st["s"], m, d,
