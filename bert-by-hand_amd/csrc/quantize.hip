@@ -195,24 +195,39 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_kernel(const f16* 
         if (t + T * i < chunks) store8<STREAM>(a.sum + off, t + T * i, D, v[i]);
     }
     if constexpr (KIND == kLayer) {
-      float s = 0.f;
+      // Twice: the mean of rows of nearly equal values is off by more than they
+      // deviate (a rounded sum), so the deviations' own mean comes off them too.
+      // Of equal values nothing is left then: the deviations are a few steps of
+      // fp32, all alike, and their sum and its quotient exact.
+      // (1 x 384 2.3 us with one mean, 2.4 with both; 8192 x 384 8.2 either way,
+      // 131072 x 32 15.4 and 16.1.)
 #pragma unroll
-      for (int i = 0; i < V; ++i)
+      for (int pass = 0; pass < 2; ++pass) {
+        float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += v[i][e];
-      const float mean = row_reduce<T>(s, AddOp{}, part[0]) / (float)D;
+        for (int i = 0; i < V; ++i)
 #pragma unroll
-      for (int i = 0; i < V; ++i)
+          for (int e = 0; e < 8; ++e) s += v[i][e];
+        const float mean = row_reduce<T>(s, AddOp{}, part[pass]) / (float)D;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          v[i][e] = (t + T * i) * 8 + e < D ? v[i][e] - mean : 0.f;
+        for (int i = 0; i < V; ++i) {
+          const int n = D - (t + T * i) * 8;  // values of this chunk
+          if (n >= 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] -= mean;
+          } else if (n > 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] -= e < n ? mean : 0.f;
+          }
+        }
+      }
     }
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += v[i][e] * v[i][e];
-    const float rstd = rsqrtf(row_reduce<T>(s, AddOp{}, part[1]) / (float)D + a.eps);
+    const float rstd = rsqrtf(row_reduce<T>(s, AddOp{}, part[2]) / (float)D + a.eps);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
 #pragma unroll
@@ -228,7 +243,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_kernel(const f16* 
   for (int i = 0; i < V; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = UMaxOp{}(m, fabsf(v[i][e]));
-  const Coder k(row_reduce<T>(m, UMaxOp{}, part[2]));
+  const Coder k(row_reduce<T>(m, UMaxOp{}, part[3]));
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = t + T * i;

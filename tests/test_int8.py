@@ -856,3 +856,76 @@ def test_python_checks_sizes_and_layout(torch_cuda):
     assert e.value.name == "BBH_ERR_INVALID_ARG"
     with pytest.raises(TypeError):
         engine.launch_dequantize_rows(q.cpu(), s, x, 4, 8)
+
+
+def _layernorm64(torch, h, gamma, beta, eps):
+    """LayerNorm of h (fp32, as the kernels hold it) in 64 bits, and how far the
+    kernel's may be off.  Rows of nearly equal values: h - mean is exact, the mean
+    off by 46 u of the row's size, which the deviations' own mean takes off again up
+    to 46 u of the deviations (that error of the first mean among them)."""
+    h = h.double()
+    d = h - h.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt((d * d).mean(1, keepdim=True) + eps)
+    v = d * rstd * gamma.double() + beta.double()
+    first = 46 * U * h.abs().mean(1, keepdim=True)
+    move = 46 * U * (d.abs().mean(1, keepdim=True) + first) + U * d.abs()
+    # rstd: half of the variance's 45 u and of twice the move, 3 u of its own; three roundings more
+    rel = 26 * U + move.mean(1, keepdim=True) * rstd
+    e = gamma.double().abs() * rstd * (move + d.abs() * rel) + 3 * U * v.abs()
+    return v, e
+
+
+@gpu
+@pytest.mark.parametrize("M", [3, 5000])
+@pytest.mark.parametrize("D", [5, 24, 100, 384, 385, 500, 1000, 1536, 2047, 5000, 8191, 16384])
+def test_layernorm_of_equal_and_nearly_equal_values(torch_cuda, M, D):
+    """Rows whose sums fp32 does not hold exactly.  Equal values: the deviations
+    are a few steps of fp32, all alike, so their sum (below 2^24 steps) and its
+    quotient are exact and nothing is left of them: the result is beta, bit for
+    bit.  Nearly equal ones: the deviations count, not the mean's rounding."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, D + M)
+    size = 10 ** (6 * torch.rand(M, 1, device="cuda", generator=g) - 2)
+    x = (size * (1 + torch.rand(M, 1, device="cuda", generator=g))).clamp(max=6e4).half()
+    r = (x * 1e-4 * (1 + torch.rand(M, 1, device="cuda", generator=g))).half()
+    x[:3, 0], r[:3, 0] = 1000, 0.1
+    x, r = x.expand(M, D).contiguous(), r.expand(M, D).contiguous()
+    gamma, beta = _half(torch, g, D, scale=0.3) + 1, _half(torch, g, D)
+    q = torch.empty(M, D, dtype=torch.int8, device="cuda")
+    s = torch.empty(M, device="cuda")
+    y = torch.empty(M, D, dtype=torch.float16, device="cuda")
+    engine.launch_layernorm_quantize(x, gamma, beta, q, s, M, D, residual=r, y=y)
+    bad = (y != beta).any(1)
+    assert not bool(bad.any()), (int(bad.sum()), y[bad][0, :4].tolist(), beta[:4].tolist())
+    c64, s64 = _codes64(torch, beta.double()[None])
+    assert torch.equal(q.double(), c64.round().expand(M, D))
+    assert torch.equal(s, s64.float().expand(M))
+
+    # one value of a row, then every third, moved by a few hundredths of a per cent
+    for step in (D, 3):
+        z = r.clone()
+        z[:, ::step] = (z[:, ::step].float() * 2).half()
+        v, e = _layernorm64(torch, x.float() + z.float(), gamma, beta, 1e-12)
+        engine.launch_layernorm_quantize(x, gamma, beta, q, s, M, D, residual=z, y=y)
+        err = (y.double() - v).abs() - (v.abs() * H + e * (1 + H) + TINY)
+        assert float(err.max()) <= 0, float(err.max())
+        a, ea = v.abs().amax(1), e.amax(1)
+        assert bool(((s.double() - a / 127).abs() <= (ea + 2 * U * a) / 127).all())
+
+
+@gpu
+@pytest.mark.parametrize("M,D", [(3, 384), (5000, 384), (3, 1001), (5000, 12001)])
+def test_layernorm_of_equal_values_without_eps(torch_cuda, M, D):
+    """eps 0 is the formula's: 0 / 0, whether or not the row's sum is exact."""
+    from bbh import engine
+
+    torch = torch_cuda
+    x = _half(torch, _gen(torch, D), M, D)
+    x[1], r = 1000, torch.full((M, D), 0.1, device="cuda").half()
+    gamma, beta = torch.ones(D, device="cuda").half(), torch.zeros(D, device="cuda").half()
+    q = torch.full((M, D), 55, dtype=torch.int8, device="cuda")
+    s = torch.empty(M, device="cuda")
+    engine.launch_layernorm_quantize(x, gamma, beta, q, s, M, D, eps=0.0, residual=r)
+    assert bool((q[1] == 0).all()) and torch.isnan(s).nonzero().tolist() == [[1]]
