@@ -486,6 +486,8 @@ def _place(t, stream, *sizes):
     object 3 us."""
     if min(sizes) < 1:
         raise ValueError("sizes must be positive")
+    if max(sizes) > 2147483647:  # ctypes would pass 2^32 + 1 on as 1
+        raise ValueError("sizes must fit a C int")
     if not t.is_cuda:
         raise TypeError("operands must be CUDA tensors")
     c = _torch()._C

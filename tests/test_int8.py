@@ -929,3 +929,24 @@ def test_layernorm_of_equal_values_without_eps(torch_cuda, M, D):
     s = torch.empty(M, device="cuda")
     engine.launch_layernorm_quantize(x, gamma, beta, q, s, M, D, eps=0.0, residual=r)
     assert bool((q[1] == 0).all()) and torch.isnan(s).nonzero().tolist() == [[1]]
+
+
+@pytest.mark.parametrize("big", [2 ** 31, 2 ** 32 + 1])
+def test_python_refuses_sizes_that_c_int_does_not_hold(big):
+    """ctypes would pass 2^32 + 1 rows on as one."""
+    import torch
+    from bbh import engine
+
+    x, q, s = torch.zeros(4, 8).half(), torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4)
+    for m, d in ((big, 1), (1, big)):
+        with pytest.raises(ValueError):
+            engine.launch_quantize_rows(x, q, s, m, d)
+        with pytest.raises(ValueError):
+            engine.launch_dequantize_rows(q, s, x, m, d)
+        with pytest.raises(ValueError):
+            engine.launch_rmsnorm_quantize(x, x[0], q, s, m, d)
+        with pytest.raises(ValueError):
+            engine.launch_layernorm_quantize(x, x[0], x[1], q, s, m, d)
+    for sizes in ((big, 1, 1), (1, big, 1), (1, 1, big)):
+        with pytest.raises(ValueError):
+            engine.launch_matmul_i8(q, s, q, s, x, *sizes)
