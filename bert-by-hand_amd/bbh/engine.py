@@ -12,6 +12,7 @@ work on the current stream; errors raise ``BBHError`` instead of aborting.
 from __future__ import annotations
 
 import ctypes
+from operator import index
 
 import numpy as np
 
@@ -480,26 +481,30 @@ def _operand(name, t, dtype, n, device):
 
 
 def _place(t, stream, *sizes):
-    """(current device, stream) of a launch that has t as an operand.  A launch
+    """(current device, stream, the sizes as plain ints, whose products have no
+    width to wrap at) of a launch that has t as an operand.  A launch
     of a few microseconds on the GPU is bound by the host's part of the call:
     reading the stream from torch's C layer takes 0.2 us, a torch.cuda.Stream
     object 3 us."""
-    if min(sizes) < 1:
-        raise ValueError("sizes must be positive")
-    if max(sizes) > 2147483647:  # ctypes would pass 2^32 + 1 on as 1
-        raise ValueError("sizes must fit a C int")
+    for n in sizes:
+        if n.__class__ is not int:  # numpy's, say
+            return _place(t, stream, *(int(index(n)) for n in sizes))
+        if n < 1:
+            raise ValueError("sizes must be positive")
+        if n > 2147483647:  # ctypes would pass 2^32 + 1 on as 1
+            raise ValueError("sizes must fit a C int")
     if not t.is_cuda:
         raise TypeError("operands must be CUDA tensors")
     c = _torch()._C
     device = c._cuda_getDevice()
-    return device, c._cuda_getCurrentRawStream(device) if stream is None else stream
+    return device, c._cuda_getCurrentRawStream(device) if stream is None else stream, *sizes
 
 
 def launch_quantize_rows(x, q, scale, M, D, stream=None):
     """x (M, D) fp16 -> q (M, D) int8, scale (M) fp32: one scale a row, the
     largest magnitude / 127 (bbh_quantize_rows)."""
     torch = _torch()
-    dev, s = _place(x, stream, M, D)
+    dev, s, M, D = _place(x, stream, M, D)
     call("bbh_quantize_rows", _operand("x", x, torch.float16, M * D, dev),
          _operand("q", q, torch.int8, M * D, dev), _operand("scale", scale, torch.float32, M, dev),
          M, D, s)
@@ -509,7 +514,7 @@ def launch_quantize_rows(x, q, scale, M, D, stream=None):
 def launch_dequantize_rows(q, scale, x, M, D, stream=None):
     """x (M, D) fp16 = q * scale, row by row (bbh_dequantize_rows)."""
     torch = _torch()
-    dev, s = _place(q, stream, M, D)
+    dev, s, M, D = _place(q, stream, M, D)
     call("bbh_dequantize_rows", _operand("q", q, torch.int8, M * D, dev),
          _operand("scale", scale, torch.float32, M, dev),
          _operand("x", x, torch.float16, M * D, dev), M, D, s)
@@ -522,8 +527,8 @@ def launch_rmsnorm_quantize(x, gamma, q, scale, M, D, eps=1e-6, residual=None, s
     q, scale; sum (x + residual) and y (the norm) get fp16 where given
     (bbh_rmsnorm_quantize)."""
     torch = _torch()
+    dev, s, M, D = _place(x, stream, M, D)
     f16, n = torch.float16, M * D
-    dev, s = _place(x, stream, M, D)
     call("bbh_rmsnorm_quantize", _operand("x", x, f16, n, dev),
          _operand("residual", residual, f16, n, dev), _operand("gamma", gamma, f16, D, dev),
          _operand("sum", sum, f16, n, dev), _operand("y", y, f16, n, dev),
@@ -536,8 +541,8 @@ def launch_layernorm_quantize(x, gamma, beta, q, scale, M, D, eps=LAYER_NORM_EPS
                               sum=None, y=None, stream=None):
     """launch_rmsnorm_quantize for LayerNorm (bbh_layernorm_quantize)."""
     torch = _torch()
+    dev, s, M, D = _place(x, stream, M, D)
     f16, n = torch.float16, M * D
-    dev, s = _place(x, stream, M, D)
     call("bbh_layernorm_quantize", _operand("x", x, f16, n, dev),
          _operand("residual", residual, f16, n, dev), _operand("gamma", gamma, f16, D, dev),
          _operand("beta", beta, f16, D, dev), _operand("sum", sum, f16, n, dev),
@@ -551,7 +556,7 @@ def launch_matmul_i8(A, a_scale, B, b_scale, C, M, N, K, bias=None, gelu=False, 
     (A (M, K) . B (N, K)^T) [+ bias] [GELU], the sums exact (bbh_linear_i8)."""
     torch = _torch()
     i8, f32, f16 = torch.int8, torch.float32, torch.float16
-    dev, s = _place(A, stream, M, N, K)
+    dev, s, M, N, K = _place(A, stream, M, N, K)
     call("bbh_linear_i8", _operand("A", A, i8, M * K, dev), _operand("a_scale", a_scale, f32, M, dev),
          _operand("B", B, i8, N * K, dev), _operand("b_scale", b_scale, f32, N, dev),
          _operand("C", C, f16, M * N, dev), M, N, K, _operand("bias", bias, f16, N, dev),

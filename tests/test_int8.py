@@ -950,3 +950,31 @@ def test_python_refuses_sizes_that_c_int_does_not_hold(big):
     for sizes in ((big, 1, 1), (1, big, 1), (1, 1, big)):
         with pytest.raises(ValueError):
             engine.launch_matmul_i8(q, s, q, s, x, *sizes)
+
+
+@gpu
+def test_python_sizes_of_other_integer_types(torch_cuda, monkeypatch):
+    """numpy's 32-bit integers: their product would wrap to 0, and an operand of any
+    size would do.  Nothing is launched here."""
+    from bbh import engine
+
+    torch = torch_cuda
+    launched = []
+    monkeypatch.setattr(engine, "call", lambda *a: launched.append(a))
+    x = torch.zeros(4, 8, dtype=torch.float16, device="cuda")
+    q, s = torch.zeros(4, 8, dtype=torch.int8, device="cuda"), torch.zeros(65536, device="cuda")
+    n = np.int32(65536)
+    with np.errstate(over="ignore"):
+        with pytest.raises(ValueError):
+            engine.launch_quantize_rows(x, q, s, n, n)
+        with pytest.raises(ValueError):
+            engine.launch_dequantize_rows(q, s, x, n, n)
+        with pytest.raises(ValueError):
+            engine.launch_rmsnorm_quantize(x, s.half(), q, s, n, n)
+        with pytest.raises(ValueError):
+            engine.launch_layernorm_quantize(x, s.half(), s.half(), q, s, n, n)
+        with pytest.raises(ValueError):
+            engine.launch_matmul_i8(q, s, q, s, x, n, n, n)
+    assert not launched
+    engine.launch_quantize_rows(x, q, s, np.int32(4), np.int64(8))
+    assert len(launched) == 1 and launched[0][4:6] == (4, 8)
