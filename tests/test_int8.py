@@ -978,3 +978,45 @@ def test_python_sizes_of_other_integer_types(torch_cuda, monkeypatch):
     assert not launched
     engine.launch_quantize_rows(x, q, s, np.int32(4), np.int64(8))
     assert len(launched) == 1 and launched[0][4:6] == (4, 8)
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_linear_i8_every_tile_with_gelu(torch_cuda, M, N, K):
+    """And without: every output is a number (a comparison with NaN finds none too
+    far off)."""
+    from bbh import engine
+
+    torch = torch_cuda
+    for k in (K, (K + 3) // 4 * 4, (K + 15) // 16 * 16):
+        A, sa, B, sb, bias = _operands(torch, M + N + k, M, N, k)
+        for gelu in (False, True):
+            buf, C = _guarded(torch, M * N, torch.float16, 3.0)
+            engine.launch_matmul_i8(A, sa, B, sb, C, M, N, k, bias=bias, gelu=gelu)
+            assert bool(torch.isfinite(C).all())
+            _linear_check(torch, A, sa, B, sb, bias, gelu, C.view(M, N))
+            assert bool((buf[M * N:] == 3).all())
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(4548, 1, 1777), (106, 1566, 2413), (1, 8094, 6753), (6, 158037, 8437)])
+def test_linear_i8_four_groups_of_16_x_16_shifted(torch_cuda, M, N, K):
+    """Tiles of 16 x 16 over several rounds with a long odd K: four groups share it,
+    and each row of a tile is shifted by its own number of bytes."""
+    from bbh import engine
+
+    torch = torch_cuda
+    a, sa, b, sb, bias = _operands(torch, M + N, M, N, K)
+    for gelu in (False, True):
+        buf, C = _guarded(torch, M * N, torch.float16, 3.0)
+        engine.launch_matmul_i8(a, sa, b, sb, C, M, N, K, bias=bias, gelu=gelu)
+        assert bool(torch.isfinite(C).all())
+        _linear_check(torch, a, sa, b, sb, bias, gelu, C.view(M, N))
+        assert bool((buf[M * N:] == 3).all())
+    for oa, ob in ((1, 0), (0, 2), (3, 3)):  # the same codes from other addresses: the same bits
+        A, B = (torch.empty(t.numel() + 4, dtype=torch.int8, device="cuda")[o:o + t.numel()].view(t.shape)
+                for t, o in ((a, oa), (b, ob)))
+        A.copy_(a), B.copy_(b)
+        D = torch.empty(M, N, dtype=torch.float16, device="cuda")
+        engine.launch_matmul_i8(A, sa, B, sb, D, M, N, K, bias=bias, gelu=True)
+        assert torch.equal(D, C.view(M, N))
