@@ -1020,3 +1020,36 @@ def test_linear_i8_four_groups_of_16_x_16_shifted(torch_cuda, M, N, K):
         D = torch.empty(M, N, dtype=torch.float16, device="cuda")
         engine.launch_matmul_i8(A, sa, B, sb, D, M, N, K, bias=bias, gelu=True)
         assert torch.equal(D, C.view(M, N))
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K,lds", [(1024, 2048, 2048, 75008), (4096, 4096, 4096, 138240),
+                                       (16, 4096, 4096, 65728)])
+def test_large_lds_captured_before_any_eager_call(torch_cuda, M, N, K, lds):
+    """Launches whose kernels need more LDS than 64 KB (64 x 128 tiles in a ring of
+    three slices, 256 x 256 in one of two, four groups of 16 x 16), which has to be
+    allowed once: also where that first time is inside a capture."""
+    code = """
+import sys; sys.path.insert(0, %r)
+import torch
+from bbh import engine
+M, N, K = %d, %d, %d
+A = torch.randint(-128, 128, (M, K), dtype=torch.int8, device="cuda")
+B = torch.randint(-128, 128, (N, K), dtype=torch.int8, device="cuda")
+s = torch.rand(max(M, N), device="cuda") / 64
+C = torch.zeros(M, N, dtype=torch.float16, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    engine.launch_matmul_i8(A, s, B, s, C, M, N, K)
+D = torch.empty_like(C)
+for i in range(3):
+    C.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    engine.launch_matmul_i8(A, s, B, s, D, M, N, K)
+    assert bool(C.any()) and bool(torch.isfinite(C).all()) and torch.equal(C, D)
+print("SAME")
+""" % (os.path.join(ROOT, "bert-by-hand_amd"), M, N, K)
+    assert lds > 64 * 1024
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "SAME" in r.stdout, r.stdout + r.stderr
