@@ -1053,3 +1053,34 @@ print("SAME")
     assert lds > 64 * 1024
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and "SAME" in r.stdout, r.stdout + r.stderr
+
+
+@gpu
+def test_quantize_rows_every_pair_of_mantissas(torch_cuda):
+    """Codes depend on the mantissas of x and a, 1024 each, and the gap g of their
+    exponents (9 and more: |127 x / a| < 0.5).  The nearest that a quotient comes to
+    a tie without being one is 2^-18.97 of itself (a = 2033, x = 2025; absolutely
+    2^-18.99 at a = 2031, x = 2047 / 256), which 64 bits and fp32's 2^-24 resolve."""
+    from bbh import engine
+
+    torch = torch_cuda
+    m = torch.arange(1024, 2048, device="cuda")
+    x = torch.cat([m.double() * 2.0 ** -g for g in range(10)])
+    x = torch.cat([x, -x])
+    rows = torch.minimum(x.abs()[None], m.double()[:, None]) * torch.sign(x)  # no value above a
+    rows = torch.cat([m.double()[:, None], rows], 1).half()
+    M, D = rows.shape
+    q = torch.empty(M, D, dtype=torch.int8, device="cuda")
+    s = torch.empty(M, device="cuda")
+    for D1 in (D, 10001, 1):  # rows read twice, kept in registers, and of a itself
+        part = rows[:, :D1].contiguous()
+        q1 = q.view(-1)[:M * D1].view(M, D1)
+        engine.launch_quantize_rows(part, q1, s, M, D1)
+        c64, s64 = _codes64(torch, part.double())
+        assert torch.equal(q1.double(), c64.round()) and torch.equal(s, s64.float())
+    near = torch.tensor([[2034, 1025 / 128, -1025 / 128], [2031, 2047 / 256, -2047 / 256],
+                         [2033, 2025, -2025]], device="cuda").half()
+    q = torch.empty(3, 3, dtype=torch.int8, device="cuda")
+    engine.launch_quantize_rows(near, q, s, 3, 3)
+    # 127 x / a: 0.5 - 2^-18, 0.5 + 2^-18.99 and 126.5 + 2^-12
+    assert q.tolist() == [[127, 0, 0], [127, 1, -1], [127, round(127 * 2025 / 2033), -round(127 * 2025 / 2033)]]
