@@ -265,6 +265,7 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
   extern __shared__ __align__(16) char smem[];
   constexpr bool SHIFTED = FEED == kShifted;
   constexpr bool TAIL = FEED != kCopies;  // the last slice goes through registers
+  static_assert(!TAIL || C::R > 1, "a ring of one slice has whole slices only");
   int bm, bn;
   if (!tile_of(tm, tn, bm, bn)) return;
   const int K = g.K, m0 = bm * C::BM, n0 = bn * C::BN;
@@ -710,31 +711,33 @@ hipError_t dispatch(const Args& g, bool gelu, hipStream_t s) {
   // 3488 60.8 and 58.6).  Where the last slice goes through registers a second
   // slice hides that better (4000 x 4000 x 2004 52.0 and 50.0, 5336 x 3392 x 1969
   // 77.0 and 67.5).
-  const bool one_slice = FEED == kCopies && rounds > 1 && K < 4096;
-  const bool shortk = one_slice && K <= 512;
+  if constexpr (FEED == kCopies) {
+    if (rounds > 1 && K < 4096) {
+      if (t == 2) return run<Cfg<128, 128, 4, 2, 1, 1>, FEED>(g, gelu, s);
+      if (t == 3 && K <= 512) return run<Cfg<64, 128, 1, 4, 1, 1>, FEED>(g, gelu, s);
+      if (t == 5 && K <= 512) return run<Cfg<64, 64, 2, 2, 1, 1>, FEED>(g, gelu, s);
+      if (t == 6 && K <= 512) return run<Cfg<32, 64, 1, 2, 1, 1>, FEED>(g, gelu, s);
+    }
+  }
   switch (t) {
     case 0: return run<Cfg<256, 256, 2, 4, 1, 2>, FEED>(g, gelu, s);
     case 1: return run<Cfg<256, 128, 4, 2, 1, 3>, FEED>(g, gelu, s);
     case 2:
-      return alone       ? run<Cfg<128, 128, 2, 4, 1, 3>, FEED>(g, gelu, s)
-             : one_slice ? run<Cfg<128, 128, 4, 2, 1, 1>, FEED>(g, gelu, s)
-                         : run<Cfg<128, 128, 4, 2, 1, 2>, FEED>(g, gelu, s);
+      return alone ? run<Cfg<128, 128, 2, 4, 1, 3>, FEED>(g, gelu, s)
+                   : run<Cfg<128, 128, 4, 2, 1, 2>, FEED>(g, gelu, s);
     case 3:
-      return alone    ? run<Cfg<64, 128, 2, 2, 1, 3>, FEED>(g, gelu, s)
-             : shortk ? run<Cfg<64, 128, 1, 4, 1, 1>, FEED>(g, gelu, s)
-                      : run<Cfg<64, 128, 1, 4, 1, 2>, FEED>(g, gelu, s);
+      return alone ? run<Cfg<64, 128, 2, 2, 1, 3>, FEED>(g, gelu, s)
+                   : run<Cfg<64, 128, 1, 4, 1, 2>, FEED>(g, gelu, s);
     case 4:
       return alone ? run<Cfg<128, 64, 2, 2, 1, 3>, FEED>(g, gelu, s)
                    : run<Cfg<128, 64, 2, 2, 1, 2>, FEED>(g, gelu, s);
     case 5:
-      return alone                    ? run<Cfg<64, 64, 2, 2, 2, 3>, FEED>(g, gelu, s)
-             : shortk                 ? run<Cfg<64, 64, 2, 2, 1, 1>, FEED>(g, gelu, s)
+      return alone                      ? run<Cfg<64, 64, 2, 2, 2, 3>, FEED>(g, gelu, s)
              : rounds == 2 && K >= 1024 ? run<Cfg<64, 64, 2, 2, 1, 3>, FEED>(g, gelu, s)
                                         : run<Cfg<64, 64, 2, 2, 1, 2>, FEED>(g, gelu, s);
     case 6:
-      return shortk       ? run<Cfg<32, 64, 1, 2, 1, 1>, FEED>(g, gelu, s)
-             : rounds > 2 ? run<Cfg<32, 64, 1, 2, 1, 2>, FEED>(g, gelu, s)
-                          : run<Cfg<32, 64, 1, 2, 2, 3>, FEED>(g, gelu, s);
+      return rounds > 2 ? run<Cfg<32, 64, 1, 2, 1, 2>, FEED>(g, gelu, s)
+                        : run<Cfg<32, 64, 1, 2, 2, 3>, FEED>(g, gelu, s);
     case 7:
       return alone                    ? run<Cfg<32, 32, 1, 1, 4, 4>, FEED>(g, gelu, s)
              : K <= 512 || rounds > 2 ? run<Cfg<32, 32, 1, 1, 1, 2>, FEED>(g, gelu, s)
