@@ -577,18 +577,19 @@ __global__ __launch_bounds__(C::THREADS) void gemm_i8_kernel(Args g, int tm, int
       }
     };
     // An output beyond an XCD's L2 is written past it, where it would displace the
-    // operands that other tiles read again: 8192 x 1536 x 384 12.4 -> 10.7 us, with
-    // the quantising that reads it 23.9 -> 22.3; but 512 x 1536 x 384 with that 8.0
-    // -> 8.2, and tiles of 256 x 256, whose operands are read less often, 51.8 ->
-    // 55.8 (8192 x 4096 x 1024).  Rows that are not whole lines, whose parts L2 would
-    // put together, only beside larger operands that no L2 holds (64 x 200003 x 384
-    // 24.3 -> 21.3, but 8192 x 1537 x 384 15.9 -> 17.7, 11678 x 3845 x 48 27 -> 40).
+    // operands that other tiles read again: 8192 x 1536 x 384 with GELU 15.9 -> 13.6
+    // us, 131072 x 384 x 384 47.9 -> 38.3, 2048 x 1536 x 384 6.5 -> 6.2 (inputs that
+    // change from call to call; the same ones again 14.9 -> 14.0, 38.6 -> 40.2, 5.9 both);
+    // but 512 x 1536 x 384 with the quantising that reads it 8.0 -> 8.2, and tiles of
+    // 256 x 256, whose operands are read less often, 51.8 -> 55.8 (8192 x 4096 x 1024).
+    // Only in rows of whole lines: L2 puts the parts of others together, which past
+    // it are written one by one (64 x 1000003 x 128 60 -> 119, 64 x 200003 x 384 25.7
+    // -> 31.0, 18.4 -> 21.5 with the same index again).
     // (The comments in the assembly keep the compiler from merging the two, which
     // would make every store an ordinary one.)
-    const int64_t written = (int64_t)g.M * g.N * 2, read = ((int64_t)g.M + g.N) * K;
+    const int64_t written = (int64_t)g.M * g.N * 2;
     const bool lines = ((uintptr_t)g.C | (uint32_t)g.N * 2) % 128 == 0;
-    if (C::BM * C::BN < 256 * 256 && written >= kXcdL2 &&
-        (lines || read > max(written, kXcds * kXcdL2))) {
+    if (C::BM * C::BN < 256 * 256 && written >= kXcdL2 && lines) {
       asm volatile("; past L2" ::: "memory");
       write(std::true_type{});
       asm volatile("; end past L2" ::: "memory");
