@@ -10,12 +10,17 @@
 // transposed tile D(n, m) = B . A^T, so that a lane holds runs of four
 // consecutive output columns of one row.
 //
-// Bounds, measured on MI355X: large products the matrix cores at the clock that
-// power leaves them (8192^3 440 us, 2.5 POP/s, at 1.65 GHz; independent products
-// on random codes reach 3.5); few rows against many the reading of B (64 x 200003
-// x 384 21.0 us, 4.9 TB/s with its output); a short K its copies from L2, epilogue
-// and stores in turn (8192 x 1536 x 384 with GELU 14.4 us); the smallest a launch
-// and one latency (16 x 1536 x 384 2.7 us, 1 x 4096 x 4096 5.4).
+// Bounds, measured on MI355X: large products the clock that power leaves the
+// matrix cores, and that they idle a third of its cycles (8192^3 440-470 us, 2.3-2.5
+// POP/s, 66% busy at 1.65-1.7 GHz; independent products on random codes reach 3.48,
+// always busy at that clock): a slice's copies take as long as its products, and
+// with two slots they are asked for in one burst after each barrier; few rows
+// against many the waits of a workgroup's three steps a slice more than the reading
+// of B (64 x 200003 x 384 25.7 us, 4.0 TB/s with its output, of a new index each time;
+// 18.4 of the same one, from the memory-side cache in part), as each of the 64 x 64
+// tiles copies A again; a short K its copies from L2, epilogue and stores in turn
+// (8192 x 1536 x 384 with GELU 14.0 us); the smallest a launch and one latency (16 x
+// 1536 x 384 3.0 us, 1 x 4096 x 4096 5.6).
 //
 // K goes in slices of 128 bytes: a row of a slice is one cache line, eight
 // 16-byte chunks, and logical chunk c of row r sits in slot c ^ ((r >> 1) & 7)

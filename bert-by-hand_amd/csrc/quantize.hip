@@ -3,10 +3,10 @@
 //
 // A row's codes need its largest magnitude first, so the row stays in
 // registers between the reductions and its values are read once and written
-// once: bound by HBM, at 5.8-6.5 TB/s of those bytes from 100 MB of rows on
-// (65536 x 1536 quantised in 52 us and read back in 50; LayerNorm of 131072 x
-// 384 with residual and y 55, RMS norm of 16384 x 4096 73), and by a launch and
-// its first latency below a few hundred rows (2003 x 384: 2.8-3.6 us).  T
+// once: bound by HBM, at 6.1-6.7 TB/s of those bytes from 100 MB of rows on
+// (65536 x 1536 quantised in 49 us and read back in 50; LayerNorm of 131072 x
+// 384 with residual and y 56, RMS norm of 16384 x 4096 71), and by a launch and
+// its first latency below a few hundred rows (2003 x 384: 2.8-4.1 us).  T
 // threads own a row, thread t the 8-wide chunks t, t + T, ..., V of them:
 // 16-byte loads, 8-byte stores of codes, any row length and alignment (the last
 // chunk of a row goes element by element).
@@ -334,18 +334,26 @@ hipError_t quantize_as(const f16* x, int8_t* q, float* scale, int M, int D, cons
   // Threads a row: as few as leave a thread at most four chunks, so that the
   // lanes are full and the reductions short; more where rows are too few to fill
   // the GPU and a thread's chunks would queue behind each other.  Measured, us
-  // (quantise / LayerNorm with residual and y):
-  //   131072 x 32     16 threads  8.4 / 15.4   64 threads  27.5 / 52.1
-  //   131072 x 384    16 x 3     26.1 / 55.3   64 x 1      37.2 / 62.7
-  //   2003 x 384      16 x 3      3.1 /  4.5   64 x 1       2.8 /  3.6
-  //   131072 x 512    16 x 4     33.4 / 72.1   64 x 1      37.9 / 73.9
-  //   30000 x 512     16 x 4     10.1 / 22.1   64 x 1       9.7 / 20.4
-  //   65536 x 1536    64 x 3     52.2 / 112    256 x 1     66.2 / 128
-  //   65536 x 1792    64 x 4     60.3 / 134    256 x 1     73.4 / 141
-  //   5000 x 1700     64 x 4      8.8 / 17.5   256 x 1      8.2 / 16.9
-  //   700 x 2048      64 x 4      3.6 /  5.4   256 x 1      3.1 /  4.5
-  //   8192 x 8192    256 x 4     34.3 / 76.1   1024 x 1    43.2 / 93.2
-  //   1 x 8192       256 x 4      3.1 /  4.8   1024 x 1     2.7 /  4.0
+  // (quantise / LayerNorm with residual and y; inputs that change from call to
+  // call):
+  //   131072 x 32     16 threads  8.3 / 16.5   64 threads  25.9 / 56.0
+  //   2003 x 384      16 x 3      3.1 /  4.8   64 x 1       2.8 /  4.1
+  //   4096 x 384      16 x 3      3.5 /  5.5   64 x 1       3.5 /  5.5
+  //   8192 x 384      16 x 3      4.3 /  7.5   64 x 1       4.4 /  7.9
+  //   32768 x 384     16 x 3      9.8 / 20.3   64 x 1      11.5 / 20.8
+  //   131072 x 384    16 x 3     26.7 / 55.9   64 x 1      34.5 / 69.4
+  //   2048 x 256      16 x 2      2.7 /  3.8   64 x 1       2.7 /  3.6
+  //   4096 x 256      16 x 2      2.8 /  4.5   64 x 1       3.1 /  5.2
+  //   30000 x 512     16 x 4     11.9 / 23.9   64 x 1      12.0 / 22.1
+  //   131072 x 512    16 x 4     34.2 / 74.1   64 x 1      38.0 / 74.9
+  //   700 x 2048      64 x 4      3.6 /  5.8   256 x 1      3.3 /  5.3
+  //   5000 x 1700     64 x 4      9.1 / 21.3   256 x 1      9.0 / 22.4
+  //   65536 x 1536    64 x 3     48.8 / 105    256 x 1     64.7 / 137
+  //   65536 x 1792    64 x 4     57.7 / 126    256 x 1     70.1 / 146
+  //   1 x 8192       256 x 4      3.0 /  5.2   1024 x 1     2.7 /  4.3
+  //   100 x 8192     256 x 4      3.4 /  6.0   1024 x 1     3.0 /  5.3
+  //   2048 x 8192    256 x 4     13.0 / 26.6   1024 x 1    14.0 / 28.4
+  //   8192 x 8192    256 x 4     34.5 / 78.5   1024 x 1    43.7 / 93.7
   const int chunks = (D + 7) / 8;
   const bool many = M >= 4096;
   if (chunks <= 16) return launch<16, 1, KIND, STREAM>(x, q, scale, M, D, a, s);
@@ -374,11 +382,13 @@ hipError_t quantize_as(const f16* x, int8_t* q, float* scale, int M, int D, cons
 // fp16 rows of this many bytes and more are read and written past the caches
 // (non-temporal): they would push out of the memory-side cache what the next
 // operators find there, the codes among it, and be gone themselves before anyone
-// came back to them.  Quantising and reading back 131072 x 384 (96 MB) 55.2 us
-// without, 50.0 with; LayerNorm with residual and y, read back, and the values
-// quantised again, where the reader right behind finds less: 115 and 104; the
-// first of 43690 x 384 (32 MB) 19.8 and 20.8.  Values read back stay in the
-// caches up to twice the size.
+// came back to them.  Quantising and reading back 131072 x 384 (96 MB) 54.5 us
+// without, 49.4 with; LayerNorm with residual and y 64.0 and 55.9, of 65536 x 384 34.5
+// and 30.5.  Inputs that the call before read are the other side: 47.2 and 49.6,
+// 62.4 and 56.2, 28.5 and 30.0; 20.1 and 23.9 for quantising and reading back 43690 x
+// 384 (32 MB), so smaller ones stay in the caches.  (Rows of 63, whose lines are
+// shared: LayerNorm of 400003 93.5 and 98.0, 68.3 and 96.8.)  Values read back stay
+// up to twice the size.
 constexpr int64_t kStreamBytes = 48 << 20;
 bool streams(int M, int D, int64_t bytes) { return (int64_t)M * D * 2 >= bytes; }
 

@@ -35,7 +35,8 @@ extern "C" {
  * scale a token), weights (N, K) (a scale an output channel) and embeddings. */
 bbh_status bbh_quantize_rows(const void *x, int8_t *q, float *scale, int M, int D,
                              bbh_stream_t stream);
-/* x (M, D) fp16 = q * scale, one rounding; D <= BBH_I8_MAX_K.  Any int8 codes. */
+/* x (M, D) fp16 = q * scale in fp32, rounded to fp16; D <= BBH_I8_MAX_K.  Any int8
+ * codes. */
 bbh_status bbh_dequantize_rows(const int8_t *q, const float *scale, void *x, int M, int D,
                                bbh_stream_t stream);
 
@@ -48,7 +49,9 @@ bbh_status bbh_dequantize_rows(const int8_t *q, const float *scale, void *x, int
  * (optional, fp16) gets v, which a post-norm block adds later.  x, residual,
  * gamma, beta: fp16.  sum and y may each be x or residual, but not each other;
  * q and scale overlap nothing.  With eps 0 a row of zeros (rmsnorm) or of equal
- * values (layernorm) is the formula's 0 / 0: a row with a NaN. */
+ * values (layernorm) is the formula's 0 / 0: a row with a NaN.  Sums are fp32, in
+ * an order that goes with D and M, so a row's last bits may differ with the number
+ * of rows it is among (its codes where a value lies at a tie). */
 bbh_status bbh_rmsnorm_quantize(const void *x, const void *residual, const void *gamma,
                                 void *sum, void *y, int8_t *q, float *scale, int M, int D,
                                 float eps, bbh_stream_t stream);
@@ -59,9 +62,11 @@ bbh_status bbh_layernorm_quantize(const void *x, const void *residual, const voi
 /* bbh_linear on 8-bit rows: C(M,N) fp16 = a_scale[m] * b_scale[n] *
  * sum_k A[m,k] B[n,k] [+ bias[n]] [then GELU]; A (M, K) and B (N, K) int8,
  * a_scale (M) and b_scale (N) fp32, bias (N) fp16 or NULL.  The sum is exact in
- * int32, the rest fp32, rounded to fp16 once, so a result does not depend on M
- * or on how the work is split.  GELU is within 7.6e-5 of the exact-erf form for
- * values of any size.  Any M, N >= 1 and 1 <= K <= BBH_I8_MAX_K, any alignment
+ * int32, the rest fp32 (the sum times a_scale, that times b_scale), rounded to fp16
+ * once, so a result does not depend on M or on how the work is split.  GELU is
+ * within 7.6e-5 of the exact-erf form for values of any size; that is absolute: of
+ * values below about -4.1, whose GELU is as small, no digit need be right (-3.0e-5
+ * from -4.5 on).  Any M, N >= 1 and 1 <= K <= BBH_I8_MAX_K, any alignment
  * of A and B (of which, where it is no multiple of 4, the 4-byte words around
  * the first and last bytes are read); fastest where K and the addresses of A and
  * B are multiples of 16, then of 4. */
