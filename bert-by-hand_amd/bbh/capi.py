@@ -1,5 +1,5 @@
-"""ctypes binding of include/bbh.h and include/bbh_int8.h (libbbh.so, built
-in-tree by the Makefile).
+"""ctypes binding of include/bbh.h, include/bbh_int8.h and include/bbh_attend.h
+(libbbh.so, built in-tree by the Makefile).
 
 There is deliberately no fallback: if libbbh.so is missing or fails to load,
 importing the product path raises.  Nothing here computes anything on the CPU.
@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(os.path.dirname(_HERE), "libbbh.so")
 
 c_int, c_float, c_size_t, c_void_p, c_char_p = (ctypes.c_int, ctypes.c_float, ctypes.c_size_t,
                                                ctypes.c_void_p, ctypes.c_char_p)
+c_i64 = ctypes.c_int64
 c_i32p = ctypes.POINTER(ctypes.c_int32)
 
 
@@ -32,6 +33,36 @@ class LaunchTime(ctypes.Structure):
     """bbh_launch_time: one timed op launch of a pool."""
     _fields_ = [("op", c_int), ("tile", c_int), ("fused_ln", c_int), ("m", c_int), ("n", c_int),
                 ("k", c_int), ("ms", c_float)]
+
+
+def _heads(*names):
+    """The fields of some bbh_heads, one after the other."""
+    return [(f"{n}_{f}", t) for n in names for f, t in
+            (("data", c_void_p), ("batch", c_i64), ("row", c_i64), ("head", c_i64))]
+
+
+class RopeConfig(ctypes.Structure):
+    """bbh_rope_config."""
+    _fields_ = [("rot_dim", c_int), ("interleaved", c_int), ("scaling", c_int)] + [
+        (n, ctypes.c_double) for n in ("base", "factor", "original", "low", "high", "magnitude")
+    ] + [("frequencies", ctypes.POINTER(ctypes.c_double))]
+
+
+class RopeArgs(ctypes.Structure):
+    """bbh_rope_args, its bbh_heads field by field."""
+    _fields_ = _heads("q", "k", "v", "q_out", "k_out", "v_out") + [
+        (n, c_void_p) for n in ("q_gamma", "k_gamma", "positions", "kv_rows")] + [
+        ("kv_out_rows", c_i64)] + [
+        (n, c_int) for n in ("rows", "seq", "heads", "kv_heads", "head_dim")] + [("eps", c_float)]
+
+
+class AttendArgs(ctypes.Structure):
+    """bbh_attend_args, its bbh_heads field by field."""
+    _fields_ = _heads("q", "k", "v", "out") + [("q_rows", c_i64), ("k_rows", c_i64)] + [
+        (n, c_void_p) for n in ("q_offsets", "k_offsets", "q_lengths", "k_lengths", "prefix", "mask",
+                                "slopes", "table", "scratch")] + [("scratch_bytes", c_size_t)] + [
+        (n, c_int) for n in ("batch", "q_len", "k_len", "heads", "kv_heads", "head_dim", "left",
+                             "right", "table_half")] + [("scale", c_float), ("cap", c_float)]
 
 
 _AWp, _FWp = ctypes.POINTER(AttnWeights), ctypes.POINTER(FfnWeights)
@@ -122,6 +153,16 @@ SIGNATURES_INT8 = {
     "bbh_linear_i8": (c_int, [c_void_p] * 5 + [c_int] * 3 + [c_void_p, c_int, c_void_p]),
 }
 
+# Every symbol declared in include/bbh_attend.h.
+SIGNATURES_ATTEND = {
+    "bbh_rope_create": (c_int, [ctypes.POINTER(RopeConfig), ctypes.POINTER(c_void_p)]),
+    "bbh_rope_free": (c_int, [c_void_p]),
+    "bbh_rope_frequencies": (c_int, [c_void_p, ctypes.POINTER(ctypes.c_double)]),
+    "bbh_rope_heads": (c_int, [c_void_p, ctypes.POINTER(RopeArgs), c_void_p]),
+    "bbh_attend": (c_int, [ctypes.POINTER(AttendArgs), c_void_p]),
+    "bbh_attend_scratch": (c_size_t, [ctypes.POINTER(AttendArgs)]),
+}
+
 # Exported for profile tables only: what the launchers choose.
 QUERIES = {
     "bbh_linear_tile": (c_int, [c_int, c_int, c_int, c_int]),
@@ -159,7 +200,8 @@ def lib():
         import torch  # noqa: F401
 
         L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in {**SIGNATURES, **SIGNATURES_INT8, **QUERIES}.items():
+        for name, (res, args) in {**SIGNATURES, **SIGNATURES_INT8, **SIGNATURES_ATTEND,
+                                   **QUERIES}.items():
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

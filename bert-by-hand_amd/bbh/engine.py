@@ -564,6 +564,217 @@ def launch_matmul_i8(A, a_scale, B, b_scale, C, M, N, K, bias=None, gelu=False, 
     return C
 
 
+# ---- rotary positions and attention for other models (include/bbh_attend.h) ----
+
+ROPE_MAX_DIM = 256  # BBH_ROPE_MAX_DIM
+ATTEND_MAX_DIM = 256  # BBH_ATTEND_MAX_DIM
+ROPE_SCALINGS = ("none", "linear", "base", "ramp", "bands")  # bbh_rope_scaling
+
+
+class Rope:
+    """The frequencies of rotary positions (bbh_rope_create): rot_dim leading
+    values of each head turn, as pairs (i, i + rot_dim / 2) or, interleaved,
+    (2i, 2i + 1).  scaling: one of ROPE_SCALINGS with its factor, original
+    context and low / high turns; frequencies (rot_dim / 2, radians a position)
+    replaces base and scaling.  Host memory only: one handle serves every device
+    and any number of calls."""
+
+    def __init__(self, rot_dim: int, base: float = 10000.0, interleaved: bool = False,
+                 scaling: str = "none", factor: float = 1.0, original: float = 0.0,
+                 low: float = 0.0, high: float = 0.0, magnitude: float = 1.0, frequencies=None):
+        self.handle = ctypes.c_void_p()
+        if scaling not in ROPE_SCALINGS:
+            raise ValueError(f"scaling must be one of {ROPE_SCALINGS}")
+        rot_dim = _int("rot_dim", rot_dim)
+        f = None
+        if frequencies is not None:
+            f = np.ascontiguousarray(frequencies, np.float64)
+            if f.shape != (rot_dim // 2,):
+                raise ValueError(f"frequencies: expected {rot_dim // 2} values, got {f.shape}")
+            f = f.ctypes.data_as(ctypes.POINTER(ctypes.c_double))
+        config = capi.RopeConfig(rot_dim, int(bool(interleaved)), ROPE_SCALINGS.index(scaling), base,
+                                 factor, original, low, high, magnitude, f)
+        call("bbh_rope_create", ctypes.byref(config), ctypes.byref(self.handle))
+        self.rot_dim = rot_dim
+
+    def frequencies(self):
+        """Radians a position of each pair, float64 (rot_dim / 2)."""
+        out = np.empty(self.rot_dim // 2)
+        call("bbh_rope_frequencies", self.handle,
+             out.ctypes.data_as(ctypes.POINTER(ctypes.c_double)))
+        return out
+
+    def close(self):
+        if self.handle:
+            call("bbh_rope_free", self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _int(name, n):
+    n = n if n.__class__ is int else int(index(n))
+    if not -2147483648 <= n <= 2147483647:
+        raise ValueError(f"{name} must fit a C int")
+    return n
+
+
+def _head_strides(name, t, dims, device):
+    """(address, batch, row, head strides) of a (rows, heads, head_dim) tensor, or of a
+    (batch, rows, heads, head_dim) one, on the current device.  A dimension of one
+    element has no stride that matters."""
+    if t.dtype is not _torch().float16 or t.dim() not in dims or not t.is_cuda:
+        raise TypeError(f"{name} must be a float16 CUDA tensor of {' or '.join(map(str, dims))} "
+                        "dimensions")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on cuda:{t.get_device()}, not on cuda:{device}, the current device")
+    shape, stride = t.shape, t.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name}: the values of a head must be contiguous")
+    return (t.data_ptr(), stride[0] if len(shape) == 4 and shape[0] > 1 else 0,
+            stride[-3] if shape[-3] > 1 else 0, stride[-2] if shape[-2] > 1 else 0)
+
+
+_NO_HEADS = (None, 0, 0, 0)
+
+
+def launch_rope(rope, q, q_out=None, k=None, k_out=None, v=None, v_out=None, positions=None,
+                seq=None, q_gamma=None, k_gamma=None, eps=1e-6, kv_rows=None, stream=None):
+    """q (rows, heads, head_dim) and k (rows, kv_heads, head_dim) fp16, of any row and
+    head strides (views of fused QKV rows, say): each head normed (RMS, where its gamma is
+    given) and rotated by rope (None: normed only) at positions (rows) int32, or at row % seq
+    without them; v moved along where v_out is given.  q_out and k_out default to q and k (in
+    place).  kv_rows (rows) int64: the rows of k_out and v_out that k and v go to, as the
+    slots of a cache; one outside them is not written (bbh_rope_heads)."""
+    torch = _torch()
+    if not q.is_cuda:
+        raise TypeError("operands must be CUDA tensors")
+    c = torch._C
+    dev = c._cuda_getDevice()
+    q_out = q if q_out is None else q_out
+    if k_out is None and k is not None:
+        if kv_rows is not None:
+            raise ValueError("kv_rows needs k_out")
+        k_out = k
+    if (v is None) != (v_out is None) or (k is None and k_out is not None):
+        raise ValueError("k and k_out, v and v_out go together")
+    three = (3,)
+    places = [_NO_HEADS if t is None else _head_strides(n, t, three, dev)
+              for n, t in (("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_out", k_out),
+                           ("v_out", v_out))]
+    rows, heads, dim = q.shape
+    if q_out.shape != q.shape:
+        raise ValueError("q_out must have q's shape")
+    kv_heads, out_rows = 0, None
+    for n, x, y in (("k", k, k_out), ("v", v, v_out)):
+        if x is None:
+            continue
+        if x.shape[0] != rows or x.shape[2] != dim or (kv_heads and x.shape[1] != kv_heads):
+            raise ValueError(f"{n} must have q's rows and head_dim, and k and v the same heads")
+        kv_heads = x.shape[1]
+        if y.shape[1:] != x.shape[1:] or (kv_rows is None and y.shape[0] != rows):
+            raise ValueError(f"{n}_out must have {n}'s shape (but its rows with kv_rows)")
+        if out_rows is not None and y.shape[0] != out_rows:
+            raise ValueError("k_out and v_out must have the same rows")
+        out_rows = y.shape[0]
+    seq = 0 if seq is None else _int("seq", seq)
+    if rope is not None and positions is None and seq < 1:
+        raise ValueError("positions or seq must be given")
+    if rows == 0:
+        return q_out
+    args = capi.RopeArgs(
+        *places[0], *places[1], *places[2], *places[3], *places[4], *places[5],
+        _operand("q_gamma", q_gamma, torch.float16, dim, dev),
+        _operand("k_gamma", k_gamma, torch.float16, dim, dev),
+        _operand("positions", positions, torch.int32, rows, dev),
+        _operand("kv_rows", kv_rows, torch.int64, rows, dev), out_rows or 0, rows, seq, heads,
+        kv_heads, dim, eps)
+    call("bbh_rope_heads", rope.handle if rope is not None else None, ctypes.byref(args),
+         c._cuda_getCurrentRawStream(dev) if stream is None else stream)
+    return q_out
+
+
+def _attend_args(q, k, v, out, q_len=None, k_len=None, q_offsets=None, k_offsets=None,
+                 q_lengths=None, k_lengths=None, left=-1, right=-1, scale=None, cap=0.0,
+                 mask=None, prefix=None, slopes=None, table=None, scratch=None):
+    torch = _torch()
+    if not q.is_cuda:
+        raise TypeError("operands must be CUDA tensors")
+    dev = torch._C._cuda_getDevice()
+    qp, kp = q_offsets is not None, k_offsets is not None
+    qd, kd = ((3,) if qp else (4,)), ((3,) if kp else (4,))
+    places = (_head_strides("q", q, qd, dev), _head_strides("k", k, kd, dev),
+              _head_strides("v", v, kd, dev), _head_strides("out", out, qd, dev))
+    if k.shape != v.shape or q.shape != out.shape or q.shape[-1] != k.shape[-1]:
+        raise ValueError("k and v, q and out must have the same shapes, and all the same head_dim")
+    heads, dim = q.shape[-2:]
+    batch = q_offsets.numel() - 1 if qp else q.shape[0]
+    if batch < 0:
+        raise ValueError("q_offsets: expected batch + 1 elements")
+    if not kp and k.shape[0] != batch:
+        raise ValueError(f"k and v: expected a batch of {batch}, got {k.shape[0]}")
+    lens = []
+    for n, m, t, packed in (("q_len", q_len, q, qp), ("k_len", k_len, k, kp)):
+        have = t.shape[0] if packed else t.shape[1]
+        if m is None:
+            if packed:
+                raise ValueError(f"packed sequences need {n}, the longest one's length")
+            m = have
+        m = _int(n, m)
+        if m < 0 or (m > have and not packed):
+            raise ValueError(f"{n} must be in [0, {have}]")
+        lens.append(min(m, have))
+    q_len, k_len = lens
+    i32, f32 = torch.int32, torch.float32
+    half = 0
+    if table is not None:
+        if table.dim() != 2 or table.shape[0] != heads or table.shape[1] % 2 == 0:
+            raise ValueError(f"table must be ({heads}, odd)")
+        half = table.shape[1] // 2
+    if mask is not None and tuple(mask.shape) != (batch, k_len):
+        raise ValueError(f"mask must be ({batch}, {k_len})")
+    return dev, capi.AttendArgs(
+        *places[0], *places[1], *places[2], *places[3], q.shape[0] if qp else 0,
+        k.shape[0] if kp else 0, _operand("q_offsets", q_offsets, i32, batch + 1, dev),
+        _operand("k_offsets", k_offsets, i32, batch + 1, dev),
+        _operand("q_lengths", q_lengths, i32, batch, dev),
+        _operand("k_lengths", k_lengths, i32, batch, dev),
+        _operand("prefix", prefix, i32, batch, dev), _operand("mask", mask, i32, batch * k_len, dev),
+        _operand("slopes", slopes, f32, heads, dev),
+        _operand("table", table, f32, heads * (2 * half + 1), dev),
+        None if scratch is None else _operand("scratch", scratch, scratch.dtype, 0, dev),
+        0 if scratch is None else scratch.numel() * scratch.element_size(), batch, q_len, k_len,
+        heads, k.shape[-2], dim, _int("left", left), _int("right", right), half,
+        dim ** -0.5 if scale is None else scale, cap)
+
+
+def launch_attend(q, k, v, out, q_len=None, k_len=None, q_offsets=None, k_offsets=None,
+                  q_lengths=None, k_lengths=None, left=-1, right=-1, scale=None, cap=0.0, mask=None,
+                  prefix=None, slopes=None, table=None, scratch=None, stream=None):
+    """Attention (bbh_attend) of q over k and v into out, fp16, of any row and head strides:
+    (batch, length, heads, head_dim), or packed (rows, heads, head_dim) with offsets
+    (batch + 1) int32 and the longest length.  k and v may have fewer heads (a divisor).
+    q_lengths, k_lengths, prefix: (batch) int32; mask: (batch, k_len) int32; slopes (heads)
+    and table (heads, 2 * half + 1): fp32 biases by distance; left, right: how far back and
+    ahead a query sees (negative: all; right=0: causal); scale: 1 / sqrt(head_dim) by
+    default; scratch: a tensor of attend_scratch(...) bytes, with which few queries over many
+    keys run faster."""
+    dev, args = _attend_args(q, k, v, out, q_len, k_len, q_offsets, k_offsets, q_lengths, k_lengths,
+                             left, right, scale, cap, mask, prefix, slopes, table, scratch)
+    call("bbh_attend", ctypes.byref(args),
+         _torch()._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
+    return out
+
+
+def attend_scratch(q, k, v, out, **kwargs) -> int:
+    """Bytes of scratch that launch_attend makes use of with these arguments."""
+    return capi.lib().bbh_attend_scratch(ctypes.byref(_attend_args(q, k, v, out, **kwargs)[1]))
+
+
 class Tokenizer:
     """The uncased BERT WordPiece tokenizer (bbh_tokenizer_load / bbh_tokenize):
     texts -> host int32 (n, seq) ids, types, mask, as

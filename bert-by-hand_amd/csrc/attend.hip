@@ -1,0 +1,632 @@
+// Attention for models other than MiniLM: any head size up to 256, shared
+// key/value heads, capped scores, a bias by distance, a window, a prefix, a key
+// mask, documents packed end to end, and few queries over a long cache.
+#include <limits.h>
+
+#include <algorithm>
+
+#include "attend.h"
+#include "pipe.h"
+
+namespace bbh {
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+enum Feat { kPlain = 0, kCap = 1, kAny = 2 };
+
+// Key (within a 32-key chunk) held by row r of the K tile.
+__device__ __forceinline__ int key_of_row(int r) {
+  const int a = r >> 3, c = (r >> 2) & 1, b = r & 3;
+  return 16 * (a >> 1) + 8 * c + 4 * (a & 1) + b;
+}
+
+// Chunk c (16 bytes) of a row r of a tile of HD-wide rows sits in slot c ^ f(r).
+template <int HD>
+struct Tile {
+  static constexpr int CPR = HD / 8;
+  __device__ static __forceinline__ int fk(int r) {
+    if constexpr (HD % 128 == 0) return r & 15;
+    if constexpr (HD % 64 == 0) return (r >> 1) & 7;
+    return (r >> 2) & 3;
+  }
+  __device__ static __forceinline__ int fv(int r) {
+    if constexpr (HD % 128 == 0) return 4 * (r & 3);
+    if constexpr (HD % 64 == 0) return 4 * ((r >> 1) & 1);
+    return 0;
+  }
+};
+
+constexpr float kLazy = 8.f;
+
+template <int HD_, int NW_, int T_, int KS_, int R_, int OCC_>
+struct Cfg {
+  static constexpr int HD = HD_, NW = NW_, T = T_, KS = KS_, R = R_, OCC = OCC_;
+  static_assert(KS == 1 || KS == NW, "waves go along the rows or along the keys");
+  static constexpr int RW = NW / KS;
+  static constexpr int BM = RW * T * 32;         // rows of a workgroup
+  static constexpr int SK = KS == 1 ? 64 : 32;   // keys of a tile
+  static constexpr int CW = KS == 1 ? NW : 1;    // wavefronts that share a tile's copies
+  static constexpr int N = SK * HD / 512 / CW;   // copies of a wavefront: a tile of K, of V
+  static constexpr int STAGE = 2 * SK * HD;      // halves of a stage: K, V
+  static constexpr int RINGS = KS;               // a ring each wavefront where it has tiles of its own
+  static constexpr size_t RING = (size_t)RINGS * R * STAGE * 2;
+  static constexpr size_t OUT = KS == 1 ? (size_t)NW * 32 * (HD + 8) * 2
+                                        : (size_t)KS * 32 * (HD + 4) * 4 + KS * 32 * 8;
+  static constexpr size_t LDS = RING > OUT ? RING : OUT;
+  static constexpr int THREADS = 64 * NW;
+};
+
+struct Seq {
+  int64_t q0, k0;  // first row (packed) of queries and keys
+  int nq, nk;
+};
+
+__device__ __forceinline__ int span_of(const int32_t* offsets, const int32_t* lengths, int b,
+                                       int len, int64_t rows, int64_t& start) {
+  start = 0;
+  int n = len;
+  if (offsets) {
+    const int64_t a = offsets[b], e = offsets[b + 1];
+    start = a < 0 ? 0 : a > rows ? rows : a;
+    const int64_t end = e > rows ? rows : e;
+    n = (int)(end - start < len ? end - start : len);
+  }
+  if (lengths) n = min(n, lengths[b]);
+  return max(n, 0);
+}
+__device__ __forceinline__ Seq seq_of(const AttendParams& p, int b) {
+  Seq s;
+  s.nq = span_of(p.q_offsets, p.q_lengths, b, p.q_len, p.q_rows, s.q0);
+  s.nk = span_of(p.k_offsets, p.k_lengths, b, p.k_len, p.k_rows, s.k0);
+  return s;
+}
+
+__device__ __forceinline__ int wave_id() {
+  return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+}
+__device__ __forceinline__ float imax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+template <class C, int FEAT>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams p) {
+  constexpr int HD = C::HD, T = C::T, SK = C::SK, CH = SK / 32, NS = HD / 16, ND = HD / 32;
+  HIP_DYNAMIC_SHARED(f16, smem);
+  // (sequence, key/value head), row block and split of this workgroup
+  const int rows_all = p.batch * p.kv_heads, cols = p.blocks * p.splits;
+  int item, col;
+  {
+    const int x = blockIdx.x % kXcds, n = blockIdx.x / kXcds;
+    if (rows_all >= kXcdRows) {
+      const int qd = n / cols;
+      item = qd * kXcds + x;
+      col = n - qd * cols;
+      if (item >= rows_all) return;
+    } else {
+      const int64_t items = (int64_t)rows_all * cols;
+      const int each = (int)(items / kXcds), r = (int)(items % kXcds);
+      if (n >= each + (x < r ? 1 : 0)) return;
+      const int64_t i = (int64_t)x * each + min(x, r) + n;
+      item = (int)(i / cols);
+      col = (int)(i - (int64_t)item * cols);
+    }
+  }
+  const int split = col % p.splits, block = p.blocks - 1 - col / p.splits;
+  const int bi = item / p.kv_heads, kvh = item - bi * p.kv_heads, b = p.b0 + bi;
+  const Seq sq = seq_of(p, b);
+  const int nq = sq.nq, nk = sq.nk, rows = nq * p.group;
+  const int row0 = block * C::BM;
+  if (row0 >= rows) return;
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, r32 = lane & 31, kh = lane >> 5;
+  const int rw = C::KS == 1 ? wave : 0;
+
+  // ---- the rows of this lane: row = query * group + head of the group
+  const int shift = nk - nq;
+  const int prefix = p.prefix ? min(max(p.prefix[b], 0), nk) : 0;
+  int lo[T], hi[T];
+  float slope[T];
+  int qpos[T], thead[T];
+  f16x8 q[T][NS];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int row = min(row0 + (rw * T + t) * 32 + r32, rows - 1);
+    const int i = row / p.group, g = row - i * p.group, h = kvh * p.group + g;
+    const f16* src = p.q + (p.q_offsets ? (sq.q0 + i) * p.qs.row : b * p.qs.batch + i * p.qs.row) +
+                     h * p.qs.head;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      q[t][s] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (16 * s + 8 * kh < p.dim) q[t][s] = *reinterpret_cast<const f16x8*>(src + 16 * s + 8 * kh);
+    }
+    const int pos = i + shift;
+    lo[t] = p.left < 0 ? 0 : max(pos - p.left, 0);
+    hi[t] = p.right < 0 ? nk : min(pos + p.right + 1, nk);
+    qpos[t] = pos;
+    thead[t] = h;
+    slope[t] = FEAT == kAny && p.slopes ? p.slopes[h] * 1.44269504088896f : 0.f;
+  }
+  // ---- the tiles of this block: those of the prefix, then those of the window
+  const int first_q = row0 / p.group, last_q = (min(row0 + C::BM, rows) - 1) / p.group;
+  const int wlo = p.left < 0 ? 0 : max(first_q + shift - p.left, 0);
+  const int whi = p.right < 0 ? nk : min(max(last_q + shift + p.right + 1, 0), nk);
+  const int np = (prefix + SK - 1) / SK;
+  const int t0 = max(np, wlo / SK), t1 = (whi + SK - 1) / SK;
+  const int tiles = np + max(t1 - t0, 0);
+  // per wavefront where each has its own: tiles first, first + step, ...
+  int begin = split * p.chunk, end = min(tiles, begin + p.chunk);
+  if constexpr (C::KS > 1) begin += wave;
+  const int count = begin >= end ? 0 : (end - begin + C::KS - 1) / C::KS;
+  auto tile_at = [&](int i) {
+    const int n = begin + i * C::KS;
+    return n < np ? n : t0 + (n - np);
+  };
+  // interior tiles, which every row of the block sees whole: [full_lo, full_hi)
+  const int full_lo = p.left < 0 ? 0 : max(last_q + shift - p.left, 0);
+  const int full_hi = p.right < 0 ? nk : min(max(first_q + shift + p.right + 1, 0), nk);
+
+  const f16* kbase = p.k + (p.k_offsets ? sq.k0 * p.ks.row : b * p.ks.batch) + kvh * p.ks.head;
+  const f16* vbase = p.v + (p.k_offsets ? sq.k0 * p.vs.row : b * p.vs.batch) + kvh * p.vs.head;
+  const int32_t* mrow = p.mask ? p.mask + (int64_t)b * p.k_len : nullptr;
+  f16* ring = smem + (C::KS == 1 ? 0 : wave * C::R * C::STAGE);
+  const int cwave = C::KS == 1 ? wave : 0;
+
+  constexpr uint32_t kNowhere = 0x80000000u;  // past every resource: reads nothing, writes zeros
+  uint32_t koff[C::N], voff[C::N];
+  int krow[C::N], vrow[C::N];
+#pragma unroll
+  for (int j = 0; j < C::N; ++j) {
+    const int s = (cwave * C::N + j) * 64 + lane, r = s / Tile<HD>::CPR, slot = s % Tile<HD>::CPR;
+    const int kc = slot ^ Tile<HD>::fk(r & 31), vc = slot ^ Tile<HD>::fv(r);
+    krow[j] = (r & ~31) + key_of_row(r & 31);
+    vrow[j] = r;
+    koff[j] = 8 * kc < p.dim ? (uint32_t)(krow[j] * (int)p.ks.row + 8 * kc) * 2u : kNowhere;
+    voff[j] = 8 * vc < p.dim ? (uint32_t)(r * (int)p.vs.row + 8 * vc) * 2u : kNowhere;
+  }
+  auto mask_bits = [&](int k0) -> uint64_t {  // unmasked keys of the tile
+    if (!mrow) {
+      const int left = nk - k0;
+      return left >= 64 ? ~0ull : left <= 0 ? 0ull : ((1ull << left) - 1);
+    }
+    const int key = k0 + (SK == 64 ? lane : (lane & 31));
+    const int on = key < nk ? mrow[key] : 0;
+    return __ballot(on != 0);
+  };
+  auto issue = [&](int i, uint64_t bits) {
+    const int k0 = tile_at(i) * SK;
+    f16* ks = ring + (i % C::R) * C::STAGE;
+    f16* vs = ks + SK * HD;
+    const int valid = min(nk - k0, SK);
+    const auto rk = buffer_of(kbase + (int64_t)k0 * p.ks.row,
+                              (uint32_t)((valid - 1) * (int)p.ks.row + p.dim) * 2u);
+    const auto rv = buffer_of(vbase + (int64_t)k0 * p.vs.row,
+                              (uint32_t)((valid - 1) * (int)p.vs.row + p.dim) * 2u);
+#pragma unroll
+    for (int j = 0; j < C::N; ++j) {
+      uint32_t off = koff[j];
+      if (mrow && !((bits >> krow[j]) & 1)) off = kNowhere;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rk, (__attribute__((address_space(3))) void*)(ks + (cwave * C::N + j) * 512), 16, (int)off, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < C::N; ++j) {
+      uint32_t off = voff[j];
+      if (mrow && !((bits >> vrow[j]) & 1)) off = kNowhere;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rv, (__attribute__((address_space(3))) void*)(vs + (cwave * C::N + j) * 512), 16, (int)off, 0, 0, 0);
+    }
+  };
+
+  const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const f16x2 ones = {(f16)1.f, (f16)1.f};
+  f32x16 o[T][ND];
+  float m[T], l[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[t][d] = zero;
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+  }
+  const float lag = FEAT == kPlain ? kLazy / p.c : kLazy;
+  const float mscale = FEAT == kPlain ? p.c : 1.f;
+
+  uint64_t bits_now = 0, bits_next = 0;
+  if (count > 0) {
+    bits_now = mask_bits(tile_at(0) * SK);
+    issue(0, bits_now);
+    if (count > 1) bits_next = mask_bits(tile_at(1) * SK);
+  }
+  for (int it = 0; it < count; ++it) {
+    wait_vm<0>();
+    if constexpr (C::KS == 1) lds_barrier();
+    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (it + 1 < count) issue(it + 1, bits_next);
+    const uint64_t bits = bits_now;
+    bits_now = bits_next;
+    if (it + 2 < count) bits_next = mask_bits(tile_at(it + 2) * SK);
+    const int k0 = tile_at(it) * SK;
+    const f16* ks = ring + (it % C::R) * C::STAGE;
+    const f16* vs = ks + SK * HD;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      const int kb = k0 + 32 * ch;
+      const uint32_t on = (uint32_t)(bits >> (32 * ch));
+      if (on == 0) continue;
+      const bool whole = on == 0xffffffffu && (kb + 32 <= prefix || (kb >= full_lo && kb + 32 <= full_hi));
+      uint32_t see[T];
+      if (!whole) {
+        uint32_t some = 0;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          // bits [max(lo, 0), hi) or below prefix, relative to kb
+          auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };
+          see[t] = ((below(hi[t] - kb) & ~below(lo[t] - kb)) | below(prefix - kb)) & on;
+          some |= see[t];
+          see[t] >>= 8 * kh;
+        }
+        if (!__ballot(some != 0)) continue;
+      }
+      f32x16 s[T];
+#pragma unroll
+      for (int t = 0; t < T; ++t) s[t] = zero;
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
+        const f16x8 kf = *reinterpret_cast<const f16x8*>(
+            ks + (32 * ch + r32) * HD + (((2 * st + kh) ^ Tile<HD>::fk(r32)) << 3));
+#pragma unroll
+        for (int t = 0; t < T; ++t) s[t] = mfma32(kf, q[t][st], s[t]);
+      }
+      // s[i]: key kb + 16*(i/8) + 8*kh + i%8
+      if constexpr (FEAT != kPlain) {
+        if (FEAT == kCap || p.cap_l > 0.f) {
+#pragma unroll
+          for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float e = __builtin_amdgcn_exp2f(s[t][i] * p.cap_k);
+              s[t][i] = fmaf(-2.f * p.cap_l, __builtin_amdgcn_rcpf(e + 1.f), p.cap_l);
+            }
+        } else {
+#pragma unroll
+          for (int t = 0; t < T; ++t) s[t] *= p.c;
+        }
+      }
+      if constexpr (FEAT == kAny) {
+        if (p.slopes) {
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+            const float d0 = (float)(kb + 8 * kh - qpos[t]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              s[t][i] = fmaf(-slope[t], fabsf(d0 + (float)(16 * (i >> 3) + (i & 7))), s[t][i]);
+          }
+        }
+        if (p.table) {
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+            const float* tab = p.table + (int64_t)thead[t] * (2 * p.half + 1) + p.half;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int d = kb + 8 * kh + 16 * (i >> 3) + (i & 7) - qpos[t];
+              const float w = tab[min(max(d, -p.half), p.half)];
+              s[t][i] += w == -INFINITY ? w : imax(w * 1.44269504088896f, -1e30f);
+            }
+          }
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[t][i] = (see[t] >> (16 * (i >> 3) + (i & 7))) & 1 ? s[t][i] : -INFINITY;
+      }
+      bool up = false;
+      float mx[T];
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        float v = imax(imax(s[t][0], s[t][1]), s[t][2]);
+#pragma unroll
+        for (int i = 3; i < 15; i += 2) v = imax(imax(v, s[t][i]), s[t][i + 1]);
+        v = imax(v, s[t][15]);
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        mx[t] = imax(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        up = up || !(mx[t] <= m[t] + lag);
+      }
+      if (__ballot(up)) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          const float mn = imax(m[t], mx[t]);
+          const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[t] - mn) * mscale);
+          l[t] *= corr;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) o[t][d] *= corr;
+          m[t] = mn;
+        }
+      }
+      f16x8 pr[T][2];
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const float mc = m[t] == -INFINITY ? 0.f : m[t] * mscale;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = FEAT == kPlain ? fmaf(s[t][i], p.c, -mc) : s[t][i] - mc;
+          pr[t][i >> 3][i & 7] = (f16)__builtin_amdgcn_exp2f(x);
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+          for (int i = 0; i < 8; i += 2)
+            l[t] = __builtin_amdgcn_fdot2(f16x2{pr[t][hf][i], pr[t][hf][i + 1]}, ones, l[t], false);
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const int r = 32 * ch + 16 * hf + 8 * kh + ((lane >> 2) & 3);
+          const int c16 = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+          auto* a = (__attribute__((address_space(3))) s16x4*)(vs + r * HD + ((c16 ^ Tile<HD>::fv(r)) << 3) + 4 * (lane & 1));
+          auto* a4 = (__attribute__((address_space(3))) s16x4*)(vs + (r + 4) * HD + ((c16 ^ Tile<HD>::fv(r)) << 3) + 4 * (lane & 1));
+          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(a);
+          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(a4);
+          const auto vv = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+          const f16x8 vf = __builtin_bit_cast(f16x8, vv);
+#pragma unroll
+          for (int t = 0; t < T; ++t) o[t][d] = mfma32(vf, pr[t][hf], o[t][d]);
+        }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t) l[t] = xor32_sum(l[t]);
+
+  // ---- out.  o[t][d][i]: row lane%32, dim 32 d + 8 (i/4) + 4 kh + i%4
+  const int cpr = p.dim / 8;
+  auto out_at = [&](int row) {
+    const int i = row / p.group, g = row - i * p.group;
+    return p.out + (p.q_offsets ? (sq.q0 + i) * p.os.row : b * p.os.batch + i * p.os.row) +
+           (kvh * p.group + g) * p.os.head;
+  };
+  auto slot_of = [&](int row) {
+    return (((int64_t)item * p.q_len * p.group) + row) * p.splits + split;
+  };
+  __syncthreads();  // the rings are free
+  if constexpr (C::KS == 1) {
+    if (p.splits > 1) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const int row = row0 + (rw * T + t) * 32 + r32;
+        if (row >= rows) continue;
+        const int64_t sl = slot_of(row);
+        if (kh == 0) p.part_ml[sl] = make_float2(m[t] * mscale, l[t]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<f32x4*>(p.part_o + sl * HD + 32 * d + 8 * j + 4 * kh) =
+                f32x4{o[t][d][4 * j], o[t][d][4 * j + 1], o[t][d][4 * j + 2], o[t][d][4 * j + 3]};
+      }
+      return;
+    }
+    f16* st = smem + wave * 32 * (HD + 8);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const float inv = l[t] != 0.f ? 1.f / l[t] : 0.f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f16x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = (f16)(o[t][d][4 * j + e] * inv);
+          *reinterpret_cast<f16x4*>(st + r32 * (HD + 8) + 32 * d + 8 * j + 4 * kh) = w;
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      for (int x = lane; x < 32 * Tile<HD>::CPR; x += 64) {
+        const int r = x / Tile<HD>::CPR, cc = x % Tile<HD>::CPR;
+        const int row = row0 + (rw * T + t) * 32 + r;
+        const f16x8 w = *reinterpret_cast<const f16x8*>(st + r * (HD + 8) + 8 * cc);
+        if (row < rows && cc < cpr) *reinterpret_cast<f16x8*>(out_at(row) + 8 * cc) = w;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  } else {
+    float* area = reinterpret_cast<float*>(smem);  // [KS][32][HD + 4]
+    float2* ml = reinterpret_cast<float2*>(area + C::KS * 32 * (HD + 4));
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      if (t > 0) __syncthreads();
+      if (kh == 0) ml[wave * 32 + r32] = make_float2(m[t] * mscale, l[t]);
+      __syncthreads();
+      float top = -INFINITY, mine = m[t] * mscale;
+#pragma unroll
+      for (int w = 0; w < C::KS; ++w) top = imax(top, ml[w * 32 + r32].x);
+      const float f = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - top);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<f32x4*>(area + (wave * 32 + r32) * (HD + 4) + 32 * d + 8 * j + 4 * kh) =
+              f32x4{o[t][d][4 * j] * f, o[t][d][4 * j + 1] * f, o[t][d][4 * j + 2] * f,
+                    o[t][d][4 * j + 3] * f};
+      __syncthreads();
+      for (int x = tid; x < 32 * (HD / 8); x += C::THREADS) {
+        const int r = x / (HD / 8), cc = x % (HD / 8);
+        const int row = row0 + t * 32 + r;
+        if (row >= rows || cc >= cpr) continue;
+        float tp = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < C::KS; ++w) tp = imax(tp, ml[w * 32 + r].x);
+#pragma unroll
+        for (int w = 0; w < C::KS; ++w) {
+          const float2 a = ml[w * 32 + r];
+          sum += a.x == -INFINITY ? 0.f : a.y * __builtin_amdgcn_exp2f(a.x - tp);
+        }
+        float v[8] = {};
+#pragma unroll
+        for (int w = 0; w < C::KS; ++w)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += area[(w * 32 + r) * (HD + 4) + 8 * cc + e];
+        if (p.splits > 1) {
+          const int64_t sl = slot_of(row);
+          if (cc == 0) p.part_ml[sl] = make_float2(tp, sum);
+          *reinterpret_cast<f32x4*>(p.part_o + sl * HD + 8 * cc) = f32x4{v[0], v[1], v[2], v[3]};
+          *reinterpret_cast<f32x4*>(p.part_o + sl * HD + 8 * cc + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+          const float inv = sum != 0.f ? 1.f / sum : 0.f;
+          f16x8 w;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = (f16)(v[e] * inv);
+          *reinterpret_cast<f16x8*>(out_at(row) + 8 * cc) = w;
+        }
+      }
+    }
+  }
+}
+
+// Joins the splits of each row: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
+template <int HD>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
+  constexpr int L = HD / 8, RB = 256 / L;
+  const int lane = threadIdx.x % L, per = p.q_len * p.group;
+  if (threadIdx.x / L >= RB) return;
+  const int64_t slot = (int64_t)blockIdx.x * RB + threadIdx.x / L;
+  const int64_t item = slot / per;
+  const int row = (int)(slot - item * per);
+  if (item >= (int64_t)p.batch * p.kv_heads) return;
+  const int b = (int)(item / p.kv_heads), kvh = (int)(item - (int64_t)b * p.kv_heads);  // b0 is 0 here
+  const Seq sq = seq_of(p, b);
+  if (row >= sq.nq * p.group || 8 * lane >= p.dim) return;
+  const float2* ml = p.part_ml + slot * p.splits;
+  float top = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) top = imax(top, ml[s].x);
+  float sum = 0.f, v[8] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 a = ml[s];
+    if (a.x == -INFINITY) continue;
+    const float f = __builtin_amdgcn_exp2f(a.x - top);
+    sum = fmaf(a.y, f, sum);
+    const f32x4* src = reinterpret_cast<const f32x4*>(p.part_o + (slot * p.splits + s) * HD + 8 * lane);
+    const f32x4 x = src[0], y = src[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = fmaf(x[e], f, v[e]);
+      v[4 + e] = fmaf(y[e], f, v[4 + e]);
+    }
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  const int i = row / p.group, g = row - i * p.group;
+  f16* dst = p.out + (p.q_offsets ? (sq.q0 + i) * p.os.row : b * p.os.batch + i * p.os.row) +
+             (kvh * p.group + g) * p.os.head + 8 * lane;
+  f16x8 w;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = (f16)(v[e] * inv);
+  *reinterpret_cast<f16x8*>(dst) = w;
+}
+
+template <class C, int FEAT>
+hipError_t launch_as(const AttendParams& p, int64_t grid, hipStream_t s) {
+  static const hipError_t attr =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(attend_kernel<C, FEAT>),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)C::LDS);
+  if (attr != hipSuccess) return attr;
+  hipLaunchKernelGGL((attend_kernel<C, FEAT>), dim3((unsigned)grid), dim3(C::THREADS), C::LDS, s, p);
+  return hipGetLastError();
+}
+
+constexpr int64_t kMostThreads = 0xffffffffll;  // of a launch
+
+// Longest run of keys that a block of rows may see.
+int64_t longest(const AttendParams& p) {
+  if (p.prefix || p.left < 0) return p.k_len;
+  return std::min<int64_t>(p.k_len, (int64_t)p.left + p.q_len + (p.right < 0 ? p.k_len : p.right));
+}
+
+template <class C>
+void plan(AttendParams& p, size_t scratch_bytes) {
+  const int64_t rows = (int64_t)p.q_len * p.group, items = (int64_t)p.batch * p.kv_heads;
+  p.blocks = (int)((rows + C::BM - 1) / C::BM);
+  const int64_t tiles = (longest(p) + C::SK - 1) / C::SK + 2;
+  p.splits = 1;
+  p.chunk = INT_MAX / 2;
+  const int64_t groups = items * p.blocks;
+  if (groups >= 1024) return;
+  const int64_t least = 512 / C::SK;  // keys of a split
+  int64_t want = std::min<int64_t>(tiles / least, (1024 + groups - 1) / groups);
+  const int64_t a_split = items * rows * (C::HD * 4 + 8);
+  want = std::min<int64_t>(want, (int64_t)(scratch_bytes / a_split));
+  if (want < 2) return;
+  p.chunk = (int)((tiles + want - 1) / want);
+  p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
+}
+
+template <class C>
+hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream_t s) {
+  plan<C>(p, scratch ? scratch_bytes : 0);
+  const int64_t cols = (int64_t)p.blocks * p.splits;
+  const int64_t slots = (int64_t)p.batch * p.kv_heads * p.q_len * p.group;
+  p.part_o = static_cast<float*>(scratch);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * p.splits * C::HD);
+  const int feat = p.slopes || p.table ? kAny : p.cap_l > 0.f ? kCap : kPlain;
+  // sequences a launch: its work-items are counted in 32 bits
+  const int64_t per = cols * p.kv_heads * C::THREADS;
+  const int most = (int)std::min<int64_t>(p.batch, std::max<int64_t>(1, (kMostThreads / per) - 8));
+  const int batch = p.batch;
+  for (p.b0 = 0; p.b0 < batch; p.b0 += most) {
+    p.batch = std::min(most, batch - p.b0);
+    const int64_t rows = (int64_t)p.batch * p.kv_heads;
+    const int64_t grid = rows >= kXcdRows ? (rows + kXcds - 1) / kXcds * cols * kXcds
+                                          : (rows * cols + kXcds - 1) / kXcds * kXcds;
+    const hipError_t e = feat == kPlain ? launch_as<C, kPlain>(p, grid, s)
+                         : feat == kCap ? launch_as<C, kCap>(p, grid, s)
+                                        : launch_as<C, kAny>(p, grid, s);
+    if (e != hipSuccess) return e;
+  }
+  if (p.splits > 1) {
+    p.b0 = 0;
+    p.batch = batch;
+    constexpr int RB = 256 / (C::HD / 8);
+    hipLaunchKernelGGL((attend_join_kernel<C::HD>), dim3((unsigned)((slots + RB - 1) / RB)), dim3(256),
+                       0, s, p);
+    return hipGetLastError();
+  }
+  return hipSuccess;
+}
+
+//                 HD  NW T KS R OCC
+using P32 = Cfg<32, 4, 2, 1, 2, 2>;
+using P64 = Cfg<64, 4, 2, 1, 2, 2>;
+using P96 = Cfg<96, 4, 2, 1, 2, 1>;
+using P128 = Cfg<128, 4, 2, 1, 2, 1>;
+using P256 = Cfg<256, 4, 1, 1, 2, 1>;
+using K32 = Cfg<32, 4, 1, 4, 2, 2>;
+using K64 = Cfg<64, 4, 1, 4, 2, 2>;
+using K96 = Cfg<96, 4, 1, 4, 2, 1>;
+using K128 = Cfg<128, 4, 1, 4, 2, 1>;
+using K256 = Cfg<256, 2, 1, 2, 2, 1>;
+
+template <class F>
+auto with_config(const AttendParams& p, F&& f) {
+  const bool few = (int64_t)p.q_len * p.group <= 32;
+  if (p.dim <= 32) return few ? f(K32{}) : f(P32{});
+  if (p.dim <= 64) return few ? f(K64{}) : f(P64{});
+  if (p.dim <= 96) return few ? f(K96{}) : f(P96{});
+  if (p.dim <= 128) return few ? f(K128{}) : f(P128{});
+  return few ? f(K256{}) : f(P256{});
+}
+
+}  // namespace
+
+hipError_t attend(AttendParams p, void* scratch, size_t scratch_bytes, hipStream_t s) {
+  return with_config(p, [&](auto c) { return launch<decltype(c)>(p, scratch, scratch_bytes, s); });
+}
+
+size_t attend_scratch(const AttendParams& p) {
+  return with_config(p, [&](auto c) -> size_t {
+    AttendParams a = p;
+    plan<decltype(c)>(a, SIZE_MAX / 2);
+    if (a.splits < 2) return 0;
+    return (size_t)p.batch * p.kv_heads * p.q_len * p.group * a.splits * (decltype(c)::HD * 4 + 8);
+  });
+}
+
+}  // namespace bbh
