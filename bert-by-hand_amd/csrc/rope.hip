@@ -9,9 +9,9 @@
 // its product with the position are the fraction of a turn without any loss, and the
 // high word of them is off by less than 2^-31 turns for every int32 position.
 //
-// A wavefront takes a row.  Its lanes compute the sines and cosines of the row's
-// pairs once (one or two a lane), pass them through LDS, and every group of lanes
-// then walks heads with them in registers.
+// A workgroup takes some whole rows (or a part of the heads of one, where rows are few):
+// its threads compute the sines and cosines of the rows' pairs into LDS while the first
+// heads are on their way, then every thread turns its pieces of heads.
 #include <algorithm>
 
 #include "attend.h"
@@ -19,21 +19,28 @@
 namespace bbh {
 namespace {
 
-constexpr int kWaves = 4;  // a workgroup
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
 
-// (cos, sin) of the row's pairs, times the magnitude, into this wavefront's part of LDS.
-__device__ __forceinline__ void angles(const RopeParams& p, const RopeSteps& steps, int position,
-                                       float2* cs, int lane) {
-  for (int i = lane; 2 * i < p.rot; i += kWave) {
-    const uint2 st = steps.step[i];
-    const uint32_t at = (uint32_t)position;
-    // high word of (int64)position * step
-    uint32_t turn = __umulhi(at, st.x) + at * st.y;
-    if (position < 0) turn -= st.x;
-    float s, c;
-    sincospif((float)(int32_t)turn * 0x1p-31f, &s, &c);  // half turns
-    cs[i] = make_float2(c * p.magnitude, s * p.magnitude);
-  }
+// (cos, sin), times the magnitude, of pair i at a position.
+__device__ __forceinline__ float2 angle(const RopeParams& p, const RopeSteps& steps, int position,
+                                        int i) {
+  const uint2 st = steps.step[i];
+  const uint32_t at = (uint32_t)position;
+  // high word of (int64)position * step
+  uint32_t turn = __umulhi(at, st.x) + at * st.y;
+  if (position < 0) turn -= st.x;
+  float s, c;
+  sincospif((float)(int32_t)turn * 0x1p-31f, &s, &c);  // half turns
+  return make_float2(c * p.magnitude, s * p.magnitude);
+}
+__device__ __forceinline__ int position_of(const RopeParams& p, int row) {
+  return p.rot == 0 ? 0 : p.positions ? p.positions[row] : row % p.seq;
+}
+
+__device__ __forceinline__ void turn(float& a, float& b, float2 cs) {
+  const float a0 = a;
+  a = a0 * cs.x - b * cs.y;
+  b = b * cs.x + a0 * cs.y;
 }
 
 // Sum over groups of G neighbouring lanes.
@@ -43,139 +50,158 @@ __device__ __forceinline__ float lanes_sum(float v) {
   if constexpr (G >= 4) v = xor_op<2>(v, AddOp{});
   if constexpr (G >= 8) v = xor_op<4>(v, AddOp{});
   if constexpr (G >= 16) v = xor_op<8>(v, AddOp{});
+  if constexpr (G >= 32) v = xor_op<16>(v, AddOp{});
+  if constexpr (G >= 64) v = xor_op<32>(v, AddOp{});
   return v;
 }
 
-// G lanes a head, 16 values (two chunks of eight) a lane: in the half layout the
-// chunks of a lane hold the two halves of eight pairs, otherwise they are neighbours.
-template <int G, bool NORM>
-__global__ __launch_bounds__(64 * kWaves) void rope_kernel(RopeParams p, RopeSteps steps, int waves) {
-  constexpr int HW = kWave / G, U = 4;  // heads a wavefront takes at once; steps in flight
-  __shared__ float2 lds[kWaves][kMaxRopePairs];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * kWaves + wave;
-  const int64_t rw = w / waves;
-  const int row = p.row0 + (int)rw, part = (int)(w - rw * waves);
-  if (row >= p.rows) return;
-  const int u = lane % G, first = part * HW + lane / G, step = waves * HW;
-  const int heads = p.q.heads + p.k.heads + p.v.heads;
-  int64_t out_row = row;
-  if (p.kv_rows) out_row = p.kv_rows[row];
-  const bool kv_on = !p.kv_rows || (out_row >= 0 && out_row < p.kv_out_rows);
-  const int position = p.rot == 0 ? 0 : p.positions ? p.positions[row] : row % p.seq;
+template <int W>
+using Half = _Float16 __attribute__((ext_vector_type(W)));
 
-  const bool turns = 16 * u < p.rot, half = turns && !p.interleaved;
-  const int ca = half ? 8 * u : 16 * u, cb = half ? ca + p.rot / 2 : ca + 8;
-  const bool has_a = ca < p.dim, has_b = cb < p.dim;
-  const f16x8 none = {0, 0, 0, 0, 0, 0, 0, 0};
+// How a launch is cut: pieces of 2 W values (`units` a head), U a thread.
+struct Cut {
+  int rows, parts;  // rows of a workgroup; workgroups a row's heads are spread over
+  int units, unit_div, head_div;  // division by units and heads: (n * div) >> 20, n < 1024
+};
+constexpr int kMaxItems = 1024;  // pieces of a workgroup
+
+// A piece is two runs of W values: the same place in both halves of the turning part, or
+// neighbours (interleaved pairs, and the values that do not turn).  G: lanes a head, a power
+// of two, where heads are normed (their squares are added across lanes); 0: as many as it has
+// pieces.
+template <int W, int G, int U>
+__global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p, RopeSteps steps, Cut cut) {
+  constexpr bool NORM = G > 0;
+  using V = Half<W>;
+  HIP_DYNAMIC_SHARED(float2, cs);  // [rows][rot / 2]
+  __shared__ f16 gammas[NORM ? 2 : 1][NORM ? 2 * kMaxRopePairs : 1];
+  const int tid = threadIdx.x;
+  const int block = blockIdx.x / cut.parts, part = blockIdx.x - block * cut.parts;
+  const int r0 = p.row0 + block * cut.rows, rows = min(cut.rows, p.rows - r0);
+  const int heads = p.q.heads + p.k.heads + p.v.heads, lanes = NORM ? G : cut.units;
+  const V none = {};
+
   struct At {
     const f16* x;
     f16* y;
-    int kind;  // 0 q, 1 k, 2 v, 3 nothing
+    int kind, u, row;  // kind 0 q, 1 k, 2 v, 3 nothing; row of the workgroup's
   };
-  auto locate = [&](int h) {
-    At a{nullptr, nullptr, 3};
+  auto locate = [&](int n) {  // piece n of this thread
+    const int i = tid + n * kThreads;
+    const int hs = NORM ? i / (G ? G : 1) : (i * cut.unit_div) >> 20;
+    At a{nullptr, nullptr, 3, i - hs * lanes, 0};
+    int h = hs;
+    if (cut.parts > 1) {
+      h += part * (U * kThreads / lanes);
+      if (hs >= U * kThreads / lanes) h = heads;
+    } else {
+      a.row = (hs * cut.head_div) >> 20;
+      h -= a.row * heads;
+      if (a.row >= rows) h = heads;
+    }
+    const int row = r0 + a.row;
+    if (h >= heads) a.row = 0;
     if (h < p.q.heads) {
-      a = {p.q.x + row * p.q.x_row + h * p.q.x_head, p.q.y + row * p.q.y_row + h * p.q.y_head, 0};
-    } else if (h < heads && kv_on) {
+      a.x = p.q.x + row * p.q.x_row + h * p.q.x_head;
+      a.y = p.q.y + row * p.q.y_row + h * p.q.y_head;
+      a.kind = 0;
+    } else if (h < heads) {
       h -= p.q.heads;
       const bool k = h < p.k.heads;
       const RopeParams::Part& t = k ? p.k : p.v;
       if (!k) h -= p.k.heads;
-      a = {t.x + row * t.x_row + h * t.x_head, t.y + out_row * t.y_row + h * t.y_head, k ? 1 : 2};
+      const int64_t to = p.kv_rows ? p.kv_rows[row] : row;
+      if (!p.kv_rows || (to >= 0 && to < p.kv_out_rows)) {
+        a.x = t.x + row * t.x_row + h * t.x_head;
+        a.y = t.y + to * t.y_row + h * t.y_head;
+        a.kind = k ? 1 : 2;
+      }
     }
     return a;
   };
   At at[U];
-  f16x8 a[U], b[U];
-  auto load = [&](int h0) {
-#pragma unroll
-    for (int e = 0; e < U; ++e) {
-      at[e] = locate(h0 + e * step);
-      a[e] = b[e] = none;
-      if (at[e].kind < 3 && has_a) a[e] = *reinterpret_cast<const f16x8*>(at[e].x + ca);
-      if (at[e].kind < 3 && has_b) b[e] = *reinterpret_cast<const f16x8*>(at[e].x + cb);
-    }
+  V a[U], b[U];
+  auto place = [&](int u, int& ca, int& cb) {  // first values of a piece's runs
+    const bool half = !p.interleaved && 2 * W * u < p.rot;
+    ca = half ? W * u : 2 * W * u;
+    cb = half ? ca + p.rot / 2 : ca + W;
   };
-  load(first);
-  f16x8 ga[2], gb[2];
+#pragma unroll
+  for (int e = 0; e < U; ++e) {
+    at[e] = locate(e);
+    int ca, cb;
+    place(at[e].u, ca, cb);
+    a[e] = b[e] = none;
+    if (at[e].kind < 3 && ca < p.dim) a[e] = *reinterpret_cast<const V*>(at[e].x + ca);
+    if (at[e].kind < 3 && cb < p.dim) b[e] = *reinterpret_cast<const V*>(at[e].x + cb);
+  }
   if constexpr (NORM) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const f16* g = e == 0 ? p.q.gamma : p.k.gamma;
-      ga[e] = gb[e] = none;
-      if (g && has_a)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ga[e][i] = g[ca + i];
-      if (g && has_b)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) gb[e][i] = g[cb + i];
+    if (tid < p.dim) {
+      if (p.q.gamma) gammas[0][tid] = p.q.gamma[tid];
+      if (p.k.gamma) gammas[1][tid] = p.k.gamma[tid];
     }
   }
-  float2* cs = lds[wave];
-  angles(p, steps, position, cs, lane);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wavefront's own writes
-  float c[8], s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 v = turns ? cs[8 * u + i] : make_float2(1.f, 0.f);
-    c[i] = v.x;
-    s[i] = v.y;
+  const int pairs = p.rot / 2;
+  for (int i = tid; i < rows * pairs; i += kThreads) {
+    const int r = i / pairs;
+    cs[i] = angle(p, steps, position_of(p, r0 + r), i - r * pairs);
   }
-  for (int h0 = first; h0 - lane / G < heads; h0 += U * step) {
-    if (h0 != first) load(h0);
+  __syncthreads();
 #pragma unroll
-    for (int e = 0; e < U; ++e) {
-      if (at[e].kind > 1) {  // moved as it is, or nothing
-        if (at[e].kind == 2 && has_a) *reinterpret_cast<f16x8*>(at[e].y + ca) = a[e];
-        if (at[e].kind == 2 && has_b) *reinterpret_cast<f16x8*>(at[e].y + cb) = b[e];
-      }
-      float x[8], y[8];
+  for (int e = 0; e < U; ++e) {
+    const int kind = at[e].kind, u = at[e].u;
+    int ca, cb;
+    place(u, ca, cb);
+    V oa = a[e], ob = b[e];
+    float x[W], y[W];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = (float)a[e][i];
-        y[i] = (float)b[e][i];
-      }
-      if constexpr (NORM) {
-        float q = 0.f;
+    for (int i = 0; i < W; ++i) {
+      x[i] = (float)oa[i];
+      y[i] = (float)ob[i];
+    }
+    bool changed = false;
+    if constexpr (NORM) {
+      float q = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q = fmaf(x[i], x[i], fmaf(y[i], y[i], q));
-        q = lanes_sum<G>(q);
-        const bool k = at[e].kind == 1;
-        if (k ? p.k.gamma != nullptr : p.q.gamma != nullptr) {
-          const float r = rsqrtf(q / (float)p.dim + p.eps);
+      for (int i = 0; i < W; ++i) q = fmaf(x[i], x[i], fmaf(y[i], y[i], q));
+      q = lanes_sum<G>(q);
+      changed = kind == 0 ? p.q.gamma != nullptr : kind == 1 && p.k.gamma != nullptr;
+      if (changed) {
+        const float r = rsqrtf(q / (float)p.dim + p.eps);
+        const f16* g = gammas[kind];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            x[i] *= r * (float)(k ? ga[1][i] : ga[0][i]);
-            y[i] *= r * (float)(k ? gb[1][i] : gb[0][i]);
-          }
+        for (int i = 0; i < W; ++i) {
+          x[i] *= r * (float)g[min(ca, p.dim - W) + i];
+          y[i] *= r * (float)g[min(cb, p.dim - W) + i];
         }
       }
-      f16x8 oa, ob;
-      if (!turns) {
+    }
+    if (kind < 2 && 2 * W * u < p.rot) {
+      changed = true;
+      const float2* t = cs + at[e].row * pairs + W * u;
+      float2 v[W];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          oa[i] = (f16)x[i];
-          ob[i] = (f16)y[i];
-        }
-      } else if (p.interleaved) {  // pairs (x0, x1), (x2, x3), ... (y0, y1), ...
+      for (int i = 0; i < W; ++i) v[i] = t[i];
+      if (p.interleaved) {  // pairs (x0, x1), (x2, x3), ... (y0, y1), ...
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          oa[i] = (f16)(x[i] * c[i / 2] - x[i + 1] * s[i / 2]);
-          oa[i + 1] = (f16)(x[i + 1] * c[i / 2] + x[i] * s[i / 2]);
-          ob[i] = (f16)(y[i] * c[4 + i / 2] - y[i + 1] * s[4 + i / 2]);
-          ob[i + 1] = (f16)(y[i + 1] * c[4 + i / 2] + y[i] * s[4 + i / 2]);
+        for (int i = 0; i < W / 2; ++i) {
+          turn(x[2 * i], x[2 * i + 1], v[i]);
+          turn(y[2 * i], y[2 * i + 1], v[W / 2 + i]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          oa[i] = (f16)(x[i] * c[i] - y[i] * s[i]);
-          ob[i] = (f16)(y[i] * c[i] + x[i] * s[i]);
-        }
+        for (int i = 0; i < W; ++i) turn(x[i], y[i], v[i]);
       }
-      if (at[e].kind < 2 && has_a) *reinterpret_cast<f16x8*>(at[e].y + ca) = oa;
-      if (at[e].kind < 2 && has_b) *reinterpret_cast<f16x8*>(at[e].y + cb) = ob;
     }
+    if (changed) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        oa[i] = (f16)x[i];
+        ob[i] = (f16)y[i];
+      }
+    }
+    if (kind < 3 && ca < p.dim) *reinterpret_cast<V*>(at[e].y + ca) = oa;
+    if (kind < 3 && cb < p.dim) *reinterpret_cast<V*>(at[e].y + cb) = ob;
   }
 }
 
@@ -189,12 +215,12 @@ __global__ __launch_bounds__(64 * kWaves) void rope_any_kernel(RopeParams p, Rop
   int64_t out_row = row;
   if (p.kv_rows) out_row = p.kv_rows[row];
   const bool kv_on = !p.kv_rows || (out_row >= 0 && out_row < p.kv_out_rows);
-  const int position = p.rot == 0 ? 0 : p.positions ? p.positions[row] : row % p.seq;
+  const int position = position_of(p, row);
   float2* cs = lds[wave];
-  angles(p, steps, position, cs, lane);
+  for (int i = lane; 2 * i < p.rot; i += kWave) cs[i] = angle(p, steps, position, i);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   const int pairs = p.rot / 2;
-  auto heads = [&](const RopeParams::Part& t, int64_t yr, bool turn) {
+  auto heads = [&](const RopeParams::Part& t, int64_t yr, bool turns) {
     for (int h = 0; h < t.heads; ++h) {
       const f16* x = t.x + row * t.x_row + h * t.x_head;
       f16* y = t.y + yr * t.y_row + h * t.y_head;
@@ -220,7 +246,7 @@ __global__ __launch_bounds__(64 * kWaves) void rope_any_kernel(RopeParams p, Rop
           q = fmaf(rest[e], rest[e], q);
         }
       }
-      const bool norm = turn && t.gamma;
+      const bool norm = turns && t.gamma;
       float r = 1.f;
       if (norm) r = rsqrtf(wave_sum(q) / (float)p.dim + p.eps);
 #pragma unroll
@@ -233,9 +259,9 @@ __global__ __launch_bounds__(64 * kWaves) void rope_any_kernel(RopeParams p, Rop
             u *= r * (float)t.gamma[ia];
             v *= r * (float)t.gamma[ib];
           }
-          const float2 a = turn ? cs[i] : make_float2(1.f, 0.f);
-          y[ia] = (f16)(turn ? u * a.x - v * a.y : u);
-          y[ib] = (f16)(turn ? v * a.x + u * a.y : v);
+          if (turns) turn(u, v, cs[i]);
+          y[ia] = (f16)u;
+          y[ib] = (f16)v;
         }
       }
 #pragma unroll
@@ -252,48 +278,83 @@ __global__ __launch_bounds__(64 * kWaves) void rope_any_kernel(RopeParams p, Rop
   }
 }
 
-bool wide(const RopeParams::Part& t) {
-  if (!t.heads) return true;
-  return (((uintptr_t)t.x | (uintptr_t)t.y) & 15) == 0 &&
-         ((t.x_row | t.x_head | t.y_row | t.y_head) & 7) == 0;
+// Values that every address and stride of a part allows to be moved at once.
+int width(const RopeParams::Part& t, int w) {
+  if (!t.heads) return w;
+  const uint64_t all = ((uint64_t)(uintptr_t)t.x | (uint64_t)(uintptr_t)t.y) / 2 |
+                       (uint64_t)(t.x_row | t.x_head | t.y_row | t.y_head);
+  while (w > 1 && (all & (w - 1))) w /= 2;
+  return ((uintptr_t)t.x | (uintptr_t)t.y) & 1 ? 1 : w;
 }
 
-template <int G>
-hipError_t launch(const RopeParams& p, const RopeSteps& steps, int rows, hipStream_t s) {
-  const int heads = p.q.heads + p.k.heads + p.v.heads, at_once = 64 / G;
-  // few rows: their heads over several wavefronts
-  const int most = (heads + at_once - 1) / at_once;
-  const int waves = std::min(most, std::max(1, 4096 / rows));
-  const dim3 grid((unsigned)(((int64_t)rows * waves + kWaves - 1) / kWaves)), block(64 * kWaves);
-  if (p.q.gamma || p.k.gamma)
-    hipLaunchKernelGGL((rope_kernel<G, true>), grid, block, 0, s, p, steps, waves);
-  else
-    hipLaunchKernelGGL((rope_kernel<G, false>), grid, block, 0, s, p, steps, waves);
+int pow2(int n) {
+  int p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+
+template <int W, int G, int U>
+hipError_t launch_as(const RopeParams& p, const RopeSteps& steps, hipStream_t s) {
+  const int heads = p.q.heads + p.k.heads + p.v.heads;
+  Cut c{};
+  c.units = (p.dim + 2 * W - 1) / (2 * W);
+  const int lanes = G ? G : c.units, at_once = U * kThreads / lanes;  // heads of a workgroup
+  c.rows = std::max(1, std::min(at_once / heads, 2048 / std::max(1, p.rot / 2)));
+  c.parts = (heads + at_once - 1) / at_once;
+  c.unit_div = ((1 << 20) + c.units - 1) / c.units;
+  c.head_div = ((1 << 20) + heads - 1) / heads;
+  const int rows = p.rows - p.row0;
+  const int64_t grid = (int64_t)((rows + c.rows - 1) / c.rows) * c.parts;
+  const size_t lds = (size_t)c.rows * (p.rot / 2) * sizeof(float2);
+  hipLaunchKernelGGL((rope_kernel<W, G, U>), dim3((unsigned)grid), dim3(kThreads), lds, s, p, steps, c);
   return hipGetLastError();
+}
+template <int W, int G>
+hipError_t launch(const RopeParams& p, const RopeSteps& steps, hipStream_t s) {
+  const int64_t items = (int64_t)(p.rows - p.row0) * (p.q.heads + p.k.heads + p.v.heads) *
+                        (G ? G : (p.dim + 2 * W - 1) / (2 * W));
+  return items < 1 << 18 ? launch_as<W, G, 1>(p, steps, s) : launch_as<W, G, 4>(p, steps, s);
+}
+template <int W>
+hipError_t launch_w(const RopeParams& p, const RopeSteps& steps, hipStream_t s) {
+  if (!p.q.gamma && !p.k.gamma) return launch<W, 0>(p, steps, s);
+  const int g = pow2((p.dim + 2 * W - 1) / (2 * W));
+  if constexpr (W <= 2) {
+    if (g > 32) return launch<W, 64>(p, steps, s);
+  }
+  if constexpr (W <= 4) {
+    if (g > 16) return launch<W, 32>(p, steps, s);
+  }
+  return g > 8 ? launch<W, 16>(p, steps, s)
+         : g > 4 ? launch<W, 8>(p, steps, s)
+         : g > 2 ? launch<W, 4>(p, steps, s)
+         : g > 1 ? launch<W, 2>(p, steps, s)
+                 : launch<W, 1>(p, steps, s);
 }
 
 }  // namespace
 
 hipError_t rope_heads(const RopeParams& args, const RopeSteps& steps, hipStream_t s) {
-  const bool fast = args.dim % 8 == 0 && args.rot % 16 == 0 && wide(args.q) && wide(args.k) &&
-                    wide(args.v);
-  constexpr int kRows = 1 << 25;  // of a launch, whose threads are counted in 32 bits
+  // values moved at once: what addresses, strides, the head and the turning part allow
+  int w = width(args.v, width(args.k, width(args.q, 8)));
+  while (w > 1 && (args.dim % w || args.rot % (2 * w))) w /= 2;
+  const int heads = args.q.heads + args.k.heads + args.v.heads;
+  // rows of a launch: threads are counted in 32 bits, and 64 * heads cover a row's
+  const int most = std::max(1, (1 << 30) / (64 * heads + kThreads));
   for (int row0 = 0; row0 < args.rows;) {
     RopeParams p = args;
-    const int rows = std::min(kRows, args.rows - row0);
+    const int rows = std::min(most, args.rows - row0);
     p.row0 = row0;
     p.rows = row0 + rows;
     hipError_t e;
-    if (!fast) {
+    if (w == 1) {
       hipLaunchKernelGGL(rope_any_kernel, dim3((unsigned)((rows + kWaves - 1) / kWaves)),
-                         dim3(64 * kWaves), 0, s, p, steps);
+                         dim3(kThreads), 0, s, p, steps);
       e = hipGetLastError();
     } else {
-      e = p.dim <= 16    ? launch<1>(p, steps, rows, s)
-          : p.dim <= 32  ? launch<2>(p, steps, rows, s)
-          : p.dim <= 64  ? launch<4>(p, steps, rows, s)
-          : p.dim <= 128 ? launch<8>(p, steps, rows, s)
-                         : launch<16>(p, steps, rows, s);
+      e = w == 8   ? launch_w<8>(p, steps, s)
+          : w == 4 ? launch_w<4>(p, steps, s)
+                   : launch_w<2>(p, steps, s);
     }
     if (e != hipSuccess) return e;
     row0 += rows;
