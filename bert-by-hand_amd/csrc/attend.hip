@@ -41,15 +41,16 @@ struct Tile {
 constexpr float kLazy = 8.f;
 constexpr int kMaxSplits = 256;  // a thread of the joining workgroup each
 
-template <int HD_, int NW_, int T_, int KS_, int R_, int OCC_>
+template <int HD_, int NW_, int T_, int KS_, int SK_, int R_, int OCC_>
 struct Cfg {
   static constexpr int HD = HD_, NW = NW_, T = T_, KS = KS_, R = R_, OCC = OCC_;
   static_assert(KS == 1 || KS == NW, "waves go along the rows or along the keys");
   static constexpr int RW = NW / KS;
   static constexpr int BM = RW * T * 32;         // rows of a workgroup
-  static constexpr int SK = KS == 1 ? 64 : 32;   // keys of a tile
+  static constexpr int SK = SK_;                 // keys of a tile
   static constexpr int CW = KS == 1 ? NW : 1;    // wavefronts that share a tile's copies
   static constexpr int N = SK * HD / 512 / CW;   // copies of a wavefront: a tile of K, of V
+  static_assert(SK * HD % (512 * CW) == 0, "whole copies a wavefront");
   static constexpr int STAGE = 2 * SK * HD;      // halves of a stage: K, V
   static constexpr int RINGS = KS;               // a ring each wavefront where it has tiles of its own
   static constexpr size_t RING = (size_t)RINGS * R * STAGE * 2;
@@ -93,9 +94,240 @@ struct IeeeMax {
   __device__ __forceinline__ float operator()(float a, float b) const { return imax(a, b); }
 };
 
+#define BBH_LDS __attribute__((address_space(3)))
+typedef BBH_LDS f16 lds_f16;
+
+// Scheduling of STEPS steps, each of READS LDS reads and M products of what they read: the
+// reads run A steps ahead of the products, no further (left alone the compiler reads the whole
+// tile first, into more registers than there are).
+template <int STEPS, int READS, int M, int A>
+__device__ __forceinline__ void ahead() {
+  constexpr int P = A < STEPS ? A : STEPS;
+  __builtin_amdgcn_sched_group_barrier(0x100, READS * P, 0);
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+    if (i + P < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
+}
+constexpr int kAheadK = 3, kAheadV = 2;
+
+// What a lane knows of its T rows, and the running state of their softmax.
+template <class C>
+struct Rows {
+  f16x8 q[C::T][C::HD / 16];
+  int lo[C::T], hi[C::T];  // keys it sees, apart from the prefix
+  int qpos[C::T];
+  float slope[C::T];  // in units of log2
+  f32x16 o[C::T][C::HD / 32];
+  float m[C::T], l[C::T];
+};
+
+// One tile of keys at LDS rows ks (K, chunked by fk) and vs (V, by fv): scores, softmax,
+// output.  edge: some pair of the tile is not seen (`on`: its unmasked keys).  The tile's
+// pointers are restrict beside the stage being filled: otherwise every transposed read
+// waits for the copies in flight.
+template <class C, int FEAT>
+__device__ __forceinline__ void tile_step(const AttendParams& p, Rows<C>& r,
+                                          const lds_f16* __restrict__ ks,
+                                          const lds_f16* __restrict__ vs, const float* tab, int k0,
+                                          bool edge, uint64_t on, int prefix, float lag,
+                                          float mscale) {
+  constexpr int HD = C::HD, T = C::T, CH = C::SK / 32, NS = HD / 16, ND = HD / 32;
+  const int lane = threadIdx.x & 63, r32 = lane & 31, kh = lane >> 5;
+  const f16x2 ones = {(f16)1.f, (f16)1.f};
+  uint32_t see[T][CH];
+  if (edge) {
+    uint32_t some = 0;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) {
+        const int kb = k0 + 32 * ch;
+        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };
+        const uint32_t w = ((below(r.hi[t] - kb) & ~below(r.lo[t] - kb)) | below(prefix - kb)) &
+                           (uint32_t)(on >> (32 * ch));
+        some |= w;
+        see[t][ch] = w >> (8 * kh);
+      }
+    if (!__ballot(some != 0)) return;
+  }
+  f32x16 s[T][CH];
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch) {
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+      const f16x8 kf = *reinterpret_cast<const BBH_LDS f16x8*>(
+          ks + (32 * ch + r32) * HD + (((2 * st + kh) ^ Tile<HD>::fk(r32)) << 3));
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        s[t][ch] = mfma32(kf, r.q[t][st], st == 0 ? f32x16{} : s[t][ch]);
+    }
+  }
+  ahead<CH * NS, 1, T, kAheadK>();
+  // s[t][ch][i]: key k0 + 32 ch + 16 (i / 8) + 8 kh + i % 8
+  if constexpr (FEAT != kPlain) {
+    if (FEAT == kCap || p.cap_l > 0.f) {
+      const float cap2 = -2.f * p.cap_l;
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(s[t][ch][i] * p.cap_k);
+            s[t][ch][i] = fmaf(cap2, __builtin_amdgcn_rcpf(e + 1.f), p.cap_l);
+          }
+    } else {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) s[t][ch] *= p.c;
+    }
+  }
+  if constexpr (FEAT == kAny) {
+    if (p.slopes) {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+          const float df = (float)(k0 + 32 * ch + 8 * kh - r.qpos[t]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[t][ch][i] = fmaf(-r.slope[t], fabsf(df + (float)(16 * (i >> 3) + (i & 7))), s[t][ch][i]);
+        }
+    }
+    if (p.table) {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int d = k0 + 32 * ch + 8 * kh - r.qpos[t] + 16 * (i >> 3) + (i & 7);
+            const float w = tab[min(max(d, -p.half), p.half)];
+            s[t][ch][i] += w == -INFINITY ? w : imax(w * 1.44269504088896f, -1e30f);
+          }
+    }
+  }
+  if (edge) {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[t][ch][i] = (see[t][ch] >> (16 * (i >> 3) + (i & 7))) & 1 ? s[t][ch][i] : -INFINITY;
+  }
+  bool up = false;
+  float mx[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    float v = imax(s[t][0][0], s[t][0][1]);
+#pragma unroll
+    for (int i = 2; i < 16; i += 2) v = imax(imax(v, s[t][0][i]), s[t][0][i + 1]);
+#pragma unroll
+    for (int ch = 1; ch < CH; ++ch)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) v = imax(imax(v, s[t][ch][i]), s[t][ch][i + 1]);
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    mx[t] = imax(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    up = up || !(mx[t] <= r.m[t] + lag);
+  }
+  if (__ballot(up)) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const float mn = imax(r.m[t], mx[t]);
+      const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((r.m[t] - mn) * mscale);
+      r.l[t] *= corr;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) r.o[t][d] *= corr;
+      r.m[t] = mn;
+    }
+  }
+  f16x8 pr[T][CH][2];
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      // a row that has seen nothing yet: every weight 2^(-inf) = 0
+      const float mc = r.m[t] == -INFINITY ? 0.f : r.m[t] * mscale;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = FEAT == kPlain ? fmaf(s[t][ch][i], p.c, -mc) : s[t][ch][i] - mc;
+        pr[t][ch][i >> 3][i & 7] = (f16)__builtin_amdgcn_exp2f(x);
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+          r.l[t] = __builtin_amdgcn_fdot2(f16x2{pr[t][ch][hf][i], pr[t][ch][hf][i + 1]}, ones, r.l[t], false);
+    }
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const int row = 32 * ch + 16 * hf + 8 * kh + ((lane >> 2) & 3);
+        const int c16 = (4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ Tile<HD>::fv((lane >> 2) & 3);
+        const lds_f16* at = vs + row * HD + (c16 << 3) + 4 * (lane & 1);
+        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((BBH_LDS s16x4*)at);
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((BBH_LDS s16x4*)(at + 4 * HD));
+        const f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int t = 0; t < T; ++t) r.o[t][d] = mfma32(vf, pr[t][ch][hf], r.o[t][d]);
+      }
+  }
+  ahead<CH * 2 * ND, 2, T, kAheadV>();
+}
+
+// One wavefront's share of a tile's copies.
+template <class C>
+struct Copies {
+  uint32_t koff[C::N], voff[C::N];
+  int cwave;
+  static constexpr uint32_t kNowhere = 0x80000000u;  // past every resource: reads nothing, writes zeros
+
+  __device__ __forceinline__ void init(const AttendParams& p, int wave, int lane) {
+    cwave = C::KS == 1 ? wave : 0;
+#pragma unroll
+    for (int j = 0; j < C::N; ++j) {
+      const int s = (cwave * C::N + j) * 64 + lane, r = s / Tile<C::HD>::CPR, slot = s % Tile<C::HD>::CPR;
+      const int kc = slot ^ Tile<C::HD>::fk(r & 31), vc = slot ^ Tile<C::HD>::fv(r);
+      const int kr = (r & ~31) + key_of_row(r & 31);
+      koff[j] = 8 * kc < p.dim ? (uint32_t)(kr * (int)p.ks.row + 8 * kc) * 2u : kNowhere;
+      voff[j] = 8 * vc < p.dim ? (uint32_t)(r * (int)p.vs.row + 8 * vc) * 2u : kNowhere;
+    }
+  }
+  // Keys from k0 on (`valid` of them) into a stage.  Rows behind them are zeros, and so are
+  // values whose key is masked (`bits`, where `masked`): nothing they hold reaches a sum.
+  __device__ __forceinline__ void issue(const AttendParams& p, const f16* k, const f16* v, int valid,
+                                        bool masked, uint64_t bits, lds_f16* __restrict__ stage,
+                                        int lane) {
+    const auto rk = buffer_of(k, (uint32_t)((valid - 1) * (int)p.ks.row + p.dim) * 2u);
+    const auto rv = buffer_of(v, (uint32_t)((valid - 1) * (int)p.vs.row + p.dim) * 2u);
+    lds_f16* ks = stage + cwave * C::N * 512;
+    lds_f16* vs = ks + C::SK * C::HD;
+#pragma unroll
+    for (int j = 0; j < C::N; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (BBH_LDS void*)(ks + j * 512), 16, (int)koff[j], 0, 0, 0);
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < C::N; ++j) {
+        const int r = ((cwave * C::N + j) * 64 + lane) / Tile<C::HD>::CPR;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (BBH_LDS void*)(vs + j * 512), 16,
+                                                 (int)((bits >> r) & 1 ? voff[j] : kNowhere), 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::N; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (BBH_LDS void*)(vs + j * 512), 16, (int)voff[j], 0, 0, 0);
+    }
+  }
+};
+
 template <class C, int FEAT>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams p) {
-  constexpr int HD = C::HD, T = C::T, SK = C::SK, CH = SK / 32, NS = HD / 16, ND = HD / 32;
+  constexpr int HD = C::HD, T = C::T, SK = C::SK, NS = HD / 16, ND = HD / 32;
   HIP_DYNAMIC_SHARED(f16, smem);
   // (sequence, key/value head), row block and split of this workgroup
   const int rows_all = p.batch * p.kv_heads, cols = p.blocks * p.splits;
@@ -128,10 +360,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   // ---- the rows of this lane: row = query * group + head of the group
   const int shift = nk - nq;
   const int prefix = p.prefix ? min(max(p.prefix[b], 0), nk) : 0;
-  int lo[T], hi[T];
-  float slope[T];
-  int qpos[T], thead[T];
-  f16x8 q[T][NS];
+  Rows<C> r;
+  const float* tab = nullptr;
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     const int row = min(row0 + (rw * T + t) * 32 + r32, rows - 1);
@@ -140,15 +370,15 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
                      h * p.qs.head;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      q[t][s] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (16 * s + 8 * kh < p.dim) q[t][s] = *reinterpret_cast<const f16x8*>(src + 16 * s + 8 * kh);
+      r.q[t][s] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (16 * s + 8 * kh < p.dim) r.q[t][s] = *reinterpret_cast<const f16x8*>(src + 16 * s + 8 * kh);
     }
     const int pos = i + shift;
-    lo[t] = p.left < 0 ? 0 : max(pos - p.left, 0);
-    hi[t] = p.right < 0 ? nk : min(pos + p.right + 1, nk);
-    qpos[t] = pos;
-    thead[t] = h;
-    slope[t] = FEAT == kAny && p.slopes ? p.slopes[h] * 1.44269504088896f : 0.f;
+    r.lo[t] = p.left < 0 ? 0 : max(pos - p.left, 0);
+    r.hi[t] = p.right < 0 ? nk : min(pos + p.right + 1, nk);
+    r.qpos[t] = pos;
+    r.slope[t] = FEAT == kAny && p.slopes ? p.slopes[h] * 1.44269504088896f : 0.f;
+    if (FEAT == kAny && p.table) tab = p.table + (int64_t)h * (2 * p.half + 1) + p.half;
   }
   // ---- the tiles of this block: those of the prefix, then those of the window
   const int first_q = row0 / p.group, last_q = (min(row0 + C::BM, rows) - 1) / p.group;
@@ -161,9 +391,9 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   int begin = split * p.chunk, end = min(tiles, begin + p.chunk);
   if constexpr (C::KS > 1) begin += wave;
   const int count = begin >= end ? 0 : (end - begin + C::KS - 1) / C::KS;
-  auto tile_at = [&](int i) {
+  auto key_at = [&](int i) {
     const int n = begin + i * C::KS;
-    return n < np ? n : t0 + (n - np);
+    return (n < np ? n : t0 + (n - np)) * SK;
   };
   // interior tiles, which every row of the block sees whole: [full_lo, full_hi)
   const int full_lo = p.left < 0 ? 0 : max(last_q + shift - p.left, 0);
@@ -172,215 +402,65 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   const f16* kbase = p.k + (p.k_offsets ? sq.k0 * p.ks.row : b * p.ks.batch) + kvh * p.ks.head;
   const f16* vbase = p.v + (p.k_offsets ? sq.k0 * p.vs.row : b * p.vs.batch) + kvh * p.vs.head;
   const int32_t* mrow = p.mask ? p.mask + (int64_t)b * p.k_len : nullptr;
-  f16* ring = smem + (C::KS == 1 ? 0 : wave * C::R * C::STAGE);
-  const int cwave = C::KS == 1 ? wave : 0;
+  lds_f16* ring = (lds_f16*)smem + (C::KS == 1 ? 0 : wave * C::R * C::STAGE);
 
-  constexpr uint32_t kNowhere = 0x80000000u;  // past every resource: reads nothing, writes zeros
-  uint32_t koff[C::N], voff[C::N];
-  int krow[C::N], vrow[C::N];
-#pragma unroll
-  for (int j = 0; j < C::N; ++j) {
-    const int s = (cwave * C::N + j) * 64 + lane, r = s / Tile<HD>::CPR, slot = s % Tile<HD>::CPR;
-    const int kc = slot ^ Tile<HD>::fk(r & 31), vc = slot ^ Tile<HD>::fv(r);
-    krow[j] = (r & ~31) + key_of_row(r & 31);
-    vrow[j] = r;
-    koff[j] = 8 * kc < p.dim ? (uint32_t)(krow[j] * (int)p.ks.row + 8 * kc) * 2u : kNowhere;
-    voff[j] = 8 * vc < p.dim ? (uint32_t)(r * (int)p.vs.row + 8 * vc) * 2u : kNowhere;
-  }
-  auto mask_bits = [&](int k0) -> uint64_t {  // unmasked keys of the tile
-    if (!mrow) {
-      const int left = nk - k0;
-      return left >= 64 ? ~0ull : left <= 0 ? 0ull : ((1ull << left) - 1);
-    }
-    const int key = k0 + (SK == 64 ? lane : (lane & 31));
-    const int on = key < nk ? mrow[key] : 0;
-    return __ballot(on != 0);
-  };
+  Copies<C> copies;
+  copies.init(p, wave, lane);
   auto issue = [&](int i, uint64_t bits) {
-    const int k0 = tile_at(i) * SK;
-    f16* ks = ring + (i % C::R) * C::STAGE;
-    f16* vs = ks + SK * HD;
-    const int valid = min(nk - k0, SK);
-    const auto rk = buffer_of(kbase + (int64_t)k0 * p.ks.row,
-                              (uint32_t)((valid - 1) * (int)p.ks.row + p.dim) * 2u);
-    const auto rv = buffer_of(vbase + (int64_t)k0 * p.vs.row,
-                              (uint32_t)((valid - 1) * (int)p.vs.row + p.dim) * 2u);
-#pragma unroll
-    for (int j = 0; j < C::N; ++j) {
-      uint32_t off = koff[j];
-      if (mrow && !((bits >> krow[j]) & 1)) off = kNowhere;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rk, (__attribute__((address_space(3))) void*)(ks + (cwave * C::N + j) * 512), 16, (int)off, 0, 0, 0);
-    }
-#pragma unroll
-    for (int j = 0; j < C::N; ++j) {
-      uint32_t off = voff[j];
-      if (mrow && !((bits >> vrow[j]) & 1)) off = kNowhere;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rv, (__attribute__((address_space(3))) void*)(vs + (cwave * C::N + j) * 512), 16, (int)off, 0, 0, 0);
-    }
+    const int k0 = key_at(i);
+    copies.issue(p, kbase + (int64_t)k0 * p.ks.row, vbase + (int64_t)k0 * p.vs.row, min(nk - k0, SK),
+                 mrow != nullptr, bits, ring + (i % C::R) * C::STAGE, lane);
   };
-
-  const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const f16x2 ones = {(f16)1.f, (f16)1.f};
-  f32x16 o[T][ND];
-  float m[T], l[T];
+  // the lane's mask value of tile i, and the tile's unmasked keys from it
+  auto load_mask = [&](int i) {
+    const int key = key_at(i) + (SK == 64 ? lane : r32);
+    return mrow && key < nk ? mrow[key] : 0;
+  };
+  auto bits_of = [&](int i, int value) -> uint64_t {
+    if (mrow) return __ballot(value != 0);
+    const int n = nk - key_at(i);
+    return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+  };
 #pragma unroll
   for (int t = 0; t < T; ++t) {
 #pragma unroll
-    for (int d = 0; d < ND; ++d) o[t][d] = zero;
-    m[t] = -INFINITY;
-    l[t] = 0.f;
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r.o[t][d][i] = 0.f;
+    r.m[t] = -INFINITY;
+    r.l[t] = 0.f;
   }
   const float lag = FEAT == kPlain ? kLazy / p.c : kLazy;
   const float mscale = FEAT == kPlain ? p.c : 1.f;
+  constexpr uint64_t kAll = SK == 64 ? ~0ull : 0xffffffffull;
 
   uint64_t bits_now = 0, bits_next = 0;
+  int mask_next = 0;
   if (count > 0) {
-    bits_now = mask_bits(tile_at(0) * SK);
+    bits_now = bits_of(0, load_mask(0));
     issue(0, bits_now);
-    if (count > 1) bits_next = mask_bits(tile_at(1) * SK);
+    if (count > 1) mask_next = load_mask(1);
   }
   for (int it = 0; it < count; ++it) {
     wait_vm<0>();
     if constexpr (C::KS == 1) lds_barrier();
     else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (it + 1 < count) issue(it + 1, bits_next);
-    const uint64_t bits = bits_now;
-    bits_now = bits_next;
-    if (it + 2 < count) bits_next = mask_bits(tile_at(it + 2) * SK);
-    const int k0 = tile_at(it) * SK;
-    const f16* ks = ring + (it % C::R) * C::STAGE;
-    const f16* vs = ks + SK * HD;
-#pragma unroll
-    for (int ch = 0; ch < CH; ++ch) {
-      const int kb = k0 + 32 * ch;
-      const uint32_t on = (uint32_t)(bits >> (32 * ch));
-      if (on == 0) continue;
-      const bool whole = on == 0xffffffffu && (kb + 32 <= prefix || (kb >= full_lo && kb + 32 <= full_hi));
-      uint32_t see[T];
-      if (!whole) {
-        uint32_t some = 0;
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-          // bits [max(lo, 0), hi) or below prefix, relative to kb
-          auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };
-          see[t] = ((below(hi[t] - kb) & ~below(lo[t] - kb)) | below(prefix - kb)) & on;
-          some |= see[t];
-          see[t] >>= 8 * kh;
-        }
-        if (!__ballot(some != 0)) continue;
-      }
-      f32x16 s[T];
-#pragma unroll
-      for (int t = 0; t < T; ++t) s[t] = zero;
-#pragma unroll
-      for (int st = 0; st < NS; ++st) {
-        const f16x8 kf = *reinterpret_cast<const f16x8*>(
-            ks + (32 * ch + r32) * HD + (((2 * st + kh) ^ Tile<HD>::fk(r32)) << 3));
-#pragma unroll
-        for (int t = 0; t < T; ++t) s[t] = mfma32(kf, q[t][st], s[t]);
-      }
-      // s[i]: key kb + 16*(i/8) + 8*kh + i%8
-      if constexpr (FEAT != kPlain) {
-        if (FEAT == kCap || p.cap_l > 0.f) {
-#pragma unroll
-          for (int t = 0; t < T; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float e = __builtin_amdgcn_exp2f(s[t][i] * p.cap_k);
-              s[t][i] = fmaf(-2.f * p.cap_l, __builtin_amdgcn_rcpf(e + 1.f), p.cap_l);
-            }
-        } else {
-#pragma unroll
-          for (int t = 0; t < T; ++t) s[t] *= p.c;
-        }
-      }
-      if constexpr (FEAT == kAny) {
-        if (p.slopes) {
-#pragma unroll
-          for (int t = 0; t < T; ++t) {
-            const float d0 = (float)(kb + 8 * kh - qpos[t]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              s[t][i] = fmaf(-slope[t], fabsf(d0 + (float)(16 * (i >> 3) + (i & 7))), s[t][i]);
-          }
-        }
-        if (p.table) {
-#pragma unroll
-          for (int t = 0; t < T; ++t) {
-            const float* tab = p.table + (int64_t)thead[t] * (2 * p.half + 1) + p.half;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int d = kb + 8 * kh + 16 * (i >> 3) + (i & 7) - qpos[t];
-              const float w = tab[min(max(d, -p.half), p.half)];
-              s[t][i] += w == -INFINITY ? w : imax(w * 1.44269504088896f, -1e30f);
-            }
-          }
-        }
-      }
-      if (!whole) {
-#pragma unroll
-        for (int t = 0; t < T; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            s[t][i] = (see[t] >> (16 * (i >> 3) + (i & 7))) & 1 ? s[t][i] : -INFINITY;
-      }
-      bool up = false;
-      float mx[T];
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        float v = imax(imax(s[t][0], s[t][1]), s[t][2]);
-#pragma unroll
-        for (int i = 3; i < 15; i += 2) v = imax(imax(v, s[t][i]), s[t][i + 1]);
-        v = imax(v, s[t][15]);
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        mx[t] = imax(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        up = up || !(mx[t] <= m[t] + lag);
-      }
-      if (__ballot(up)) {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-          const float mn = imax(m[t], mx[t]);
-          const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[t] - mn) * mscale);
-          l[t] *= corr;
-#pragma unroll
-          for (int d = 0; d < ND; ++d) o[t][d] *= corr;
-          m[t] = mn;
-        }
-      }
-      f16x8 pr[T][2];
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const float mc = m[t] == -INFINITY ? 0.f : m[t] * mscale;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = FEAT == kPlain ? fmaf(s[t][i], p.c, -mc) : s[t][i] - mc;
-          pr[t][i >> 3][i & 7] = (f16)__builtin_amdgcn_exp2f(x);
-        }
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-          for (int i = 0; i < 8; i += 2)
-            l[t] = __builtin_amdgcn_fdot2(f16x2{pr[t][hf][i], pr[t][hf][i + 1]}, ones, l[t], false);
-      }
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const int r = 32 * ch + 16 * hf + 8 * kh + ((lane >> 2) & 3);
-          const int c16 = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-          auto* a = (__attribute__((address_space(3))) s16x4*)(vs + r * HD + ((c16 ^ Tile<HD>::fv(r)) << 3) + 4 * (lane & 1));
-          auto* a4 = (__attribute__((address_space(3))) s16x4*)(vs + (r + 4) * HD + ((c16 ^ Tile<HD>::fv(r)) << 3) + 4 * (lane & 1));
-          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(a);
-          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(a4);
-          const auto vv = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-          const f16x8 vf = __builtin_bit_cast(f16x8, vv);
-#pragma unroll
-          for (int t = 0; t < T; ++t) o[t][d] = mfma32(vf, pr[t][hf], o[t][d]);
-        }
+    if (it + 1 < count) {
+      bits_next = bits_of(it + 1, mask_next);
+      issue(it + 1, bits_next);
+      if (mrow && it + 2 < count) mask_next = load_mask(it + 2);
     }
+    const uint64_t bits = bits_now & kAll;
+    bits_now = bits_next;
+    const int k0 = key_at(it);
+    const lds_f16* ks = ring + (it % C::R) * C::STAGE;
+    const bool edge = bits != kAll || !(k0 + SK <= prefix || (k0 >= full_lo && k0 + SK <= full_hi));
+    if (bits)
+      tile_step<C, FEAT>(p, r, ks, ks + SK * HD, tab, k0, edge, bits, prefix, lag, mscale);
   }
+  f32x16 (&o)[T][ND] = r.o;
+  float (&m)[T] = r.m;
+  float (&l)[T] = r.l;
 #pragma unroll
   for (int t = 0; t < T; ++t) l[t] = xor32_sum(l[t]);
 
@@ -518,6 +598,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
   const int g = tid / L, c = tid % L;
   f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
   if (g < GR) {
+#pragma unroll 2
     for (int s = g; s < p.splits; s += GR) {
       const float ws2 = w[s];
       if (ws2 == 0.f) continue;  // an empty split wrote nothing
@@ -536,6 +617,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
   if (tid >= L || 8 * tid >= p.dim) return;
   x = sums[0][tid][0];
   y = sums[0][tid][1];
+#pragma unroll 4
   for (int i = 1; i < GR; ++i) {
     x += sums[i][tid][0];
     y += sums[i][tid][1];
@@ -620,17 +702,17 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
   return hipSuccess;
 }
 
-//                 HD  NW T KS R OCC
-using P32 = Cfg<32, 4, 2, 1, 2, 2>;
-using P64 = Cfg<64, 4, 2, 1, 2, 2>;
-using P96 = Cfg<96, 4, 2, 1, 2, 1>;
-using P128 = Cfg<128, 4, 2, 1, 2, 1>;
-using P256 = Cfg<256, 4, 1, 1, 2, 1>;
-using K32 = Cfg<32, 4, 1, 4, 2, 2>;
-using K64 = Cfg<64, 4, 1, 4, 2, 2>;
-using K96 = Cfg<96, 4, 1, 4, 2, 1>;
-using K128 = Cfg<128, 4, 1, 4, 2, 1>;
-using K256 = Cfg<256, 2, 1, 2, 2, 1>;
+//                HD  NW T KS SK R OCC
+using P32 = Cfg<32, 4, 1, 1, 64, 2, 4>;
+using P64 = Cfg<64, 8, 1, 1, 64, 2, 3>;
+using P96 = Cfg<96, 4, 1, 1, 64, 2, 2>;
+using P128 = Cfg<128, 8, 1, 1, 64, 2, 2>;
+using P256 = Cfg<256, 4, 1, 1, 32, 2, 1>;
+using K32 = Cfg<32, 4, 1, 4, 32, 2, 2>;
+using K64 = Cfg<64, 4, 1, 4, 32, 2, 2>;
+using K96 = Cfg<96, 4, 1, 4, 32, 2, 1>;
+using K128 = Cfg<128, 4, 1, 4, 32, 2, 1>;
+using K256 = Cfg<256, 2, 1, 2, 32, 2, 1>;
 
 template <class F>
 auto with_config(const AttendParams& p, F&& f) {
