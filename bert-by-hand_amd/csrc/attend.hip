@@ -41,13 +41,14 @@ struct Tile {
 constexpr float kLazy = 8.f;
 constexpr int kMaxSplits = 256;  // a thread of the joining workgroup each
 
-template <int HD_, int NW_, int T_, int KS_, int SK_, int R_, int OCC_>
+template <int HD_, int NW_, int KS_, int SK_, int R_, int OCC_>
 struct Cfg {
-  static constexpr int HD = HD_, NW = NW_, T = T_, KS = KS_, R = R_, OCC = OCC_;
+  static constexpr int HD = HD_, NW = NW_, KS = KS_, R = R_, OCC = OCC_;
   static_assert(KS == 1 || KS == NW, "waves go along the rows or along the keys");
   static constexpr int RW = NW / KS;
-  static constexpr int BM = RW * T * 32;         // rows of a workgroup
+  static constexpr int BM = RW * 32;             // rows of a workgroup
   static constexpr int SK = SK_;                 // keys of a tile
+  static constexpr int CH = SK / 32;             // 32-key chunks of a tile
   static constexpr int CW = KS == 1 ? NW : 1;    // wavefronts that share a tile's copies
   static constexpr int N = SK * HD / 512 / CW;   // copies of a wavefront: a tile of K, of V
   static_assert(SK * HD % (512 * CW) == 0, "whole copies a wavefront");
@@ -56,7 +57,8 @@ struct Cfg {
   static constexpr size_t RING = (size_t)RINGS * R * STAGE * 2;
   static constexpr size_t OUT = KS == 1 ? (size_t)NW * 32 * (HD + 8) * 2
                                         : (size_t)KS * 32 * (HD + 4) * 4 + KS * 32 * 8;
-  static constexpr size_t LDS = RING > OUT ? RING : OUT;
+  static constexpr size_t MASKS = (size_t)RINGS * R * 64 * 4;  // a tile's mask beside it
+  static constexpr size_t LDS = RING + MASKS > OUT ? RING + MASKS : OUT;
   static constexpr int THREADS = 64 * NW;
 };
 
@@ -97,187 +99,203 @@ struct IeeeMax {
 #define BBH_LDS __attribute__((address_space(3)))
 typedef BBH_LDS f16 lds_f16;
 
-// Scheduling of STEPS steps, each of READS LDS reads and M products of what they read: the
-// reads run A steps ahead of the products, no further (left alone the compiler reads the whole
-// tile first, into more registers than there are).
-template <int STEPS, int READS, int M, int A>
+// Scheduling of STEPS steps, each of READS LDS reads and a product of what they read: the reads
+// run A steps ahead of the products, no further (left alone the compiler reads the whole tile
+// first, into more registers than there are).  VALU and TRANS other operations of the block go
+// beside each product.
+template <int STEPS, int READS, int A, int VALU = 0, int TRANS = 0>
 __device__ __forceinline__ void ahead() {
   constexpr int P = A < STEPS ? A : STEPS;
   __builtin_amdgcn_sched_group_barrier(0x100, READS * P, 0);
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     if (i + P < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    if constexpr (VALU > 0) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+    if constexpr (TRANS > 0) __builtin_amdgcn_sched_group_barrier(0x400, TRANS, 0);
   }
 }
-constexpr int kAheadK = 3, kAheadV = 2;
+constexpr int kAheadK = 4, kAheadV = 4;
 
-// What a lane knows of its T rows, and the running state of their softmax.
+// What a lane knows of its row (a wavefront has 32 rows; lanes l and l + 32 share one), and the
+// running state of its softmax.  m is in the units of `scores` as they are left by shape(); times
+// mscale it is a power of two.
 template <class C>
-struct Rows {
-  f16x8 q[C::T][C::HD / 16];
-  int lo[C::T], hi[C::T];  // keys it sees, apart from the prefix
-  int qpos[C::T];
-  float slope[C::T];  // in units of log2
-  f32x16 o[C::T][C::HD / 32];
-  float m[C::T], l[C::T];
+struct Row {
+  f16x8 q[C::HD / 16];
+  int lo, hi;  // keys it sees, apart from the prefix
+  int pos;
+  float slope;  // in units of log2
+  const float* tab;
+  f32x16 o[C::HD / 32];  // o[d][i]: dim 32 d + 8 (i / 4) + 4 (lane / 32) + i % 4
+  float m, l;
+};
+// The scores of a tile: s[ch][i] is key 32 ch + 16 (i / 8) + 8 (lane / 32) + i % 8 of it.
+template <class C>
+struct Scores {
+  f32x16 s[C::CH];
+};
+template <class C>
+struct Weights {
+  f16x8 w[C::CH][2];
 };
 
-// One tile of keys at LDS rows ks (K, chunked by fk) and vs (V, by fv): scores, softmax,
-// output.  edge: some pair of the tile is not seen (`on`: its unmasked keys).  The tile's
-// pointers are restrict beside the stage being filled: otherwise every transposed read
-// waits for the copies in flight.
-template <class C, int FEAT>
-__device__ __forceinline__ void tile_step(const AttendParams& p, Rows<C>& r,
-                                          const lds_f16* __restrict__ ks,
-                                          const lds_f16* __restrict__ vs, const float* tab, int k0,
-                                          bool edge, uint64_t on, int prefix, float lag,
-                                          float mscale) {
-  constexpr int HD = C::HD, T = C::T, CH = C::SK / 32, NS = HD / 16, ND = HD / 32;
+// Scores of the tile at LDS rows ks (K, chunked by fk).
+template <class C>
+__device__ __forceinline__ void scores(const Row<C>& r, const lds_f16* __restrict__ ks, Scores<C>& x) {
   const int lane = threadIdx.x & 63, r32 = lane & 31, kh = lane >> 5;
-  const f16x2 ones = {(f16)1.f, (f16)1.f};
-  uint32_t see[T][CH];
-  if (edge) {
-    uint32_t some = 0;
 #pragma unroll
-    for (int t = 0; t < T; ++t)
+  for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
-      for (int ch = 0; ch < CH; ++ch) {
-        const int kb = k0 + 32 * ch;
-        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };
-        const uint32_t w = ((below(r.hi[t] - kb) & ~below(r.lo[t] - kb)) | below(prefix - kb)) &
-                           (uint32_t)(on >> (32 * ch));
-        some |= w;
-        see[t][ch] = w >> (8 * kh);
-      }
-    if (!__ballot(some != 0)) return;
-  }
-  f32x16 s[T][CH];
-#pragma unroll
-  for (int ch = 0; ch < CH; ++ch) {
-#pragma unroll
-    for (int st = 0; st < NS; ++st) {
+    for (int st = 0; st < C::HD / 16; ++st) {
       const f16x8 kf = *reinterpret_cast<const BBH_LDS f16x8*>(
-          ks + (32 * ch + r32) * HD + (((2 * st + kh) ^ Tile<HD>::fk(r32)) << 3));
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-        s[t][ch] = mfma32(kf, r.q[t][st], st == 0 ? f32x16{} : s[t][ch]);
+          ks + (32 * ch + r32) * C::HD + (((2 * st + kh) ^ Tile<C::HD>::fk(r32)) << 3));
+      x.s[ch] = mfma32(kf, r.q[st], st == 0 ? f32x16{} : x.s[ch]);
     }
-  }
-  ahead<CH * NS, 1, T, kAheadK>();
-  // s[t][ch][i]: key k0 + 32 ch + 16 (i / 8) + 8 kh + i % 8
-  if constexpr (FEAT != kPlain) {
-    if (FEAT == kCap || p.cap_l > 0.f) {
-      const float cap2 = -2.f * p.cap_l;
+}
+
+// Cap and bias.  kPlain leaves the products as they are (times c they are powers of two); kCap
+// leaves -1 / (1 + 2^(cap_k s)), which rises as tanh does and times 2 cap_l is cap * tanh but
+// for a constant, which a softmax does not see; kAny leaves powers of two.
+template <class C, int FEAT>
+__device__ __forceinline__ void shape(const AttendParams& p, const Row<C>& r, int k0, Scores<C>& x) {
+  if constexpr (FEAT == kPlain) return;
+  const int kh = (threadIdx.x & 63) >> 5;
+  if (FEAT == kCap || p.cap_l > 0.f) {
 #pragma unroll
-      for (int t = 0; t < T; ++t)
+    for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
-        for (int ch = 0; ch < CH; ++ch)
+      for (int i = 0; i < 16; ++i)
+        x.s[ch][i] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x.s[ch][i] * p.cap_k));
+    if constexpr (FEAT == kAny) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e = __builtin_amdgcn_exp2f(s[t][ch][i] * p.cap_k);
-            s[t][ch][i] = fmaf(cap2, __builtin_amdgcn_rcpf(e + 1.f), p.cap_l);
-          }
-    } else {
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int ch = 0; ch < CH; ++ch) s[t][ch] *= p.c;
+      for (int ch = 0; ch < C::CH; ++ch) x.s[ch] *= 2.f * p.cap_l;
     }
+  } else {
+#pragma unroll
+    for (int ch = 0; ch < C::CH; ++ch) x.s[ch] *= p.c;
   }
   if constexpr (FEAT == kAny) {
     if (p.slopes) {
 #pragma unroll
-      for (int t = 0; t < T; ++t)
+      for (int ch = 0; ch < C::CH; ++ch) {
+        const float df = (float)(k0 + 32 * ch + 8 * kh - r.pos);
 #pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-          const float df = (float)(k0 + 32 * ch + 8 * kh - r.qpos[t]);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            s[t][ch][i] = fmaf(-r.slope[t], fabsf(df + (float)(16 * (i >> 3) + (i & 7))), s[t][ch][i]);
-        }
+        for (int i = 0; i < 16; ++i)
+          x.s[ch][i] = fmaf(-r.slope, fabsf(df + (float)(16 * (i >> 3) + (i & 7))), x.s[ch][i]);
+      }
     }
     if (p.table) {
 #pragma unroll
-      for (int t = 0; t < T; ++t)
+      for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
-        for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int d = k0 + 32 * ch + 8 * kh - r.qpos[t] + 16 * (i >> 3) + (i & 7);
-            const float w = tab[min(max(d, -p.half), p.half)];
-            s[t][ch][i] += w == -INFINITY ? w : imax(w * 1.44269504088896f, -1e30f);
-          }
+        for (int i = 0; i < 16; ++i) {
+          const int d = k0 + 32 * ch + 8 * kh - r.pos + 16 * (i >> 3) + (i & 7);
+          const float w = r.tab[min(max(d, -p.half), p.half)];
+          x.s[ch][i] += w == -INFINITY ? w : imax(w * 1.44269504088896f, -1e30f);
+        }
     }
   }
-  if (edge) {
+}
+
+// The pairs of a tile that are seen, as bits of the lane's scores; false: none of the wavefront's.
+template <class C>
+struct Seen {
+  uint32_t bits[C::CH];
+};
+template <class C>
+__device__ __forceinline__ bool seen_of(const Row<C>& r, int k0, uint64_t on, int prefix, Seen<C>& see) {
+  const int kh = (threadIdx.x & 63) >> 5;
+  uint32_t some = 0;
 #pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-      for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          s[t][ch][i] = (see[t][ch] >> (16 * (i >> 3) + (i & 7))) & 1 ? s[t][ch][i] : -INFINITY;
+  for (int ch = 0; ch < C::CH; ++ch) {
+    const int kb = k0 + 32 * ch;
+    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };
+    const uint32_t w = ((below(r.hi - kb) & ~below(r.lo - kb)) | below(prefix - kb)) &
+                       (uint32_t)(on >> (32 * ch));
+    some |= w;
+    see.bits[ch] = w >> (8 * kh);
   }
-  bool up = false;
-  float mx[T];
+  return __ballot(some != 0) != 0;
+}
+template <class C>
+__device__ __forceinline__ void hide(const Seen<C>& see, Scores<C>& x) {
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    float v = imax(s[t][0][0], s[t][0][1]);
+  for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
-    for (int i = 2; i < 16; i += 2) v = imax(imax(v, s[t][0][i]), s[t][0][i + 1]);
+    for (int i = 0; i < 16; ++i)
+      x.s[ch][i] = (see.bits[ch] >> (16 * (i >> 3) + (i & 7))) & 1 ? x.s[ch][i] : -INFINITY;
+}
+
+// Four chains: an operation on the one before's result waits twice as long as its issue takes.
+template <class C>
+__device__ __forceinline__ float largest(const Scores<C>& x) {
+  float v[4];
 #pragma unroll
-    for (int ch = 1; ch < CH; ++ch)
+  for (int e = 0; e < 4; ++e) v[e] = imax(x.s[0][e], x.s[0][4 + e]);
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) v = imax(imax(v, s[t][ch][i]), s[t][ch][i + 1]);
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    mx[t] = imax(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-    up = up || !(mx[t] <= r.m[t] + lag);
-  }
-  if (__ballot(up)) {
+  for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      const float mn = imax(r.m[t], mx[t]);
-      const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((r.m[t] - mn) * mscale);
-      r.l[t] *= corr;
+    for (int i = ch == 0 ? 8 : 0; i < 16; i += 8)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) r.o[t][d] *= corr;
-      r.m[t] = mn;
+      for (int e = 0; e < 4; ++e) v[e] = imax(imax(v[e], x.s[ch][i + e]), x.s[ch][i + 4 + e]);
+  const float m = imax(imax(v[0], v[1]), imax(v[2], v[3]));
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  return imax(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+}
+
+// Brings the running maximum up to a tile's, where that is far enough above it (kLazy).
+template <class C>
+__device__ __forceinline__ void raise(Row<C>& r, float mx, float lag, float mscale) {
+  if (!__ballot(!(mx <= r.m + lag))) return;
+  const float mn = imax(r.m, mx);
+  const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((r.m - mn) * mscale);
+  r.l *= corr;
+#pragma unroll
+  for (int d = 0; d < C::HD / 32; ++d) r.o[d] *= corr;
+  r.m = mn;
+}
+
+// Weights 2^(mscale (s - m)), rounded to fp16 (half of a step of an output's own type, and the
+// matrix unit's operand) for the product with V; their sum is of the unrounded ones, in fp32.
+// It is added up with plain additions: a dot product of two does not run while the matrix unit is
+// busy (16 of them beside another wavefront's products 104 -> 230 cycles; additions 104 -> 129).
+template <class C>
+__device__ __forceinline__ void weigh(Row<C>& r, const Scores<C>& x, float mscale, Weights<C>& out) {
+  // a row that has seen nothing yet: every weight 2^(-inf) = 0
+  const float mc = r.m == -INFINITY ? 0.f : r.m * mscale;
+  float sum[4] = {};
+#pragma unroll
+  for (int ch = 0; ch < C::CH; ++ch)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float e = __builtin_amdgcn_exp2f(fmaf(x.s[ch][i], mscale, -mc));
+      sum[i & 3] += e;
+      out.w[ch][i >> 3][i & 7] = (f16)e;
     }
-  }
-  f16x8 pr[T][CH][2];
+  r.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// o += V^T w of the tile at LDS rows vs (V, chunked by fv): a transposed read hands a lane
+// the four keys of its dim that it supplies to the product.
+template <class C>
+__device__ __forceinline__ void context(Row<C>& r, const lds_f16* __restrict__ vs, const Weights<C>& x) {
+  constexpr int HD = C::HD;
+  const int lane = threadIdx.x & 63, kh = lane >> 5;
 #pragma unroll
-  for (int ch = 0; ch < CH; ++ch) {
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      // a row that has seen nothing yet: every weight 2^(-inf) = 0
-      const float mc = r.m[t] == -INFINITY ? 0.f : r.m[t] * mscale;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float x = FEAT == kPlain ? fmaf(s[t][ch][i], p.c, -mc) : s[t][ch][i] - mc;
-        pr[t][ch][i >> 3][i & 7] = (f16)__builtin_amdgcn_exp2f(x);
-      }
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int i = 0; i < 8; i += 2)
-          r.l[t] = __builtin_amdgcn_fdot2(f16x2{pr[t][ch][hf][i], pr[t][ch][hf][i + 1]}, ones, r.l[t], false);
-    }
+  for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
+      for (int d = 0; d < HD / 32; ++d) {
         const int row = 32 * ch + 16 * hf + 8 * kh + ((lane >> 2) & 3);
         const int c16 = (4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ Tile<HD>::fv((lane >> 2) & 3);
         const lds_f16* at = vs + row * HD + (c16 << 3) + 4 * (lane & 1);
         const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((BBH_LDS s16x4*)at);
         const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((BBH_LDS s16x4*)(at + 4 * HD));
         const f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int t = 0; t < T; ++t) r.o[t][d] = mfma32(vf, pr[t][ch][hf], r.o[t][d]);
+        r.o[d] = mfma32(vf, x.w[ch][hf], r.o[d]);
       }
-  }
-  ahead<CH * 2 * ND, 2, T, kAheadV>();
 }
 
 // One wavefront's share of a tile's copies.
@@ -298,36 +316,38 @@ struct Copies {
       voff[j] = 8 * vc < p.dim ? (uint32_t)(r * (int)p.vs.row + 8 * vc) * 2u : kNowhere;
     }
   }
-  // Keys from k0 on (`valid` of them) into a stage.  Rows behind them are zeros, and so are
-  // values whose key is masked (`bits`, where `masked`): nothing they hold reaches a sum.
-  __device__ __forceinline__ void issue(const AttendParams& p, const f16* k, const f16* v, int valid,
-                                        bool masked, uint64_t bits, lds_f16* __restrict__ stage,
-                                        int lane) {
-    const auto rk = buffer_of(k, (uint32_t)((valid - 1) * (int)p.ks.row + p.dim) * 2u);
-    const auto rv = buffer_of(v, (uint32_t)((valid - 1) * (int)p.vs.row + p.dim) * 2u);
-    lds_f16* ks = stage + cwave * C::N * 512;
-    lds_f16* vs = ks + C::SK * C::HD;
+  // `valid` keys (of K, of V) from src on into a stage; rows behind them become zeros.
+  __device__ __forceinline__ void issue_k(const AttendParams& p, const f16* src, int valid, lds_f16* stage) {
+    const auto r = buffer_of(src, (uint32_t)((valid - 1) * (int)p.ks.row + p.dim) * 2u);
 #pragma unroll
     for (int j = 0; j < C::N; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (BBH_LDS void*)(ks + j * 512), 16, (int)koff[j], 0, 0, 0);
-    if (masked) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (BBH_LDS void*)(stage + (cwave * C::N + j) * 512), 16,
+                                               (int)koff[j], 0, 0, 0);
+  }
+  __device__ __forceinline__ void issue_v(const AttendParams& p, const f16* src, int valid, lds_f16* stage) {
+    const auto r = buffer_of(src, (uint32_t)((valid - 1) * (int)p.vs.row + p.dim) * 2u);
+    lds_f16* vs = stage + C::SK * C::HD;
 #pragma unroll
-      for (int j = 0; j < C::N; ++j) {
-        const int r = ((cwave * C::N + j) * 64 + lane) / Tile<C::HD>::CPR;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (BBH_LDS void*)(vs + j * 512), 16,
-                                                 (int)((bits >> r) & 1 ? voff[j] : kNowhere), 0, 0, 0);
-      }
-    } else {
+    for (int j = 0; j < C::N; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (BBH_LDS void*)(vs + (cwave * C::N + j) * 512), 16,
+                                               (int)voff[j], 0, 0, 0);
+  }
+  // Zeros over this wavefront's part of a stage's V where the key is masked: a weight of 0 times
+  // what a masked key holds is not always 0.
+  __device__ __forceinline__ void clear_masked(lds_f16* stage, uint64_t bits, int lane) {
+    lds_f16* vs = stage + C::SK * C::HD;
 #pragma unroll
-      for (int j = 0; j < C::N; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (BBH_LDS void*)(vs + j * 512), 16, (int)voff[j], 0, 0, 0);
+    for (int j = 0; j < C::N; ++j) {
+      const int s = (cwave * C::N + j) * 64 + lane;
+      if (!((bits >> (s / Tile<C::HD>::CPR)) & 1))
+        *reinterpret_cast<BBH_LDS f16x8*>(vs + 8 * s) = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
     }
   }
 };
 
 template <class C, int FEAT>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams p) {
-  constexpr int HD = C::HD, T = C::T, SK = C::SK, NS = HD / 16, ND = HD / 32;
+  constexpr int HD = C::HD, SK = C::SK, NS = HD / 16, ND = HD / 32;
   HIP_DYNAMIC_SHARED(f16, smem);
   // (sequence, key/value head), row block and split of this workgroup
   const int rows_all = p.batch * p.kv_heads, cols = p.blocks * p.splits;
@@ -360,25 +380,22 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   // ---- the rows of this lane: row = query * group + head of the group
   const int shift = nk - nq;
   const int prefix = p.prefix ? min(max(p.prefix[b], 0), nk) : 0;
-  Rows<C> r;
-  const float* tab = nullptr;
-#pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int row = min(row0 + (rw * T + t) * 32 + r32, rows - 1);
-    const int i = row / p.group, g = row - i * p.group, h = kvh * p.group + g;
+  Row<C> r;
+  {
+    const int row = min(row0 + rw * 32 + r32, rows - 1);
+    const int i = row / p.group, h = kvh * p.group + row - i * p.group;
     const f16* src = p.q + (p.q_offsets ? (sq.q0 + i) * p.qs.row : b * p.qs.batch + i * p.qs.row) +
                      h * p.qs.head;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      r.q[t][s] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (16 * s + 8 * kh < p.dim) r.q[t][s] = *reinterpret_cast<const f16x8*>(src + 16 * s + 8 * kh);
+      r.q[s] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (16 * s + 8 * kh < p.dim) r.q[s] = *reinterpret_cast<const f16x8*>(src + 16 * s + 8 * kh);
     }
-    const int pos = i + shift;
-    r.lo[t] = p.left < 0 ? 0 : max(pos - p.left, 0);
-    r.hi[t] = p.right < 0 ? nk : min(pos + p.right + 1, nk);
-    r.qpos[t] = pos;
-    r.slope[t] = FEAT == kAny && p.slopes ? p.slopes[h] * 1.44269504088896f : 0.f;
-    if (FEAT == kAny && p.table) tab = p.table + (int64_t)h * (2 * p.half + 1) + p.half;
+    r.pos = i + shift;
+    r.lo = p.left < 0 ? 0 : max(r.pos - p.left, 0);
+    r.hi = p.right < 0 ? nk : min(r.pos + p.right + 1, nk);
+    r.slope = FEAT == kAny && p.slopes ? p.slopes[h] * 1.44269504088896f : 0.f;
+    r.tab = FEAT == kAny && p.table ? p.table + (int64_t)h * (2 * p.half + 1) + p.half : nullptr;
   }
   // ---- the tiles of this block: those of the prefix, then those of the window
   const int first_q = row0 / p.group, last_q = (min(row0 + C::BM, rows) - 1) / p.group;
@@ -406,65 +423,84 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
 
   Copies<C> copies;
   copies.init(p, wave, lane);
-  auto issue = [&](int i, uint64_t bits) {
-    const int k0 = key_at(i);
-    copies.issue(p, kbase + (int64_t)k0 * p.ks.row, vbase + (int64_t)k0 * p.vs.row, min(nk - k0, SK),
-                 mrow != nullptr, bits, ring + (i % C::R) * C::STAGE, lane);
+  BBH_LDS int* masks = (BBH_LDS int*)((BBH_LDS char*)smem + C::RING) + (C::KS == 1 ? 0 : wave * C::R * 64);
+  // Copies of the next tile, into the ring's next stage.
+  int ni = 0, nstage = 0;
+  auto next_k = [&] {
+    const int k0 = key_at(ni), valid = min(nk - k0, SK);
+    copies.issue_k(p, kbase + (int64_t)k0 * (int)p.ks.row, valid, ring + nstage * C::STAGE);
+    if (mrow && copies.cwave == C::CW - 1)  // the tile's mask beside it; zeros behind the last key
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_of(mrow, (uint32_t)nk * 4u),
+                                               (BBH_LDS void*)(masks + nstage * 64), 4,
+                                               (k0 + lane) * 4, 0, 0, 0);
   };
-  // the lane's mask value of tile i, and the tile's unmasked keys from it
-  auto load_mask = [&](int i) {
-    const int key = key_at(i) + (SK == 64 ? lane : r32);
-    return mrow && key < nk ? mrow[key] : 0;
+  auto next_v = [&] {
+    const int k0 = key_at(ni), valid = min(nk - k0, SK);
+    copies.issue_v(p, vbase + (int64_t)k0 * (int)p.vs.row, valid, ring + nstage * C::STAGE);
+    ++ni;
+    nstage = nstage == C::R - 1 ? 0 : nstage + 1;
   };
-  auto bits_of = [&](int i, int value) -> uint64_t {
-    if (mrow) return __ballot(value != 0);
-    const int n = nk - key_at(i);
-    return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
-  };
-#pragma unroll
-  for (int t = 0; t < T; ++t) {
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) r.o[t][d][i] = 0.f;
-    r.m[t] = -INFINITY;
-    r.l[t] = 0.f;
-  }
-  const float lag = FEAT == kPlain ? kLazy / p.c : kLazy;
-  const float mscale = FEAT == kPlain ? p.c : 1.f;
   constexpr uint64_t kAll = SK == 64 ? ~0ull : 0xffffffffull;
+  // Unmasked keys of a tile that is in place.
+  auto bits_of = [&](int i, int stage) -> uint64_t {
+    if (!mrow) {
+      const int n = nk - key_at(i);
+      return n >= SK ? kAll : (1ull << n) - 1;
+    }
+    const uint64_t bits = __ballot(masks[stage * 64 + lane] != 0) & kAll;
+    if (bits != kAll) copies.clear_masked(ring + stage * C::STAGE, bits, lane);
+    return bits;
+  };
+#pragma unroll
+  for (int d = 0; d < ND; ++d) r.o[d] = f32x16{};
+  r.m = -INFINITY;
+  r.l = 0.f;
+  const float mscale = FEAT == kPlain ? p.c : FEAT == kCap ? 2.f * p.cap_l : 1.f;
+  const float lag = kLazy / mscale;
+  auto whole = [&](int k0, uint64_t bits) {
+    return bits == kAll && (k0 + SK <= prefix || (k0 >= full_lo && k0 + SK <= full_hi));
+  };
 
-  uint64_t bits_now = 0, bits_next = 0;
-  int mask_next = 0;
+  Scores<C> x;
+  Weights<C> w;
+  Seen<C> see;
   if (count > 0) {
-    bits_now = bits_of(0, load_mask(0));
-    issue(0, bits_now);
-    if (count > 1) mask_next = load_mask(1);
+    next_k();
+    next_v();
   }
+  wait_vm<0>();  // the queries too: their first use is inside the loop
+  int now = 0;   // stage of tile it
   for (int it = 0; it < count; ++it) {
     wait_vm<0>();
     if constexpr (C::KS == 1) lds_barrier();
     else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (it + 1 < count) {
-      bits_next = bits_of(it + 1, mask_next);
-      issue(it + 1, bits_next);
-      if (mrow && it + 2 < count) mask_next = load_mask(it + 2);
+      next_k();
+      next_v();
     }
-    const uint64_t bits = bits_now & kAll;
-    bits_now = bits_next;
     const int k0 = key_at(it);
-    const lds_f16* ks = ring + (it % C::R) * C::STAGE;
-    const bool edge = bits != kAll || !(k0 + SK <= prefix || (k0 >= full_lo && k0 + SK <= full_hi));
-    if (bits)
-      tile_step<C, FEAT>(p, r, ks, ks + SK * HD, tab, k0, edge, bits, prefix, lag, mscale);
+    const uint64_t bits = bits_of(it, now);
+    if (mrow && bits != kAll) {  // all of V is cleared before any of it is read
+      if constexpr (C::KS == 1) lds_barrier();
+      else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    const lds_f16* ks = ring + now * C::STAGE;
+    now = now == C::R - 1 ? 0 : now + 1;
+    const bool edge = !whole(k0, bits);
+    if (!bits || (edge && !seen_of(r, k0, bits, prefix, see))) continue;
+    scores(r, ks, x);
+    ahead<C::CH * NS, 1, kAheadK>();
+    shape<C, FEAT>(p, r, k0, x);
+    if (edge) hide(see, x);
+    raise(r, largest(x), lag, mscale);
+    weigh(r, x, mscale, w);
+    context(r, ks + SK * HD, w);
+    ahead<C::CH * 2 * ND, 2, kAheadV>();
   }
-  f32x16 (&o)[T][ND] = r.o;
-  float (&m)[T] = r.m;
-  float (&l)[T] = r.l;
-#pragma unroll
-  for (int t = 0; t < T; ++t) l[t] = xor32_sum(l[t]);
+  f32x16 (&o)[ND] = r.o;
+  const float m = r.m, l = xor32_sum(r.l);
 
-  // ---- out.  o[t][d][i]: row lane%32, dim 32 d + 8 (i/4) + 4 kh + i%4
+  // ---- out
   const int cpr = p.dim / 8;
   auto out_at = [&](int row) {
     const int i = row / p.group, g = row - i * p.group;
@@ -477,92 +513,78 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   __syncthreads();  // the rings are free
   if constexpr (C::KS == 1) {
     if (p.splits > 1) {
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const int row = row0 + (rw * T + t) * 32 + r32;
-        if (row >= rows) continue;
-        const int64_t sl = slot_of(row);
-        if (kh == 0) p.part_ml[sl] = make_float2(m[t] * mscale, l[t]);
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<f32x4*>(p.part_o + sl * HD + 32 * d + 8 * j + 4 * kh) =
-                f32x4{o[t][d][4 * j], o[t][d][4 * j + 1], o[t][d][4 * j + 2], o[t][d][4 * j + 3]};
-      }
-      return;
-    }
-    f16* st = smem + wave * 32 * (HD + 8);
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      const float inv = l[t] != 0.f ? 1.f / l[t] : 0.f;
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f16x4 w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = (f16)(o[t][d][4 * j + e] * inv);
-          *reinterpret_cast<f16x4*>(st + r32 * (HD + 8) + 32 * d + 8 * j + 4 * kh) = w;
-        }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      for (int x = lane; x < 32 * Tile<HD>::CPR; x += 64) {
-        const int r = x / Tile<HD>::CPR, cc = x % Tile<HD>::CPR;
-        const int row = row0 + (rw * T + t) * 32 + r;
-        const f16x8 w = *reinterpret_cast<const f16x8*>(st + r * (HD + 8) + 8 * cc);
-        if (row < rows && cc < cpr) *reinterpret_cast<f16x8*>(out_at(row) + 8 * cc) = w;
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-  } else {
-    float* area = reinterpret_cast<float*>(smem);  // [KS][32][HD + 4]
-    float2* ml = reinterpret_cast<float2*>(area + C::KS * 32 * (HD + 4));
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      if (t > 0) __syncthreads();
-      if (kh == 0) ml[wave * 32 + r32] = make_float2(m[t] * mscale, l[t]);
-      __syncthreads();
-      float top = -INFINITY, mine = m[t] * mscale;
-#pragma unroll
-      for (int w = 0; w < C::KS; ++w) top = imax(top, ml[w * 32 + r32].x);
-      const float f = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - top);
+      const int row = row0 + rw * 32 + r32;
+      if (row >= rows) return;
+      const int64_t sl = slot_of(row);
+      if (kh == 0) p.part_ml[sl] = make_float2(m * mscale, l);
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<f32x4*>(area + (wave * 32 + r32) * (HD + 4) + 32 * d + 8 * j + 4 * kh) =
-              f32x4{o[t][d][4 * j] * f, o[t][d][4 * j + 1] * f, o[t][d][4 * j + 2] * f,
-                    o[t][d][4 * j + 3] * f};
-      __syncthreads();
-      for (int x = tid; x < 32 * (HD / 8); x += C::THREADS) {
-        const int r = x / (HD / 8), cc = x % (HD / 8);
-        const int row = row0 + t * 32 + r;
-        if (row >= rows || cc >= cpr) continue;
-        float tp = -INFINITY, sum = 0.f;
+          *reinterpret_cast<f32x4*>(p.part_o + sl * HD + 32 * d + 8 * j + 4 * kh) =
+              f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+      return;
+    }
+    f16* st = smem + wave * 32 * (HD + 8);
+    const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
-        for (int w = 0; w < C::KS; ++w) tp = imax(tp, ml[w * 32 + r].x);
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int w = 0; w < C::KS; ++w) {
-          const float2 a = ml[w * 32 + r];
-          sum += a.x == -INFINITY ? 0.f : a.y * __builtin_amdgcn_exp2f(a.x - tp);
-        }
-        float v[8] = {};
+      for (int j = 0; j < 4; ++j) {
+        f16x4 w;
 #pragma unroll
-        for (int w = 0; w < C::KS; ++w)
+        for (int e = 0; e < 4; ++e) w[e] = (f16)(o[d][4 * j + e] * inv);
+        *reinterpret_cast<f16x4*>(st + r32 * (HD + 8) + 32 * d + 8 * j + 4 * kh) = w;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    for (int x = lane; x < 32 * Tile<HD>::CPR; x += 64) {
+      const int rr = x / Tile<HD>::CPR, cc = x % Tile<HD>::CPR, row = row0 + rw * 32 + rr;
+      const f16x8 w = *reinterpret_cast<const f16x8*>(st + rr * (HD + 8) + 8 * cc);
+      if (row < rows && cc < cpr) *reinterpret_cast<f16x8*>(out_at(row) + 8 * cc) = w;
+    }
+  } else {
+    float* area = reinterpret_cast<float*>(smem);  // [KS][32][HD + 4]
+    float2* ml = reinterpret_cast<float2*>(area + C::KS * 32 * (HD + 4));
+    if (kh == 0) ml[wave * 32 + r32] = make_float2(m * mscale, l);
+    __syncthreads();
+    float top = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += area[(w * 32 + r) * (HD + 4) + 8 * cc + e];
-        if (p.splits > 1) {
-          const int64_t sl = slot_of(row);
-          if (cc == 0) p.part_ml[sl] = make_float2(tp, sum);
-          *reinterpret_cast<f32x4*>(p.part_o + sl * HD + 8 * cc) = f32x4{v[0], v[1], v[2], v[3]};
-          *reinterpret_cast<f32x4*>(p.part_o + sl * HD + 8 * cc + 4) = f32x4{v[4], v[5], v[6], v[7]};
-        } else {
-          const float inv = sum != 0.f ? 1.f / sum : 0.f;
-          f16x8 w;
+    for (int w = 0; w < C::KS; ++w) top = imax(top, ml[w * 32 + r32].x);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * mscale - top);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = (f16)(v[e] * inv);
-          *reinterpret_cast<f16x8*>(out_at(row) + 8 * cc) = w;
-        }
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(area + (wave * 32 + r32) * (HD + 4) + 32 * d + 8 * j + 4 * kh) =
+            f32x4{o[d][4 * j] * f, o[d][4 * j + 1] * f, o[d][4 * j + 2] * f, o[d][4 * j + 3] * f};
+    __syncthreads();
+    for (int x = tid; x < 32 * (HD / 8); x += C::THREADS) {
+      const int rr = x / (HD / 8), cc = x % (HD / 8), row = row0 + rr;
+      if (row >= rows || cc >= cpr) continue;
+      float tp = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < C::KS; ++w) tp = imax(tp, ml[w * 32 + rr].x);
+#pragma unroll
+      for (int w = 0; w < C::KS; ++w) {
+        const float2 a = ml[w * 32 + rr];
+        sum += a.x == -INFINITY ? 0.f : a.y * __builtin_amdgcn_exp2f(a.x - tp);
+      }
+      float v[8] = {};
+#pragma unroll
+      for (int w = 0; w < C::KS; ++w)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += area[(w * 32 + rr) * (HD + 4) + 8 * cc + e];
+      if (p.splits > 1) {
+        const int64_t sl = slot_of(row);
+        if (cc == 0) p.part_ml[sl] = make_float2(tp, sum);
+        *reinterpret_cast<f32x4*>(p.part_o + sl * HD + 8 * cc) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(p.part_o + sl * HD + 8 * cc + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      } else {
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        f16x8 w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = (f16)(v[e] * inv);
+        *reinterpret_cast<f16x8*>(out_at(row) + 8 * cc) = w;
       }
     }
   }
@@ -702,17 +724,17 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
   return hipSuccess;
 }
 
-//                HD  NW T KS SK R OCC
-using P32 = Cfg<32, 4, 1, 1, 64, 2, 4>;
-using P64 = Cfg<64, 8, 1, 1, 64, 2, 3>;
-using P96 = Cfg<96, 4, 1, 1, 64, 2, 2>;
-using P128 = Cfg<128, 8, 1, 1, 64, 2, 2>;
-using P256 = Cfg<256, 4, 1, 1, 32, 2, 1>;
-using K32 = Cfg<32, 4, 1, 4, 32, 2, 2>;
-using K64 = Cfg<64, 4, 1, 4, 32, 2, 2>;
-using K96 = Cfg<96, 4, 1, 4, 32, 2, 1>;
-using K128 = Cfg<128, 4, 1, 4, 32, 2, 1>;
-using K256 = Cfg<256, 2, 1, 2, 32, 2, 1>;
+//               HD  NW KS SK R OCC
+using P32 = Cfg<32, 4, 1, 64, 2, 4>;
+using P64 = Cfg<64, 4, 1, 64, 2, 3>;
+using P96 = Cfg<96, 4, 1, 64, 2, 2>;
+using P128 = Cfg<128, 8, 1, 64, 2, 2>;
+using P256 = Cfg<256, 4, 1, 32, 2, 1>;
+using K32 = Cfg<32, 4, 4, 32, 2, 2>;
+using K64 = Cfg<64, 4, 4, 32, 2, 2>;
+using K96 = Cfg<96, 4, 4, 32, 2, 1>;
+using K128 = Cfg<128, 4, 4, 32, 2, 1>;
+using K256 = Cfg<256, 2, 2, 32, 2, 1>;
 
 template <class F>
 auto with_config(const AttendParams& p, F&& f) {
