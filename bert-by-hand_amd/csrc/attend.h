@@ -24,7 +24,9 @@ struct AttendParams {
   int b0;  // first sequence of a launch
   int batch, q_len, k_len, heads, kv_heads, dim, group;
   int left, right, half;
-  float c;      // scale * log2(e): scores in units of log2
+  float c;           // scale * log2(e)
+  float bias_scale;  // log2(e) / (c, or 2 * cap_l under a cap): biases in the units of the scores
+  bool table_lds;    // the table fits beside the tiles
   float cap_k;  // 2 * log2(e) * scale / cap
   float cap_l;  // cap * log2(e); 0: no cap
   int blocks, splits, chunk;  // row blocks; splits of a block's key tiles, `chunk` tiles each

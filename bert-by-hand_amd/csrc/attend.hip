@@ -11,10 +11,11 @@
 namespace bbh {
 namespace {
 
+#define BBH_LDS __attribute__((address_space(3)))
+typedef BBH_LDS f16 lds_f16;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-enum Feat { kPlain = 0, kCap = 1, kAny = 2 };
+enum Feat { kPlain = 0, kCap = 1, kAny = 2 };  // a softmax of the products, of capped ones, any bias
 
 // Key (within a 32-key chunk) held by row r of the K tile.
 __device__ __forceinline__ int key_of_row(int r) {
@@ -96,9 +97,6 @@ struct IeeeMax {
   __device__ __forceinline__ float operator()(float a, float b) const { return imax(a, b); }
 };
 
-#define BBH_LDS __attribute__((address_space(3)))
-typedef BBH_LDS f16 lds_f16;
-
 // Scheduling of STEPS steps, each of READS LDS reads and a product of what they read: the reads
 // run A steps ahead of the products, no further (left alone the compiler reads the whole tile
 // first, into more registers than there are).  VALU and TRANS other operations of the block go
@@ -118,18 +116,25 @@ __device__ __forceinline__ void ahead() {
 constexpr int kAheadK = 4, kAheadV = 4;
 
 // What a lane knows of its row (a wavefront has 32 rows; lanes l and l + 32 share one), and the
-// running state of its softmax.  m is in the units of `scores` as they are left by shape(); times
-// mscale it is a power of two.
+// running state of its softmax.  m is in the units that shape() leaves the scores in; times mscale
+// they are powers of two.
 template <class C>
 struct Row {
   f16x8 q[C::HD / 16];
   int lo, hi;  // keys it sees, apart from the prefix
   int pos;
-  float slope;  // in units of log2
-  const float* tab;
+  int first, last;  // of the wavefront's rows: least and largest position
+  float slope;
+  const float* tab;          // distance 0 of the head's table,
+  const BBH_LDS float* ltab;  // in LDS where it is there
+  float below, above;        // its ends
   f32x16 o[C::HD / 32];  // o[d][i]: dim 32 d + 8 (i / 4) + 4 (lane / 32) + i % 4
   float m, l;
 };
+// A bias in the units of the scores.  Finite ones stay finite.
+__device__ __forceinline__ float bias_units(const AttendParams& p, float w) {
+  return w == -INFINITY ? w : imax(w * p.bias_scale, -1e38f);
+}
 // The scores of a tile: s[ch][i] is key 32 ch + 16 (i / 8) + 8 (lane / 32) + i % 8 of it.
 template <class C>
 struct Scores {
@@ -154,9 +159,15 @@ __device__ __forceinline__ void scores(const Row<C>& r, const lds_f16* __restric
     }
 }
 
-// Cap and bias.  kPlain leaves the products as they are (times c they are powers of two); kCap
-// leaves -1 / (1 + 2^(cap_k s)), which rises as tanh does and times 2 cap_l is cap * tanh but
-// for a constant, which a softmax does not see; kAny leaves powers of two.
+// Cap and bias.  The products s of q and k become -1 / (1 + 2^(cap_k s)) under a cap, which rises
+// as tanh does and times 2 cap_l is cap * tanh but for a constant, which a softmax does not see.
+// Biases arrive in the units of either (divided by mscale), so that nothing is scaled here.
+//
+// The table of a head lies in LDS with its ends repeated kPad times, so that the distances of a
+// chunk (32 keys from at most 32 neighbouring queries: 62 apart at most) are either all past one
+// end, where the bias is a constant, or all inside the padded table, where a lane reads eight
+// neighbouring values with no clamping.  Tables too long for that are read from memory.
+constexpr int kPad = 64;
 template <class C, int FEAT>
 __device__ __forceinline__ void shape(const AttendParams& p, const Row<C>& r, int k0, Scores<C>& x) {
   if constexpr (FEAT == kPlain) return;
@@ -167,13 +178,6 @@ __device__ __forceinline__ void shape(const AttendParams& p, const Row<C>& r, in
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         x.s[ch][i] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x.s[ch][i] * p.cap_k));
-    if constexpr (FEAT == kAny) {
-#pragma unroll
-      for (int ch = 0; ch < C::CH; ++ch) x.s[ch] *= 2.f * p.cap_l;
-    }
-  } else {
-#pragma unroll
-    for (int ch = 0; ch < C::CH; ++ch) x.s[ch] *= p.c;
   }
   if constexpr (FEAT == kAny) {
     if (p.slopes) {
@@ -187,13 +191,24 @@ __device__ __forceinline__ void shape(const AttendParams& p, const Row<C>& r, in
     }
     if (p.table) {
 #pragma unroll
-      for (int ch = 0; ch < C::CH; ++ch)
+      for (int ch = 0; ch < C::CH; ++ch) {
+        const int kb = k0 + 32 * ch;
+        if (kb + 31 - r.first <= -p.half || kb - r.last >= p.half) {
+          const float w = kb < r.last ? r.below : r.above;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int d = k0 + 32 * ch + 8 * kh - r.pos + 16 * (i >> 3) + (i & 7);
-          const float w = r.tab[min(max(d, -p.half), p.half)];
-          x.s[ch][i] += w == -INFINITY ? w : imax(w * 1.44269504088896f, -1e30f);
+          for (int i = 0; i < 16; ++i) x.s[ch][i] += w;
+        } else if (r.ltab) {
+          const BBH_LDS float* t = r.ltab + (kb + 8 * kh - r.pos);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x.s[ch][i] += t[16 * (i >> 3) + (i & 7)];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int d = kb + 8 * kh - r.pos + 16 * (i >> 3) + (i & 7);
+            x.s[ch][i] += bias_units(p, r.tab[min(max(d, -p.half), p.half)]);
+          }
         }
+      }
     }
   }
 }
@@ -316,21 +331,20 @@ struct Copies {
       voff[j] = 8 * vc < p.dim ? (uint32_t)(r * (int)p.vs.row + 8 * vc) * 2u : kNowhere;
     }
   }
-  // `valid` keys (of K, of V) from src on into a stage; rows behind them become zeros.
-  __device__ __forceinline__ void issue_k(const AttendParams& p, const f16* src, int valid, lds_f16* stage) {
-    const auto r = buffer_of(src, (uint32_t)((valid - 1) * (int)p.ks.row + p.dim) * 2u);
+  // `valid` keys from k and v on into a stage; rows behind them become zeros.
+  __device__ __forceinline__ void issue(const AttendParams& p, const f16* k, const f16* v, int valid,
+                                        lds_f16* stage) {
+    const bool any = valid > 0;
+    const auto rk = buffer_of(k, any ? (uint32_t)((valid - 1) * (int)p.ks.row + p.dim) * 2u : 0u);
+    const auto rv = buffer_of(v, any ? (uint32_t)((valid - 1) * (int)p.vs.row + p.dim) * 2u : 0u);
+    lds_f16* ks = stage + cwave * C::N * 512;
+    lds_f16* vs = ks + C::SK * C::HD;
 #pragma unroll
     for (int j = 0; j < C::N; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (BBH_LDS void*)(stage + (cwave * C::N + j) * 512), 16,
-                                               (int)koff[j], 0, 0, 0);
-  }
-  __device__ __forceinline__ void issue_v(const AttendParams& p, const f16* src, int valid, lds_f16* stage) {
-    const auto r = buffer_of(src, (uint32_t)((valid - 1) * (int)p.vs.row + p.dim) * 2u);
-    lds_f16* vs = stage + C::SK * C::HD;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (BBH_LDS void*)(ks + j * 512), 16, (int)koff[j], 0, 0, 0);
 #pragma unroll
     for (int j = 0; j < C::N; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (BBH_LDS void*)(vs + (cwave * C::N + j) * 512), 16,
-                                               (int)voff[j], 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (BBH_LDS void*)(vs + j * 512), 16, (int)voff[j], 0, 0, 0);
   }
   // Zeros over this wavefront's part of a stage's V where the key is masked: a weight of 0 times
   // what a masked key holds is not always 0.
@@ -394,8 +408,29 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
     r.pos = i + shift;
     r.lo = p.left < 0 ? 0 : max(r.pos - p.left, 0);
     r.hi = p.right < 0 ? nk : min(r.pos + p.right + 1, nk);
-    r.slope = FEAT == kAny && p.slopes ? p.slopes[h] * 1.44269504088896f : 0.f;
-    r.tab = FEAT == kAny && p.table ? p.table + (int64_t)h * (2 * p.half + 1) + p.half : nullptr;
+    if constexpr (FEAT == kAny) {
+      const int w0 = row0 + rw * 32;
+      r.first = min(w0, rows - 1) / p.group + shift;
+      r.last = min(w0 + 31, rows - 1) / p.group + shift;
+      r.slope = p.slopes ? p.slopes[h] * p.bias_scale : 0.f;
+      r.ltab = nullptr;
+      if (p.table) {
+        r.tab = p.table + (int64_t)h * (2 * p.half + 1) + p.half;
+        r.below = bias_units(p, r.tab[-p.half]);
+        r.above = bias_units(p, r.tab[p.half]);
+        if (p.table_lds) {
+          const int len = 2 * p.half + 1 + 2 * kPad;
+          BBH_LDS float* t = (BBH_LDS float*)((BBH_LDS char*)smem + C::LDS);
+          for (int e = tid; e < p.group * len; e += C::THREADS) {
+            const int g = e / len, d = e - g * len - kPad;
+            t[e] = bias_units(p, p.table[(int64_t)(kvh * p.group + g) * (2 * p.half + 1) +
+                                         min(max(d, 0), 2 * p.half)]);
+          }
+          __syncthreads();
+          r.ltab = t + (h - kvh * p.group) * len + kPad + p.half;
+        }
+      }
+    }
   }
   // ---- the tiles of this block: those of the prefix, then those of the window
   const int first_q = row0 / p.group, last_q = (min(row0 + C::BM, rows) - 1) / p.group;
@@ -426,17 +461,14 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   BBH_LDS int* masks = (BBH_LDS int*)((BBH_LDS char*)smem + C::RING) + (C::KS == 1 ? 0 : wave * C::R * 64);
   // Copies of the next tile, into the ring's next stage.
   int ni = 0, nstage = 0;
-  auto next_k = [&] {
-    const int k0 = key_at(ni), valid = min(nk - k0, SK);
-    copies.issue_k(p, kbase + (int64_t)k0 * (int)p.ks.row, valid, ring + nstage * C::STAGE);
+  auto next = [&] {
+    const int k0 = key_at(ni), valid = ni < count ? min(nk - k0, SK) : 0;
+    copies.issue(p, kbase + (int64_t)k0 * (int)p.ks.row, vbase + (int64_t)k0 * (int)p.vs.row, valid,
+                 ring + nstage * C::STAGE);
     if (mrow && copies.cwave == C::CW - 1)  // the tile's mask beside it; zeros behind the last key
       __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_of(mrow, (uint32_t)nk * 4u),
                                                (BBH_LDS void*)(masks + nstage * 64), 4,
-                                               (k0 + lane) * 4, 0, 0, 0);
-  };
-  auto next_v = [&] {
-    const int k0 = key_at(ni), valid = min(nk - k0, SK);
-    copies.issue_v(p, vbase + (int64_t)k0 * (int)p.vs.row, valid, ring + nstage * C::STAGE);
+                                               ni < count ? (k0 + lane) * 4 : (int)Copies<C>::kNowhere, 0, 0, 0);
     ++ni;
     nstage = nstage == C::R - 1 ? 0 : nstage + 1;
   };
@@ -455,7 +487,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   for (int d = 0; d < ND; ++d) r.o[d] = f32x16{};
   r.m = -INFINITY;
   r.l = 0.f;
-  const float mscale = FEAT == kPlain ? p.c : FEAT == kCap ? 2.f * p.cap_l : 1.f;
+  const float mscale = FEAT == kPlain ? p.c : FEAT == kCap || p.cap_l > 0.f ? 2.f * p.cap_l : p.c;
   const float lag = kLazy / mscale;
   auto whole = [&](int k0, uint64_t bits) {
     return bits == kAll && (k0 + SK <= prefix || (k0 >= full_lo && k0 + SK <= full_hi));
@@ -464,19 +496,22 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   Scores<C> x;
   Weights<C> w;
   Seen<C> see;
-  if (count > 0) {
-    next_k();
-    next_v();
-  }
-  wait_vm<0>();  // the queries too: their first use is inside the loop
-  int now = 0;   // stage of tile it
+  // R - 1 tiles on their way (past the last one: of nothing, so that their number is known).
+  constexpr int kTile = 2 * C::N;  // copies of a tile (a wavefront that copies masks has one more,
+                                   // and waits for more than it has to)
+  wait_vm<0>();  // the queries: their first use is inside the loop
+  for (int i = 0; i < C::R - 1; ++i) next();
+  int now = 0;  // stage of tile it
   for (int it = 0; it < count; ++it) {
-    wait_vm<0>();
-    if constexpr (C::KS == 1) lds_barrier();
-    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (it + 1 < count) {
-      next_k();
-      next_v();
+    if constexpr (C::KS == 1) {
+      wait_vm<(C::R - 2) * kTile>();
+      lds_barrier();
+      next();
+    } else {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last tile of that stage has been read
+      next();
+      wait_vm<(C::R - 1) * kTile>();
+      asm volatile("" ::: "memory");
     }
     const int k0 = key_at(it);
     const uint64_t bits = bits_of(it, now);
@@ -510,6 +545,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   auto slot_of = [&](int row) {
     return (((int64_t)item * p.q_len * p.group) + row) * p.splits + split;
   };
+  wait_vm<0>();
   __syncthreads();  // the rings are free
   if constexpr (C::KS == 1) {
     if (p.splits > 1) {
@@ -657,13 +693,19 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
   *reinterpret_cast<f16x8*>(dst) = o;
 }
 
+// LDS of the padded tables of a group's heads.
+int64_t table_bytes(const AttendParams& p) {
+  return (int64_t)p.group * (2 * (int64_t)p.half + 1 + 2 * kPad) * 4;
+}
+
 template <class C, int FEAT>
 hipError_t launch_as(const AttendParams& p, int64_t grid, hipStream_t s) {
   static const hipError_t attr =
       hipFuncSetAttribute(reinterpret_cast<const void*>(attend_kernel<C, FEAT>),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)C::LDS);
+                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLdsMax);
   if (attr != hipSuccess) return attr;
-  hipLaunchKernelGGL((attend_kernel<C, FEAT>), dim3((unsigned)grid), dim3(C::THREADS), C::LDS, s, p);
+  const size_t lds = C::LDS + (FEAT == kAny && p.table_lds ? table_bytes(p) : 0);
+  hipLaunchKernelGGL((attend_kernel<C, FEAT>), dim3((unsigned)grid), dim3(C::THREADS), lds, s, p);
   return hipGetLastError();
 }
 
@@ -675,6 +717,9 @@ int64_t longest(const AttendParams& p) {
   return std::min<int64_t>(p.k_len, (int64_t)p.left + p.q_len + (p.right < 0 ? p.k_len : p.right));
 }
 
+// Row blocks, and how a block's keys are split over workgroups: enough of those that they all
+// end at about the same time, none with less than 512 keys.  (64 tokens over caches of up to 8192
+// keys, workgroups of one wavefront: 8192 workgroups 195 us, 1024 221; of 1024 keys each 208.)
 template <class C>
 void plan(AttendParams& p, size_t scratch_bytes) {
   const int64_t rows = (int64_t)p.q_len * p.group, items = (int64_t)p.batch * p.kv_heads;
@@ -682,10 +727,9 @@ void plan(AttendParams& p, size_t scratch_bytes) {
   const int64_t tiles = (longest(p) + C::SK - 1) / C::SK + 2;
   p.splits = 1;
   p.chunk = INT_MAX / 2;
-  const int64_t groups = items * p.blocks;
-  if (groups >= 1024) return;
-  const int64_t least = 512 / C::SK;  // keys of a split
-  int64_t want = std::min<int64_t>(tiles / least, (1024 + groups - 1) / groups);
+  const int64_t groups = items * p.blocks, target = C::NW == 1 ? 8192 : 1024;
+  if (groups >= target) return;
+  int64_t want = std::min<int64_t>(tiles / (512 / C::SK), (target + groups - 1) / groups);
   const int64_t a_split = items * rows * (C::HD * 4 + 8);
   want = std::min<int64_t>(std::min<int64_t>(want, kMaxSplits), (int64_t)(scratch_bytes / a_split));
   if (want < 2) return;
@@ -700,6 +744,7 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
   const int64_t slots = (int64_t)p.batch * p.kv_heads * p.q_len * p.group;
   p.part_o = static_cast<float*>(scratch);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * p.splits * C::HD);
+  p.table_lds = p.table && table_bytes(p) <= std::min<int64_t>(16384, (int64_t)kLdsMax - (int64_t)C::LDS);
   const int feat = p.slopes || p.table ? kAny : p.cap_l > 0.f ? kCap : kPlain;
   // sequences a launch: its work-items are counted in 32 bits
   const int64_t per = cols * p.kv_heads * C::THREADS;
@@ -726,34 +771,55 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
 
 //               HD  NW KS SK R OCC
 using P32 = Cfg<32, 4, 1, 64, 2, 4>;
-using P64 = Cfg<64, 4, 1, 64, 2, 3>;
+using P64 = Cfg<64, 4, 1, 32, 2, 3>;
 using P96 = Cfg<96, 4, 1, 64, 2, 2>;
 using P128 = Cfg<128, 8, 1, 64, 2, 2>;
 using P256 = Cfg<256, 4, 1, 32, 2, 1>;
+using S32 = Cfg<32, 2, 1, 32, 2, 4>;
+using S64 = Cfg<64, 2, 1, 32, 2, 3>;
+using S96 = Cfg<96, 2, 1, 32, 2, 2>;
+using S128 = Cfg<128, 2, 1, 32, 2, 2>;
+using S256 = Cfg<256, 2, 1, 32, 2, 1>;
 using K32 = Cfg<32, 4, 4, 32, 2, 2>;
 using K64 = Cfg<64, 4, 4, 32, 2, 2>;
 using K96 = Cfg<96, 4, 4, 32, 2, 1>;
 using K128 = Cfg<128, 4, 4, 32, 2, 1>;
 using K256 = Cfg<256, 2, 2, 32, 2, 1>;
+using L32 = Cfg<32, 1, 1, 32, 2, 4>;
+using L64 = Cfg<64, 1, 1, 32, 2, 3>;
+using L96 = Cfg<96, 1, 1, 32, 2, 2>;
+using L128 = Cfg<128, 1, 1, 32, 2, 2>;
+using L256 = Cfg<256, 1, 1, 32, 2, 1>;
 
 template <class F>
-auto with_config(const AttendParams& p, F&& f) {
-  const bool few = (int64_t)p.q_len * p.group <= 32;
-  if (p.dim <= 32) return few ? f(K32{}) : f(P32{});
-  if (p.dim <= 64) return few ? f(K64{}) : f(P64{});
-  if (p.dim <= 96) return few ? f(K96{}) : f(P96{});
-  if (p.dim <= 128) return few ? f(K128{}) : f(P128{});
-  return few ? f(K256{}) : f(P256{});
+auto with_config(const AttendParams& p, bool scratch, F&& f) {
+  const int64_t rows = (int64_t)p.q_len * p.group, keys = longest(p);
+  const int64_t mean = p.q_offsets ? p.q_rows * p.group / p.batch : rows;
+#define BBH_BY_SIZE(SET)                \
+  do {                                  \
+    if (p.dim <= 32) return f(SET##32{});   \
+    if (p.dim <= 64) return f(SET##64{});   \
+    if (p.dim <= 96) return f(SET##96{});   \
+    if (p.dim <= 128) return f(SET##128{}); \
+    return f(SET##256{});               \
+  } while (0)
+  if (rows <= 32 && keys > 128) {
+    if (scratch && (int64_t)p.batch * p.kv_heads * keys >= 1 << 18) BBH_BY_SIZE(L);
+    BBH_BY_SIZE(K);
+  }
+  if (mean <= 64) BBH_BY_SIZE(S);
+  BBH_BY_SIZE(P);
+#undef BBH_BY_SIZE
 }
 
 }  // namespace
 
 hipError_t attend(AttendParams p, void* scratch, size_t scratch_bytes, hipStream_t s) {
-  return with_config(p, [&](auto c) { return launch<decltype(c)>(p, scratch, scratch_bytes, s); });
+  return with_config(p, scratch != nullptr, [&](auto c) { return launch<decltype(c)>(p, scratch, scratch_bytes, s); });
 }
 
 size_t attend_scratch(const AttendParams& p) {
-  return with_config(p, [&](auto c) -> size_t {
+  return with_config(p, true, [&](auto c) -> size_t {
     AttendParams a = p;
     plan<decltype(c)>(a, SIZE_MAX / 2);
     if (a.splits < 2) return 0;

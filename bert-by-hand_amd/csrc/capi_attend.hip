@@ -275,8 +275,12 @@ static bbh_status attend_params(const bbh_attend_args* a, bbh::AttendParams& p) 
     return fail(BBH_ERR_UNSUPPORTED, what, "k_len or q_len * heads / kv_heads above 2^28");
   if ((int64_t)a->batch * a->heads > INT_MAX)
     return fail(BBH_ERR_UNSUPPORTED, what, "batch * heads above 2^31 - 1");
-  if (!(a->scale > 0.f) || !isfinite(a->scale)) return invalid(what, "scale must be finite and positive");
-  if (!(a->cap >= 0.f) || !isfinite(a->cap)) return invalid(what, "cap must be finite and not negative");
+  // (so that biases divided by either keep their size)
+  constexpr float kLeast = 0x1p-24f, kMost = 0x1p24f;
+  if (!(a->scale >= kLeast && a->scale <= kMost))
+    return invalid(what, "scale must lie between 2^-24 and 2^24");
+  if (!(a->cap == 0.f || (a->cap >= kLeast && a->cap <= kMost)))
+    return invalid(what, "cap must be 0 or lie between 2^-24 and 2^24");
   if (a->table && (a->table_half < 0 || a->table_half > kMaxLen))
     return invalid(what, "table_half out of range");
   if ((a->q_offsets && a->q_rows < 0) || (a->k_offsets && a->k_rows < 0))
@@ -315,6 +319,7 @@ static bbh_status attend_params(const bbh_attend_args* a, bbh::AttendParams& p) 
   p.c = (float)(a->scale * log2e);
   p.cap_k = a->cap > 0.f ? (float)(2 * log2e * a->scale / a->cap) : 0.f;
   p.cap_l = (float)(a->cap * log2e);
+  p.bias_scale = (float)(a->cap > 0.f ? 0.5 / a->cap : 1.0 / a->scale);
   return BBH_OK;
 }
 

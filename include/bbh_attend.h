@@ -124,7 +124,8 @@ bbh_status bbh_rope_heads(const bbh_rope *rope, const bbh_rope_args *args, bbh_s
  * must be finite (its weight here is 0, and 0 times infinity is not).
  *
  * Scores, softmax and sums are fp32; the weights are rounded to fp16 for the product
- * with v, the output once.  table entries are finite (below -6.9e29 they count as that) or
+ * with v, the output once.  table entries are of magnitude up to
+ * 1e30, lower ones count as some such value, or
  * -infinity (the pair is not seen).  Offsets, lengths, prefix, mask: int32, on the
  * device; slopes and table: fp32.  head_dim is a multiple of 8 up to
  * BBH_ATTEND_MAX_DIM; addresses of q, k, v and out are multiples of 16 bytes, their
@@ -150,7 +151,7 @@ typedef struct bbh_attend_args {
   int batch, q_len, k_len; /* of the longest sequence */
   int heads, kv_heads, head_dim;
   int left, right, table_half;
-  float scale, cap; /* scale > 0; cap 0: none */
+  float scale, cap; /* between 2^-24 and 2^24; cap 0: none */
 } bbh_attend_args;
 bbh_status bbh_attend(const bbh_attend_args *args, bbh_stream_t stream);
 /* Bytes of scratch for these sizes (pointers of args are not read, but those that are
