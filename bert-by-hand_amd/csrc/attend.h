@@ -12,6 +12,10 @@ struct Heads {
   int64_t batch, row, head;
 };
 
+struct Divisor {
+  uint32_t hi, lo;  // ceil(2^64 / d); 0: d is 1
+};
+
 struct AttendParams {
   const f16 *q, *k, *v;
   f16* out;
@@ -23,6 +27,8 @@ struct AttendParams {
   int64_t q_rows, k_rows;
   int b0;  // first sequence of a launch
   int batch, q_len, k_len, heads, kv_heads, dim, group;
+  Divisor by_cols, by_splits, by_kv;  // blocks * splits, splits, kv_heads
+  uint32_t group_magic;  // ceil(2^32 / group), or 0
   int left, right, half;
   float c;           // scale * log2(e)
   float bias_scale;  // log2(e) / (c, or 2 * cap_l under a cap): biases in the units of the scores

@@ -81,6 +81,19 @@ __device__ __forceinline__ int span_of(const int32_t* offsets, const int32_t* le
   if (lengths) n = min(n, lengths[b]);
   return max(n, 0);
 }
+// n / d for any 32-bit n, with the host's ceil(2^64 / d) (0: d is 1): a division takes some thirty
+// instructions, as many as part of a short sequence's tile.
+__device__ __forceinline__ int divide(int n, Divisor d) {
+  if ((d.hi | d.lo) == 0) return n;
+  const uint64_t low = (uint64_t)(uint32_t)n * d.lo, high = (uint64_t)(uint32_t)n * d.hi;
+  return (int)((high + (low >> 32)) >> 32);
+}
+// row / group: rows of up to 2^28 by groups of up to 16 with one multiplication (a division
+// takes forty instructions, as many as a short sequence's tile).
+__device__ __forceinline__ int query_of(const AttendParams& p, int row) {
+  if (p.group == 1) return row;
+  return p.group_magic ? (int)__umulhi((uint32_t)row, p.group_magic) : row / p.group;
+}
 __device__ __forceinline__ Seq seq_of(const AttendParams& p, int b) {
   Seq s;
   s.nq = span_of(p.q_offsets, p.q_lengths, b, p.q_len, p.q_rows, s.q0);
@@ -233,13 +246,17 @@ __device__ __forceinline__ bool seen_of(const Row<C>& r, int k0, uint64_t on, in
   }
   return __ballot(some != 0) != 0;
 }
+// -infinity over the scores of pairs that are not seen: a bit spread over the word, and a bitwise
+// choice by it (two operations, none of them on a condition register).
 template <class C>
 __device__ __forceinline__ void hide(const Seen<C>& see, Scores<C>& x) {
 #pragma unroll
   for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      x.s[ch][i] = (see.bits[ch] >> (16 * (i >> 3) + (i & 7))) & 1 ? x.s[ch][i] : -INFINITY;
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t on = (uint32_t)((int)(see.bits[ch] << (31 - 16 * (i >> 3) - (i & 7))) >> 31);
+      x.s[ch][i] = __uint_as_float((on & __float_as_uint(x.s[ch][i])) | (~on & 0xff800000u));
+    }
 }
 
 // Four chains: an operation on the one before's result waits twice as long as its issue takes.
@@ -264,6 +281,10 @@ template <class C>
 __device__ __forceinline__ void raise(Row<C>& r, float mx, float lag, float mscale) {
   if (!__ballot(!(mx <= r.m + lag))) return;
   const float mn = imax(r.m, mx);
+  if (!__ballot(r.m != -INFINITY)) {  // the first tile: nothing to bring along
+    r.m = mn;
+    return;
+  }
   const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((r.m - mn) * mscale);
   r.l *= corr;
 #pragma unroll
@@ -369,21 +390,21 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   {
     const int x = blockIdx.x % kXcds, n = blockIdx.x / kXcds;
     if (rows_all >= kXcdRows) {
-      const int qd = n / cols;
+      const int qd = divide(n, p.by_cols);
       item = qd * kXcds + x;
       col = n - qd * cols;
       if (item >= rows_all) return;
     } else {
-      const int64_t items = (int64_t)rows_all * cols;
-      const int each = (int)(items / kXcds), r = (int)(items % kXcds);
+      const int items = rows_all * cols, each = items / kXcds, r = items % kXcds;
       if (n >= each + (x < r ? 1 : 0)) return;
-      const int64_t i = (int64_t)x * each + min(x, r) + n;
-      item = (int)(i / cols);
-      col = (int)(i - (int64_t)item * cols);
+      const int i = x * each + min(x, r) + n;
+      item = divide(i, p.by_cols);
+      col = i - item * cols;
     }
   }
-  const int split = col % p.splits, block = p.blocks - 1 - col / p.splits;
-  const int bi = item / p.kv_heads, kvh = item - bi * p.kv_heads, b = p.b0 + bi;
+  const int over = divide(col, p.by_splits);
+  const int split = col - over * p.splits, block = p.blocks - 1 - over;
+  const int bi = divide(item, p.by_kv), kvh = item - bi * p.kv_heads, b = p.b0 + bi;
   const Seq sq = seq_of(p, b);
   const int nq = sq.nq, nk = sq.nk, rows = nq * p.group;
   const int row0 = block * C::BM;
@@ -397,7 +418,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   Row<C> r;
   {
     const int row = min(row0 + rw * 32 + r32, rows - 1);
-    const int i = row / p.group, h = kvh * p.group + row - i * p.group;
+    const int i = query_of(p, row), h = kvh * p.group + row - i * p.group;
     const f16* src = p.q + (p.q_offsets ? (sq.q0 + i) * p.qs.row : b * p.qs.batch + i * p.qs.row) +
                      h * p.qs.head;
 #pragma unroll
@@ -410,8 +431,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
     r.hi = p.right < 0 ? nk : min(r.pos + p.right + 1, nk);
     if constexpr (FEAT == kAny) {
       const int w0 = row0 + rw * 32;
-      r.first = min(w0, rows - 1) / p.group + shift;
-      r.last = min(w0 + 31, rows - 1) / p.group + shift;
+      r.first = query_of(p, min(w0, rows - 1)) + shift;
+      r.last = query_of(p, min(w0 + 31, rows - 1)) + shift;
       r.slope = p.slopes ? p.slopes[h] * p.bias_scale : 0.f;
       r.ltab = nullptr;
       if (p.table) {
@@ -433,7 +454,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
     }
   }
   // ---- the tiles of this block: those of the prefix, then those of the window
-  const int first_q = row0 / p.group, last_q = (min(row0 + C::BM, rows) - 1) / p.group;
+  const int first_q = query_of(p, row0), last_q = query_of(p, min(row0 + C::BM, rows) - 1);
   const int wlo = p.left < 0 ? 0 : max(first_q + shift - p.left, 0);
   const int whi = p.right < 0 ? nk : min(max(last_q + shift + p.right + 1, 0), nk);
   const int np = (prefix + SK - 1) / SK;
@@ -538,7 +559,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   // ---- out
   const int cpr = p.dim / 8;
   auto out_at = [&](int row) {
-    const int i = row / p.group, g = row - i * p.group;
+    const int i = query_of(p, row), g = row - i * p.group;
     return p.out + (p.q_offsets ? (sq.q0 + i) * p.os.row : b * p.os.batch + i * p.os.row) +
            (kvh * p.group + g) * p.os.head;
   };
@@ -681,7 +702,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
     y += sums[i][tid][1];
   }
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  const int i = row / p.group, gh = row - i * p.group;
+  const int i = query_of(p, row), gh = row - i * p.group;
   f16* dst = p.out + (p.q_offsets ? (sq.q0 + i) * p.os.row : b * p.os.batch + i * p.os.row) +
              (kvh * p.group + gh) * p.os.head + 8 * tid;
   f16x8 o;
@@ -737,6 +758,12 @@ void plan(AttendParams& p, size_t scratch_bytes) {
   p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
 }
 
+Divisor divisor(uint64_t d) {
+  if (d == 1) return {0, 0};
+  const uint64_t m = ~0ull / d + 1;
+  return {(uint32_t)(m >> 32), (uint32_t)m};
+}
+
 template <class C>
 hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream_t s) {
   plan<C>(p, scratch ? scratch_bytes : 0);
@@ -744,6 +771,11 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
   const int64_t slots = (int64_t)p.batch * p.kv_heads * p.q_len * p.group;
   p.part_o = static_cast<float*>(scratch);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * p.splits * C::HD);
+  p.by_cols = divisor((uint64_t)cols);
+  p.by_splits = divisor((uint64_t)p.splits);
+  p.by_kv = divisor((uint64_t)p.kv_heads);
+  // exact for rows below 2^32 / group
+  p.group_magic = p.group > 1 && p.group <= 16 ? (uint32_t)(((1ull << 32) + p.group - 1) / p.group) : 0;
   p.table_lds = p.table && table_bytes(p) <= std::min<int64_t>(16384, (int64_t)kLdsMax - (int64_t)C::LDS);
   const int feat = p.slopes || p.table ? kAny : p.cap_l > 0.f ? kCap : kPlain;
   // sequences a launch: its work-items are counted in 32 bits
@@ -774,7 +806,7 @@ using P32 = Cfg<32, 4, 1, 64, 2, 4>;
 using P64 = Cfg<64, 4, 1, 32, 2, 3>;
 using P96 = Cfg<96, 4, 1, 64, 2, 2>;
 using P128 = Cfg<128, 8, 1, 64, 2, 2>;
-using P256 = Cfg<256, 4, 1, 32, 2, 1>;
+using P256 = Cfg<256, 4, 1, 64, 2, 1>;
 using S32 = Cfg<32, 2, 1, 32, 2, 4>;
 using S64 = Cfg<64, 2, 1, 32, 2, 3>;
 using S96 = Cfg<96, 2, 1, 32, 2, 2>;
