@@ -58,18 +58,32 @@ __device__ __forceinline__ float lanes_sum(float v) {
 template <int W>
 using Half = _Float16 __attribute__((ext_vector_type(W)));
 
+template <bool STREAM, class V>
+__device__ __forceinline__ V take(const f16* p) {
+  const V* v = reinterpret_cast<const V*>(p);
+  if constexpr (STREAM) return __builtin_nontemporal_load(v);
+  return *v;
+}
+template <bool STREAM, class V>
+__device__ __forceinline__ void put(f16* p, V v) {
+  V* o = reinterpret_cast<V*>(p);
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(v, o);
+  else
+    *o = v;
+}
+
 // How a launch is cut: pieces of 2 W values (`units` a head), U a thread.
 struct Cut {
   int rows, parts;  // rows of a workgroup; workgroups a row's heads are spread over
   int units, unit_div, head_div;  // division by units and heads: (n * div) >> 20, n < 1024
 };
-constexpr int kMaxItems = 1024;  // pieces of a workgroup
 
 // A piece is two runs of W values: the same place in both halves of the turning part, or
 // neighbours (interleaved pairs, and the values that do not turn).  G: lanes a head, a power
 // of two, where heads are normed (their squares are added across lanes); 0: as many as it has
 // pieces.
-template <int W, int G, int U>
+template <int W, int G, int U, bool STREAM>
 __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p, RopeSteps steps, Cut cut) {
   constexpr bool NORM = G > 0;
   using V = Half<W>;
@@ -132,8 +146,8 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p, RopeSteps 
     int ca, cb;
     place(at[e].u, ca, cb);
     a[e] = b[e] = none;
-    if (at[e].kind < 3 && ca < p.dim) a[e] = *reinterpret_cast<const V*>(at[e].x + ca);
-    if (at[e].kind < 3 && cb < p.dim) b[e] = *reinterpret_cast<const V*>(at[e].x + cb);
+    if (at[e].kind < 3 && ca < p.dim) a[e] = take<STREAM, V>(at[e].x + ca);
+    if (at[e].kind < 3 && cb < p.dim) b[e] = take<STREAM, V>(at[e].x + cb);
   }
   if constexpr (NORM) {
     if (tid < p.dim) {
@@ -200,8 +214,8 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p, RopeSteps 
         ob[i] = (f16)y[i];
       }
     }
-    if (kind < 3 && ca < p.dim) *reinterpret_cast<V*>(at[e].y + ca) = oa;
-    if (kind < 3 && cb < p.dim) *reinterpret_cast<V*>(at[e].y + cb) = ob;
+    if (kind < 3 && ca < p.dim) put<STREAM>(at[e].y + ca, oa);
+    if (kind < 3 && cb < p.dim) put<STREAM>(at[e].y + cb, ob);
   }
 }
 
@@ -287,13 +301,26 @@ int width(const RopeParams::Part& t, int w) {
   return ((uintptr_t)t.x | (uintptr_t)t.y) & 1 ? 1 : w;
 }
 
+// Whether rows are read and written past the caches: from 48 MB on, where every store is of whole
+// lines (32768 x 40 x 128 142 -> 131 us; 131072 x 24 x 32, whose stores are of half lines, 81 ->
+// 139).  Three pieces a thread then (four 134, two 137).
+constexpr int64_t kStreamBytes = 48 << 20;
+bool lines(const RopeParams::Part& t) {
+  return !t.heads || (((uintptr_t)t.y & 127) == 0 && ((t.y_row | t.y_head) & 63) == 0);
+}
+bool streams(const RopeParams& p) {
+  const int64_t bytes = 2 * (int64_t)(p.rows - p.row0) * (p.q.heads + p.k.heads + p.v.heads) * p.dim;
+  return bytes >= kStreamBytes && !p.interleaved && p.rot == p.dim && p.dim % 128 == 0 && lines(p.q) &&
+         lines(p.k) && lines(p.v);
+}
+
 int pow2(int n) {
   int p = 1;
   while (p < n) p *= 2;
   return p;
 }
 
-template <int W, int G, int U>
+template <int W, int G, int U, bool STREAM>
 hipError_t launch_as(const RopeParams& p, const RopeSteps& steps, hipStream_t s) {
   const int heads = p.q.heads + p.k.heads + p.v.heads;
   Cut c{};
@@ -306,14 +333,20 @@ hipError_t launch_as(const RopeParams& p, const RopeSteps& steps, hipStream_t s)
   const int rows = p.rows - p.row0;
   const int64_t grid = (int64_t)((rows + c.rows - 1) / c.rows) * c.parts;
   const size_t lds = (size_t)c.rows * (p.rot / 2) * sizeof(float2);
-  hipLaunchKernelGGL((rope_kernel<W, G, U>), dim3((unsigned)grid), dim3(kThreads), lds, s, p, steps, c);
+  hipLaunchKernelGGL((rope_kernel<W, G, U, STREAM>), dim3((unsigned)grid), dim3(kThreads), lds, s, p, steps, c);
   return hipGetLastError();
 }
 template <int W, int G>
 hipError_t launch(const RopeParams& p, const RopeSteps& steps, hipStream_t s) {
   const int64_t items = (int64_t)(p.rows - p.row0) * (p.q.heads + p.k.heads + p.v.heads) *
                         (G ? G : (p.dim + 2 * W - 1) / (2 * W));
-  return items < 1 << 18 ? launch_as<W, G, 1>(p, steps, s) : launch_as<W, G, 4>(p, steps, s);
+  // A piece a thread for calls of few tokens (16 tokens of 48 heads of 128: 4.0 us against 5.5 with
+  // four), two otherwise (131072 x 24 x 32 81 us with two, 93 with four).
+  if (items < 1 << 18) return launch_as<W, G, 1, false>(p, steps, s);
+  if constexpr (W == 8) {
+    if (streams(p)) return launch_as<W, G, 3, true>(p, steps, s);
+  }
+  return launch_as<W, G, 2, false>(p, steps, s);
 }
 template <int W>
 hipError_t launch_w(const RopeParams& p, const RopeSteps& steps, hipStream_t s) {
