@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "libbbh.so")
@@ -64,6 +65,19 @@ class AttendArgs(ctypes.Structure):
         (n, c_int) for n in ("batch", "q_len", "k_len", "heads", "kv_heads", "head_dim", "left",
                              "right", "table_half")] + [("scale", c_float), ("cap", c_float)]
 
+
+_CODES = {c_void_p: "P", c_i64: "q", c_size_t: "N", c_int: "i", c_float: "f"}
+
+
+def packer(cls):
+    """A function from the values of cls's fields, in order, to the struct's bytes: a third
+    of the time that ctypes takes to fill one."""
+    pack = struct.Struct("@" + "".join(_CODES[t] for _, t in cls._fields_) + "0P")
+    assert pack.size == ctypes.sizeof(cls)
+    return pack.pack
+
+
+pack_rope_args, pack_attend_args = packer(RopeArgs), packer(AttendArgs)
 
 _AWp, _FWp = ctypes.POINTER(AttnWeights), ctypes.POINTER(FfnWeights)
 
@@ -158,9 +172,9 @@ SIGNATURES_ATTEND = {
     "bbh_rope_create": (c_int, [ctypes.POINTER(RopeConfig), ctypes.POINTER(c_void_p)]),
     "bbh_rope_free": (c_int, [c_void_p]),
     "bbh_rope_frequencies": (c_int, [c_void_p, ctypes.POINTER(ctypes.c_double)]),
-    "bbh_rope_heads": (c_int, [c_void_p, ctypes.POINTER(RopeArgs), c_void_p]),
-    "bbh_attend": (c_int, [ctypes.POINTER(AttendArgs), c_void_p]),
-    "bbh_attend_scratch": (c_size_t, [ctypes.POINTER(AttendArgs)]),
+    "bbh_rope_heads": (c_int, [c_void_p, c_void_p, c_void_p]),
+    "bbh_attend": (c_int, [c_void_p, c_void_p]),
+    "bbh_attend_scratch": (c_size_t, [c_void_p]),
 }
 
 # Exported for profile tables only: what the launchers choose.

@@ -623,23 +623,27 @@ def _int(name, n):
     return n
 
 
-def _head_strides(name, t, dims, device):
-    """(address, batch, row, head strides) of a (rows, heads, head_dim) tensor, or of a
-    (batch, rows, heads, head_dim) one, on the current device.  A dimension of one
+def _place_of_heads(name, t, n, device):
+    """(address, batch, row, head strides) of a (rows, heads, head_dim) tensor (n = 3), or
+    of a (batch, rows, heads, head_dim) one, on the current device.  A dimension of one
     element has no stride that matters."""
-    if t.dtype is not _torch().float16 or t.dim() not in dims or not t.is_cuda:
-        raise TypeError(f"{name} must be a float16 CUDA tensor of {' or '.join(map(str, dims))} "
-                        "dimensions")
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not _torch().float16 or len(shape) != n or not t.is_cuda:
+        raise TypeError(f"{name} must be a float16 CUDA tensor of {n} dimensions")
     if t.get_device() != device:
         raise ValueError(f"{name} is on cuda:{t.get_device()}, not on cuda:{device}, the current device")
-    shape, stride = t.shape, t.stride()
-    if stride[-1] != 1 and shape[-1] > 1:
+    if n == 3:
+        batch, (i, h, d), (row, head, one) = 0, shape, stride
+    else:
+        (b, i, h, d), (batch, row, head, one) = shape, stride
+        if b == 1:
+            batch = 0
+    if one != 1 and d > 1:
         raise ValueError(f"{name}: the values of a head must be contiguous")
-    return (t.data_ptr(), stride[0] if len(shape) == 4 and shape[0] > 1 else 0,
-            stride[-3] if shape[-3] > 1 else 0, stride[-2] if shape[-2] > 1 else 0)
+    return t.data_ptr(), batch, row if i > 1 else 0, head if h > 1 else 0
 
 
-_NO_HEADS = (None, 0, 0, 0)
+_NO_HEADS = (0, 0, 0, 0)
 
 
 def launch_rope(rope, q, q_out=None, k=None, k_out=None, v=None, v_out=None, positions=None,
@@ -651,49 +655,53 @@ def launch_rope(rope, q, q_out=None, k=None, k_out=None, v=None, v_out=None, pos
     place).  kv_rows (rows) int64: the rows of k_out and v_out that k and v go to, as the
     slots of a cache; one outside them is not written (bbh_rope_heads)."""
     torch = _torch()
-    if not q.is_cuda:
-        raise TypeError("operands must be CUDA tensors")
     c = torch._C
-    dev = c._cuda_getDevice()
-    q_out = q if q_out is None else q_out
-    if k_out is None and k is not None:
-        if kv_rows is not None:
-            raise ValueError("kv_rows needs k_out")
-        k_out = k
-    if (v is None) != (v_out is None) or (k is None and k_out is not None):
-        raise ValueError("k and k_out, v and v_out go together")
-    three = (3,)
-    places = [_NO_HEADS if t is None else _head_strides(n, t, three, dev)
-              for n, t in (("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_out", k_out),
-                           ("v_out", v_out))]
-    rows, heads, dim = q.shape
-    if q_out.shape != q.shape:
-        raise ValueError("q_out must have q's shape")
-    kv_heads, out_rows = 0, None
+    dev = c._cuda_getDevice() if q.is_cuda else -1
+    rows, heads, dim = q.shape if q.dim() == 3 else (0, 0, 0)
+    at_q = at_out = _place_of_heads("q", q, 3, dev)
+    if q_out is None:
+        q_out = q
+    else:
+        at_out = _place_of_heads("q_out", q_out, 3, dev)
+        if q_out.shape != q.shape:
+            raise ValueError("q_out must have q's shape")
+    kv_heads = out_rows = 0
+    at_kv = []
     for n, x, y in (("k", k, k_out), ("v", v, v_out)):
         if x is None:
+            if y is not None:
+                raise ValueError(f"{n}_out without {n}")
+            at_kv.append(_NO_HEADS)
+            at_kv.append(_NO_HEADS)
             continue
-        if x.shape[0] != rows or x.shape[2] != dim or (kv_heads and x.shape[1] != kv_heads):
+        if y is None:
+            if n == "v" or kv_rows is not None:
+                raise ValueError(f"{n} needs {n}_out")
+            y = x
+        at_kv.append(_place_of_heads(n, x, 3, dev))
+        at_kv.append(_place_of_heads(n + "_out", y, 3, dev))
+        shape, to = x.shape, y.shape
+        if shape[0] != rows or shape[2] != dim or (kv_heads and shape[1] != kv_heads):
             raise ValueError(f"{n} must have q's rows and head_dim, and k and v the same heads")
-        kv_heads = x.shape[1]
-        if y.shape[1:] != x.shape[1:] or (kv_rows is None and y.shape[0] != rows):
+        if to[1:] != shape[1:] or (kv_rows is None and to[0] != rows):
             raise ValueError(f"{n}_out must have {n}'s shape (but its rows with kv_rows)")
-        if out_rows is not None and y.shape[0] != out_rows:
+        if kv_heads and to[0] != out_rows:
             raise ValueError("k_out and v_out must have the same rows")
-        out_rows = y.shape[0]
+        kv_heads, out_rows = shape[1], to[0]
     seq = 0 if seq is None else _int("seq", seq)
     if rope is not None and positions is None and seq < 1:
         raise ValueError("positions or seq must be given")
-    if rows == 0:
+    if rows == 0 or heads == 0 or dim == 0:
         return q_out
-    args = capi.RopeArgs(
-        *places[0], *places[1], *places[2], *places[3], *places[4], *places[5],
-        _operand("q_gamma", q_gamma, torch.float16, dim, dev),
-        _operand("k_gamma", k_gamma, torch.float16, dim, dev),
-        _operand("positions", positions, torch.int32, rows, dev),
-        _operand("kv_rows", kv_rows, torch.int64, rows, dev), out_rows or 0, rows, seq, heads,
-        kv_heads, dim, eps)
-    call("bbh_rope_heads", rope.handle if rope is not None else None, ctypes.byref(args),
+    f16 = torch.float16
+    args = capi.pack_rope_args(
+        *at_q, *at_kv[0], *at_kv[2], *at_out, *at_kv[1], *at_kv[3],
+        0 if q_gamma is None else _operand("q_gamma", q_gamma, f16, dim, dev),
+        0 if k_gamma is None else _operand("k_gamma", k_gamma, f16, dim, dev),
+        0 if positions is None else _operand("positions", positions, torch.int32, rows, dev),
+        0 if kv_rows is None else _operand("kv_rows", kv_rows, torch.int64, rows, dev), out_rows,
+        rows, seq, heads, kv_heads, dim, eps)
+    call("bbh_rope_heads", None if rope is None else rope.handle, args,
          c._cuda_getCurrentRawStream(dev) if stream is None else stream)
     return q_out
 
@@ -702,13 +710,11 @@ def _attend_args(q, k, v, out, q_len=None, k_len=None, q_offsets=None, k_offsets
                  q_lengths=None, k_lengths=None, left=-1, right=-1, scale=None, cap=0.0,
                  mask=None, prefix=None, slopes=None, table=None, scratch=None):
     torch = _torch()
-    if not q.is_cuda:
-        raise TypeError("operands must be CUDA tensors")
-    dev = torch._C._cuda_getDevice()
+    dev = torch._C._cuda_getDevice() if q.is_cuda else -1
     qp, kp = q_offsets is not None, k_offsets is not None
-    qd, kd = ((3,) if qp else (4,)), ((3,) if kp else (4,))
-    places = (_head_strides("q", q, qd, dev), _head_strides("k", k, kd, dev),
-              _head_strides("v", v, kd, dev), _head_strides("out", out, qd, dev))
+    qd, kd = 3 if qp else 4, 3 if kp else 4
+    places = (*_place_of_heads("q", q, qd, dev), *_place_of_heads("k", k, kd, dev),
+              *_place_of_heads("v", v, kd, dev), *_place_of_heads("out", out, qd, dev))
     if k.shape != v.shape or q.shape != out.shape or q.shape[-1] != k.shape[-1]:
         raise ValueError("k and v, q and out must have the same shapes, and all the same head_dim")
     heads, dim = q.shape[-2:]
@@ -737,16 +743,16 @@ def _attend_args(q, k, v, out, q_len=None, k_len=None, q_offsets=None, k_offsets
         half = table.shape[1] // 2
     if mask is not None and tuple(mask.shape) != (batch, k_len):
         raise ValueError(f"mask must be ({batch}, {k_len})")
-    return dev, capi.AttendArgs(
-        *places[0], *places[1], *places[2], *places[3], q.shape[0] if qp else 0,
-        k.shape[0] if kp else 0, _operand("q_offsets", q_offsets, i32, batch + 1, dev),
-        _operand("k_offsets", k_offsets, i32, batch + 1, dev),
-        _operand("q_lengths", q_lengths, i32, batch, dev),
-        _operand("k_lengths", k_lengths, i32, batch, dev),
-        _operand("prefix", prefix, i32, batch, dev), _operand("mask", mask, i32, batch * k_len, dev),
-        _operand("slopes", slopes, f32, heads, dev),
-        _operand("table", table, f32, heads * (2 * half + 1), dev),
-        None if scratch is None else _operand("scratch", scratch, scratch.dtype, 0, dev),
+    def of(name, t, dtype, n):
+        return 0 if t is None else _operand(name, t, dtype, n, dev)
+
+    return dev, capi.pack_attend_args(
+        *places, q.shape[0] if qp else 0, k.shape[0] if kp else 0,
+        of("q_offsets", q_offsets, i32, batch + 1), of("k_offsets", k_offsets, i32, batch + 1),
+        of("q_lengths", q_lengths, i32, batch), of("k_lengths", k_lengths, i32, batch),
+        of("prefix", prefix, i32, batch), of("mask", mask, i32, batch * k_len),
+        of("slopes", slopes, f32, heads), of("table", table, f32, heads * (2 * half + 1)),
+        0 if scratch is None else _operand("scratch", scratch, scratch.dtype, 0, dev),
         0 if scratch is None else scratch.numel() * scratch.element_size(), batch, q_len, k_len,
         heads, k.shape[-2], dim, _int("left", left), _int("right", right), half,
         dim ** -0.5 if scale is None else scale, cap)
@@ -765,14 +771,14 @@ def launch_attend(q, k, v, out, q_len=None, k_len=None, q_offsets=None, k_offset
     keys run faster."""
     dev, args = _attend_args(q, k, v, out, q_len, k_len, q_offsets, k_offsets, q_lengths, k_lengths,
                              left, right, scale, cap, mask, prefix, slopes, table, scratch)
-    call("bbh_attend", ctypes.byref(args),
+    call("bbh_attend", args,
          _torch()._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
     return out
 
 
 def attend_scratch(q, k, v, out, **kwargs) -> int:
     """Bytes of scratch that launch_attend makes use of with these arguments."""
-    return capi.lib().bbh_attend_scratch(ctypes.byref(_attend_args(q, k, v, out, **kwargs)[1]))
+    return capi.lib().bbh_attend_scratch(_attend_args(q, k, v, out, **kwargs)[1])
 
 
 class Tokenizer:
