@@ -352,20 +352,20 @@ struct Copies {
       voff[j] = 8 * vc < p.dim ? (uint32_t)(r * (int)p.vs.row + 8 * vc) * 2u : kNowhere;
     }
   }
-  // `valid` keys from k and v on into a stage; rows behind them become zeros.
-  __device__ __forceinline__ void issue(const AttendParams& p, const f16* k, const f16* v, int valid,
-                                        lds_f16* stage) {
-    const bool any = valid > 0;
-    const auto rk = buffer_of(k, any ? (uint32_t)((valid - 1) * (int)p.ks.row + p.dim) * 2u : 0u);
-    const auto rv = buffer_of(v, any ? (uint32_t)((valid - 1) * (int)p.vs.row + p.dim) * 2u : 0u);
-    lds_f16* ks = stage + cwave * C::N * 512;
-    lds_f16* vs = ks + C::SK * C::HD;
+  // `valid` keys' K (V) from src on into a stage; rows behind them become zeros.
+  __device__ __forceinline__ void issue_k(const AttendParams& p, const f16* src, int valid, lds_f16* stage) {
+    const auto r = buffer_of(src, valid > 0 ? (uint32_t)((valid - 1) * (int)p.ks.row + p.dim) * 2u : 0u);
+    lds_f16* to = stage + cwave * C::N * 512;
 #pragma unroll
     for (int j = 0; j < C::N; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (BBH_LDS void*)(ks + j * 512), 16, (int)koff[j], 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (BBH_LDS void*)(to + j * 512), 16, (int)koff[j], 0, 0, 0);
+  }
+  __device__ __forceinline__ void issue_v(const AttendParams& p, const f16* src, int valid, lds_f16* stage) {
+    const auto r = buffer_of(src, valid > 0 ? (uint32_t)((valid - 1) * (int)p.vs.row + p.dim) * 2u : 0u);
+    lds_f16* to = stage + C::SK * C::HD + cwave * C::N * 512;
 #pragma unroll
     for (int j = 0; j < C::N; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (BBH_LDS void*)(vs + j * 512), 16, (int)voff[j], 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (BBH_LDS void*)(to + j * 512), 16, (int)voff[j], 0, 0, 0);
   }
   // Zeros over this wavefront's part of a stage's V where the key is masked: a weight of 0 times
   // what a masked key holds is not always 0.
@@ -480,18 +480,18 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   Copies<C> copies;
   copies.init(p, wave, lane);
   BBH_LDS int* masks = (BBH_LDS int*)((BBH_LDS char*)smem + C::RING) + (C::KS == 1 ? 0 : wave * C::R * 64);
-  // Copies of the next tile, into the ring's next stage.
-  int ni = 0, nstage = 0;
-  auto next = [&] {
-    const int k0 = key_at(ni), valid = ni < count ? min(nk - k0, SK) : 0;
-    copies.issue(p, kbase + (int64_t)k0 * (int)p.ks.row, vbase + (int64_t)k0 * (int)p.vs.row, valid,
-                 ring + nstage * C::STAGE);
+  // Copies of tile i into a stage (past the last tile: of nothing).
+  auto copy_k = [&](int i, int stage) {
+    const int k0 = key_at(i), valid = i < count ? min(nk - k0, SK) : 0;
+    copies.issue_k(p, kbase + (int64_t)k0 * (int)p.ks.row, valid, ring + stage * C::STAGE);
     if (mrow && copies.cwave == C::CW - 1)  // the tile's mask beside it; zeros behind the last key
       __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_of(mrow, (uint32_t)nk * 4u),
-                                               (BBH_LDS void*)(masks + nstage * 64), 4,
-                                               ni < count ? (k0 + lane) * 4 : (int)Copies<C>::kNowhere, 0, 0, 0);
-    ++ni;
-    nstage = nstage == C::R - 1 ? 0 : nstage + 1;
+                                               (BBH_LDS void*)(masks + stage * 64), 4,
+                                               i < count ? (k0 + lane) * 4 : (int)Copies<C>::kNowhere, 0, 0, 0);
+  };
+  auto copy_v = [&](int i, int stage) {
+    const int k0 = key_at(i), valid = i < count ? min(nk - k0, SK) : 0;
+    copies.issue_v(p, vbase + (int64_t)k0 * (int)p.vs.row, valid, ring + stage * C::STAGE);
   };
   constexpr uint64_t kAll = SK == 64 ? ~0ull : 0xffffffffull;
   // Unmasked keys of a tile that is in place.
@@ -500,9 +500,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
       const int n = nk - key_at(i);
       return n >= SK ? kAll : (1ull << n) - 1;
     }
-    const uint64_t bits = __ballot(masks[stage * 64 + lane] != 0) & kAll;
-    if (bits != kAll) copies.clear_masked(ring + stage * C::STAGE, bits, lane);
-    return bits;
+    return __ballot(masks[stage * 64 + lane] != 0) & kAll;
   };
 #pragma unroll
   for (int d = 0; d < ND; ++d) r.o[d] = f32x16{};
@@ -517,41 +515,82 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   Scores<C> x;
   Weights<C> w;
   Seen<C> see;
-  // R - 1 tiles on their way (past the last one: of nothing, so that their number is known).
-  constexpr int kTile = 2 * C::N;  // copies of a tile (a wavefront that copies masks has one more,
-                                   // and waits for more than it has to)
-  wait_vm<0>();  // the queries: their first use is inside the loop
-  for (int i = 0; i < C::R - 1; ++i) next();
-  int now = 0;  // stage of tile it
-  for (int it = 0; it < count; ++it) {
-    if constexpr (C::KS == 1) {
-      wait_vm<(C::R - 2) * kTile>();
-      lds_barrier();
-      next();
-    } else {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last tile of that stage has been read
-      next();
-      wait_vm<(C::R - 1) * kTile>();
-      asm volatile("" ::: "memory");
-    }
-    const int k0 = key_at(it);
-    const uint64_t bits = bits_of(it, now);
-    if (mrow && bits != kAll) {  // all of V is cleared before any of it is read
-      if constexpr (C::KS == 1) lds_barrier();
-      else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-    const lds_f16* ks = ring + now * C::STAGE;
-    now = now == C::R - 1 ? 0 : now + 1;
-    const bool edge = !whole(k0, bits);
-    if (!bits || (edge && !seen_of(r, k0, bits, prefix, see))) continue;
+  // A tile's products, softmax and output; false where no row of the wavefront sees any of it.
+  auto tile_scores = [&](int k0, uint64_t bits, const lds_f16* ks, bool& edge) {
+    edge = !whole(k0, bits);
+    if (!bits || (edge && !seen_of(r, k0, bits, prefix, see))) return false;
     scores(r, ks, x);
     ahead<C::CH * NS, 1, kAheadK>();
+    return true;
+  };
+  auto tile_weights = [&](int k0, bool edge) {
     shape<C, FEAT>(p, r, k0, x);
     if (edge) hide(see, x);
     raise(r, largest(x), lag, mscale);
     weigh(r, x, mscale, w);
-    context(r, ks + SK * HD, w);
+  };
+  auto tile_output = [&](const lds_f16* vs) {
+    context(r, vs, w);
     ahead<C::CH * 2 * ND, 2, kAheadV>();
+  };
+  auto lds_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+  wait_vm<0>();  // the queries: their first use is inside the loop
+  if constexpr (C::R == 1) {
+    // A wavefront's own tile, one stage: K of the next tile is on its way from the end of this
+    // one's scores on, V from the end of its output on.  Half the LDS of two stages is twice the
+    // wavefronts, and those are what keeps the memory busy here.  (A copied mask is one copy more
+    // than is counted: the waits are for more than they have to be.)
+    static_assert(C::CW == 1, "tiles of its own");
+    copy_k(0, 0);
+    copy_v(0, 0);
+    for (int it = 0; it < count; ++it) {
+      wait_vm<C::N>();
+      asm volatile("" ::: "memory");
+      const int k0 = key_at(it);
+      const uint64_t bits = bits_of(it, 0);
+      bool edge;
+      const bool some = tile_scores(k0, bits, ring, edge);
+      lds_done();
+      copy_k(it + 1, 0);
+      if (some) tile_weights(k0, edge);
+      wait_vm<C::N>();
+      asm volatile("" ::: "memory");
+      if (mrow && bits != kAll) {
+        copies.clear_masked(ring, bits, lane);
+        lds_done();
+      }
+      if (some) tile_output(ring + SK * HD);
+      lds_done();
+      copy_v(it + 1, 0);
+    }
+  } else {
+    // R - 1 tiles on their way, shared by the workgroup's wavefronts.
+    static_assert(C::KS == 1, "a barrier a tile");
+    constexpr int kTile = 2 * C::N;  // copies of a tile
+    for (int i = 0; i < C::R - 1; ++i) {
+      copy_k(i, i);
+      copy_v(i, i);
+    }
+    int now = 0, next = C::R - 1;  // stages of tile it and of tile it + R - 1
+    for (int it = 0; it < count; ++it) {
+      wait_vm<(C::R - 2) * kTile>();
+      lds_barrier();
+      copy_k(it + C::R - 1, next);
+      copy_v(it + C::R - 1, next);
+      next = next == C::R - 1 ? 0 : next + 1;
+      const int k0 = key_at(it);
+      const uint64_t bits = bits_of(it, now);
+      lds_f16* ks = ring + now * C::STAGE;
+      if (mrow && bits != kAll) {  // all of V is cleared before any of it is read
+        copies.clear_masked(ks, bits, lane);
+        lds_barrier();
+      }
+      now = now == C::R - 1 ? 0 : now + 1;
+      bool edge;
+      if (!tile_scores(k0, bits, ks, edge)) continue;
+      tile_weights(k0, edge);
+      tile_output(ks + SK * HD);
+    }
   }
   f32x16 (&o)[ND] = r.o;
   const float m = r.m, l = xor32_sum(r.l);
@@ -812,16 +851,16 @@ using S64 = Cfg<64, 2, 1, 32, 2, 3>;
 using S96 = Cfg<96, 2, 1, 32, 2, 2>;
 using S128 = Cfg<128, 2, 1, 32, 2, 2>;
 using S256 = Cfg<256, 2, 1, 32, 2, 1>;
-using K32 = Cfg<32, 4, 4, 32, 2, 2>;
-using K64 = Cfg<64, 4, 4, 32, 2, 2>;
-using K96 = Cfg<96, 4, 4, 32, 2, 1>;
-using K128 = Cfg<128, 4, 4, 32, 2, 1>;
-using K256 = Cfg<256, 2, 2, 32, 2, 1>;
-using L32 = Cfg<32, 1, 1, 32, 2, 4>;
-using L64 = Cfg<64, 1, 1, 32, 2, 3>;
+using K32 = Cfg<32, 4, 4, 32, 1, 2>;
+using K64 = Cfg<64, 4, 4, 32, 1, 2>;
+using K96 = Cfg<96, 4, 4, 32, 1, 2>;
+using K128 = Cfg<128, 4, 4, 32, 1, 2>;
+using K256 = Cfg<256, 4, 4, 32, 1, 1>;
+using L32 = Cfg<32, 1, 1, 64, 2, 4>;
+using L64 = Cfg<64, 1, 1, 64, 2, 2>;
 using L96 = Cfg<96, 1, 1, 32, 2, 2>;
 using L128 = Cfg<128, 1, 1, 32, 2, 2>;
-using L256 = Cfg<256, 1, 1, 32, 2, 1>;
+using L256 = Cfg<256, 1, 1, 32, 1, 1>;
 
 template <class F>
 auto with_config(const AttendParams& p, bool scratch, F&& f) {
