@@ -840,9 +840,16 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
   return hipSuccess;
 }
 
+// The sets of configurations, by head size (sizes between them are padded with zeros in LDS and
+// registers, never in memory):
+//  P  many rows a sequence: 128 rows a workgroup, 256 for 128 values a head
+//  S  fewer: 64, whose copies wait for less company
+//  T  up to 16 rows: a wavefront, one stage
+//  K  up to 32 rows over many keys, whose four wavefronts take tiles of keys in turn
+//  L  the same with work for a wavefront everywhere
 //               HD  NW KS SK R OCC
 using P32 = Cfg<32, 4, 1, 64, 2, 4>;
-using P64 = Cfg<64, 4, 1, 32, 2, 3>;
+using P64 = Cfg<64, 4, 1, 32, 2, 4>;
 using P96 = Cfg<96, 4, 1, 64, 2, 2>;
 using P128 = Cfg<128, 8, 1, 64, 2, 2>;
 using P256 = Cfg<256, 4, 1, 64, 2, 1>;
@@ -851,6 +858,11 @@ using S64 = Cfg<64, 2, 1, 32, 2, 3>;
 using S96 = Cfg<96, 2, 1, 32, 2, 2>;
 using S128 = Cfg<128, 2, 1, 32, 2, 2>;
 using S256 = Cfg<256, 2, 1, 32, 2, 1>;
+using T32 = Cfg<32, 1, 1, 32, 1, 4>;
+using T64 = Cfg<64, 1, 1, 32, 1, 4>;
+using T96 = Cfg<96, 1, 1, 32, 1, 2>;
+using T128 = Cfg<128, 1, 1, 32, 1, 2>;
+using T256 = Cfg<256, 1, 1, 32, 1, 1>;
 using K32 = Cfg<32, 4, 4, 32, 1, 2>;
 using K64 = Cfg<64, 4, 4, 32, 1, 2>;
 using K96 = Cfg<96, 4, 4, 32, 1, 2>;
@@ -860,25 +872,36 @@ using L32 = Cfg<32, 1, 1, 64, 2, 4>;
 using L64 = Cfg<64, 1, 1, 64, 2, 2>;
 using L96 = Cfg<96, 1, 1, 32, 2, 2>;
 using L128 = Cfg<128, 1, 1, 32, 2, 2>;
-using L256 = Cfg<256, 1, 1, 32, 1, 1>;
+using L256 = T256;
 
+// By rows a sequence (on average, where documents are packed) and keys.  Measured on 40000 tokens
+// of 12 heads in sequences of one length, us on P / S / T:
+//   64 values a head:   8 tokens 221 / 127 / 73, 16: 118 / 70 / 49, 32: 66 / 52 / 56, 64: 52 / 54 / 59,
+//                       200: 68 / 74 / 95, 500: 102 / 111 / 146
+//   128 values a head:  8 tokens 1142 / 243 / 148, 16: 601 / 139 / 98, 32: 336 / 99 / 99, 128: 145 / 109 / 134,
+//                       300: 210 / 156 / 209, 300 by 4 heads a key/value head: 138 / 133 / 160, 500 so: 180 / 188 / 222
 template <class F>
 auto with_config(const AttendParams& p, bool scratch, F&& f) {
   const int64_t rows = (int64_t)p.q_len * p.group, keys = longest(p);
+  const int64_t items = (int64_t)p.batch * p.kv_heads;
   const int64_t mean = p.q_offsets ? p.q_rows * p.group / p.batch : rows;
-#define BBH_BY_SIZE(SET)                \
-  do {                                  \
+#define BBH_BY_SIZE(SET)                    \
+  do {                                      \
     if (p.dim <= 32) return f(SET##32{});   \
     if (p.dim <= 64) return f(SET##64{});   \
     if (p.dim <= 96) return f(SET##96{});   \
     if (p.dim <= 128) return f(SET##128{}); \
-    return f(SET##256{});               \
+    return f(SET##256{});                   \
   } while (0)
   if (rows <= 32 && keys > 128) {
-    if (scratch && (int64_t)p.batch * p.kv_heads * keys >= 1 << 18) BBH_BY_SIZE(L);
+    if (items >= 1024 || (scratch && items * keys >= 1 << 18)) BBH_BY_SIZE(L);
     BBH_BY_SIZE(K);
   }
-  if (mean <= 64) BBH_BY_SIZE(S);
+  if (mean <= 16) BBH_BY_SIZE(T);
+  // Rows of S at most.  Above 64 values of 64 a head P is 3-8% faster where all sequences are as long,
+  // and far behind where they are not (2000 documents of 8 to 160 tokens: 301 us against 172).
+  const int64_t most = p.dim <= 96 ? 128 : p.dim <= 128 ? 1024 : 64;
+  if (mean <= most) BBH_BY_SIZE(S);
   BBH_BY_SIZE(P);
 #undef BBH_BY_SIZE
 }
