@@ -4,6 +4,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "attend.h"
 #include "pipe.h"
@@ -40,6 +41,11 @@ struct Tile {
 };
 
 constexpr float kLazy = 8.f;
+// A weight's exponent is fma(mscale, s, -(m mscale rounded)): one operation, and the product's
+// rounding error, the same in all of a row's weights, cancels with their sum.  With scores of 2^28
+// and more it would itself be far from 0 (a bias of the type's lowest value: 2^100), so that
+// above kFar the difference is taken first.
+constexpr float kFar = 65536.f;
 constexpr int kMaxSplits = 256;  // a thread of the joining workgroup each
 
 template <int HD_, int NW_, int KS_, int SK_, int R_, int OCC_>
@@ -68,6 +74,8 @@ struct Seq {
   int nq, nk;
 };
 
+// Rows of sequence b, inside the tensor whatever the offsets hold (both ends clamped: their
+// difference then fits an int) and whatever the length.
 __device__ __forceinline__ int span_of(const int32_t* offsets, const int32_t* lengths, int b,
                                        int len, int64_t rows, int64_t& start) {
   start = 0;
@@ -75,7 +83,7 @@ __device__ __forceinline__ int span_of(const int32_t* offsets, const int32_t* le
   if (offsets) {
     const int64_t a = offsets[b], e = offsets[b + 1];
     start = a < 0 ? 0 : a > rows ? rows : a;
-    const int64_t end = e > rows ? rows : e;
+    const int64_t end = e < 0 ? 0 : e > rows ? rows : e;
     n = (int)(end - start < len ? end - start : len);
   }
   if (lengths) n = min(n, lengths[b]);
@@ -143,10 +151,11 @@ struct Row {
   float below, above;        // its ends
   f32x16 o[C::HD / 32];  // o[d][i]: dim 32 d + 8 (i / 4) + 4 (lane / 32) + i % 4
   float m, l;
+  bool far;  // some row's m * mscale is above kFar
 };
-// A bias in the units of the scores.  Finite ones stay finite.
+// A bias in the units of the scores.  Finite ones stay finite, in those units and as powers of two.
 __device__ __forceinline__ float bias_units(const AttendParams& p, float w) {
-  return w == -INFINITY ? w : imax(w * p.bias_scale, -1e38f);
+  return w == -INFINITY ? w : imax(imax(w, -1e38f) * p.bias_scale, -1e38f);
 }
 // The scores of a tile: s[ch][i] is key 32 ch + 16 (i / 8) + 8 (lane / 32) + i % 8 of it.
 template <class C>
@@ -281,6 +290,7 @@ template <class C>
 __device__ __forceinline__ void raise(Row<C>& r, float mx, float lag, float mscale) {
   if (!__ballot(!(mx <= r.m + lag))) return;
   const float mn = imax(r.m, mx);
+  r.far = __ballot(mn != -INFINITY && fabsf(mn * mscale) > kFar) != 0;
   if (!__ballot(r.m != -INFINITY)) {  // the first tile: nothing to bring along
     r.m = mn;
     return;
@@ -297,10 +307,17 @@ __device__ __forceinline__ void raise(Row<C>& r, float mx, float lag, float msca
 // It is added up with plain additions: a dot product of two does not run while the matrix unit is
 // busy (16 of them beside another wavefront's products 104 -> 230 cycles; additions 104 -> 129).
 template <class C>
-__device__ __forceinline__ void weigh(Row<C>& r, const Scores<C>& x, float mscale, Weights<C>& out) {
+__device__ __forceinline__ void weigh(Row<C>& r, Scores<C>& x, float mscale, Weights<C>& out) {
   // a row that has seen nothing yet: every weight 2^(-inf) = 0
-  const float mc = r.m == -INFINITY ? 0.f : r.m * mscale;
-  float sum[4] = {};
+  const float m = r.m == -INFINITY ? 0.f : r.m;
+  float mc = m * mscale, sum[4] = {};
+  if (__builtin_expect(r.far, 0)) {
+#pragma unroll
+    for (int ch = 0; ch < C::CH; ++ch)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x.s[ch][i] -= m;
+    mc = 0.f;
+  }
 #pragma unroll
   for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
@@ -367,9 +384,9 @@ struct Copies {
     for (int j = 0; j < C::N; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (BBH_LDS void*)(to + j * 512), 16, (int)voff[j], 0, 0, 0);
   }
-  // Zeros over this wavefront's part of a stage's V where the key is masked: a weight of 0 times
-  // what a masked key holds is not always 0.
-  __device__ __forceinline__ void clear_masked(lds_f16* stage, uint64_t bits, int lane) {
+  // Zeros over this wavefront's part of a stage's V where no row of the workgroup sees the key: a
+  // weight of 0 times what such a key holds is not always 0.
+  __device__ __forceinline__ void clear_unseen(lds_f16* stage, uint64_t bits, int lane) {
     lds_f16* vs = stage + C::SK * C::HD;
 #pragma unroll
     for (int j = 0; j < C::N; ++j) {
@@ -494,18 +511,21 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
     copies.issue_v(p, vbase + (int64_t)k0 * (int)p.vs.row, valid, ring + stage * C::STAGE);
   };
   constexpr uint64_t kAll = SK == 64 ? ~0ull : 0xffffffffull;
-  // Unmasked keys of a tile that is in place.
-  auto bits_of = [&](int i, int stage) -> uint64_t {
-    if (!mrow) {
-      const int n = nk - key_at(i);
-      return n >= SK ? kAll : (1ull << n) - 1;
-    }
-    return __ballot(masks[stage * 64 + lane] != 0) & kAll;
+  // Keys of a tile that is in place: those there are, and of them those that some row of the
+  // workgroup may see.
+  auto below = [](int n) -> uint64_t { return n <= 0 ? 0 : n >= SK ? kAll : (1ull << n) - 1; };
+  auto bits_of = [&](int k0, int stage, uint64_t& live) -> uint64_t {
+    live = below(nk - k0);
+    uint64_t bits = live;
+    if (k0 < wlo || k0 + SK > whi) bits &= (below(whi - k0) & ~below(wlo - k0)) | below(prefix - k0);
+    if (mrow) bits &= __ballot(masks[stage * 64 + lane] != 0);
+    return bits;
   };
 #pragma unroll
   for (int d = 0; d < ND; ++d) r.o[d] = f32x16{};
   r.m = -INFINITY;
   r.l = 0.f;
+  r.far = false;
   const float mscale = FEAT == kPlain ? p.c : FEAT == kCap || p.cap_l > 0.f ? 2.f * p.cap_l : p.c;
   const float lag = kLazy / mscale;
   auto whole = [&](int k0, uint64_t bits) {
@@ -547,7 +567,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
       wait_vm<C::N>();
       asm volatile("" ::: "memory");
       const int k0 = key_at(it);
-      const uint64_t bits = bits_of(it, 0);
+      uint64_t live;
+      const uint64_t bits = bits_of(k0, 0, live);
       bool edge;
       const bool some = tile_scores(k0, bits, ring, edge);
       lds_done();
@@ -555,8 +576,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
       if (some) tile_weights(k0, edge);
       wait_vm<C::N>();
       asm volatile("" ::: "memory");
-      if (mrow && bits != kAll) {
-        copies.clear_masked(ring, bits, lane);
+      if (bits != live) {
+        copies.clear_unseen(ring, bits, lane);
         lds_done();
       }
       if (some) tile_output(ring + SK * HD);
@@ -579,10 +600,11 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
       copy_v(it + C::R - 1, next);
       next = next == C::R - 1 ? 0 : next + 1;
       const int k0 = key_at(it);
-      const uint64_t bits = bits_of(it, now);
+      uint64_t live;
+      const uint64_t bits = bits_of(k0, now, live);
       lds_f16* ks = ring + now * C::STAGE;
-      if (mrow && bits != kAll) {  // all of V is cleared before any of it is read
-        copies.clear_masked(ks, bits, lane);
+      if (bits != live) {  // all of V is cleared before any of it is read
+        copies.clear_unseen(ks, bits, lane);
         lds_barrier();
       }
       now = now == C::R - 1 ? 0 : now + 1;
@@ -760,10 +782,17 @@ int64_t table_bytes(const AttendParams& p) {
 
 template <class C, int FEAT>
 hipError_t launch_as(const AttendParams& p, int64_t grid, hipStream_t s) {
-  static const hipError_t attr =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(attend_kernel<C, FEAT>),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLdsMax);
-  if (attr != hipSuccess) return attr;
+  static std::atomic<uint64_t> set{0};  // a bit a device
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(set.load(std::memory_order_relaxed) & bit)) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(attend_kernel<C, FEAT>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLdsMax);
+    if (e != hipSuccess) return e;
+    set.fetch_or(bit, std::memory_order_relaxed);
+  }
   const size_t lds = C::LDS + (FEAT == kAny && p.table_lds ? table_bytes(p) : 0);
   hipLaunchKernelGGL((attend_kernel<C, FEAT>), dim3((unsigned)grid), dim3(C::THREADS), lds, s, p);
   return hipGetLastError();
@@ -821,7 +850,8 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
   const int64_t per = cols * p.kv_heads * C::THREADS;
   const int most = (int)std::min<int64_t>(p.batch, std::max<int64_t>(1, (kMostThreads / per) - 8));
   const int batch = p.batch;
-  for (p.b0 = 0; p.b0 < batch; p.b0 += most) {
+  for (int64_t b0 = 0; b0 < batch; b0 += most) {
+    p.b0 = (int)b0;
     p.batch = std::min(most, batch - p.b0);
     const int64_t rows = (int64_t)p.batch * p.kv_heads;
     const int64_t grid = rows >= kXcdRows ? (rows + kXcds - 1) / kXcds * cols * kXcds

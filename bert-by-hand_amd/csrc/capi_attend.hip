@@ -275,6 +275,9 @@ static bbh_status attend_params(const bbh_attend_args* a, bbh::AttendParams& p) 
     return fail(BBH_ERR_UNSUPPORTED, what, "k_len or q_len * heads / kv_heads above 2^28");
   if ((int64_t)a->batch * a->heads > INT_MAX)
     return fail(BBH_ERR_UNSUPPORTED, what, "batch * heads above 2^31 - 1");
+  // (a sequence's work-items fit a launch's 2^32)
+  if (a->heads > 65536 || (int64_t)a->q_len * a->heads > 1 << 30)
+    return fail(BBH_ERR_UNSUPPORTED, what, "more than 65536 heads, or q_len * heads above 2^30");
   // (so that biases divided by either keep their size)
   constexpr float kLeast = 0x1p-24f, kMost = 0x1p24f;
   if (!(a->scale >= kLeast && a->scale <= kMost))
@@ -355,11 +358,19 @@ bbh_status bbh_attend(const bbh_attend_args* a, bbh_stream_t stream) {
   if (!apart(out)) return invalid(what, "rows or heads of out overlap");
   for (const Region& r : in)
     if (overlap(out, r)) return invalid(what, "out overlaps an input");
-  if (a->scratch) {
-    const Region sc{a->scratch, 1, 0, 1, 0, 1, 0, (int64_t)(a->scratch_bytes / 2)};
-    if (overlap(sc, out) || overlap(sc, in[0]) || overlap(sc, in[1]) || overlap(sc, in[2]))
-      return invalid(what, "scratch overlaps an operand");
+  auto words = [](const void* data, int64_t n) { return Region{data, 1, 0, 1, 0, 1, 0, 2 * n}; };
+  const Region small[8] = {
+      words(a->q_offsets, (int64_t)a->batch + 1), words(a->k_offsets, (int64_t)a->batch + 1),
+      words(a->q_lengths, a->batch),              words(a->k_lengths, a->batch),
+      words(a->prefix, a->batch),                 words(a->mask, (int64_t)a->batch * a->k_len),
+      words(a->slopes, a->heads),                 words(a->table, a->heads * (2 * (int64_t)a->table_half + 1))};
+  const Region sc{a->scratch, 1, 0, 1, 0, 1, 0, (int64_t)(a->scratch_bytes / 2)};
+  for (const Region& r : small) {
+    if (overlap(out, r)) return invalid(what, "out overlaps an input");
+    if (overlap(sc, r)) return invalid(what, "scratch overlaps an operand");
   }
+  if (overlap(sc, out) || overlap(sc, in[0]) || overlap(sc, in[1]) || overlap(sc, in[2]))
+    return invalid(what, "scratch overlaps an operand");
   return done(bbh::attend(p, a->scratch, a->scratch ? a->scratch_bytes : 0,
                           static_cast<hipStream_t>(stream)),
               what);

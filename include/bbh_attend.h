@@ -119,17 +119,19 @@ bbh_status bbh_rope_heads(const bbh_rope *rope, const bbh_rope_args *args, bbh_s
  *    k_rows), at most q_len (k_len) of them, and at most q_lengths[b] where given.
  *    Offsets outside the rows are clamped to them.
  * q and k choose separately: packed new tokens over a padded cache, say.  Rows of out
- * behind a sequence's n_q are left as they were.  Keys behind n_k, and keys whose mask
- * is 0, have no effect whatever they hold; a key that is seen by another query only
- * must be finite (its weight here is 0, and 0 times infinity is not).
+ * behind a sequence's n_q are left as they were.  Keys that no query sees (behind n_k,
+ * with a mask of 0, outside of every window and the prefix) have no effect whatever they
+ * hold; a value that some query sees must be finite, or may reach the others (its weight
+ * there is 0, and 0 times infinity is not).
  *
  * Scores, softmax and sums are fp32; the weights are rounded to fp16 for the product
- * with v, the output once.  table entries are of magnitude up to
- * 1e30, lower ones count as some such value, or
- * -infinity (the pair is not seen).  Offsets, lengths, prefix, mask: int32, on the
- * device; slopes and table: fp32.  head_dim is a multiple of 8 up to
- * BBH_ATTEND_MAX_DIM; addresses of q, k, v and out are multiples of 16 bytes, their
- * strides of 8 elements, row strides below 2^23.
+ * with v, the output once.  Offsets, lengths, prefix, mask: int32, on the device.  slopes
+ * and table: fp32, on the device, finite and at most 1e20 and 1e30 in magnitude.  A table
+ * may also hold -infinity (the pair is not seen) and any lower finite value, the type's
+ * lowest say, which counts as about -1e38 or, divided by scale, that.  head_dim is a
+ * multiple of 8 up to BBH_ATTEND_MAX_DIM; heads at most 65536, q_len * heads 2^30;
+ * addresses of q, k, v and out are multiples of 16 bytes, their strides of 8 elements, row
+ * strides below 2^23.  out and scratch overlap nothing.
  *
  * scratch (optional, 16-byte aligned): with it, calls with few rows spread the keys over
  * more workgroups and join their results; bbh_attend_scratch gives the bytes that it

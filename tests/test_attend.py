@@ -420,6 +420,8 @@ def test_rope_norm_of_zeros_and_large_values(torch_cuda):
 def _attend64(torch, q, k, v, nq, nk, left=-1, right=-1, scale=None, cap=0.0, mask=None, prefix=0,
               slopes=None, table=None):
     """One sequence (its first nq queries, nk keys) in 64 bits, and what a result may be off by."""
+    if nk == 0 or nq == 0:
+        return q[:nq].double() * 0, q[:nq].double() * 0
     q, k, v = q[:nq].double(), k[:nk].double(), v[:nk].double()
     h, d = q.shape[1:]
     rep = h // k.shape[1]
@@ -514,3 +516,612 @@ def test_attend(torch_cuda, batch, q_len, k_len, heads, kv, dim, form):
         for b in range(batch):
             _check(torch, out[b], q[b], k[b], v[b], q_len, k_len, mask=None if mask is None else mask[b],
                    prefix=0 if prefix is None else min(int(prefix[b]), k_len), **kw)
+
+
+SETS = [  # every set of kernels: batch, q_len, k_len, heads, kv_heads
+    (3, 9, 9, 2, 2), (2, 11, 150, 2, 1), (2, 60, 60, 2, 2), (1, 140, 140, 3, 3), (1, 1100, 1100, 1, 1),
+    (1, 2, 700, 4, 2), (2, 1, 70000, 4, 2), (1, 300, 5000, 8, 4),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dim", [24, 32, 64, 80, 96, 128, 136, 256])
+@pytest.mark.parametrize("form", ["plain", "cap", "any"])
+@pytest.mark.parametrize("batch,q_len,k_len,heads,kv", SETS)
+def test_attend_every_set(torch_cuda, batch, q_len, k_len, heads, kv, form, dim):
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, q_len + k_len + dim)
+    q = _normal(torch, g, batch, q_len, heads, dim)
+    k, v = _normal(torch, g, batch, k_len, kv, dim), _normal(torch, g, batch, k_len, kv, dim)
+    kw, mask, prefix = dict(right=0), None, None
+    if form == "cap":
+        kw["cap"] = 8.0
+    elif form == "any":
+        mask = (torch.rand(batch, k_len, device="cuda", generator=g) < 0.8).int()
+        prefix = torch.full((batch,), 70, device="cuda", dtype=torch.int32)
+        kw.update(left=200, right=3, cap=8.0, slopes=0.02 * torch.rand(heads, device="cuda", generator=g),
+                  table=torch.randn(heads, 201, device="cuda", generator=g))
+    out = torch.full_like(q, float("nan"))
+    scratch = torch.empty(max(engine.attend_scratch(q, k, v, out, mask=mask, prefix=prefix, **kw), 16),
+                          dtype=torch.uint8, device="cuda")
+    engine.launch_attend(q, k, v, out, mask=mask, prefix=prefix, scratch=scratch, **kw)
+    torch.cuda.synchronize()
+    for b in range(batch):
+        _check(torch, out[b], q[b], k[b], v[b], q_len, k_len, mask=None if mask is None else mask[b],
+               prefix=0 if prefix is None else min(70, k_len), **kw)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens", [[5, 0, 1, 70, 33, 64, 128, 3], [200] * 3 + [0] * 70 + [1], [0, 0], [7] * 300,
+                                  [1, 900, 2]])
+def test_packed_documents(torch_cuda, lens, dim):
+    """Out of fused rows with gaps between the documents, bounded by q_len: each as alone, and
+    every row of no document left as it was."""
+    from bbh import engine
+
+    torch = torch_cuda
+    heads, kv, gap = 6, 2, 2
+    starts = np.cumsum([0] + [n for n in lens])
+    rows = int(starts[-1]) + gap + 3
+    g = _gen(torch, rows)
+    qkv = _normal(torch, g, rows, heads + 2 * kv, dim)
+    q, k, v = qkv.split((heads, kv, kv), dim=1)
+    offsets = torch.tensor(starts + gap, device="cuda", dtype=torch.int32)  # two rows before the first
+    slopes = torch.rand(heads, device="cuda", generator=g)
+    most = max(max(lens) - 10, 1)  # the longest lose their last ten
+    for kw in (dict(), dict(slopes=slopes, left=40, right=40), dict(right=0, cap=5.0)):
+        out = torch.full((rows, heads, dim), float("nan"), device="cuda").half()
+        engine.launch_attend(q, k, v, out, q_offsets=offsets, k_offsets=offsets, q_len=most, k_len=most, **kw)
+        torch.cuda.synchronize()
+        left = torch.ones(rows, dtype=torch.bool, device="cuda")
+        for n, s in zip(lens, starts):
+            n, at = min(n, most), int(s) + gap
+            if n:
+                _check(torch, out[at:at + n], q[at:], k[at:], v[at:], n, n, **kw)
+                left[at:at + n] = False
+        assert bool(out[left].isnan().all())
+
+
+@gpu
+def test_offsets_outside_the_rows_are_clamped(torch_cuda):
+    """Offsets before, behind and out of order: nothing outside the tensors is read or written."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, 3)
+    q, k, v = (_normal(torch, g, 50, 2, 64) for _ in range(3))
+    out = torch.full_like(q, float("nan"))
+    offsets = torch.tensor([-7, 10, 4, 30, 2147483647, -2147483648, 45, 60], device="cuda", dtype=torch.int32)
+    engine.launch_attend(q, k, v, out, q_offsets=offsets, k_offsets=offsets, q_len=50, k_len=50)
+    torch.cuda.synchronize()
+    # [0, 10), [10, 4) none, [4, 30), [30, 50), none, [0, 45) and [45, 50): later ones overlap
+    # earlier ones here, so each row holds one of its sequences' results
+    assert not bool(out.isnan().any())
+    a, _ = _attend64(torch, q[45:], k[45:], v[45:], 5, 5)
+    b, _ = _attend64(torch, q[30:], k[30:], v[30:], 20, 20)
+    d = torch.minimum((out[45:].double() - a).abs(), (out[45:].double() - b[15:]).abs())
+    assert float(d.max()) < 4e-3
+
+
+@gpu
+@pytest.mark.parametrize("q_len,lens", [(1, [1, 700, 64, 0, 333]), (4, [4, 1000, 65, 17, 2]), (70, [70, 71, 500, 64, 0])])
+def test_cache_of_ragged_lengths(torch_cuda, q_len, lens):
+    """Padded and packed queries over a padded cache whose rows behind each length hold NaN and
+    infinities; a sequence with fewer keys than queries, and one with none."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g, heads, kv, dim, cap = _gen(torch, q_len), 8, 4, 128, 1024
+    n = len(lens)
+    q = _normal(torch, g, n, q_len, heads, dim)
+    k, v = _normal(torch, g, n, cap, kv, dim), _normal(torch, g, n, cap, kv, dim)
+    for b, m in enumerate(lens):
+        k[b, m:] = float("nan")
+        v[b, m:] = float("inf")
+    kl = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    ql = torch.tensor([q_len, q_len, max(q_len - 1, 0), q_len, q_len], device="cuda", dtype=torch.int32)
+    scratch = torch.empty(1 << 22, device="cuda")
+    for sc in (None, scratch):
+        out = torch.full_like(q, float("nan"))
+        engine.launch_attend(q, k, v, out, k_lengths=kl, q_lengths=ql, right=0, scratch=sc)
+        torch.cuda.synchronize()
+        for b, m in enumerate(lens):
+            nq = int(ql[b])
+            _check(torch, out[b], q[b], k[b], v[b], nq, m, right=0)
+            assert bool(out[b, nq:].isnan().all())
+    # the same queries packed end to end
+    packed = torch.cat([q[b, :int(ql[b])] for b in range(n)])
+    offsets = torch.cat([torch.zeros(1, device="cuda"), ql.cumsum(0)]).int()
+    po = torch.full_like(packed, float("nan"))
+    engine.launch_attend(packed, k, v, po, q_offsets=offsets, q_len=q_len, k_lengths=kl, right=0)
+    torch.cuda.synchronize()
+    for b, m in enumerate(lens):
+        a, e = int(offsets[b]), int(offsets[b + 1])
+        _check(torch, po[a:e], q[b], k[b], v[b], e - a, m, right=0)
+
+
+@gpu
+@pytest.mark.parametrize("q_len,k_len", [(1, 300), (30, 30), (200, 200)])
+def test_masked_keys_have_no_effect_whatever_they_hold(torch_cuda, q_len, k_len):
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, k_len)
+    q = _normal(torch, g, 2, q_len, 4, 64)
+    k, v = _normal(torch, g, 2, k_len, 4, 64), _normal(torch, g, 2, k_len, 4, 64)
+    mask = (torch.rand(2, k_len, device="cuda", generator=g) < 0.7).int()
+    clean = torch.empty_like(q)
+    engine.launch_attend(q, k, v, clean, mask=mask)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        k2, v2 = (torch.where((mask == 0)[..., None, None], bad, t.float()).half() for t in (k, v))
+        out = torch.empty_like(q)
+        engine.launch_attend(q, k2, v2, out, mask=mask)
+        torch.cuda.synchronize()
+        assert torch.equal(out, clean)
+    # a NaN in a key that is seen reaches the rows that see it, and no others
+    k[0, 3, 1] = float("nan")
+    mask[0, 3] = 1
+    engine.launch_attend(q, k, v, out, mask=mask, right=0)
+    torch.cuda.synchronize()
+    bad = out.isnan().all(-1)
+    first = max(3 - (k_len - q_len), 0)
+    assert bool(bad[0, first:, 1].all()) and int(out.isnan().any(-1).sum()) == q_len - first
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_len,k_len,left,right,prefix", [
+    (1, 300, 100, 0, 0), (1, 1000, 7, 0, 5), (3, 1000, 50, 0, 33), (10, 90, 11, -1, 0), (70, 500, 100, 0, 40),
+    (200, 400, 13, 2, 70), (64, 64, -1, 0, 0), (300, 2000, 64, 64, 0)])
+def test_keys_that_no_query_sees_have_no_effect(torch_cuda, q_len, k_len, left, right, prefix, dim):
+    """Behind the windows of all queries, as in a cache whose oldest slots were given away."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, k_len)
+    q = _normal(torch, g, 1, q_len, 4, dim)
+    k, v = _normal(torch, g, 1, k_len, 2, dim), _normal(torch, g, 1, k_len, 2, dim)
+    unseen = torch.arange(k_len, device="cuda")
+    unseen = (unseen >= prefix) & ((left >= 0) & (unseen < k_len - q_len - left))
+    pf = torch.tensor([prefix], device="cuda", dtype=torch.int32)
+    for scratch in (None, torch.empty(1 << 20, device="cuda")):
+        clean = torch.empty_like(q)
+        engine.launch_attend(q, k, v, clean, left=left, right=right, prefix=pf, scratch=scratch)
+        torch.cuda.synchronize()
+        _check(torch, clean[0], q[0], k[0], v[0], q_len, k_len, left=left, right=right, prefix=prefix)
+        for bad in (float("nan"), float("inf")):
+            k2, v2 = (torch.where(unseen[None, :, None, None], bad, t.float()).half() for t in (k, v))
+            out = torch.empty_like(q)
+            engine.launch_attend(q, k2, v2, out, left=left, right=right, prefix=pf, scratch=scratch)
+            torch.cuda.synchronize()
+            assert torch.equal(out, clean)
+
+
+@gpu
+@pytest.mark.parametrize("half,heads,kv", [(0, 4, 4), (1, 4, 1), (63, 6, 2), (500, 8, 1), (3000, 4, 2), (9000, 2, 2)])
+def test_tables(torch_cuda, half, heads, kv):
+    """Short tables and ones too long for LDS; entries of -infinity hide pairs, the type's lowest
+    value does not (a row of nothing else is an average)."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, half)
+    n, dim = 333, 64
+    q = _normal(torch, g, 1, n, heads, dim)
+    k, v = _normal(torch, g, 1, n, kv, dim), _normal(torch, g, 1, n, kv, dim)
+    table = torch.randn(heads, 2 * half + 1, device="cuda", generator=g)
+    table[torch.rand(table.shape, device="cuda", generator=g) < 0.2] = -float("inf")
+    for kw in (dict(), dict(cap=4.0), dict(left=50, right=70)):
+        out = torch.full_like(q, float("nan"))
+        engine.launch_attend(q, k, v, out, table=table, **kw)
+        torch.cuda.synchronize()
+        _check(torch, out[0], q[0], k[0], v[0], n, n, table=table, **kw)
+    lowest = torch.full_like(table, torch.finfo(torch.float32).min)
+    mean = v[0].double().mean(0).repeat_interleave(heads // kv, 0)
+    for kw in (dict(), dict(scale=2.0 ** -24), dict(scale=1.0), dict(scale=9.0), dict(cap=50.0),
+               dict(cap=2.0 ** -24), dict(cap=2.0 ** 24)):
+        engine.launch_attend(q, k, v, out, table=lowest, **kw)
+        torch.cuda.synchronize()
+        assert float((out[0].double() - mean).abs().max()) <= 4 * H, kw
+    table.fill_(-float("inf"))
+    engine.launch_attend(q, k, v, out, table=table)
+    torch.cuda.synchronize()
+    assert bool((out == 0).all())
+
+
+@gpu
+def test_attend_other_layouts(torch_cuda):
+    """Heads before rows, gaps between rows and sequences, keys shared by all (stride 0): the bits
+    of contiguous operands."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, 1)
+    b, n, h, kv, d = 3, 77, 6, 3, 64
+    q, k, v = _normal(torch, g, b, n, h, d), _normal(torch, g, b, n, kv, d), _normal(torch, g, b, n, kv, d)
+    want = torch.empty_like(q)
+    engine.launch_attend(q, k, v, want, left=30)
+
+    def head_major(t):
+        return t.transpose(1, 2).contiguous().transpose(1, 2)
+
+    def spread(t):
+        room = torch.full((t.shape[0] + 1, t.shape[1] + 5, t.shape[2] + 2, d + 8), float("nan"),
+                          device="cuda").half()
+        part = room[:t.shape[0], 2:2 + t.shape[1], 1:1 + t.shape[2], :d]
+        part.copy_(t)
+        return part, room
+
+    out = head_major(torch.empty_like(q))
+    engine.launch_attend(head_major(q), head_major(k), head_major(v), out, left=30)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    out, room = spread(torch.full_like(q, float("nan")))
+    engine.launch_attend(spread(q)[0], spread(k)[0], spread(v)[0], out, left=30)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and int((~room.isnan()).sum()) == q.numel()
+    one = k[:1].expand(b, -1, -1, -1)
+    got, same = torch.empty_like(q), torch.empty_like(q)
+    engine.launch_attend(q, one, v, got, left=30)
+    engine.launch_attend(q, one.contiguous(), v, same, left=30)
+    torch.cuda.synchronize()
+    assert torch.equal(got, same)
+
+
+@gpu
+def test_attend_no_keys(torch_cuda):
+    from bbh import engine
+
+    torch = torch_cuda
+    q = torch.randn(2, 5, 4, 64, device="cuda").half()
+    out = torch.full_like(q, float("nan"))
+    none = torch.empty(2, 0, 4, 64, device="cuda").half()
+    engine.launch_attend(q, none, none, out)
+    torch.cuda.synchronize()
+    assert bool((out == 0).all())
+    engine.launch_attend(q[:, :0], q, q, out[:, :0])
+    engine.launch_attend(q[:0], q[:0], q[:0], out[:0])
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_offsets_past_32_bits(torch_cuda):
+    """A cache of more than 2^31 elements, and its slots filled behind them."""
+    from bbh import engine
+
+    torch = torch_cuda
+    keys, kv, dim, heads = 1060000, 16, 128, 16
+    g = _gen(torch, 9)
+    k = torch.empty(1, keys, kv, dim, device="cuda", dtype=torch.float16)
+    v = torch.empty_like(k)
+    assert k.numel() > 2 ** 31
+    for t in (k, v):
+        for i in range(0, keys, 53000):
+            t[0, i:i + 53000] = torch.randn((53000, kv, dim), device="cuda", generator=g, dtype=torch.float16)
+    # the last three slots are written by launch_rope
+    rope = engine.Rope(dim)
+    nk, nv = _normal(torch, g, 3, kv, dim), _normal(torch, g, 3, kv, dim)
+    nq = _normal(torch, g, 3, heads, dim)
+    slots = torch.arange(keys - 3, keys, device="cuda")
+    pos = slots.int()
+    q = torch.empty_like(nq)
+    engine.launch_rope(rope, nq, q, k=nk, k_out=k[0], v=nv, v_out=v[0], kv_rows=slots, positions=pos)
+    torch.cuda.synchronize()
+    want, tol = _rope64(torch, nk, pos, _frequencies64(dim, 10000.0), False, 1.0, None, 0)
+    assert bool(((k[0, -3:].double() - want).abs() <= tol).all()) and torch.equal(v[0, -3:], nv)
+    # a window at the far end, and the whole cache
+    q, out = q[None], torch.empty_like(q)[None]
+    scratch = torch.empty(1 << 24, device="cuda")
+    for left, sc in ((500, None), (500, scratch), (-1, scratch)):
+        engine.launch_attend(q, k, v, out, left=left, right=0, scratch=sc)
+        torch.cuda.synchronize()
+        for h in (0, 15):
+            n = keys if left < 0 else 600
+            w, t = _attend64(torch, q[0, :, h:h + 1], k[0, -n:, h:h + 1], v[0, -n:, h:h + 1], 3, n, left=left,
+                             right=0)
+            d = (out[0, :, h:h + 1].double() - w).abs()
+            # (over the whole cache the bound's share for weights below 2^-14 is larger than a value)
+            assert bool((d <= (t if left >= 0 else 5e-4)).all()), (left, h, float(d.max()))
+
+
+@gpu
+def test_rope_past_32_bits(torch_cuda):
+    from bbh import engine
+
+    torch = torch_cuda
+    rows, heads, dim = 2 ** 18 + 3, 64, 128
+    x = torch.empty(rows, heads, dim, device="cuda", dtype=torch.float16)
+    assert x.numel() > 2 ** 31
+    for i in range(0, rows, 1 << 16):
+        x[i:i + (1 << 16)] = torch.randn(x[i:i + (1 << 16)].shape, device="cuda", dtype=torch.float16)
+    y = torch.empty_like(x)
+    rope = engine.Rope(dim)
+    engine.launch_rope(rope, x, y, seq=2 ** 30)
+    torch.cuda.synchronize()
+    for part in (slice(0, 5), slice(rows - 70, rows)):
+        pos = torch.arange(rows, device="cuda")[part]
+        want, tol = _rope64(torch, x[part], pos, _frequencies64(dim, 10000.0), False, 1.0, None, 0)
+        assert bool(((y[part].double() - want).abs() <= tol).all())
+
+
+@gpu
+def test_many_workgroups(torch_cuda):
+    """More sequences than one launch counts threads for would need: 2^21 of one token."""
+    from bbh import engine
+
+    torch = torch_cuda
+    n, heads = 1 << 21, 40
+    v = torch.randn(n, 1, heads, 8, device="cuda").half()
+    out = torch.full_like(v, float("nan"))
+    engine.launch_attend(v, v, v, out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, v)  # one key: its value
+
+
+@gpu
+def test_a_block_of_a_model(torch_cuda):
+    """As a decoder-style embedding model uses them: the QKV Linear, norms and rotation with keys
+    and values put into a cache, causal attention over it; a prompt at once, and the same
+    tokens in pieces, down to one at a time, which see the same keys."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, 21)
+    heads, kv, dim, hidden, n = 8, 2, 64, 512, 150
+    width = (heads + 2 * kv) * dim
+    x = _normal(torch, g, n, hidden)
+    w = (torch.randn(width, hidden, device="cuda", generator=g) * hidden ** -0.5).half()
+    bias = (0.1 * torch.randn(width, device="cuda", generator=g)).half()
+    gq, gk = ((0.5 + torch.rand(dim, device="cuda", generator=g)).half() for _ in range(2))
+    rope = engine.Rope(dim, 10000.0, scaling="bands", factor=8.0, original=64.0, low=1.0, high=4.0)
+    freq = _frequencies64(dim, 10000.0, "bands", 8.0, 64.0, 1.0, 4.0)
+    cache = [torch.full((1, 256, kv, dim), float("nan"), device="cuda").half() for _ in range(2)]
+    scratch = torch.empty(1 << 20, device="cuda")
+
+    def step(first, last):
+        m = last - first
+        qkv = torch.empty(m, heads + 2 * kv, dim, device="cuda", dtype=torch.float16)
+        engine.launch_matmul(x[first:last], w, qkv, m, width, hidden, bias=bias)
+        q, k, v = qkv.split((heads, kv, kv), dim=1)
+        slots = torch.arange(first, last, device="cuda")
+        qr = torch.empty(m, heads, dim, device="cuda", dtype=torch.float16)
+        engine.launch_rope(rope, q, qr, k=k, k_out=cache[0][0], v=v, v_out=cache[1][0], kv_rows=slots,
+                           positions=slots.int(), q_gamma=gq, k_gamma=gk)
+        out = torch.full_like(qr, float("nan"))
+        length = torch.tensor([last], device="cuda", dtype=torch.int32)
+        engine.launch_attend(qr[None], *cache, out[None], k_lengths=length, right=0, scratch=scratch)
+        return qkv, qr, out
+
+    qkv, qr, out = step(0, n)
+    torch.cuda.synchronize()
+    pos = torch.arange(n, device="cuda")
+    for got, raw, gamma in ((qr, qkv[:, :heads], gq), (cache[0][0, :n], qkv[:, heads:heads + kv], gk)):
+        want, tol = _rope64(torch, raw, pos, freq, False, 1.0, gamma, 1e-6)
+        assert bool(((got.double() - want).abs() <= tol).all())
+    assert torch.equal(cache[1][0, :n], qkv[:, heads + kv:])
+    _check(torch, out, qr, cache[0][0], cache[1][0], n, n, right=0)
+    whole = out.clone()
+    for t in cache:
+        t.fill_(float("nan"))
+    parts = torch.cat([step(a, b)[2] for a, b in ((0, 64), (64, 65), (65, 100), (100, 101), (101, 149), (149, 150))])
+    torch.cuda.synchronize()
+    # the Linear's rows do not depend on how many there are; attention's order of sums does
+    assert float((parts.float() - whole.float()).abs().max()) <= 8 * H * float(whole.abs().max())
+
+
+@gpu
+def test_attend_captured_and_replayed_beside_eager_work(torch_cuda):
+    """Two graphs with scratch of their own replayed on two streams, eager calls between the
+    replays: every replay the eager bits of the same inputs."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, 4)
+    rope = engine.Rope(128)
+    k, v = _normal(torch, g, 2, 9000, 4, 128), _normal(torch, g, 2, 9000, 4, 128)
+    slopes = torch.rand(8, device="cuda", generator=g)
+
+    def state():
+        x = _normal(torch, g, 2, 8, 128)
+        return dict(x=x, q=torch.empty_like(x), out=torch.empty_like(x)[:, None],
+                    scratch=torch.empty(1 << 22, device="cuda"))
+
+    def call(s):
+        engine.launch_rope(rope, s["x"], s["q"], seq=7)
+        engine.launch_attend(s["q"][:, None], k, v, s["out"], right=0, slopes=slopes, scratch=s["scratch"])
+
+    states = [state(), state()]
+    graphs = []
+    for s in states:
+        call(s)  # (first launches outside of the capture; the next test has them inside)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            call(s)
+        graphs.append(gr)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(4):
+        want = []
+        for s in states:
+            s["x"].copy_(_normal(torch, g, 2, 8, 128))
+            call(s)
+            want.append(s["out"].clone())
+            s["out"].fill_(float("nan"))
+        torch.cuda.synchronize()
+        for st, gr in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                gr.replay()
+        eager = state()
+        call(eager)
+        torch.cuda.synchronize()
+        for s, w in zip(states, want):
+            assert torch.equal(s["out"], w), i
+        _check(torch, eager["out"][0], eager["q"][:1], k[0], v[0], 1, 9000, right=0, slopes=slopes)
+
+
+@gpu
+def test_captured_before_any_eager_call(torch_cuda):
+    """A process whose first launches (of kernels with more than 64 KB of LDS too) are captured."""
+    import subprocess
+    import sys
+
+    code = """
+import torch, sys
+sys.path.insert(0, %r)
+from bbh import engine
+rope = engine.Rope(128)
+x = torch.randn(1, 2000, 4, 128, device="cuda").half()
+q, out, out2 = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+s = torch.empty(1 << 22, device="cuda")
+one = torch.empty(1, 1, 4, 128, device="cuda").half()
+def call(o):
+    engine.launch_rope(rope, x[0], q[0], seq=2000)
+    engine.launch_attend(q, x, x, o, right=0)
+    engine.launch_attend(q[:, :1], x, x, one, cap=3.0, scratch=s)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    call(out)
+for i in range(3):
+    x.copy_(torch.randn_like(x)); g.replay(); torch.cuda.synchronize()
+    first = one.clone(); call(out2); torch.cuda.synchronize()
+    assert torch.equal(out, out2) and torch.equal(first, one), i
+print("captured")
+""" % os.path.join(ROOT, "bert-by-hand_amd")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+@gpu
+def test_on_a_stream_of_the_caller(torch_cuda):
+    from bbh import engine
+
+    torch = torch_cuda
+    x = torch.randn(1, 300, 4, 64, device="cuda").half()
+    a, b = torch.empty_like(x), torch.empty_like(x)
+    rope = engine.Rope(64)
+    y = torch.empty_like(x)
+    engine.launch_rope(rope, x[0], y[0], seq=300)
+    engine.launch_attend(y, x, x, a)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    y.zero_()
+    torch.cuda.synchronize()
+    engine.launch_rope(rope, x[0], y[0], seq=300, stream=st.cuda_stream)
+    engine.launch_attend(y, x, x, b, stream=st.cuda_stream)
+    st.synchronize()
+    assert torch.equal(a, b)
+
+
+@gpu
+def test_python_checks(torch_cuda):
+    from bbh import engine
+
+    torch = torch_cuda
+    rope = engine.Rope(64)
+    x = torch.randn(10, 4, 64, device="cuda").half()
+    y = torch.empty_like(x)
+    pos = torch.arange(10, device="cuda", dtype=torch.int32)
+    for error, kw in [
+        (TypeError, dict(q=x.float())), (TypeError, dict(q=x[0])), (TypeError, dict(q_out=y.cpu())),
+        (ValueError, dict(q=x.transpose(1, 2).contiguous().transpose(1, 2))),
+        (ValueError, dict(q_out=y[:9])), (ValueError, dict(positions=None)),
+        (ValueError, dict(positions=pos[:9])), (TypeError, dict(positions=pos.long())),
+        (ValueError, dict(k=x[:9], k_out=y[:9])), (ValueError, dict(k=x, k_out=y[:, :2])),
+        (ValueError, dict(v=x)), (ValueError, dict(k_out=y)), (ValueError, dict(k=x, kv_rows=pos.long())),
+        (TypeError, dict(k=x, k_out=y, kv_rows=pos)),
+        (ValueError, dict(k=x, k_out=y, v=x[:, :2], v_out=y[:, :2])),
+        (TypeError, dict(q_gamma=torch.ones(64, device="cuda"))),
+        (ValueError, dict(q_gamma=torch.ones(32, device="cuda").half())),
+        (engine.BBHError, dict(q_out=x[:, :, :], k=x, k_out=x)),
+    ]:
+        a = dict(q=x, q_out=y, positions=pos)
+        a.update(kw)
+        with pytest.raises(error):
+            engine.launch_rope(rope, **a)
+    q, k = torch.randn(2, 8, 4, 64, device="cuda").half(), torch.randn(2, 9, 2, 64, device="cuda").half()
+    i32 = torch.int32
+    for error, kw in [
+        (TypeError, dict(q=q.float())), (TypeError, dict(q=q[0])), (TypeError, dict(k=k.cpu())),
+        (ValueError, dict(k=k[:, :8])), (ValueError, dict(out=q[:, :7])), (ValueError, dict(v=k[:1], k=k[:1])),
+        (ValueError, dict(q_len=9)), (ValueError, dict(k_len=-1)), (ValueError, dict(q_len=2 ** 32 + 1)),
+        (ValueError, dict(left=2 ** 31)), (TypeError, dict(q_offsets=torch.zeros(3, device="cuda", dtype=i32))),
+        (ValueError, dict(q=q[0], out=q[1], q_offsets=torch.zeros(3, device="cuda", dtype=i32))),
+        (ValueError, dict(mask=torch.ones(2, 8, device="cuda", dtype=i32))),
+        (TypeError, dict(mask=torch.ones(2, 9, device="cuda"))),
+        (ValueError, dict(table=torch.ones(4, 6, device="cuda"))),
+        (ValueError, dict(table=torch.ones(2, 5, device="cuda"))),
+        (TypeError, dict(slopes=torch.ones(4, device="cuda").half())),
+        (ValueError, dict(slopes=torch.ones(3, device="cuda"))),
+        (ValueError, dict(k_lengths=torch.ones(1, device="cuda", dtype=i32))),
+        (TypeError, dict(scratch=torch.empty(64, 64, device="cuda").t()[:, 1:])),
+        (engine.BBHError, dict(out=q)), (engine.BBHError, dict(scale=0.0)),
+        (engine.BBHError, dict(q=q[..., :36], k=k[..., :36], v=k[..., :36], out=torch.empty_like(q)[..., :36])),
+    ]:
+        a = dict(q=q, k=k, v=k, out=torch.empty_like(q))
+        a.update(kw)
+        if "k" in kw and "v" not in kw:
+            a["v"] = k
+        with pytest.raises(error):
+            engine.launch_attend(**a)
+    # numpy's integers are sizes too
+    out = torch.empty_like(q)
+    engine.launch_attend(q, k, k, out, q_len=np.int64(8), left=np.int32(-1))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(heads=65544, kv_heads=8, batch=1, q_len=1), b"65536"),
+    (dict(heads=1024, kv_heads=1024, batch=1, q_len=1 << 21), b"2^30"),
+])
+def test_attend_refuses_more_than_a_launch_holds(change, message):
+    L, a = _lib(), _args(**change)
+    assert L.bbh_attend(ctypes.byref(a), None) == 7 and message in L.bbh_last_error()
+    assert L.bbh_attend_scratch(ctypes.byref(a)) == 0
+
+
+@pytest.mark.parametrize("name,n", [("q_offsets", 3), ("k_offsets", 3), ("q_lengths", 2), ("k_lengths", 2),
+                                    ("prefix", 2), ("mask", 100), ("slopes", 8), ("table", 40)])
+def test_attend_refuses_outputs_over_small_operands(name, n):
+    out, scratch = 4 * P, 7 * P
+    for where, message in ((out + 16, b"out overlaps"), (out - 4 * n + 4, b"out overlaps"),
+                           (scratch + 4092, b"scratch overlaps"), (scratch - 4 * n + 4, b"scratch overlaps")):
+        a = _args(scratch=scratch, scratch_bytes=4096, q_rows=80, k_rows=100, table_half=2, **{name: where})
+        assert _lib().bbh_attend(ctypes.byref(a), None) == 1, hex(where)
+        assert message in _lib().bbh_last_error(), _lib().bbh_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("dim,n", [(32, 9), (64, 70), (96, 130), (128, 300), (256, 600), (64, 1), (128, 2000)])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_scores_far_from_zero(torch_cuda, dim, n, slopes):
+    """Products of up to 2^38, next ones 2^21 apart: each row is the value of its largest, whether
+    they rise or fall along the keys, and of the mean of equal ones."""
+    from bbh import engine
+
+    torch = torch_cuda
+    q = torch.zeros(1, n, 4, dim, device="cuda").half()
+    k = torch.zeros(1, n, 2, dim, device="cuda").half()
+    v = torch.randint(-8, 9, k.shape, device="cuda").half()
+    q[..., 0] = 32768.0
+    step = torch.arange(1, n + 1, device="cuda") % 1000 * 64.0
+    sl = torch.full((4,), 0.5, device="cuda") if slopes else None  # (at most 1000 in all)
+    scratch = torch.empty(1 << 20, device="cuda")
+    for sign in (1, -1):
+        k[..., 0] = (sign * step).half()[None, :, None]
+        for q_len in (n, 1):
+            out = torch.empty_like(q[:, :q_len])
+            engine.launch_attend(q[:, :q_len], k, v, out, right=0, scale=1.0, slopes=sl, scratch=scratch)
+            torch.cuda.synchronize()
+            for i in range(0, q_len, 7):
+                top = int((sign * step[:n - q_len + i + 1]).argmax())
+                if (step[:n - q_len + i + 1] == step[top]).sum() == 1:
+                    assert torch.equal(out[0, i], v[0, top].repeat_interleave(2, 0)), (sign, q_len, i)
+    k[..., 0] = -65472.0
+    engine.launch_attend(q, k, v, q_out := torch.empty_like(q), scale=1.0)
+    torch.cuda.synchronize()
+    mean = v[0].double().mean(0).repeat_interleave(2, 0)
+    assert float((q_out[0].double() - mean).abs().max()) <= 8 * H  # one rounding of at most 8, fp32 sums
