@@ -43,8 +43,9 @@ struct Tile {
 constexpr float kLazy = 8.f;
 // A weight's exponent is fma(mscale, s, -(m mscale rounded)): one operation, and the product's
 // rounding error, the same in all of a row's weights, cancels with their sum.  With scores of 2^28
-// and more it would itself be far from 0 (a bias of the type's lowest value: 2^100), so that
-// above kFar the difference is taken first.
+// and more that error would itself be far from 0 (a bias of the type's lowest value: 2^100).  So a
+// wavefront that meets a maximum above kFar counts its rows' scores from there on from what their
+// maxima were (base), a subtraction a score, which only such wavefronts make.
 constexpr float kFar = 65536.f;
 constexpr int kMaxSplits = 256;  // a thread of the joining workgroup each
 
@@ -146,12 +147,11 @@ struct Row {
   int pos;
   int first, last;  // of the wavefront's rows: least and largest position
   float slope;
-  const float* tab;          // distance 0 of the head's table,
-  const BBH_LDS float* ltab;  // in LDS where it is there
-  float below, above;        // its ends
+  int tab;  // where distance 0 of the head's table is in LDS, or the head (a table in memory)
   f32x16 o[C::HD / 32];  // o[d][i]: dim 32 d + 8 (i / 4) + 4 (lane / 32) + i % 4
   float m, l;
-  bool far;  // some row's m * mscale is above kFar
+  float base;  // m and the scores are counted from here: 0, but where
+  bool far;    // some row's m came to lie above kFar
 };
 // A bias in the units of the scores.  Finite ones stay finite, in those units and as powers of two.
 __device__ __forceinline__ float bias_units(const AttendParams& p, float w) {
@@ -190,6 +190,11 @@ __device__ __forceinline__ void scores(const Row<C>& r, const lds_f16* __restric
 // end, where the bias is a constant, or all inside the padded table, where a lane reads eight
 // neighbouring values with no clamping.  Tables too long for that are read from memory.
 constexpr int kPad = 64;
+template <class C>
+__device__ __forceinline__ BBH_LDS float* table_area() {
+  HIP_DYNAMIC_SHARED(f16, smem);
+  return (BBH_LDS float*)((BBH_LDS char*)smem + C::LDS);
+}
 template <class C, int FEAT>
 __device__ __forceinline__ void shape(const AttendParams& p, const Row<C>& r, int k0, Scores<C>& x) {
   if constexpr (FEAT == kPlain) return;
@@ -215,19 +220,30 @@ __device__ __forceinline__ void shape(const AttendParams& p, const Row<C>& r, in
 #pragma unroll
       for (int ch = 0; ch < C::CH; ++ch) {
         const int kb = k0 + 32 * ch;
-        if (kb + 31 - r.first <= -p.half || kb - r.last >= p.half) {
-          const float w = kb < r.last ? r.below : r.above;
+        const bool past = kb + 31 - r.first <= -p.half || kb - r.last >= p.half;
+        const int end = kb < r.last ? -p.half : p.half;
+        if (p.table_lds) {
+          const BBH_LDS float* t = table_area<C>() + r.tab + (past ? end : kb + 8 * kh - r.pos);
+          if (past) {
+            const float w = *t;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x.s[ch][i] += w;
-        } else if (r.ltab) {
-          const BBH_LDS float* t = r.ltab + (kb + 8 * kh - r.pos);
+            for (int i = 0; i < 16; ++i) x.s[ch][i] += w;
+          } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x.s[ch][i] += t[16 * (i >> 3) + (i & 7)];
+            for (int i = 0; i < 16; ++i) x.s[ch][i] += t[16 * (i >> 3) + (i & 7)];
+          }
         } else {
+          const float* t = p.table + (int64_t)r.tab * (2 * p.half + 1) + p.half;
+          if (past) {
+            const float w = bias_units(p, t[end]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int d = kb + 8 * kh - r.pos + 16 * (i >> 3) + (i & 7);
-            x.s[ch][i] += bias_units(p, r.tab[min(max(d, -p.half), p.half)]);
+            for (int i = 0; i < 16; ++i) x.s[ch][i] += w;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int d = kb + 8 * kh - r.pos + 16 * (i >> 3) + (i & 7);
+              x.s[ch][i] += bias_units(p, t[min(max(d, -p.half), p.half)]);
+            }
           }
         }
       }
@@ -287,19 +303,26 @@ __device__ __forceinline__ float largest(const Scores<C>& x) {
 
 // Brings the running maximum up to a tile's, where that is far enough above it (kLazy).
 template <class C>
-__device__ __forceinline__ void raise(Row<C>& r, float mx, float lag, float mscale) {
+__device__ __forceinline__ void raise(Row<C>& r, Scores<C>& x, float mx, float lag, float mscale) {
   if (!__ballot(!(mx <= r.m + lag))) return;
   const float mn = imax(r.m, mx);
-  r.far = __ballot(mn != -INFINITY && fabsf(mn * mscale) > kFar) != 0;
-  if (!__ballot(r.m != -INFINITY)) {  // the first tile: nothing to bring along
-    r.m = mn;
-    return;
-  }
-  const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((r.m - mn) * mscale);
-  r.l *= corr;
+  if (__ballot(r.m != -INFINITY)) {  // (at the first tile there is nothing to bring along)
+    const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((r.m - mn) * mscale);
+    r.l *= corr;
 #pragma unroll
-  for (int d = 0; d < C::HD / 32; ++d) r.o[d] *= corr;
+    for (int d = 0; d < C::HD / 32; ++d) r.o[d] *= corr;
+  }
   r.m = mn;
+  if (__ballot(mn != -INFINITY && fabsf(mn * mscale) > kFar)) {
+    const float by = mn == -INFINITY ? 0.f : mn;
+    r.far = true;
+    r.base += by;
+    r.m -= by;
+#pragma unroll
+    for (int ch = 0; ch < C::CH; ++ch)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x.s[ch][i] -= by;
+  }
 }
 
 // Weights 2^(mscale (s - m)), rounded to fp16 (half of a step of an output's own type, and the
@@ -307,17 +330,10 @@ __device__ __forceinline__ void raise(Row<C>& r, float mx, float lag, float msca
 // It is added up with plain additions: a dot product of two does not run while the matrix unit is
 // busy (16 of them beside another wavefront's products 104 -> 230 cycles; additions 104 -> 129).
 template <class C>
-__device__ __forceinline__ void weigh(Row<C>& r, Scores<C>& x, float mscale, Weights<C>& out) {
+__device__ __forceinline__ void weigh(Row<C>& r, const Scores<C>& x, float mscale, Weights<C>& out) {
   // a row that has seen nothing yet: every weight 2^(-inf) = 0
-  const float m = r.m == -INFINITY ? 0.f : r.m;
-  float mc = m * mscale, sum[4] = {};
-  if (__builtin_expect(r.far, 0)) {
-#pragma unroll
-    for (int ch = 0; ch < C::CH; ++ch)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x.s[ch][i] -= m;
-    mc = 0.f;
-  }
+  const float mc = r.m == -INFINITY ? 0.f : r.m * mscale;
+  float sum[4] = {};
 #pragma unroll
   for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
@@ -451,21 +467,18 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
       r.first = query_of(p, min(w0, rows - 1)) + shift;
       r.last = query_of(p, min(w0 + 31, rows - 1)) + shift;
       r.slope = p.slopes ? p.slopes[h] * p.bias_scale : 0.f;
-      r.ltab = nullptr;
+      r.tab = h;
       if (p.table) {
-        r.tab = p.table + (int64_t)h * (2 * p.half + 1) + p.half;
-        r.below = bias_units(p, r.tab[-p.half]);
-        r.above = bias_units(p, r.tab[p.half]);
         if (p.table_lds) {
           const int len = 2 * p.half + 1 + 2 * kPad;
-          BBH_LDS float* t = (BBH_LDS float*)((BBH_LDS char*)smem + C::LDS);
+          BBH_LDS float* t = table_area<C>();
           for (int e = tid; e < p.group * len; e += C::THREADS) {
             const int g = e / len, d = e - g * len - kPad;
             t[e] = bias_units(p, p.table[(int64_t)(kvh * p.group + g) * (2 * p.half + 1) +
                                          min(max(d, 0), 2 * p.half)]);
           }
           __syncthreads();
-          r.ltab = t + (h - kvh * p.group) * len + kPad + p.half;
+          r.tab = (h - kvh * p.group) * len + kPad + p.half;
         }
       }
     }
@@ -514,17 +527,23 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   // Keys of a tile that is in place: those there are, and of them those that some row of the
   // workgroup may see.
   auto below = [](int n) -> uint64_t { return n <= 0 ? 0 : n >= SK ? kAll : (1ull << n) - 1; };
-  auto bits_of = [&](int k0, int stage, uint64_t& live) -> uint64_t {
-    live = below(nk - k0);
-    uint64_t bits = live;
-    if (k0 < wlo || k0 + SK > whi) bits &= (below(whi - k0) & ~below(wlo - k0)) | below(prefix - k0);
-    if (mrow) bits &= __ballot(masks[stage * 64 + lane] != 0);
+  // (one condition that is the same for all tiles: windows and prefixes often end with a tile)
+  const bool some_unseen = mrow || ((wlo | prefix) & (SK - 1)) || (whi < nk && (whi & (SK - 1)));
+  auto bits_of = [&](int k0, int stage, bool& unseen) -> uint64_t {
+    uint64_t bits = below(nk - k0);
+    unseen = false;
+    if (some_unseen) {
+      const uint64_t live = bits;
+      if (k0 < wlo || k0 + SK > whi) bits &= (below(whi - k0) & ~below(wlo - k0)) | below(prefix - k0);
+      if (mrow) bits &= __ballot(masks[stage * 64 + lane] != 0);
+      unseen = bits != live;
+    }
     return bits;
   };
 #pragma unroll
   for (int d = 0; d < ND; ++d) r.o[d] = f32x16{};
   r.m = -INFINITY;
-  r.l = 0.f;
+  r.l = r.base = 0.f;
   r.far = false;
   const float mscale = FEAT == kPlain ? p.c : FEAT == kCap || p.cap_l > 0.f ? 2.f * p.cap_l : p.c;
   const float lag = kLazy / mscale;
@@ -537,7 +556,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   Seen<C> see;
   // A tile's products, softmax and output; false where no row of the wavefront sees any of it.
   auto tile_scores = [&](int k0, uint64_t bits, const lds_f16* ks, bool& edge) {
-    edge = !whole(k0, bits);
+    edge = r.far || !whole(k0, bits);
     if (!bits || (edge && !seen_of(r, k0, bits, prefix, see))) return false;
     scores(r, ks, x);
     ahead<C::CH * NS, 1, kAheadK>();
@@ -545,8 +564,16 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   };
   auto tile_weights = [&](int k0, bool edge) {
     shape<C, FEAT>(p, r, k0, x);
-    if (edge) hide(see, x);
-    raise(r, largest(x), lag, mscale);
+    if (edge) {
+      hide(see, x);
+      if (r.far) {
+#pragma unroll
+        for (int ch = 0; ch < C::CH; ++ch)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x.s[ch][i] -= r.base;
+      }
+    }
+    raise(r, x, largest(x), lag, mscale);
     weigh(r, x, mscale, w);
   };
   auto tile_output = [&](const lds_f16* vs) {
@@ -567,8 +594,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
       wait_vm<C::N>();
       asm volatile("" ::: "memory");
       const int k0 = key_at(it);
-      uint64_t live;
-      const uint64_t bits = bits_of(k0, 0, live);
+      bool unseen;
+      const uint64_t bits = bits_of(k0, 0, unseen);
       bool edge;
       const bool some = tile_scores(k0, bits, ring, edge);
       lds_done();
@@ -576,7 +603,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
       if (some) tile_weights(k0, edge);
       wait_vm<C::N>();
       asm volatile("" ::: "memory");
-      if (bits != live) {
+      if (unseen) {
         copies.clear_unseen(ring, bits, lane);
         lds_done();
       }
@@ -600,10 +627,10 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
       copy_v(it + C::R - 1, next);
       next = next == C::R - 1 ? 0 : next + 1;
       const int k0 = key_at(it);
-      uint64_t live;
-      const uint64_t bits = bits_of(k0, now, live);
+      bool unseen;
+      const uint64_t bits = bits_of(k0, now, unseen);
       lds_f16* ks = ring + now * C::STAGE;
-      if (bits != live) {  // all of V is cleared before any of it is read
+      if (unseen) {  // all of V is cleared before any of it is read
         copies.clear_unseen(ks, bits, lane);
         lds_barrier();
       }
@@ -615,7 +642,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
     }
   }
   f32x16 (&o)[ND] = r.o;
-  const float m = r.m, l = xor32_sum(r.l);
+  const float m = r.m + r.base, l = xor32_sum(r.l);
 
   // ---- out
   const int cpr = p.dim / 8;

@@ -127,9 +127,9 @@ bbh_status bbh_rope_heads(const bbh_rope *rope, const bbh_rope_args *args, bbh_s
  * Scores, softmax and sums are fp32; the weights are rounded to fp16 for the product
  * with v, the output once.  Offsets, lengths, prefix, mask: int32, on the device.  slopes
  * and table: fp32, on the device, finite and at most 1e20 and 1e30 in magnitude.  A table
- * may also hold -infinity (the pair is not seen) and any lower finite value, the type's
- * lowest say, which counts as about -1e38 or, divided by scale, that.  head_dim is a
- * multiple of 8 up to BBH_ATTEND_MAX_DIM; heads at most 65536, q_len * heads 2^30;
+ * may also hold -infinity (the pair is not seen) and lower finite values, the type's
+ * lowest say, which count as some value below -1e30.  head_dim is a multiple of 8 up to
+ * BBH_ATTEND_MAX_DIM; heads at most 65536, q_len * heads 2^30;
  * addresses of q, k, v and out are multiples of 16 bytes, their strides of 8 elements, row
  * strides below 2^23.  out and scratch overlap nothing.
  *
