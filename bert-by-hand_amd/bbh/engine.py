@@ -654,6 +654,8 @@ def launch_rope(rope, q, q_out=None, k=None, k_out=None, v=None, v_out=None, pos
     without them; v moved along where v_out is given.  q_out and k_out default to q and k (in
     place).  kv_rows (rows) int64: the rows of k_out and v_out that k and v go to, as the
     slots of a cache; one outside them is not written (bbh_rope_heads)."""
+    if rope is not None and not rope.handle:
+        raise ValueError("rope is closed")
     torch = _torch()
     c = torch._C
     dev = c._cuda_getDevice() if q.is_cuda else -1

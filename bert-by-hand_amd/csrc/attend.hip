@@ -1,6 +1,34 @@
 // Attention for models other than MiniLM: any head size up to 256, shared
 // key/value heads, capped scores, a bias by distance, a window, a prefix, a key
 // mask, documents packed end to end, and few queries over a long cache.
+//
+// Mathematics.  One pass over the keys with a running maximum m, sum l and output o for each
+// row (a query of a head), in base 2: for each tile of keys
+//   s = q K^T,  w = 2^(mscale s - m),  l += sum w,  o += w V,
+// where o and l are rescaled only when m rises by more than kLazy.  A cap's tanh is 1 - 2 / (1 + e^2x):
+// the constant drops out of the softmax, and one exp2 and one reciprocal are left (shape()).
+//
+// Rows.  A wavefront has 32 rows: the heads that share a key/value head lie side by side in them
+// (row = query * group + head), so that a tile of K and V serves all of them, and one token of 8
+// heads fills 8 rows where a row a query would leave 31 empty.
+//
+// Layout.  Scores are computed as S^T = K Q^T (32x32x16): a lane then has 16 scores of ONE row,
+// the maximum takes one exchange between lanes, and the weights are, in the lane that computed them,
+// the operand of the second product O^T = V^T W^T, given that K's rows lie permuted in LDS
+// (key_of_row).  V^T comes from rows of V by transposed LDS reads.  K and V go to LDS by buffer
+// loads without passing registers; chunks of 16 bytes lie XORed by the row so that the reads of
+// both hit all banks evenly; rows behind the last key and values behind the head's size are past the
+// resource's end and become zeros.
+//
+// What bounds it (the cases as sequences x tokens x heads (key/value heads) x head size, fp16):
+//  8192 causal, 32 (8) x 128  540-560 us, 980-1020 TFLOP/s of the 1311 that a library product of
+//                             8192^3 reaches: matrix cores busy half of the time, vector units 41-46%
+//                             (exponentials first); one wavefront's softmax runs beside another's
+//                             products, at 1.65-1.7 GHz.
+//  4 x 4096, window of 1023, prefix, cap, 16 (4) x 256  469 us, 545 TFLOP/s: 32 rows of 256 values
+//                             leave one wavefront a SIMD, whose products and softmax take turns.
+//  64 tokens over caches of up to 8192, 32 (8) x 128  195 us, 4.6 TB/s of K and V.
+//  heads of 64 and short sequences: vector units (50-63% busy) and the fixed cost of a tile.
 #include <limits.h>
 
 #include <algorithm>

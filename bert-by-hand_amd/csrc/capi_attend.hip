@@ -3,6 +3,7 @@
 
 #include <limits.h>
 #include <math.h>
+#include <stdint.h>
 #include <string.h>
 
 #include <new>
@@ -50,9 +51,11 @@ struct Region {
   int64_t batch, batch_stride, rows, row, heads, head, dim;
   bool none() const { return !data || batch < 1 || rows < 1 || heads < 1; }
   uintptr_t begin() const { return (uintptr_t)data; }
+  // (as far as addresses go: sizes that no memory holds overlap what lies behind them)
   uintptr_t end() const {
-    return begin() + 2 * (uintptr_t)((batch - 1) * batch_stride + (rows - 1) * row +
-                                     (heads - 1) * head + dim);
+    const __int128 e = (__int128)begin() + 2 * ((__int128)(batch - 1) * batch_stride +
+                                                (__int128)(rows - 1) * row + (heads - 1) * head + dim);
+    return e > (__int128)UINTPTR_MAX ? UINTPTR_MAX : (uintptr_t)e;
   }
   int64_t width() const { return (heads - 1) * head + dim; }  // of a row
 };
@@ -79,14 +82,16 @@ bool apart(const Region& r) {
   if (r.none()) return true;
   if (r.heads > 1 && r.head < r.dim) return false;
   if (r.rows > 1 && r.row < r.dim) return false;
+  const __int128 column = (__int128)(r.rows - 1) * r.row + r.dim;
   if (r.rows > 1 && r.heads > 1) {
     // rows of heads, or heads of rows
-    if (r.row < r.width() && r.head < (r.rows - 1) * r.row + r.dim) return false;
+    if (r.row < r.width() && r.head < column) return false;
   }
   if (r.batch > 1) {
-    const int64_t one = (r.rows - 1) * r.row + (r.heads - 1) * r.head + r.dim;
+    const __int128 one = column + (r.heads - 1) * r.head;
     if (r.batch_stride < one &&
-        !(r.row > 0 && r.width() <= r.batch_stride && r.row >= (r.batch - 1) * r.batch_stride + r.width()))
+        !(r.row > 0 && r.width() <= r.batch_stride &&
+          r.row >= (__int128)(r.batch - 1) * r.batch_stride + r.width()))
       return false;
   }
   return true;
@@ -297,6 +302,8 @@ static bbh_status attend_params(const bbh_attend_args* a, bbh::AttendParams& p) 
   p.ks = heads(a->k);
   p.vs = heads(a->v);
   p.os = heads(a->out);
+  // (a row that is the only one has no stride that matters, and rows behind it have to be elsewhere)
+  if ((a->k_offsets ? a->k_rows : a->k_len) <= 1) p.ks.row = p.vs.row = a->head_dim;
   p.q_offsets = a->q_offsets;
   p.k_offsets = a->k_offsets;
   p.q_lengths = a->q_lengths;

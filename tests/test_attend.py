@@ -1125,3 +1125,56 @@ def test_scores_far_from_zero(torch_cuda, dim, n, slopes):
     torch.cuda.synchronize()
     mean = v[0].double().mean(0).repeat_interleave(2, 0)
     assert float((q_out[0].double() - mean).abs().max()) <= 8 * H  # one rounding of at most 8, fp32 sums
+
+
+@gpu
+def test_through_the_cpp_layer(torch_cuda, tmp_path):
+    """cpp/attend_check: the operators through bert_by_hand_attend.hpp."""
+    import subprocess
+
+    prog = os.path.join(ROOT, "bert-by-hand_amd", "cpp", "attend_check")
+    if not os.path.exists(prog):
+        pytest.fail(f"{prog} is not built (run __graft_entry__.build())")
+    r = subprocess.run([prog], cwd=str(tmp_path), capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout.count(" PASS") == 5, r.stdout + r.stderr
+
+
+def test_a_closed_rope_is_refused():
+    from bbh import engine
+
+    rope = engine.Rope(64)
+    rope.close()
+    with pytest.raises(ValueError, match="closed"):
+        engine.launch_rope(rope, None)
+
+
+def test_sizes_that_no_memory_holds_are_refused():
+    """Strides times sizes past 64 bits do not wrap into memory that seems apart."""
+    L = _lib()
+    for change in (dict(batch=1 << 24, out_batch=1 << 40), dict(batch=1 << 24, q_batch=1 << 40),
+                   dict(q_offsets=9 * P, q_rows=1 << 62), dict(k_offsets=9 * P, k_rows=1 << 60)):
+        assert L.bbh_attend(ctypes.byref(_args(**change)), None) == 1, change
+        assert b"overlap" in L.bbh_last_error(), L.bbh_last_error()
+    from bbh import engine
+
+    a = _rope_args(kv_rows=9 * P, kv_out_rows=1 << 40, k_out_data=8 * P, k_out_row=1 << 40)
+    assert L.bbh_rope_heads(engine.Rope(64).handle, ctypes.byref(a), None) == 1
+    assert b"overlap" in L.bbh_last_error(), L.bbh_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_one_key_of_any_value(torch_cuda, q_len):
+    """Its value, infinite or not, whatever the strides of a lone row."""
+    from bbh import engine
+
+    torch = torch_cuda
+    q = torch.randn(2, q_len, 4, 64, device="cuda").half()
+    k, v = torch.randn(2, 1, 4, 64, device="cuda").half(), torch.randn(2, 1, 4, 64, device="cuda").half()
+    v[0, 0, 1, 5], v[1, 0, 2, 9] = float("inf"), -float("inf")
+    for kk, vv in ((k, v), (k.transpose(1, 2).contiguous().transpose(1, 2),
+                            v.transpose(1, 2).contiguous().transpose(1, 2))):
+        out = torch.empty_like(q)
+        engine.launch_attend(q, kk, vv, out)
+        torch.cuda.synchronize()
+        assert torch.equal(out, v.expand_as(out))
