@@ -22,13 +22,14 @@
 //
 // What bounds it (the cases as sequences x tokens x heads (key/value heads) x head size, fp16):
 //  8192 causal, 32 (8) x 128  540-560 us, 980-1020 TFLOP/s of the 1311 that a library product of
-//                             8192^3 reaches: matrix cores busy half of the time, vector units 41-46%
+//                             8192^3 reaches: matrix cores busy half of the time, vector units 39-46%
 //                             (exponentials first); one wavefront's softmax runs beside another's
 //                             products, at 1.65-1.7 GHz.
 //  4 x 4096, window of 1023, prefix, cap, 16 (4) x 256  469 us, 545 TFLOP/s: 32 rows of 256 values
 //                             leave one wavefront a SIMD, whose products and softmax take turns.
 //  64 tokens over caches of up to 8192, 32 (8) x 128  195 us, 4.6 TB/s of K and V.
-//  heads of 64 and short sequences: vector units (50-63% busy) and the fixed cost of a tile.
+//  heads of 64 and short sequences: a tile's steps one after another (vector units 37-47% busy by
+//                             instructions, matrix cores 10-16%) and each workgroup's start.
 #include <limits.h>
 
 #include <algorithm>
