@@ -797,7 +797,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
 #pragma unroll 2
     for (int s = g; s < p.splits; s += GR) {
       const float ws2 = w[s];
-      if (ws2 == 0.f) continue;  // an empty split wrote nothing
+      if (ws2 == 0.f) continue;  // an empty split, or one far below the others
       const f32x4* src = reinterpret_cast<const f32x4*>(p.part_o + (slot * p.splits + s) * HD + 8 * c);
       const f32x4 u = src[0], v = src[1];
 #pragma unroll
