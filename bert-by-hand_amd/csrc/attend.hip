@@ -936,17 +936,17 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
 //               HD  NW KS SK R OCC
 using P32 = Cfg<32, 4, 1, 64, 2, 4>;
 using P64 = Cfg<64, 4, 1, 32, 2, 4>;
-using P96 = Cfg<96, 4, 1, 64, 2, 2>;
+using P96 = Cfg<96, 4, 1, 64, 2, 3>;
 using P128 = Cfg<128, 8, 1, 64, 2, 2>;
 using P256 = Cfg<256, 4, 1, 64, 2, 1>;
 using S32 = Cfg<32, 2, 1, 32, 2, 4>;
-using S64 = Cfg<64, 2, 1, 32, 2, 3>;
-using S96 = Cfg<96, 2, 1, 32, 2, 2>;
+using S64 = Cfg<64, 2, 1, 32, 2, 4>;
+using S96 = Cfg<96, 2, 1, 32, 2, 3>;
 using S128 = Cfg<128, 2, 1, 32, 2, 2>;
 using S256 = Cfg<256, 2, 1, 32, 2, 1>;
 using T32 = Cfg<32, 1, 1, 32, 1, 4>;
 using T64 = Cfg<64, 1, 1, 32, 1, 4>;
-using T96 = Cfg<96, 1, 1, 32, 1, 2>;
+using T96 = Cfg<96, 1, 1, 32, 1, 3>;
 using T128 = Cfg<128, 1, 1, 32, 1, 2>;
 using T256 = Cfg<256, 1, 1, 32, 1, 1>;
 using K32 = Cfg<32, 4, 4, 32, 1, 2>;
@@ -984,9 +984,11 @@ auto with_config(const AttendParams& p, bool scratch, F&& f) {
     BBH_BY_SIZE(K);
   }
   if (mean <= 16) BBH_BY_SIZE(T);
-  // Rows of S at most.  Above 64 values of 64 a head P is 3-8% faster where all sequences are as long,
-  // and far behind where they are not (2000 documents of 8 to 160 tokens: 301 us against 172).
-  const int64_t most = p.dim <= 96 ? 128 : p.dim <= 128 ? 1024 : 64;
+  // Rows of S at most.  Sequences of one length run as fast or faster on P from about 200 rows of 64
+  // values on (above), ones of 80 to 160 tokens far slower, whose last rows fill little of a
+  // workgroup (300 of them, 12 heads, us on P / S: 32 values 50 / 35, 64 61 / 45, 96 87 / 58; 64 of
+  // 256 to 512: 45 / 45, 63 / 63, 82 / 83).
+  const int64_t most = p.dim <= 96 ? 256 : p.dim <= 128 ? 1024 : 64;
   if (mean <= most) BBH_BY_SIZE(S);
   BBH_BY_SIZE(P);
 #undef BBH_BY_SIZE
