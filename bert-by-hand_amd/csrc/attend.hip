@@ -28,7 +28,7 @@
 //  4 x 4096, window of 1023, prefix, cap, 16 (4) x 256  469 us, 545 TFLOP/s: 32 rows of 256 values
 //                             leave one wavefront a SIMD, whose products and softmax take turns.
 //  64 tokens over caches of up to 8192, 32 (8) x 128  195 us, 4.6 TB/s of K and V.
-//  heads of 64 and short sequences: a tile's steps one after another (vector units 37-47% busy by
+//  heads of 64 and short sequences: a tile's steps one after another (vector units 37-54% busy by
 //                             instructions, matrix cores 10-16%) and each workgroup's start.
 #include <limits.h>
 
@@ -933,6 +933,9 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
 //  T  up to 16 rows: a wavefront, one stage
 //  K  up to 32 rows over many keys, whose four wavefronts take tiles of keys in turn
 //  L  the same with work for a wavefront everywhere
+// OCC wavefronts a SIMD, where that is worth more than the few registers that some then spill:
+// 2000 documents of 12 heads of 64 with slopes 163 us at four, 177 at three; 64 sequences of 256 to
+// 512 tokens, 12 heads of 96, 82 at three, 86 at two.
 //               HD  NW KS SK R OCC
 using P32 = Cfg<32, 4, 1, 64, 2, 4>;
 using P64 = Cfg<64, 4, 1, 32, 2, 4>;
