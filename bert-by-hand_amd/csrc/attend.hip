@@ -992,7 +992,10 @@ auto with_config(const AttendParams& p, bool scratch, F&& f) {
   // workgroup (300 of them, 12 heads, us on P / S: 32 values 50 / 35, 64 61 / 45, 96 87 / 58; 64 of
   // 256 to 512: 45 / 45, 63 / 63, 82 / 83).
   const int64_t most = p.dim <= 96 ? 256 : p.dim <= 128 ? 1024 : 64;
-  if (mean <= most) BBH_BY_SIZE(S);
+  // Above 128 values a workgroup of P has its CU to itself, so that nothing runs beside its first
+  // copies and last stores: worth it over many keys only (16 heads of 256, us on P / S: 500 of 192
+  // tokens 965 / 659, 100 of 203 on 4 key/value heads 244 / 222, 16 of 512 121 / 118, 30 of 1000 490 / 513).
+  if (mean <= most || (p.dim > 128 && keys <= 256)) BBH_BY_SIZE(S);
   BBH_BY_SIZE(P);
 #undef BBH_BY_SIZE
 }

@@ -520,7 +520,7 @@ def test_attend(torch_cuda, batch, q_len, k_len, heads, kv, dim, form):
 
 SETS = [  # every set of kernels: batch, q_len, k_len, heads, kv_heads
     (3, 9, 9, 2, 2), (2, 11, 150, 2, 1), (2, 60, 60, 2, 2), (1, 140, 140, 3, 3), (1, 1100, 1100, 1, 1),
-    (1, 2, 700, 4, 2), (2, 1, 70000, 4, 2), (1, 300, 5000, 8, 4),
+    (1, 2, 700, 4, 2), (2, 1, 70000, 4, 2), (1, 300, 5000, 8, 4), (2, 190, 190, 4, 1),
 ]
 
 
