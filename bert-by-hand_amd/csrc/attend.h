@@ -16,6 +16,10 @@ struct Divisor {
   uint32_t hi, lo;  // ceil(2^64 / d); 0: d is 1
 };
 
+// Largest cap under which scores are computed from 1 / (1 + e^2x) and its constant left out
+// (attend.hip, shape()).
+constexpr float kNearCap = 128.f;
+
 struct AttendParams {
   const f16 *q, *k, *v;
   f16* out;
@@ -30,11 +34,11 @@ struct AttendParams {
   Divisor by_cols, by_splits, by_kv;  // blocks * splits, splits, kv_heads
   uint32_t group_magic;  // ceil(2^32 / group), or 0
   int left, right, half;
-  float c;           // scale * log2(e)
-  float bias_scale;  // log2(e) / (c, or 2 * cap_l under a cap): biases in the units of the scores
+  float mscale;      // scores times this are powers of two: scale, twice a cap or a cap, each * log2(e)
+  float bias_scale;  // log2(e) / mscale: biases in the units of the scores
   bool table_lds;    // the table fits beside the tiles
-  float cap_k;  // 2 * log2(e) * scale / cap
-  float cap_l;  // cap * log2(e); 0: no cap
+  float cap_k;  // 2 * log2(e) * scale / cap of a cap up to kNearCap; 0: none
+  float cap_x;  // scale / cap of a larger one; 0: none
   int blocks, splits, chunk;  // row blocks; splits of a block's key tiles, `chunk` tiles each
 };
 

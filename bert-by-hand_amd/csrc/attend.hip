@@ -6,7 +6,8 @@
 // row (a query of a head), in base 2: for each tile of keys
 //   s = q K^T,  w = 2^(mscale s - m),  l += sum w,  o += w V,
 // where o and l are rescaled only when m rises by more than kLazy.  A cap's tanh is 1 - 2 / (1 + e^2x):
-// the constant drops out of the softmax, and one exp2 and one reciprocal are left (shape()).
+// the constant drops out of the softmax, and one exp2 and one reciprocal are left, for caps of up
+// to kNearCap (shape()).
 //
 // Rows.  A wavefront has 32 rows: the heads that share a key/value head lie side by side in them
 // (row = query * group + head), so that a tile of K and V serves all of them, and one token of 8
@@ -45,7 +46,8 @@ namespace {
 typedef BBH_LDS f16 lds_f16;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-enum Feat { kPlain = 0, kCap = 1, kAny = 2 };  // a softmax of the products, of capped ones, any bias
+// A softmax of the products, of ones under a cap up to kNearCap, with any bias or cap.
+enum Feat { kPlain = 0, kCap = 1, kAny = 2 };
 
 // Key (within a 32-key chunk) held by row r of the K tile.
 __device__ __forceinline__ int key_of_row(int r) {
@@ -211,9 +213,23 @@ __device__ __forceinline__ void scores(const Row<C>& r, const lds_f16* __restric
 }
 
 // Cap and bias.  The products s of q and k become -1 / (1 + 2^(cap_k s)) under a cap, which rises
-// as tanh does and times 2 cap_l is cap * tanh but for a constant, which a softmax does not see.
+// as tanh does and times 2 cap is cap * tanh but for a constant, which a softmax does not see.
 // Biases arrive in the units of either (divided by mscale), so that nothing is scaled here.
 //
+// That value lies near -1/2 wherever s is small against the cap, so that a score is off by up to
+// 8 * 2^-24 of the cap: 6e-5 at kNearCap, an eighth of a rounding of the weights to fp16, but more
+// than 1 at 2^24.  Under larger caps the value is tanh(x) itself, off by 2^-21 of its own size: up
+// to 3/4 the quotient x (945 + 105 x^2 + x^4) / (945 + 420 x^2 + 15 x^4), a convergent of tanh's
+// continued fraction (3e-9 of it at 3/4), from there on 1 - 2 / (1 + e^2|x|).  Three times the
+// operations, in the kernels for biases only.
+__device__ __forceinline__ float tanh_of(float x) {
+  const float a = fabsf(x), x2 = x * x;
+  const float n = fmaf(x2, x2 + 105.f, 945.f), d = fmaf(x2, fmaf(x2, 15.f, 420.f), 945.f);
+  const float e = __builtin_amdgcn_exp2f(a * 2.8853900817779268f);  // 2 log2(e)
+  const float far = copysignf(fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + e), 1.f), x);
+  return a < 0.75f ? x * n * __builtin_amdgcn_rcpf(d) : far;
+}
+
 // The table of a head lies in LDS with its ends repeated kPad times, so that the distances of a
 // chunk (32 keys from at most 32 neighbouring queries: 62 apart at most) are either all past one
 // end, where the bias is a constant, or all inside the padded table, where a lane reads eight
@@ -228,7 +244,7 @@ template <class C, int FEAT>
 __device__ __forceinline__ void shape(const AttendParams& p, const Row<C>& r, int k0, Scores<C>& x) {
   if constexpr (FEAT == kPlain) return;
   const int kh = (threadIdx.x & 63) >> 5;
-  if (FEAT == kCap || p.cap_l > 0.f) {
+  if (FEAT == kCap || p.cap_k > 0.f) {
 #pragma unroll
     for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
@@ -236,6 +252,12 @@ __device__ __forceinline__ void shape(const AttendParams& p, const Row<C>& r, in
         x.s[ch][i] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x.s[ch][i] * p.cap_k));
   }
   if constexpr (FEAT == kAny) {
+    if (p.cap_x > 0.f) {
+#pragma unroll
+      for (int ch = 0; ch < C::CH; ++ch)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x.s[ch][i] = tanh_of(x.s[ch][i] * p.cap_x);
+    }
     if (p.slopes) {
 #pragma unroll
       for (int ch = 0; ch < C::CH; ++ch) {
@@ -574,7 +596,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   r.m = -INFINITY;
   r.l = r.base = 0.f;
   r.far = false;
-  const float mscale = FEAT == kPlain ? p.c : FEAT == kCap || p.cap_l > 0.f ? 2.f * p.cap_l : p.c;
+  const float mscale = p.mscale;
   const float lag = kLazy / mscale;
   auto whole = [&](int k0, uint64_t bits) {
     return bits == kAll && (k0 + SK <= prefix || (k0 >= full_lo && k0 + SK <= full_hi));
@@ -901,7 +923,7 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
   // exact for rows below 2^32 / group
   p.group_magic = p.group > 1 && p.group <= 16 ? (uint32_t)(((1ull << 32) + p.group - 1) / p.group) : 0;
   p.table_lds = p.table && table_bytes(p) <= std::min<int64_t>(16384, (int64_t)kLdsMax - (int64_t)C::LDS);
-  const int feat = p.slopes || p.table ? kAny : p.cap_l > 0.f ? kCap : kPlain;
+  const int feat = p.slopes || p.table || p.cap_x > 0.f ? kAny : p.cap_k > 0.f ? kCap : kPlain;
   // sequences a launch: its work-items are counted in 32 bits
   const int64_t per = cols * p.kv_heads * C::THREADS;
   const int most = (int)std::min<int64_t>(p.batch, std::max<int64_t>(1, (kMostThreads / per) - 8));

@@ -326,10 +326,12 @@ static bbh_status attend_params(const bbh_attend_args* a, bbh::AttendParams& p) 
   p.right = a->right < 0 || a->right > 2 * kMaxLen ? -1 : a->right;
   p.half = a->table_half;
   const double log2e = 1.4426950408889634;
-  p.c = (float)(a->scale * log2e);
-  p.cap_k = a->cap > 0.f ? (float)(2 * log2e * a->scale / a->cap) : 0.f;
-  p.cap_l = (float)(a->cap * log2e);
-  p.bias_scale = (float)(a->cap > 0.f ? 0.5 / a->cap : 1.0 / a->scale);
+  const bool near = a->cap > 0.f && a->cap <= bbh::kNearCap, wide = a->cap > bbh::kNearCap;
+  const double unit = near ? 2.0 * a->cap : wide ? a->cap : a->scale;
+  p.mscale = (float)(unit * log2e);
+  p.bias_scale = (float)(1.0 / unit);
+  p.cap_k = near ? (float)(2 * log2e * a->scale / a->cap) : 0.f;
+  p.cap_x = wide ? a->scale / a->cap : 0.f;
   return BBH_OK;
 }
 

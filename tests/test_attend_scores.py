@@ -1,0 +1,97 @@
+"""Attention for other models (include/bbh_attend.h): scores far from zero and under
+large caps, small weights, every tile of a long cache, scratch of any size.
+
+u is half a step of fp32 relative to the value, 2^-24; H the same of fp16,
+2^-11; below fp16's normal range a rounding is off by up to 2^-25."""
+
+import math
+
+import pytest
+
+from test_attend import H, TINY, U, _gen, _normal
+
+gpu = pytest.mark.gpu
+
+
+# Scores of caps up to this are computed from an exponential next to 1, to half a
+# step of fp32 of the cap; those of larger ones to a few steps of their own size.
+NEAR_CAP = 128.0
+
+
+def _attend64(torch, q, k, v, right=-1, scale=None, cap=0.0, slopes=None, table=None):
+    """One sequence in 64 bits, and what a result may be off by, where only scores that
+    carry weight count: a key of weight 0 may have a score of any size."""
+    q, k, v = q.double(), k.double(), v.double()
+    (nq, h, d), nk = q.shape, k.shape[0]
+    rep = h // k.shape[1]
+    k, v = k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1)
+    scale = d ** -0.5 if scale is None else scale
+    qt, kt = q.transpose(0, 1), k.permute(1, 2, 0).contiguous()
+    s = torch.matmul(qt, kt) * scale
+    off = torch.matmul(qt.abs(), kt.abs()) * scale * (d + 4) * U  # fp32 sums of D products
+    if cap:
+        s = cap * torch.tanh(s / cap)
+        # the small ones: twice the cap times 1 / (1 + e), whose exponential (a quarter of 2 u),
+        # sum (u) and reciprocal (2 u) are off by less than 4 u together; the large ones: the
+        # argument (2 u) and a quotient of polynomials (6 u), or, of a result above 0.6, the
+        # same four and a difference
+        off = off + (8 * min(cap, NEAR_CAP) + 16 * s.abs()) * U
+    dist = torch.arange(nk, device="cuda") - (torch.arange(nq, device="cuda")[:, None] + nk - nq)
+    for b in ([] if slopes is None else [-slopes.double()[:, None, None] * dist.abs()]) + \
+            ([] if table is None else
+             [table.double()[:, dist.clamp(-(table.shape[1] // 2), table.shape[1] // 2) + table.shape[1] // 2]]):
+        s, off = s + b, off + 3 * U * (b.abs() + s.abs())
+    if right >= 0:
+        s = s.masked_fill(dist > right, -math.inf)
+    p = torch.softmax(s, -1)
+    # difference from the maximum and its product, rounded each
+    carry = p > 1e-12
+    off = torch.where(carry, off + 4 * U * s.abs(), 0.0).amax(-1, keepdim=True)
+    v = v.transpose(0, 1).contiguous()
+    out, size = torch.matmul(p, v), torch.matmul(p, v.abs())
+    # weights rounded to fp16 (those below 2^-21 of the largest by up to 2^-32 of it);
+    # the output rounded once; fp32 sums
+    small = torch.matmul(((p > 0) & (p < 2 ** -13)).double(), v.abs()) * 2.0 ** -32
+    tol = H * out.abs() + size * (2 * H + 4 * off + 2 * (nk ** 0.5 + 40) * U) + small + TINY + 1e-12 * nk
+    return out.transpose(0, 1), tol.transpose(0, 1)
+
+
+def _worst(torch, got, want, tol):
+    ratio = (got.double() - want).abs() / tol
+    assert bool(ratio.isfinite().all())
+    return float(ratio.max())
+
+
+# a set of kernels each: q_len, k_len, heads, kv_heads
+SETS = [(9, 9, 2, 2), (1, 500, 4, 2), (60, 60, 2, 2), (300, 300, 4, 2), (1100, 1100, 1, 1), (2, 66000, 4, 4)]
+
+
+@gpu
+@pytest.mark.parametrize("cap", [128.0, 129.0, 1e3, 1e5, 2.0 ** 24])
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+@pytest.mark.parametrize("q_len,k_len,heads,kv", SETS)
+def test_caps_of_any_size(torch_cuda, q_len, k_len, heads, kv, dim, cap):
+    """Ordinary scores, ones of the cap's size, and biases beside them."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, k_len + dim)
+    q = _normal(torch, g, 1, q_len, heads, dim)
+    k, v = _normal(torch, g, 1, k_len, kv, dim), _normal(torch, g, 1, k_len, kv, dim)
+    slopes = 0.05 * torch.rand(heads, device="cuda", generator=g)
+    table = torch.randn(heads, 41, device="cuda", generator=g)
+    scratch = torch.empty(1 << 22, device="cuda")
+    for kw in (dict(), dict(scale=3 * dim ** -0.5), dict(slopes=slopes), dict(table=table, right=0),
+               dict(scale=min(0.5 * cap * dim ** -0.5, 200.0))):
+        out = torch.full_like(q, float("nan"))
+        engine.launch_attend(q, k, v, out, cap=cap, scratch=scratch, **kw)
+        torch.cuda.synchronize()
+        want, tol = _attend64(torch, q[0], k[0], v[0], cap=cap, **kw)
+        assert _worst(torch, out[0], want, tol) <= 1, kw.keys()
+
+
+# batch, q_len, k_len, heads a key/value head, with scratch: kernels of a wavefront or four over
+# tiles in turn, of rows, split and not
+CACHES = [(1, 1, 70001, 2, True), (1, 1, 70001, 2, False), (1, 5, 70001, 1, True), (1, 1, 4003, 1, True),
+          (1, 3, 4003, 2, False), (70, 1, 1000, 1, True), (70, 1, 1000, 1, False), (1, 40, 9000, 1, True),
+          (1, 40, 9000, 1, False), (1, 300, 9000, 1, True), (3, 17, 140, 1, False)]
