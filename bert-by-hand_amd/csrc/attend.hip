@@ -74,9 +74,10 @@ struct Tile {
 constexpr float kLazy = 8.f;
 // A weight's exponent is fma(mscale, s, -(m mscale rounded)): one operation, and the product's
 // rounding error, the same in all of a row's weights, cancels with their sum.  With scores of 2^28
-// and more that error would itself be far from 0 (a bias of the type's lowest value: 2^100).  So a
-// wavefront that meets a maximum above kFar counts its rows' scores from there on from what their
-// maxima were (base), a subtraction a score, which only such wavefronts make.
+// and more that error would itself be far from 0 (a bias of the type's lowest value: 2^100).  So
+// while a wavefront's maxima lie further out than kFar, they are subtracted from the scores before
+// anything is scaled: exact next to the maximum.  Maxima stay what they are, never counted from an
+// earlier one: a score near 0 behind one of -10^9 would lose its digits in such a difference.
 constexpr float kFar = 65536.f;
 constexpr int kMaxSplits = 256;  // a thread of the joining workgroup each
 
@@ -181,8 +182,7 @@ struct Row {
   int tab;  // where distance 0 of the head's table is in LDS, or the head (a table in memory)
   f32x16 o[C::HD / 32];  // o[d][i]: dim 32 d + 8 (i / 4) + 4 (lane / 32) + i % 4
   float m, l;
-  float base;  // m and the scores are counted from here: 0, but where
-  bool far;    // some row's m came to lie above kFar
+  bool far;  // some row's m lies further from 0 than kFar
 };
 // A bias in the units of the scores.  Finite ones stay finite, in those units and as powers of two.
 __device__ __forceinline__ float bias_units(const AttendParams& p, float w) {
@@ -354,7 +354,7 @@ __device__ __forceinline__ float largest(const Scores<C>& x) {
 
 // Brings the running maximum up to a tile's, where that is far enough above it (kLazy).
 template <class C>
-__device__ __forceinline__ void raise(Row<C>& r, Scores<C>& x, float mx, float lag, float mscale) {
+__device__ __forceinline__ void raise(Row<C>& r, float mx, float lag, float mscale) {
   if (!__ballot(!(mx <= r.m + lag))) return;
   const float mn = imax(r.m, mx);
   if (__ballot(r.m != -INFINITY)) {  // (at the first tile there is nothing to bring along)
@@ -364,16 +364,7 @@ __device__ __forceinline__ void raise(Row<C>& r, Scores<C>& x, float mx, float l
     for (int d = 0; d < C::HD / 32; ++d) r.o[d] *= corr;
   }
   r.m = mn;
-  if (__ballot(mn != -INFINITY && fabsf(mn * mscale) > kFar)) {
-    const float by = mn == -INFINITY ? 0.f : mn;
-    r.far = true;
-    r.base += by;
-    r.m -= by;
-#pragma unroll
-    for (int ch = 0; ch < C::CH; ++ch)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x.s[ch][i] -= by;
-  }
+  r.far = __ballot(mn != -INFINITY && fabsf(mn * mscale) > kFar) != 0;
 }
 
 // Weights 2^(mscale (s - m)), rounded to fp16 (half of a step of an output's own type, and the
@@ -381,9 +372,17 @@ __device__ __forceinline__ void raise(Row<C>& r, Scores<C>& x, float mx, float l
 // It is added up with plain additions: a dot product of two does not run while the matrix unit is
 // busy (16 of them beside another wavefront's products 104 -> 230 cycles; additions 104 -> 129).
 template <class C>
-__device__ __forceinline__ void weigh(Row<C>& r, const Scores<C>& x, float mscale, Weights<C>& out) {
+__device__ __forceinline__ void weigh(Row<C>& r, Scores<C>& x, float mscale, Weights<C>& out) {
   // a row that has seen nothing yet: every weight 2^(-inf) = 0
-  const float mc = r.m == -INFINITY ? 0.f : r.m * mscale;
+  const float m = r.m == -INFINITY ? 0.f : r.m;
+  float mc = m * mscale;
+  if (r.far) {
+    mc = 0.f;
+#pragma unroll
+    for (int ch = 0; ch < C::CH; ++ch)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x.s[ch][i] -= m;
+  }
   float sum[4] = {};
 #pragma unroll
   for (int ch = 0; ch < C::CH; ++ch)
@@ -594,7 +593,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
 #pragma unroll
   for (int d = 0; d < ND; ++d) r.o[d] = f32x16{};
   r.m = -INFINITY;
-  r.l = r.base = 0.f;
+  r.l = 0.f;
   r.far = false;
   const float mscale = p.mscale;
   const float lag = kLazy / mscale;
@@ -607,7 +606,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   Seen<C> see;
   // A tile's products, softmax and output; false where no row of the wavefront sees any of it.
   auto tile_scores = [&](int k0, uint64_t bits, const lds_f16* ks, bool& edge) {
-    edge = r.far || !whole(k0, bits);
+    edge = !whole(k0, bits);
     if (!bits || (edge && !seen_of(r, k0, bits, prefix, see))) return false;
     scores(r, ks, x);
     ahead<C::CH * NS, 1, kAheadK>();
@@ -615,16 +614,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   };
   auto tile_weights = [&](int k0, bool edge) {
     shape<C, FEAT>(p, r, k0, x);
-    if (edge) {
-      hide(see, x);
-      if (r.far) {
-#pragma unroll
-        for (int ch = 0; ch < C::CH; ++ch)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x.s[ch][i] -= r.base;
-      }
-    }
-    raise(r, x, largest(x), lag, mscale);
+    if (edge) hide(see, x);
+    raise(r, largest(x), lag, mscale);
     weigh(r, x, mscale, w);
   };
   auto tile_output = [&](const lds_f16* vs) {
@@ -693,7 +684,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
     }
   }
   f32x16 (&o)[ND] = r.o;
-  const float m = r.m + r.base, l = xor32_sum(r.l);
+  const float m = r.m, l = xor32_sum(r.l);
 
   // ---- out
   const int cpr = p.dim / 8;
@@ -712,7 +703,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
       const int row = row0 + rw * 32 + r32;
       if (row >= rows) return;
       const int64_t sl = slot_of(row);
-      if (kh == 0) p.part_ml[sl] = make_float2(m * mscale, l);
+      if (kh == 0) p.part_ml[sl] = make_float2(m, l);
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -741,12 +732,12 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   } else {
     float* area = reinterpret_cast<float*>(smem);  // [KS][32][HD + 4]
     float2* ml = reinterpret_cast<float2*>(area + C::KS * 32 * (HD + 4));
-    if (kh == 0) ml[wave * 32 + r32] = make_float2(m * mscale, l);
+    if (kh == 0) ml[wave * 32 + r32] = make_float2(m, l);
     __syncthreads();
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < C::KS; ++w) top = imax(top, ml[w * 32 + r32].x);
-    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * mscale - top);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * mscale);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -763,7 +754,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
 #pragma unroll
       for (int w = 0; w < C::KS; ++w) {
         const float2 a = ml[w * 32 + rr];
-        sum += a.x == -INFINITY ? 0.f : a.y * __builtin_amdgcn_exp2f(a.x - tp);
+        sum += a.x == -INFINITY ? 0.f : a.y * __builtin_amdgcn_exp2f((a.x - tp) * mscale);
       }
       float v[8] = {};
 #pragma unroll
@@ -786,7 +777,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   }
 }
 
-// Joins the splits of a row: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  A
+// Joins the splits of a row: out = sum_s f_s o_s / sum_s f_s l_s, f_s = 2^(mscale (m_s - m)).  A
 // workgroup a row: its threads weigh the splits first, all at once, then groups of HD / 8
 // threads add every (256 / group)th split's outputs, and their sums are added through LDS.
 // (One thread for a piece of a row, split after split: 131 us for 184 splits.)
@@ -807,7 +798,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
   if ((tid & 63) == 0) red[0][tid >> 6] = wm;
   __syncthreads();
   const float top = imax(imax(red[0][0], red[0][1]), imax(red[0][2], red[0][3]));
-  const float f = mine.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine.x - top);
+  const float f = mine.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mine.x - top) * p.mscale);
   const float ws = wave_sum(f * mine.y);
   if ((tid & 63) == 0) red[1][tid >> 6] = ws;
   if (tid < p.splits) w[tid] = f;

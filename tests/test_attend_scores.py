@@ -90,6 +90,56 @@ def test_caps_of_any_size(torch_cuda, q_len, k_len, heads, kv, dim, cap):
         assert _worst(torch, out[0], want, tol) <= 1, kw.keys()
 
 
+@gpu
+@pytest.mark.parametrize("far", [-3e4, -1e6, -1e9, -3.4e38])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q_len,k_len,heads,kv", SETS[1:])
+def test_a_table_that_hides_by_large_values(torch_cuda, q_len, k_len, heads, kv, dim, far):
+    """The first keys of a row far below the ones behind them, as masks of -1e9 have it: the
+    latter's weights are those of their own differences."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, k_len + dim)
+    q = _normal(torch, g, 1, q_len, heads, dim)
+    k, v = _normal(torch, g, 1, k_len, kv, dim), _normal(torch, g, 1, k_len, kv, dim)
+    table = torch.randn(heads, 401, device="cuda", generator=g)
+    table[:, :180] = far  # more than 20 keys back
+    table[:, 230:] = far  # 30 and more ahead
+    scratch = torch.empty(1 << 22, device="cuda")
+    for cap in (0.0, 30.0):
+        for sc in (None, scratch):
+            out = torch.full_like(q, float("nan"))
+            engine.launch_attend(q, k, v, out, table=table, cap=cap, scratch=sc)
+            torch.cuda.synchronize()
+            want, tol = _attend64(torch, q[0], k[0], v[0], table=table, cap=cap)
+            assert _worst(torch, out[0], want, tol) <= 1, (cap, sc is None)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_len", [1, 64])
+@pytest.mark.parametrize("nk", [3000, 100000])
+def test_steep_slopes_over_a_long_cache(torch_cuda, nk, q_len, dim):
+    """In one pass and split: the first keys' scores lie as far as -2e6, those that carry weight
+    near zero."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, nk + dim)
+    q = 3 * _normal(torch, g, 1, q_len, 6, dim)
+    k, v = _normal(torch, g, 1, nk, 6, dim), _normal(torch, g, 1, nk, 6, dim)
+    slopes = torch.tensor([0.4, 0.6, 0.84, 1.0, 3.0, 20.0], device="cuda")
+    for sc in (None, torch.empty(1 << 22, device="cuda")):
+        out = torch.full_like(q, float("nan"))
+        engine.launch_attend(q, k, v, out, right=0, slopes=slopes, scratch=sc)
+        torch.cuda.synchronize()
+        # (keys further back than this weigh less than e^-700 against the query's own)
+        n = min(nk, 3000 + q_len)
+        want, tol = _attend64(torch, q[0], k[0, -n:], v[0, -n:], right=0, slopes=slopes)
+        assert _worst(torch, out[0], want, tol) <= 1, sc is None
+
+
 # batch, q_len, k_len, heads a key/value head, with scratch: kernels of a wavefront or four over
 # tiles in turn, of rows, split and not
 CACHES = [(1, 1, 70001, 2, True), (1, 1, 70001, 2, False), (1, 5, 70001, 1, True), (1, 1, 4003, 1, True),
