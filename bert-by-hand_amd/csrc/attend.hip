@@ -182,7 +182,9 @@ struct Row {
   int tab;  // where distance 0 of the head's table is in LDS, or the head (a table in memory)
   f32x16 o[C::HD / 32];  // o[d][i]: dim 32 d + 8 (i / 4) + 4 (lane / 32) + i % 4
   float m, l;
-  bool far;  // some row's m lies further from 0 than kFar
+  float mc;   // m * mscale, what a weight's exponent is counted from (0 where m is subtracted, or -infinity)
+  float lag;  // how far above m scores may lie: kLazy / mscale, or none at all (-infinity) while
+              // some row's m lies further from 0 than kFar
 };
 // A bias in the units of the scores.  Finite ones stay finite, in those units and as powers of two.
 __device__ __forceinline__ float bias_units(const AttendParams& p, float w) {
@@ -352,10 +354,12 @@ __device__ __forceinline__ float largest(const Scores<C>& x) {
   return imax(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
 }
 
-// Brings the running maximum up to a tile's, where that is far enough above it (kLazy).
+// Brings the running maximum up to a tile's, where that is far enough above it (r.lag), and
+// subtracts it from the tile's scores where some row's is far.
 template <class C>
-__device__ __forceinline__ void raise(Row<C>& r, float mx, float lag, float mscale) {
-  if (!__ballot(!(mx <= r.m + lag))) return;
+__device__ __forceinline__ void raise(Row<C>& r, Scores<C>& x, float mx, float lag, float mscale) {
+  // (one condition for both: a second one beside it takes 6% of 4 x 4096 causal of 12 heads of 64)
+  if (!__ballot(!(mx <= r.m + r.lag))) return;
   const float mn = imax(r.m, mx);
   if (__ballot(r.m != -INFINITY)) {  // (at the first tile there is nothing to bring along)
     const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((r.m - mn) * mscale);
@@ -364,7 +368,17 @@ __device__ __forceinline__ void raise(Row<C>& r, float mx, float lag, float msca
     for (int d = 0; d < C::HD / 32; ++d) r.o[d] *= corr;
   }
   r.m = mn;
-  r.far = __ballot(mn != -INFINITY && fabsf(mn * mscale) > kFar) != 0;
+  r.mc = mn == -INFINITY ? 0.f : mn * mscale;
+  r.lag = lag;
+  if (__ballot(fabsf(r.mc) > kFar)) {
+    r.lag = -INFINITY;
+    r.mc = 0.f;
+    const float by = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+    for (int ch = 0; ch < C::CH; ++ch)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x.s[ch][i] -= by;
+  }
 }
 
 // Weights 2^(mscale (s - m)), rounded to fp16 (half of a step of an output's own type, and the
@@ -372,23 +386,13 @@ __device__ __forceinline__ void raise(Row<C>& r, float mx, float lag, float msca
 // It is added up with plain additions: a dot product of two does not run while the matrix unit is
 // busy (16 of them beside another wavefront's products 104 -> 230 cycles; additions 104 -> 129).
 template <class C>
-__device__ __forceinline__ void weigh(Row<C>& r, Scores<C>& x, float mscale, Weights<C>& out) {
-  // a row that has seen nothing yet: every weight 2^(-inf) = 0
-  const float m = r.m == -INFINITY ? 0.f : r.m;
-  float mc = m * mscale;
-  if (r.far) {
-    mc = 0.f;
-#pragma unroll
-    for (int ch = 0; ch < C::CH; ++ch)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x.s[ch][i] -= m;
-  }
+__device__ __forceinline__ void weigh(Row<C>& r, const Scores<C>& x, float mscale, Weights<C>& out) {
   float sum[4] = {};
 #pragma unroll
   for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float e = __builtin_amdgcn_exp2f(fmaf(x.s[ch][i], mscale, -mc));
+      const float e = __builtin_amdgcn_exp2f(fmaf(x.s[ch][i], mscale, -r.mc));
       sum[i & 3] += e;
       out.w[ch][i >> 3][i & 7] = (f16)e;
     }
@@ -593,10 +597,9 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
 #pragma unroll
   for (int d = 0; d < ND; ++d) r.o[d] = f32x16{};
   r.m = -INFINITY;
-  r.l = 0.f;
-  r.far = false;
+  r.l = r.mc = 0.f;
   const float mscale = p.mscale;
-  const float lag = kLazy / mscale;
+  const float lag = r.lag = kLazy / mscale;
   auto whole = [&](int k0, uint64_t bits) {
     return bits == kAll && (k0 + SK <= prefix || (k0 >= full_lo && k0 + SK <= full_hi));
   };
@@ -615,7 +618,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   auto tile_weights = [&](int k0, bool edge) {
     shape<C, FEAT>(p, r, k0, x);
     if (edge) hide(see, x);
-    raise(r, largest(x), lag, mscale);
+    raise(r, x, largest(x), lag, mscale);
     weigh(r, x, mscale, w);
   };
   auto tile_output = [&](const lds_f16* vs) {
