@@ -35,6 +35,7 @@ struct AttendParams {
   uint32_t group_magic;  // ceil(2^32 / group), or 0
   int left, right, half;
   float mscale;      // scores times this are powers of two: scale, twice a cap or a cap, each * log2(e)
+  float lag;         // how far above a row's maximum its scores may lie before that is raised (attend.hip)
   float bias_scale;  // log2(e) / mscale: biases in the units of the scores
   bool table_lds;    // the table fits beside the tiles
   float cap_k;  // 2 * log2(e) * scale / cap of a cap up to kNearCap; 0: none

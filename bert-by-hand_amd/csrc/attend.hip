@@ -72,6 +72,11 @@ struct Tile {
 };
 
 constexpr float kLazy = 8.f;
+// Weights are 2^kRoom times what they are called here, up to 2^15 with kLazy: the factor is in the
+// sums and the output alike, and fp16, which weights are rounded to for the product with V, holds
+// ones down to 2^-21 of a row's maximum to 2^-11 of themselves, and smaller ones to 2^-32 of that (2^-25
+// without: at 10^5 equal keys e^18 below one other, all of them were zeros there and none in the sum).
+constexpr float kRoom = 7.f;
 // A weight's exponent is fma(mscale, s, -(m mscale rounded)): one operation, and the product's
 // rounding error, the same in all of a row's weights, cancels with their sum.  With scores of 2^28
 // and more that error would itself be far from 0 (a bias of the type's lowest value: 2^100).  So
@@ -182,7 +187,7 @@ struct Row {
   int tab;  // where distance 0 of the head's table is in LDS, or the head (a table in memory)
   f32x16 o[C::HD / 32];  // o[d][i]: dim 32 d + 8 (i / 4) + 4 (lane / 32) + i % 4
   float m, l;
-  float mc;   // m * mscale, what a weight's exponent is counted from (0 where m is subtracted, or -infinity)
+  float mc;   // m * mscale (0 where m is subtracted, or -infinity) - kRoom: a weight's exponent 0
   float lag;  // how far above m scores may lie: kLazy / mscale, or none at all (-infinity) while
               // some row's m lies further from 0 than kFar
 };
@@ -368,11 +373,11 @@ __device__ __forceinline__ void raise(Row<C>& r, Scores<C>& x, float mx, float l
     for (int d = 0; d < C::HD / 32; ++d) r.o[d] *= corr;
   }
   r.m = mn;
-  r.mc = mn == -INFINITY ? 0.f : mn * mscale;
+  r.mc = (mn == -INFINITY ? 0.f : mn * mscale) - kRoom;
   r.lag = lag;
   if (__ballot(fabsf(r.mc) > kFar)) {
     r.lag = -INFINITY;
-    r.mc = 0.f;
+    r.mc = -kRoom;
     const float by = mn == -INFINITY ? 0.f : mn;
 #pragma unroll
     for (int ch = 0; ch < C::CH; ++ch)
@@ -381,8 +386,8 @@ __device__ __forceinline__ void raise(Row<C>& r, Scores<C>& x, float mx, float l
   }
 }
 
-// Weights 2^(mscale (s - m)), rounded to fp16 (half of a step of an output's own type, and the
-// matrix unit's operand) for the product with V; their sum is of the unrounded ones, in fp32.
+// Weights 2^(mscale (s - m) + kRoom), rounded to fp16 (half of a step of an output's own type, and
+// the matrix unit's operand) for the product with V; their sum is of the unrounded ones, in fp32.
 // It is added up with plain additions: a dot product of two does not run while the matrix unit is
 // busy (16 of them beside another wavefront's products 104 -> 230 cycles; additions 104 -> 129).
 template <class C>
@@ -599,7 +604,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   r.m = -INFINITY;
   r.l = r.mc = 0.f;
   const float mscale = p.mscale;
-  const float lag = r.lag = kLazy / mscale;
+  r.lag = p.lag;
   auto whole = [&](int k0, uint64_t bits) {
     return bits == kAll && (k0 + SK <= prefix || (k0 >= full_lo && k0 + SK <= full_hi));
   };
@@ -618,7 +623,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
   auto tile_weights = [&](int k0, bool edge) {
     shape<C, FEAT>(p, r, k0, x);
     if (edge) hide(see, x);
-    raise(r, x, largest(x), lag, mscale);
+    raise(r, x, largest(x), p.lag, mscale);
     weigh(r, x, mscale, w);
   };
   auto tile_output = [&](const lds_f16* vs) {
@@ -911,6 +916,7 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
   const int64_t slots = (int64_t)p.batch * p.kv_heads * p.q_len * p.group;
   p.part_o = static_cast<float*>(scratch);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * p.splits * C::HD);
+  p.lag = kLazy / p.mscale;
   p.by_cols = divisor((uint64_t)cols);
   p.by_splits = divisor((uint64_t)p.splits);
   p.by_kv = divisor((uint64_t)p.kv_heads);

@@ -125,7 +125,8 @@ bbh_status bbh_rope_heads(const bbh_rope *rope, const bbh_rope_args *args, bbh_s
  * there is 0, and 0 times infinity is not).
  *
  * Scores, softmax and sums are fp32; the weights are rounded to fp16 for the product
- * with v, the output once.  Offsets, lengths, prefix, mask: int32, on the device.  slopes
+ * with v (to 2^-11 of a weight, or 2^-32 of the row's largest where that is more), the
+ * output once.  Offsets, lengths, prefix, mask: int32, on the device.  slopes
  * and table: fp32, on the device, finite and at most 1e20 and 1e30 in magnitude.  A table
  * may also hold -infinity (the pair is not seen) and lower finite values, the type's
  * lowest say, which count as some value below -1e30.  head_dim is a multiple of 8 up to

@@ -140,6 +140,32 @@ def test_steep_slopes_over_a_long_cache(torch_cuda, nk, q_len, dim):
         assert _worst(torch, out[0], want, tol) <= 1, sc is None
 
 
+@gpu
+@pytest.mark.parametrize("gap", [15.5, 17.25, 18.0, 19.0])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q_len,scratch", [(1, False), (1, True), (33, False), (700, False)])
+def test_a_long_flat_tail_keeps_its_values(torch_cuda, q_len, scratch, dim, gap):
+    """One key `gap` above 131071 equal ones, whose values alone are not zero: each weighs less
+    than 2^-22 of it, all of them 2e-2 to 7e-4."""
+    from bbh import engine
+
+    torch = torch_cuda
+    n = 131072
+    q = torch.zeros(1, q_len, 1, dim, device="cuda").half()
+    k, v = torch.zeros(1, n, 1, dim, device="cuda").half(), torch.ones(1, n, 1, dim, device="cuda").half()
+    q[..., 3], k[0, 0, 0, 3], v[0, 0] = 1.0, gap, 0.0
+    out = torch.full_like(q, float("nan"))
+    engine.launch_attend(q, k, v, out, scale=1.0,
+                         scratch=torch.empty(1 << 22, device="cuda") if scratch else None)
+    torch.cuda.synchronize()
+    tail = (n - 1) * math.exp(-gap)
+    want = tail / (1 + tail)
+    # each weight is off by up to 2^-32 of the largest; sums of up to 4096 tiles in fp32, the
+    # output rounded
+    tol = want * (2 * H + 2 * 8192 * U) + n * 2.0 ** -32 + TINY
+    assert float((out.double() - want).abs().max()) <= tol, float(out.double().mean() / want)
+
+
 # batch, q_len, k_len, heads a key/value head, with scratch: kernels of a wavefront or four over
 # tiles in turn, of rows, split and not
 CACHES = [(1, 1, 70001, 2, True), (1, 1, 70001, 2, False), (1, 5, 70001, 1, True), (1, 1, 4003, 1, True),
