@@ -251,20 +251,21 @@ template <class C, int FEAT>
 __device__ __forceinline__ void shape(const AttendParams& p, const Row<C>& r, int k0, Scores<C>& x) {
   if constexpr (FEAT == kPlain) return;
   const int kh = (threadIdx.x & 63) >> 5;
-  if (FEAT == kCap || p.cap_k > 0.f) {
-#pragma unroll
-    for (int ch = 0; ch < C::CH; ++ch)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        x.s[ch][i] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x.s[ch][i] * p.cap_k));
-  }
-  if constexpr (FEAT == kAny) {
-    if (p.cap_x > 0.f) {
+  if (FEAT == kCap || p.cap_k != 0.f) {  // (one condition a tile where there is no cap)
+    if (FEAT == kCap || p.cap_k > 0.f) {
 #pragma unroll
       for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x.s[ch][i] = tanh_of(x.s[ch][i] * p.cap_x);
+        for (int i = 0; i < 16; ++i)
+          x.s[ch][i] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x.s[ch][i] * p.cap_k));
+    } else {
+#pragma unroll
+      for (int ch = 0; ch < C::CH; ++ch)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x.s[ch][i] = tanh_of(x.s[ch][i] * -p.cap_k);
     }
+  }
+  if constexpr (FEAT == kAny) {
     if (p.slopes) {
 #pragma unroll
       for (int ch = 0; ch < C::CH; ++ch) {
@@ -923,7 +924,7 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
   // exact for rows below 2^32 / group
   p.group_magic = p.group > 1 && p.group <= 16 ? (uint32_t)(((1ull << 32) + p.group - 1) / p.group) : 0;
   p.table_lds = p.table && table_bytes(p) <= std::min<int64_t>(16384, (int64_t)kLdsMax - (int64_t)C::LDS);
-  const int feat = p.slopes || p.table || p.cap_x > 0.f ? kAny : p.cap_k > 0.f ? kCap : kPlain;
+  const int feat = p.slopes || p.table || p.cap_k < 0.f ? kAny : p.cap_k > 0.f ? kCap : kPlain;
   // sequences a launch: its work-items are counted in 32 bits
   const int64_t per = cols * p.kv_heads * C::THREADS;
   const int most = (int)std::min<int64_t>(p.batch, std::max<int64_t>(1, (kMostThreads / per) - 8));
