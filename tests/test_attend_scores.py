@@ -171,3 +171,46 @@ def test_a_long_flat_tail_keeps_its_values(torch_cuda, q_len, scratch, dim, gap)
 CACHES = [(1, 1, 70001, 2, True), (1, 1, 70001, 2, False), (1, 5, 70001, 1, True), (1, 1, 4003, 1, True),
           (1, 3, 4003, 2, False), (70, 1, 1000, 1, True), (70, 1, 1000, 1, False), (1, 40, 9000, 1, True),
           (1, 40, 9000, 1, False), (1, 300, 9000, 1, True), (3, 17, 140, 1, False)]
+
+
+@gpu
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("form", ["plain", "cap", "any", "window", "behind"])
+@pytest.mark.parametrize("batch,q_len,nk,group,scratch", CACHES)
+def test_every_tile_of_a_cache_counts_once(torch_cuda, batch, q_len, nk, group, scratch, form, dim):
+    """Equal scores, and each value of each key/value head from 32 keys of its own: a tile (or a key
+    of it) that is lost, read twice or weighed otherwise shows in the value of its own."""
+    from bbh import engine
+
+    torch = torch_cuda
+    tiles = (nk + 31) // 32
+    kv = (tiles + dim - 1) // dim
+    if batch > 1:
+        kv = max(kv, 16)
+    j = torch.arange(nk, device="cuda")
+    amount = 1 + j % 7
+    v = torch.zeros(nk, kv * dim, device="cuda", dtype=torch.float16)
+    v[j, j // 32] = amount.half()
+    v = v.view(1, nk, kv, dim).expand(batch, -1, -1, -1)
+    q = torch.zeros(batch, q_len, kv * group, dim, device="cuda").half()
+    k = _normal(torch, _gen(torch, nk), 1, nk, kv, dim).expand(batch, -1, -1, -1)
+    kw = {"plain": {}, "cap": dict(cap=8.0), "any": dict(slopes=torch.zeros(kv * group, device="cuda")),
+          "window": dict(left=nk - 45, right=0, prefix=torch.full((batch,), 10, device="cuda", dtype=torch.int32),
+                         mask=(j % 11 != 5).int().expand(batch, -1).contiguous()),
+          "behind": dict(left=nk // 3)}[form]
+    seen = torch.ones(q_len, nk, dtype=torch.bool, device="cuda")
+    if form == "window":
+        i = torch.arange(q_len, device="cuda")[:, None] + nk - q_len
+        seen = ((j <= i) & (j >= i - (nk - 45)) | (j < 10)) & (j % 11 != 5)
+    elif form == "behind":
+        seen = j >= torch.arange(nk - q_len, nk, device="cuda")[:, None] - nk // 3
+    each = torch.zeros(q_len, kv * dim, device="cuda", dtype=torch.float64)
+    each.index_add_(1, j // 32, seen.double() * amount)
+    want = (each / seen.sum(-1, keepdim=True)).view(q_len, kv, dim).repeat_interleave(group, 1)
+    out = torch.full_like(q, float("nan"))
+    room = torch.empty(max(engine.attend_scratch(q, k, v, out, **kw), 16), dtype=torch.uint8, device="cuda")
+    engine.launch_attend(q, k, v, out, scratch=room if scratch else None, **kw)
+    torch.cuda.synchronize()
+    # weights of exactly one power of two (under a cap to some steps of it, all alike), sums of
+    # whole numbers below 2^24: the reciprocal, the product and the output are rounded
+    assert bool(((out.double() - want).abs() <= (H + 64 * U) * want + TINY).all())
