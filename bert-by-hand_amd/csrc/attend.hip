@@ -878,10 +878,11 @@ hipError_t launch_as(const AttendParams& p, int64_t grid, hipStream_t s) {
 
 constexpr int64_t kMostThreads = 0xffffffffll;  // of a launch
 
-// Longest run of keys that a block of rows may see.
+// Longest run of keys that a sequence's rows may see: its last query stands at its last key, so that
+// there are none behind the window of the first, whatever `right`, but those up to there.
 int64_t longest(const AttendParams& p) {
   if (p.prefix || p.left < 0) return p.k_len;
-  return std::min<int64_t>(p.k_len, (int64_t)p.left + p.q_len + (p.right < 0 ? p.k_len : p.right));
+  return std::min<int64_t>(p.k_len, (int64_t)p.left + p.q_len);
 }
 
 // Row blocks, and how a block's keys are split over workgroups: enough of those that they all

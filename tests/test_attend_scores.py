@@ -214,3 +214,19 @@ def test_every_tile_of_a_cache_counts_once(torch_cuda, batch, q_len, nk, group, 
     # weights of exactly one power of two (under a cap to some steps of it, all alike), sums of
     # whole numbers below 2^24: the reciprocal, the product and the output are rounded
     assert bool(((out.double() - want).abs() <= (H + 64 * U) * want + TINY).all())
+
+
+@pytest.mark.parametrize("left,right", [(0, 0), (500, 0), (500, -1), (500, 7), (500, 1 << 28), (100000, -1)])
+@pytest.mark.parametrize("q_len", [1, 3, 40, 3000])
+def test_scratch_for_the_keys_that_a_window_leaves(q_len, left, right):
+    """The queries stand at the last keys: a bound behind them, or none, adds no key to what
+    their windows hold."""
+    import ctypes
+
+    from test_attend import _args, _lib
+
+    def bytes_of(**kw):
+        return _lib().bbh_attend_scratch(ctypes.byref(_args(batch=1, q_len=q_len, **kw)))
+
+    seen = min(1000000, q_len + left)
+    assert bytes_of(k_len=1000000, left=left, right=right) == bytes_of(k_len=seen, left=-1, right=-1)
