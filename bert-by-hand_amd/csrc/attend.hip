@@ -35,6 +35,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "attend.h"
 #include "pipe.h"
@@ -885,24 +886,44 @@ int64_t longest(const AttendParams& p) {
   return std::min<int64_t>(p.k_len, (int64_t)p.left + p.q_len);
 }
 
-// Row blocks, and how a block's keys are split over workgroups: enough of those that they all
-// end at about the same time, none with less than 512 keys.  (64 tokens over caches of up to 8192
-// keys, workgroups of one wavefront: 8192 workgroups 195 us, 1024 221; of 1024 keys each 208.)
+// Row blocks, and how a block's keys are split over workgroups where those are few.
+//  - Sets whose wavefronts take tiles in turn (K), the smallest of
+//    sqrt(tiles) parts: then a part's chain of tiles and the join's reading of all parts take about
+//      as long (128 values, 8 pairs of a sequence and a key/value head, us by parts: 8192 keys 8 16.7,
+//      16 14.4, 64 15.8; 32768 keys 8 36.7, 32 29.4, 128 34.1; 131072 keys 16 122, 64 101, 256 111);
+//    four rounds of the chip's places for workgroups;
+//    what the scratch holds;
+//    an odd number: the first parts, which short sequences have too, would go to the same eighth,
+//      quarter or half of the chip (512 ragged pairs of up to 8192 keys: 1 part 212, 2 217, 3 192, 4
+//      231, 6 194, 8 209; all of 8192: 356, 374, 373, 377, 383, 386).
+//    Few keys are not worth a join: up to 1024 (512 of more than 128 values, whose tile takes four
+//    times as long), twice that from 49 pairs on (32 pairs over 2048 keys: 1 part 18.0, 3 14.8; 96:
+//    19.2, 24.4 in 4; 192 over 1024: 19.0, 24.6 in 3; 256 values, 48 over 2048: 38.1, 26.0 in 4).
+//  - The others: 1024 workgroups, of 512 keys each at least.
 template <class C>
 void plan(AttendParams& p, size_t scratch_bytes) {
   const int64_t rows = (int64_t)p.q_len * p.group, items = (int64_t)p.batch * p.kv_heads;
   p.blocks = (int)((rows + C::BM - 1) / C::BM);
-  const int64_t tiles = (longest(p) + C::SK - 1) / C::SK + 2;
+  const int64_t keys = longest(p), tiles = (keys + C::SK - 1) / C::SK + 2;
   p.splits = 1;
   p.chunk = INT_MAX / 2;
-  const int64_t groups = items * p.blocks, target = C::NW == 1 ? 8192 : 1024;
+  const int64_t groups = items * p.blocks;
+  int64_t want, target = 1024;
+  if (C::KS > 1) {
+    target = C::HD > 128 ? 1024 : C::HD > 64 ? 2048 : 3072;
+    if (keys <= (C::HD > 128 ? 512 : 1024) * (groups > 48 ? 2 : 1)) return;
+    want = (int64_t)std::sqrt((double)tiles);
+  } else {
+    want = tiles / (512 / C::SK);
+  }
   if (groups >= target) return;
-  int64_t want = std::min<int64_t>(tiles / (512 / C::SK), (target + groups - 1) / groups);
+  want = std::min<int64_t>(want, (target + groups - 1) / groups);
   const int64_t a_split = items * rows * (C::HD * 4 + 8);
   want = std::min<int64_t>(std::min<int64_t>(want, kMaxSplits), (int64_t)(scratch_bytes / a_split));
+  if (C::KS > 1 && want % 2 == 0) --want;
   if (want < 2) return;
   p.chunk = (int)((tiles + want - 1) / want);
-  p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
+  p.splits = (int)want;
 }
 
 Divisor divisor(uint64_t d) {
@@ -956,7 +977,6 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
 //  S  fewer: 64, whose copies wait for less company
 //  T  up to 16 rows: a wavefront, one stage
 //  K  up to 32 rows over many keys, whose four wavefronts take tiles of keys in turn
-//  L  the same with work for a wavefront everywhere
 // OCC wavefronts a SIMD, where that is worth more than the few registers that some then spill:
 // 2000 documents of 12 heads of 64 with slopes 163 us at four, 177 at three; 64 sequences of 256 to
 // 512 tokens, 12 heads of 96, 82 at three, 86 at two.
@@ -981,11 +1001,6 @@ using K64 = Cfg<64, 4, 4, 32, 1, 2>;
 using K96 = Cfg<96, 4, 4, 32, 1, 2>;
 using K128 = Cfg<128, 4, 4, 32, 1, 2>;
 using K256 = Cfg<256, 4, 4, 32, 1, 1>;
-using L32 = Cfg<32, 1, 1, 64, 2, 4>;
-using L64 = Cfg<64, 1, 1, 64, 2, 2>;
-using L96 = Cfg<96, 1, 1, 32, 2, 2>;
-using L128 = Cfg<128, 1, 1, 32, 2, 2>;
-using L256 = T256;
 
 // By rows a sequence (on average, where documents are packed) and keys.  Measured on 40000 tokens
 // of 12 heads in sequences of one length, us on P / S / T:
@@ -994,7 +1009,7 @@ using L256 = T256;
 //   128 values a head:  8 tokens 1142 / 243 / 148, 16: 601 / 139 / 98, 32: 336 / 99 / 99, 128: 145 / 109 / 134,
 //                       300: 210 / 156 / 209, 300 by 4 heads a key/value head: 138 / 133 / 160, 500 so: 180 / 188 / 222
 template <class F>
-auto with_config(const AttendParams& p, bool scratch, F&& f) {
+auto with_config(const AttendParams& p, F&& f) {
   const int64_t rows = (int64_t)p.q_len * p.group, keys = longest(p);
   const int64_t items = (int64_t)p.batch * p.kv_heads;
   const int64_t mean = p.q_offsets ? p.q_rows * p.group / p.batch : rows;
@@ -1006,10 +1021,12 @@ auto with_config(const AttendParams& p, bool scratch, F&& f) {
     if (p.dim <= 128) return f(SET##128{}); \
     return f(SET##256{});                   \
   } while (0)
-  if (rows <= 32 && keys > 128) {
-    if (items >= 1024 || (scratch && items * keys >= 1 << 18)) BBH_BY_SIZE(L);
-    BBH_BY_SIZE(K);
-  }
+  // K for few rows over more than 128 keys.  But heads of more than 128 values, of which a CU holds one
+  // workgroup of K, run on T, a tile at a time, where there are wavefronts enough for that and few keys
+  // (8 heads a key/value head of 256, us on K / T: 520 pairs over 200 keys 36 / 26, 400: 61 / 49, 1000:
+  // 115 / 108; 2100: 118 / 98, 187 / 172, 374 / 405).
+  if (rows <= 32 && keys > 128 && !(p.dim > 128 && items >= 512 && keys <= 512)) BBH_BY_SIZE(K);
+  if (rows <= 32 && keys > 128) BBH_BY_SIZE(T);
   if (mean <= 16) BBH_BY_SIZE(T);
   // Rows of S at most.  Sequences of one length run as fast or faster on P from about 200 rows of 64
   // values on (above), ones of 80 to 160 tokens far slower, whose last rows fill little of a
@@ -1027,11 +1044,11 @@ auto with_config(const AttendParams& p, bool scratch, F&& f) {
 }  // namespace
 
 hipError_t attend(AttendParams p, void* scratch, size_t scratch_bytes, hipStream_t s) {
-  return with_config(p, scratch != nullptr, [&](auto c) { return launch<decltype(c)>(p, scratch, scratch_bytes, s); });
+  return with_config(p, [&](auto c) { return launch<decltype(c)>(p, scratch, scratch_bytes, s); });
 }
 
 size_t attend_scratch(const AttendParams& p) {
-  return with_config(p, true, [&](auto c) -> size_t {
+  return with_config(p, [&](auto c) -> size_t {
     AttendParams a = p;
     plan<decltype(c)>(a, SIZE_MAX / 2);
     if (a.splits < 2) return 0;

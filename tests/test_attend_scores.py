@@ -216,6 +216,35 @@ def test_every_tile_of_a_cache_counts_once(torch_cuda, batch, q_len, nk, group, 
     assert bool(((out.double() - want).abs() <= (H + 64 * U) * want + TINY).all())
 
 
+@gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q_len,nk,heads,kv", [(1, 300000, 4, 2), (5, 100003, 8, 4), (1, 40000, 12, 12)])
+def test_scratch_too_small_to_split_is_as_none(torch_cuda, q_len, nk, heads, kv, dim):
+    """Less scratch than it pays to have is used as far as it goes: none of it where it does not
+    hold two parts, and the call is the one without."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, nk)
+    q = _normal(torch, g, 1, q_len, heads, dim)
+    k, v = _normal(torch, g, 1, nk, kv, dim), _normal(torch, g, 1, nk, kv, dim)
+    whole = torch.empty_like(q)
+    engine.launch_attend(q, k, v, whole)
+    full = torch.empty_like(q)
+    most = engine.attend_scratch(q, k, v, full)
+    engine.launch_attend(q, k, v, full, scratch=torch.empty(most, dtype=torch.uint8, device="cuda"))
+    part = q_len * heads * (4 * dim + 8)
+    for n, same in ((16, True), (2 * part - 16, True), (2 * part, False), (3 * part, False), (most // 2, False)):
+        out = torch.full_like(q, float("nan"))
+        engine.launch_attend(q, k, v, out, scratch=torch.empty(n, dtype=torch.uint8, device="cuda"))
+        torch.cuda.synchronize()
+        assert not same or torch.equal(out, whole), n
+        # values of deviation (e / nk)^1/2 whose weights are rounded to fp16 at random on both
+        # sides, less than H of that each (ten of them allowed), and both outputs' own roundings
+        tol = 2 * H * full.double().abs() + 16 * H * nk ** -0.5 + 2 * TINY
+        assert bool(((out.double() - full.double()).abs() <= tol).all()), n
+
+
 @pytest.mark.parametrize("left,right", [(0, 0), (500, 0), (500, -1), (500, 7), (500, 1 << 28), (100000, -1)])
 @pytest.mark.parametrize("q_len", [1, 3, 40, 3000])
 def test_scratch_for_the_keys_that_a_window_leaves(q_len, left, right):
