@@ -117,7 +117,7 @@ bbh_status bbh_rope_create(const bbh_rope_config* c, bbh_rope** out) {
     return invalid(what, "rot_dim must be even and positive");
   if (c->rot_dim > BBH_ROPE_MAX_DIM)
     return fail(BBH_ERR_UNSUPPORTED, what, "rot_dim above 256 is not supported");
-  if (!isfinite(c->magnitude)) return invalid(what, "magnitude must be finite");
+  if (!isfinite((float)c->magnitude)) return invalid(what, "magnitude must be finite in fp32");
   const int pairs = c->rot_dim / 2;
   double f[bbh::kMaxRopePairs];
   if (c->frequencies) {

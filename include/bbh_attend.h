@@ -61,7 +61,7 @@ typedef struct bbh_rope_config {
   double factor;   /* >= 1 */
   double original; /* > 0 */
   double low, high; /* 0 < low < high */
-  double magnitude; /* of cos and sin; finite */
+  double magnitude; /* of cos and sin; finite in fp32 */
   /* the f_i themselves (rot_dim / 2 finite values, host memory, copied), in radians
    * a position; NULL: from base and scaling */
   const double *frequencies;
