@@ -1012,7 +1012,8 @@ template <class F>
 auto with_config(const AttendParams& p, F&& f) {
   const int64_t rows = (int64_t)p.q_len * p.group, keys = longest(p);
   const int64_t items = (int64_t)p.batch * p.kv_heads;
-  const int64_t mean = p.q_offsets ? p.q_rows * p.group / p.batch : rows;
+  // (a packed tensor may have more rows than the sequences, up to any int64)
+  const int64_t mean = p.q_offsets ? std::min(p.q_rows, p.batch * (int64_t)p.q_len) * p.group / p.batch : rows;
 #define BBH_BY_SIZE(SET)                    \
   do {                                      \
     if (p.dim <= 32) return f(SET##32{});   \

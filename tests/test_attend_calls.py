@@ -18,3 +18,14 @@ def test_a_magnitude_past_fp32_is_refused(magnitude):
     assert b"magnitude" in L.bbh_last_error() and not out.value
     ok = _rope_config(magnitude=3e38)
     assert L.bbh_rope_create(ctypes.byref(ok), ctypes.byref(out)) == 0 and L.bbh_rope_free(out) == 0
+
+
+def test_scratch_for_more_rows_than_the_longest_sequences_have():
+    """Rows of a packed tensor behind the sequences do not change what it pays to have, however
+    many there are."""
+    L = _lib()
+    kw = dict(batch=1, q_len=300, k_len=100000, heads=8, kv_heads=4, q_offsets=1 << 40)
+    want = L.bbh_attend_scratch(ctypes.byref(_args(q_rows=300, **kw)))
+    assert want > 0
+    for rows in (301, 1 << 31, 1 << 62, (1 << 63) - 1):
+        assert L.bbh_attend_scratch(ctypes.byref(_args(q_rows=rows, **kw))) == want, rows
