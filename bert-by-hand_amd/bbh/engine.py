@@ -693,8 +693,10 @@ def launch_rope(rope, q, q_out=None, k=None, k_out=None, v=None, v_out=None, pos
     seq = 0 if seq is None else _int("seq", seq)
     if rope is not None and positions is None and seq < 1:
         raise ValueError("positions or seq must be given")
-    if rows == 0 or heads == 0 or dim == 0:
+    if rows == 0 or dim == 0 or (heads == 0 and k is None and v is None):
         return q_out
+    if heads == 0:
+        raise ValueError("q has no heads")
     f16 = torch.float16
     args = capi.pack_rope_args(
         *at_q, *at_kv[0], *at_kv[2], *at_out, *at_kv[1], *at_kv[3],

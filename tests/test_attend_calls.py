@@ -29,3 +29,16 @@ def test_scratch_for_more_rows_than_the_longest_sequences_have():
     assert want > 0
     for rows in (301, 1 << 31, 1 << 62, (1 << 63) - 1):
         assert L.bbh_attend_scratch(ctypes.byref(_args(q_rows=rows, **kw))) == want, rows
+
+
+@gpu
+def test_queries_without_heads_are_refused(torch_cuda):
+    """Not passed over with the keys beside them unturned."""
+    from bbh import engine
+
+    torch = torch_cuda
+    q = torch.empty(5, 0, 64, device="cuda").half()
+    k = torch.randn(5, 2, 64, device="cuda").half()
+    with pytest.raises((ValueError, engine.BBHError)):
+        engine.launch_rope(engine.Rope(64), q, k=k, k_out=torch.empty_like(k), seq=5)
+    assert engine.launch_rope(engine.Rope(64), q, seq=5) is q
