@@ -238,7 +238,12 @@ __global__ __launch_bounds__(64 * kWaves) void rope_any_kernel(RopeParams p, Rop
     for (int h = 0; h < t.heads; ++h) {
       const f16* x = t.x + row * t.x_row + h * t.x_head;
       f16* y = t.y + yr * t.y_row + h * t.y_head;
-      float pa[2] = {}, pb[2] = {}, rest[4] = {};
+      if (!turns) {
+        for (int d = lane; d < p.dim; d += kWave) y[d] = x[d];
+        continue;
+      }
+      float pa[2] = {}, pb[2] = {};
+      f16 rest[4] = {};  // (as they are: a conversion and back makes a signalling NaN a quiet one)
       float q = 0.f;
       auto index = [&](int i, int which) {
         return p.interleaved ? 2 * i + which : i + which * pairs;
@@ -256,11 +261,11 @@ __global__ __launch_bounds__(64 * kWaves) void rope_any_kernel(RopeParams p, Rop
       for (int e = 0; e < 4; ++e) {
         const int d = p.rot + lane + 64 * e;
         if (d < p.dim) {
-          rest[e] = (float)x[d];
-          q = fmaf(rest[e], rest[e], q);
+          rest[e] = x[d];
+          q = fmaf((float)rest[e], (float)rest[e], q);
         }
       }
-      const bool norm = turns && t.gamma;
+      const bool norm = t.gamma != nullptr;
       float r = 1.f;
       if (norm) r = rsqrtf(wave_sum(q) / (float)p.dim + p.eps);
 #pragma unroll
@@ -273,7 +278,7 @@ __global__ __launch_bounds__(64 * kWaves) void rope_any_kernel(RopeParams p, Rop
             u *= r * (float)t.gamma[ia];
             v *= r * (float)t.gamma[ib];
           }
-          if (turns) turn(u, v, cs[i]);
+          turn(u, v, cs[i]);
           y[ia] = (f16)u;
           y[ib] = (f16)v;
         }
@@ -281,7 +286,7 @@ __global__ __launch_bounds__(64 * kWaves) void rope_any_kernel(RopeParams p, Rop
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = p.rot + lane + 64 * e;
-        if (d < p.dim) y[d] = (f16)(norm ? rest[e] * (r * (float)t.gamma[d]) : rest[e]);
+        if (d < p.dim) y[d] = norm ? (f16)((float)rest[e] * (r * (float)t.gamma[d])) : rest[e];
       }
     }
   };

@@ -42,3 +42,28 @@ def test_queries_without_heads_are_refused(torch_cuda):
     with pytest.raises((ValueError, engine.BBHError)):
         engine.launch_rope(engine.Rope(64), q, k=k, k_out=torch.empty_like(k), seq=5)
     assert engine.launch_rope(engine.Rope(64), q, seq=5) is q
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 33, 1])
+def test_every_bit_pattern_is_moved(torch_cuda, dim):
+    """v, and what of q and k neither turns nor is normed: signalling NaN too."""
+    from bbh import engine
+
+    torch = torch_cuda
+    bits = torch.arange(65536, device="cuda", dtype=torch.int32).to(torch.int16)
+    rows = -(-65536 // (2 * dim))
+    x = bits.repeat(2)[:rows * 2 * dim].view(rows, 2, dim).view(torch.float16).clone()
+    q, k, v = x.clone(), x.clone(), x.clone()
+    for gamma in (None, torch.ones(dim, device="cuda").half()):
+        outs = [torch.zeros_like(x) for _ in range(3)]
+        engine.launch_rope(None, q, outs[0], k=k, k_out=outs[1], v=v, v_out=outs[2], q_gamma=gamma)
+        torch.cuda.synchronize()
+        for got in outs[1 if gamma is not None else 0:]:
+            assert torch.equal(got.view(torch.int16), x.view(torch.int16))
+    if dim > 2:
+        rot = 2
+        y = torch.zeros_like(x)
+        engine.launch_rope(engine.Rope(rot), q, y, seq=1)
+        torch.cuda.synchronize()
+        assert torch.equal(y[..., rot:].view(torch.int16), x[..., rot:].view(torch.int16))
