@@ -61,7 +61,8 @@ struct Region {
 };
 
 // Whether two regions share memory, taking it as read that they do where that is not plain:
-// apart in memory, or columns of the same rows.
+// apart in memory, or columns of the same rows, or of the same heads of them (q, k and v of a head
+// side by side).
 bool overlap(const Region& a, const Region& b) {
   if (a.none() || b.none()) return false;
   if (a.begin() >= b.end() || b.begin() >= a.end()) return false;
@@ -74,7 +75,11 @@ bool overlap(const Region& a, const Region& b) {
   if (bytes % 2) return true;
   int64_t d = bytes / 2 % row;  // b's first column, seen from a's
   if (d < 0) d += row;
-  return !(d >= a.width() && d + b.width() <= row);
+  const bool wraps = d + b.width() > row;  // b's last columns lie in a's next row
+  if (d >= a.width() && !wraps) return false;
+  const int64_t head = a.heads > 1 ? a.head : b.head;
+  if (head < 1 || (b.heads > 1 && b.head != head) || (wraps && row % head)) return true;
+  return !(d % head >= a.dim && d % head + b.dim <= head);
 }
 
 // Whether an output's elements are apart from each other.

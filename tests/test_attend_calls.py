@@ -67,3 +67,55 @@ def test_every_bit_pattern_is_moved(torch_cuda, dim):
         engine.launch_rope(engine.Rope(rot), q, y, seq=1)
         torch.cuda.synchronize()
         assert torch.equal(y[..., rot:].view(torch.int16), x[..., rot:].view(torch.int16))
+
+
+@gpu
+@pytest.mark.parametrize("order", [(0, 1, 2), (2, 0, 1)])
+@pytest.mark.parametrize("rows,heads,dim", [(7, 3, 64), (50, 12, 64), (5, 2, 40)])
+def test_fused_rows_with_a_heads_q_k_and_v_side_by_side(torch_cuda, rows, heads, dim, order):
+    """In place: the heads of q, k and v interleave, and overlap nothing."""
+    from bbh import engine
+
+    torch = torch_cuda
+    g = _gen(torch, rows)
+    qkv = _normal(torch, g, rows, heads, 3, dim)
+    before = qkv.clone()
+    iq, ik, iv = order
+    rope = engine.Rope(dim)
+    pos = torch.arange(rows, device="cuda", dtype=torch.int32)
+    engine.launch_rope(rope, qkv[:, :, iq], k=qkv[:, :, ik], positions=pos)
+    torch.cuda.synchronize()
+    for i in (iq, ik):
+        want, tol = _rope64(torch, before[:, :, i], pos, _frequencies64(dim, 10000.0), False, 1.0, None, 0)
+        assert bool(((qkv[:, :, i].double() - want).abs() <= tol).all())
+    assert torch.equal(qkv[:, :, iv], before[:, :, iv])
+    # q's heads of one key/value head, then its key and value
+    group = _normal(torch, g, rows, heads, 4, dim)
+    before = group.clone()
+    # (heads of a head's group have no one stride: a call for each of them)
+    for i in (0, 1):
+        engine.launch_rope(rope, group[:, :, i], k=group[:, :, 2] if i == 0 else None, positions=pos)
+    torch.cuda.synchronize()
+    for i in (0, 1, 2):
+        want, tol = _rope64(torch, before[:, :, i], pos, _frequencies64(dim, 10000.0), False, 1.0, None, 0)
+        assert bool(((group[:, :, i].double() - want).abs() <= tol).all())
+    assert torch.equal(group[:, :, 3], before[:, :, 3])
+
+
+@pytest.mark.parametrize("change", [
+    dict(k_out_data=(1 << 30) + 64, k_out_head=192),       # k's first half over q's second
+    dict(k_out_data=(1 << 30) + 2 * 128, k_out_head=128),  # another stride
+    dict(k_out_data=(1 << 30) + 128, k_out_head=192, k_out_row=192 * 13),
+    dict(k_out_data=(1 << 30) + 12 * 192 * 2 - 64, k_out_head=192, k_out_row=192 * 12),
+])
+def test_heads_that_do_overlap_are_refused(change):
+    from bbh import engine
+
+    p = 1 << 30
+    a = dict(q_out_data=p, q_out_head=192, q_out_row=192 * 12, k_out_row=192 * 12, kv_heads=12,
+             q_data=20 * p, q_row=768, q_head=64, k_data=21 * p, k_row=768, k_head=64, v_data=None,
+             v_out_data=None)
+    a.update(change)
+    L = _lib()
+    assert L.bbh_rope_heads(engine.Rope(64).handle, ctypes.byref(_rope_args(**a)), None) == 1
+    assert b"overlap" in L.bbh_last_error()
