@@ -219,7 +219,9 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p, RopeSteps 
   }
 }
 
-// Any sizes and alignment: a wavefront a head, an element or a pair a lane.
+// Any sizes and alignment: a wavefront for the heads of a row, one after another, an element or a
+// pair a lane.  Bound by the number of accesses of 2 bytes (32768 rows of 16 heads of 65 values 93
+// us, 1.5 TB/s; 24 of 127 158 us, 2.5 TB/s).
 __global__ __launch_bounds__(64 * kWaves) void rope_any_kernel(RopeParams p, RopeSteps steps) {
   __shared__ float2 lds[kWaves][kMaxRopePairs];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -307,8 +309,11 @@ int width(const RopeParams::Part& t, int w) {
 }
 
 // Whether rows are read and written past the caches: from 48 MB on, where every store is of whole
-// lines (32768 x 40 x 128 142 -> 131 us; 131072 x 24 x 32, whose stores are of half lines, 81 ->
-// 139).  Three pieces a thread then (four 134, two 137).
+// lines (131072 x 24 x 32, whose stores are of half lines, 81 -> 139 us), with three pieces a thread
+// where heads are normed, two otherwise.  40 heads of 128, us with two pieces through the caches /
+// past them with two, three, four:
+//   normed      32 MB 17.3 / 17.5, 16.8, 19.3   48: 27.2 / 23.8, 21.7, 22.4   320: 141 / 135, 129, 132
+//   not normed  32 MB 12.9 / 13.7, 15.1, 16.6   48: 20.3 / 19.0, 20.6, 21.3   320: 117 / 105, 111, 119
 constexpr int64_t kStreamBytes = 48 << 20;
 bool lines(const RopeParams::Part& t) {
   return !t.heads || (((uintptr_t)t.y & 127) == 0 && ((t.y_row | t.y_head) & 63) == 0);
@@ -349,7 +354,7 @@ hipError_t launch(const RopeParams& p, const RopeSteps& steps, hipStream_t s) {
   // four), two otherwise (131072 x 24 x 32 81 us with two, 93 with four).
   if (items < 1 << 18) return launch_as<W, G, 1, false>(p, steps, s);
   if constexpr (W == 8) {
-    if (streams(p)) return launch_as<W, G, 3, true>(p, steps, s);
+    if (streams(p)) return launch_as<W, G, G ? 3 : 2, true>(p, steps, s);
   }
   return launch_as<W, G, 2, false>(p, steps, s);
 }
