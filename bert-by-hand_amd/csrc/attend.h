@@ -38,7 +38,8 @@ struct AttendParams {
   float lag;         // how far above a row's maximum its scores may lie before that is raised (attend.hip)
   float bias_scale;  // log2(e) / mscale: biases in the units of the scores
   bool table_lds;    // the table fits beside the tiles
-  float cap_k;  // 2 * log2(e) * scale / cap of a cap up to kNearCap, -scale / cap of a larger one; 0: none
+  float cap_k;  // 2 * log2(e) * scale / cap of a cap up to kNearCap, scale / cap of a larger one; 0: none
+  bool wide_cap;
   int blocks, splits, chunk;  // row blocks; splits of a block's key tiles, `chunk` tiles each
 };
 

@@ -22,13 +22,13 @@
 // resource's end and become zeros.
 //
 // What bounds it (the cases as sequences x tokens x heads (key/value heads) x head size, fp16):
-//  8192 causal, 32 (8) x 128  540-560 us, 980-1020 TFLOP/s of the 1311 that a library product of
-//                             8192^3 reaches: matrix cores busy half of the time, vector units 39-46%
+//  8192 causal, 32 (8) x 128  535-555 us, 990-1030 TFLOP/s of the 1311 that a library product of
+//                             8192^3 reaches: matrix cores busy half of the time, vector units 38%
 //                             (exponentials first); one wavefront's softmax runs beside another's
 //                             products, at 1.65-1.7 GHz.
-//  4 x 4096, window of 1023, prefix, cap, 16 (4) x 256  469 us, 545 TFLOP/s: 32 rows of 256 values
+//  4 x 4096, window of 1023, prefix, cap, 16 (4) x 256  471 us, 543 TFLOP/s: 32 rows of 256 values
 //                             leave one wavefront a SIMD, whose products and softmax take turns.
-//  64 tokens over caches of up to 8192, 32 (8) x 128  195 us, 4.6 TB/s of K and V.
+//  64 tokens over caches of up to 8192, 32 (8) x 128  187 us, 4.8 TB/s of K and V.
 //  heads of 64 and short sequences: a tile's steps one after another (vector units 37-54% busy by
 //                             instructions, matrix cores 10-16%) and each workgroup's start.
 #include <limits.h>
@@ -47,8 +47,9 @@ namespace {
 typedef BBH_LDS f16 lds_f16;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// A softmax of the products, of ones under a cap up to kNearCap, with any bias or cap.
-enum Feat { kPlain = 0, kCap = 1, kAny = 2 };
+// A softmax of the products, of ones under a cap up to kNearCap, with any bias beside them, with a
+// larger cap and any bias.
+enum Feat { kPlain = 0, kCap = 1, kAny = 2, kWide = 3 };
 
 // Key (within a 32-key chunk) held by row r of the K tile.
 __device__ __forceinline__ int key_of_row(int r) {
@@ -228,8 +229,10 @@ __device__ __forceinline__ void scores(const Row<C>& r, const lds_f16* __restric
 // 8 * 2^-24 of the cap: 6e-5 at kNearCap, an eighth of a rounding of the weights to fp16, but more
 // than 1 at 2^24.  Under larger caps the value is tanh(x) itself, off by 2^-21 of its own size: up
 // to 3/4 the quotient x (945 + 105 x^2 + x^4) / (945 + 420 x^2 + 15 x^4), a convergent of tanh's
-// continued fraction (3e-9 of it at 3/4), from there on 1 - 2 / (1 + e^2|x|).  Three times the
-// operations, in the kernels for biases only.
+// continued fraction (3e-9 of it at 3/4), from there on 1 - 2 / (1 + e^2|x|).  These are three
+// times the operations, in kernels of their own: beside the others' they take registers that cost
+// 5-15% of calls with a bias (4 x 4096 causal, 16 (4) x 128: 296 us without a cap, 345 up to kNearCap,
+// 567 beyond).
 __device__ __forceinline__ float tanh_of(float x) {
   const float a = fabsf(x), x2 = x * x;
   const float n = fmaf(x2, x2 + 105.f, 945.f), d = fmaf(x2, fmaf(x2, 15.f, 420.f), 945.f);
@@ -241,7 +244,9 @@ __device__ __forceinline__ float tanh_of(float x) {
 // The table of a head lies in LDS with its ends repeated kPad times, so that the distances of a
 // chunk (32 keys from at most 32 neighbouring queries: 62 apart at most) are either all past one
 // end, where the bias is a constant, or all inside the padded table, where a lane reads eight
-// neighbouring values with no clamping.  Tables too long for that are read from memory.
+// neighbouring values with no clamping.  Tables of more than 16 KB are read from memory, so that
+// every set keeps its workgroups a CU (32 x 509, 12 x 64, us: 257 entries 52.7, 1801 57.0, 3801 61.6;
+// from memory, 3969 to 18001, 88.9).
 constexpr int kPad = 64;
 template <class C>
 __device__ __forceinline__ BBH_LDS float* table_area() {
@@ -252,21 +257,19 @@ template <class C, int FEAT>
 __device__ __forceinline__ void shape(const AttendParams& p, const Row<C>& r, int k0, Scores<C>& x) {
   if constexpr (FEAT == kPlain) return;
   const int kh = (threadIdx.x & 63) >> 5;
-  if (FEAT == kCap || p.cap_k != 0.f) {  // (one condition a tile where there is no cap)
-    if (FEAT == kCap || p.cap_k > 0.f) {
+  if constexpr (FEAT == kWide) {
 #pragma unroll
-      for (int ch = 0; ch < C::CH; ++ch)
+    for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          x.s[ch][i] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x.s[ch][i] * p.cap_k));
-    } else {
+      for (int i = 0; i < 16; ++i) x.s[ch][i] = tanh_of(x.s[ch][i] * p.cap_k);
+  } else if (FEAT == kCap || p.cap_k > 0.f) {
 #pragma unroll
-      for (int ch = 0; ch < C::CH; ++ch)
+    for (int ch = 0; ch < C::CH; ++ch)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x.s[ch][i] = tanh_of(x.s[ch][i] * -p.cap_k);
-    }
+      for (int i = 0; i < 16; ++i)
+        x.s[ch][i] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x.s[ch][i] * p.cap_k));
   }
-  if constexpr (FEAT == kAny) {
+  if constexpr (FEAT >= kAny) {
     if (p.slopes) {
 #pragma unroll
       for (int ch = 0; ch < C::CH; ++ch) {
@@ -523,7 +526,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void attend_kernel(AttendParams
     r.pos = i + shift;
     r.lo = p.left < 0 ? 0 : max(r.pos - p.left, 0);
     r.hi = p.right < 0 ? nk : min(r.pos + p.right + 1, nk);
-    if constexpr (FEAT == kAny) {
+    if constexpr (FEAT >= kAny) {
       const int w0 = row0 + rw * 32;
       r.first = query_of(p, min(w0, rows - 1)) + shift;
       r.last = query_of(p, min(w0 + 31, rows - 1)) + shift;
@@ -872,7 +875,7 @@ hipError_t launch_as(const AttendParams& p, int64_t grid, hipStream_t s) {
     if (e != hipSuccess) return e;
     set.fetch_or(bit, std::memory_order_relaxed);
   }
-  const size_t lds = C::LDS + (FEAT == kAny && p.table_lds ? table_bytes(p) : 0);
+  const size_t lds = C::LDS + (FEAT >= kAny && p.table_lds ? table_bytes(p) : 0);
   hipLaunchKernelGGL((attend_kernel<C, FEAT>), dim3((unsigned)grid), dim3(C::THREADS), lds, s, p);
   return hipGetLastError();
 }
@@ -896,8 +899,8 @@ int64_t longest(const AttendParams& p) {
 //    an odd number: the first parts, which short sequences have too, would go to the same eighth,
 //      quarter or half of the chip (512 ragged pairs of up to 8192 keys: 1 part 212, 2 217, 3 192, 4
 //      231, 6 194, 8 209; all of 8192: 356, 374, 373, 377, 383, 386).
-//    Few keys are not worth a join: up to 1024 (512 of more than 128 values, whose tile takes four
-//    times as long), twice that from 49 pairs on (32 pairs over 2048 keys: 1 part 18.0, 3 14.8; 96:
+//    Few keys are not worth a join: up to 1024 (512 of more than 128 values, whose tile takes
+//    nearly three times as long), twice that from 49 pairs on (32 pairs over 2048 keys: 1 part 18.0, 3 14.8; 96:
 //    19.2, 24.4 in 4; 192 over 1024: 19.0, 24.6 in 3; 256 values, 48 over 2048: 38.1, 26.0 in 4).
 //  - The others: 1024 workgroups, of 512 keys each at least.
 template <class C>
@@ -946,7 +949,7 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
   // exact for rows below 2^32 / group
   p.group_magic = p.group > 1 && p.group <= 16 ? (uint32_t)(((1ull << 32) + p.group - 1) / p.group) : 0;
   p.table_lds = p.table && table_bytes(p) <= std::min<int64_t>(16384, (int64_t)kLdsMax - (int64_t)C::LDS);
-  const int feat = p.slopes || p.table || p.cap_k < 0.f ? kAny : p.cap_k > 0.f ? kCap : kPlain;
+  const int feat = p.wide_cap ? kWide : p.slopes || p.table ? kAny : p.cap_k > 0.f ? kCap : kPlain;
   // sequences a launch: its work-items are counted in 32 bits
   const int64_t per = cols * p.kv_heads * C::THREADS;
   const int most = (int)std::min<int64_t>(p.batch, std::max<int64_t>(1, (kMostThreads / per) - 8));
@@ -959,7 +962,8 @@ hipError_t launch(AttendParams p, void* scratch, size_t scratch_bytes, hipStream
                                           : (rows * cols + kXcds - 1) / kXcds * kXcds;
     const hipError_t e = feat == kPlain ? launch_as<C, kPlain>(p, grid, s)
                          : feat == kCap ? launch_as<C, kCap>(p, grid, s)
-                                        : launch_as<C, kAny>(p, grid, s);
+                         : feat == kAny ? launch_as<C, kAny>(p, grid, s)
+                                        : launch_as<C, kWide>(p, grid, s);
     if (e != hipSuccess) return e;
   }
   if (p.splits > 1) {

@@ -335,7 +335,8 @@ static bbh_status attend_params(const bbh_attend_args* a, bbh::AttendParams& p) 
   const double unit = near ? 2.0 * a->cap : wide ? a->cap : a->scale;
   p.mscale = (float)(unit * log2e);
   p.bias_scale = (float)(1.0 / unit);
-  p.cap_k = near ? (float)(2 * log2e * a->scale / a->cap) : wide ? -(a->scale / a->cap) : 0.f;
+  p.cap_k = near ? (float)(2 * log2e * a->scale / a->cap) : wide ? a->scale / a->cap : 0.f;
+  p.wide_cap = wide;
   return BBH_OK;
 }
 
