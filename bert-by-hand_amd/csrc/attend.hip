@@ -231,8 +231,8 @@ __device__ __forceinline__ void scores(const Row<C>& r, const lds_f16* __restric
 // to 3/4 the quotient x (945 + 105 x^2 + x^4) / (945 + 420 x^2 + 15 x^4), a convergent of tanh's
 // continued fraction (3e-9 of it at 3/4), from there on 1 - 2 / (1 + e^2|x|).  These are three
 // times the operations, in kernels of their own: beside the others' they take registers that cost
-// 5-15% of calls with a bias (4 x 4096 causal, 16 (4) x 128: 296 us without a cap, 345 up to kNearCap,
-// 567 beyond).
+// 5-15% of calls with a bias (4 x 4096 causal, 16 (4) x 128: 312 us without a cap, 374 up to kNearCap,
+// 550 beyond).
 __device__ __forceinline__ float tanh_of(float x) {
   const float a = fabsf(x), x2 = x * x;
   const float n = fmaf(x2, x2 + 105.f, 945.f), d = fmaf(x2, fmaf(x2, 15.f, 420.f), 945.f);
