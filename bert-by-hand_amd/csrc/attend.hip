@@ -894,14 +894,15 @@ int64_t longest(const AttendParams& p) {
 //    sqrt(tiles) parts: then a part's chain of tiles and the join's reading of all parts take about
 //      as long (128 values, 8 pairs of a sequence and a key/value head, us by parts: 8192 keys 8 16.7,
 //      16 14.4, 64 15.8; 32768 keys 8 36.7, 32 29.4, 128 34.1; 131072 keys 16 122, 64 101, 256 111);
-//    four rounds of the chip's places for workgroups;
+//    four rounds of the chip's places for workgroups (1, 2 and 3 a CU, by head size);
 //    what the scratch holds;
 //    an odd number: the first parts, which short sequences have too, would go to the same eighth,
 //      quarter or half of the chip (512 ragged pairs of up to 8192 keys: 1 part 212, 2 217, 3 192, 4
 //      231, 6 194, 8 209; all of 8192: 356, 374, 373, 377, 383, 386).
 //    Few keys are not worth a join: up to 1024 (512 of more than 128 values, whose tile takes
-//    nearly three times as long), twice that from 49 pairs on (32 pairs over 2048 keys: 1 part 18.0, 3 14.8; 96:
-//    19.2, 24.4 in 4; 192 over 1024: 19.0, 24.6 in 3; 256 values, 48 over 2048: 38.1, 26.0 in 4).
+//    nearly three times as long), twice that from 49 pairs on (32 pairs over 2048 keys: 1 part 18.0,
+//    3 14.8; 96: 19.2, 24.4 in 4; 192 over 1024: 19.0, 24.6 in 3; 256 values, 48 over 2048: 38.1, 26.0
+//    in 4).
 //  - The others: 1024 workgroups, of 512 keys each at least.
 template <class C>
 void plan(AttendParams& p, size_t scratch_bytes) {
