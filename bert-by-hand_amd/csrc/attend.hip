@@ -914,7 +914,7 @@ void plan(AttendParams& p, size_t scratch_bytes) {
   const int64_t groups = items * p.blocks;
   int64_t want, target = 1024;
   if (C::KS > 1) {
-    target = C::HD > 128 ? 1024 : C::HD > 64 ? 2048 : 3072;
+    target = 1024 * (C::HD > 128 ? 1 : C::HD > 64 ? 2 : 3);
     if (keys <= (C::HD > 128 ? 512 : 1024) * (groups > 48 ? 2 : 1)) return;
     want = (int64_t)std::sqrt((double)tiles);
   } else {
